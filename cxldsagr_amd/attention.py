@@ -228,3 +228,93 @@ def pack_kv_fp8(kv, kv_cache, page_table, token_offset=0, status=None):
             _native.stream_of(kv.device),
         )
     return kv_cache
+
+
+PROMPT_HEAD_DIMS = ((192, 128), (128, 128), (64, 64))
+
+
+def _check_starts(starts, device, what):
+    if (not isinstance(starts, torch.Tensor) or starts.dtype != torch.int32 or starts.ndim != 1
+            or starts.numel() < 1 or starts.device != device):
+        raise ValueError(f"{what} must be int32 [sequences + 1] on the query device")
+    return starts.contiguous()
+
+
+def _heads_layout(tensor):
+    """``tensor`` [tokens, heads, dim] as the kernels read it: the last dim
+    contiguous, the other strides multiples of 16 bytes, aligned; else a copy."""
+    token, head, dim = tensor.stride()
+    if (dim != 1 or token % 8 or head % 8 or not 0 <= token < 1 << 25 or not 0 <= head < 1 << 25
+            or tensor.data_ptr() % 16):
+        return tensor.clone(memory_format=torch.contiguous_format)
+    return tensor
+
+
+def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None, out=None):
+    """Causal attention over packed sequences with grouped heads.
+
+    ``q`` ``[Tq, H, d_qk]``, ``k`` ``[Tk, H_kv, d_qk]``, ``v`` ``[Tk, H_kv, d_v]``
+    in bf16 or fp16 (any token and head strides), ``(d_qk, d_v)`` one of
+    ``(192, 128)``, ``(128, 128)``, ``(64, 64)``; head ``h`` reads KV head
+    ``h // (H // H_kv)``. Sequence ``b`` holds queries ``cu_q[b]:cu_q[b + 1]`` and
+    keys ``cu_k[b]:cu_k[b + 1]`` (int32 ``[sequences + 1]`` on the device,
+    ascending; ``cu_k`` defaults to ``cu_q``). Query ``i`` of ``n_q`` sees keys
+    ``j <= i + n_k - n_q``: a prompt, a chunk after a history, single tokens
+    (``causal=False``: every key). A query that sees no key gives zeros.
+
+    Returns ``[Tq, H, d_v]`` in ``q``'s type, or writes it to ``out``
+    (contiguous); queries outside the sequences (before ``cu_q[0]``, from
+    ``cu_q[-1]`` on) are left as they were in ``out``. ``max_k`` (default
+    ``Tk``): an upper bound of a sequence's keys, by which few queries' keys are
+    split over the GPU; it does not change what is computed. Forward only. A
+    key that some query of its sequence does not see must have finite values.
+    """
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise ValueError("Expected q [Tq,H,Dqk], k [Tk,Hkv,Dqk], and v [Tk,Hkv,Dv]")
+    if k.shape[:2] != v.shape[:2] or q.shape[2] != k.shape[2]:
+        raise ValueError("Query, key, and value dimensions do not agree")
+    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError("q's heads must be a positive multiple of k's")
+    if (q.shape[2], v.shape[2]) not in PROMPT_HEAD_DIMS:
+        raise ValueError(f"(Dqk, Dv) must be one of {PROMPT_HEAD_DIMS}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k, and v must share bf16 or fp16")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k, and v must be on the same device")
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be positive and finite")
+    if max_k is not None and (type(max_k) is not int or max_k < 0):
+        raise ValueError("max_k must be a nonnegative integer")
+    if any(t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+        raise ValueError("prompt attention has no backward pass")
+    _native.require_gfx950(q.device, "prompt attention")
+    cu_q = _check_starts(cu_q, q.device, "cu_q")
+    cu_k = cu_q if cu_k is None else _check_starts(cu_k, q.device, "cu_k")
+    if cu_k.numel() != cu_q.numel():
+        raise ValueError("cu_q and cu_k must describe the same sequences")
+    shape = (*q.shape[:2], v.shape[2])
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != q.dtype
+          or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned [Tq, H, Dv] tensor of q's "
+                         "dtype on q's device")
+    sequences = cu_q.numel() - 1
+    if not q.shape[0] or not sequences:
+        return out
+    max_k = k.shape[0] if max_k is None else min(max_k, k.shape[0])
+    q, k, v = _heads_layout(q), _heads_layout(k), _heads_layout(v)
+    with _native.on_device(q.device):
+        needed = _native.size_of("dsa_prompt_attention_workspace_bytes", q.device.index,
+                                 q.shape[0], q.shape[1], k.shape[1], v.shape[2], sequences, max_k)
+        workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
+        _native.call(
+            "dsa_prompt_attention",
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), _native.DTYPE_CODES[q.dtype],
+            q.shape[1], k.shape[1], q.shape[2], v.shape[2],
+            cu_q.data_ptr(), cu_k.data_ptr(), sequences, q.shape[0], k.shape[0], max_k,
+            float(scale), int(causal), out.data_ptr(), _native.ptr(workspace), needed,
+            _native.raw_stream(q.device),
+        )
+    return out

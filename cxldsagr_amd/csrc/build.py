@@ -52,6 +52,10 @@ FLAGS = [
 SOURCE_FLAGS = {
     "sparse_mla.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "logits.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # prompt_attention, shared_prefix: VGPR-form MFMA as sparse_mla (their
+    # accumulators are rescaled outside the key loop's inner part).
+    "prompt_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "shared_prefix.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # topk: the exact row recompute of the candidate top-k runs the logits
     # arithmetic (logits_core.h) and must compile it as logits.hip does.
     "topk.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"],

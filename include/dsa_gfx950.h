@@ -451,6 +451,37 @@ int dsa_sparse_mla_fp8_paged_ws(const void* q, int64_t rows, int64_t heads, cons
                                 void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Causal attention over packed sequences with grouped heads. No reference
+ * counterpart (operators/flashinfer.py adapts a library's).
+ * q: [q_tokens, heads, qk_dim], k: [k_tokens, kv_heads, qk_dim], v: [k_tokens,
+ * kv_heads, v_dim], all `dtype` (bf16 or fp16), the last dim contiguous, token
+ * and head strides in elements (multiples of 8, below 2^25), 16-byte aligned;
+ * (qk_dim, v_dim) one of (192, 128), (128, 128), (64, 64); heads a multiple of
+ * kv_heads. Sequence b holds queries cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b]
+ * .. cu_k[b + 1] - 1 (int32 device arrays of sequences + 1 entries, ascending;
+ * what lies outside the tensors is cut off). With causal != 0 query i of n_q sees
+ * keys j <= i + n_k - n_q, else every key. out: dtype [q_tokens, heads, v_dim]
+ * contiguous, 16-byte aligned = softmax(scale q k^T) v, zeros for a query that
+ * sees no key; queries outside the sequences are not written. scale > 0.
+ * max_k: at least the longest sequence's keys (it decides how keys are split
+ * over work-groups, not what is computed). `workspace`: 16-byte aligned, at least
+ * dsa_prompt_attention_workspace_bytes bytes (0: not used), no initialisation,
+ * free again when the stream has passed the call; not to be shared by calls that
+ * may run at the same time.
+ */
+int dsa_prompt_attention_workspace_bytes(int64_t q_tokens, int64_t heads, int64_t kv_heads,
+                                         int64_t v_dim, int64_t sequences, int64_t max_k,
+                                         int64_t* bytes);
+int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                         int64_t heads, int64_t kv_heads, int64_t qk_dim, int64_t v_dim,
+                         const int32_t* cu_q, const int32_t* cu_k, int64_t sequences,
+                         int64_t q_tokens, int64_t k_tokens, int64_t max_k, float scale,
+                         int causal, void* out, void* workspace, int64_t workspace_bytes,
+                         hipStream_t stream);
+
+/*
  * A11 - gather whole records from pinned host memory into device memory,
  * device[device_ids[r]] = host[host_ids[r]] for r < count, or for
  * r < *valid_count when valid_count (a device int64 or uint32 scalar, kind
