@@ -79,6 +79,10 @@ SIGNATURES = {
     "dsa_prompt_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _int, _i64,
                              _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _int,
                              _ptr, _ptr, _i64, _ptr],
+    "dsa_shared_prefix_mla_workspace_bytes": [_i64, _i64, _i64, _i64,
+                                              ctypes.POINTER(ctypes.c_int64)],
+    "dsa_shared_prefix_mla_fp8": [_ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr,
+                                  _i64, _f32, _ptr, _ptr, _i64, _ptr],
     "dsa_gather_records": [_ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _int, _i64, _ptr,
                            _ptr],
     "dsa_copy_records_h2d": [_ptr, _ptr, _i64, _ptr],

@@ -318,3 +318,78 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
             _native.raw_stream(q.device),
         )
     return out
+
+
+def shared_prefix_mla(q, kv_cache, prefix_table, prefix_tokens, suffix_tables, suffix_tokens,
+                      scale, *, cu_q=None, value_dim=512, out=None):
+    """MLA attention of branches (a request's candidates) that share a prefix.
+
+    ``q`` bf16 ``[T, H, 576]``; records as in ``sparse_mla_fp8_paged``, in
+    ``kv_cache`` uint8 ``[pages, 64, 656]``: the shared prefix's
+    ``prefix_tokens`` (an int) on the pages of ``prefix_table`` (int32
+    ``[>= ceil(prefix_tokens / 64)]``), branch ``b``'s own ``suffix_tokens[b]``
+    (int32 ``[B]`` on the device; what the table does not cover is cut off) on
+    the pages of ``suffix_tables[b]`` (int32 ``[B, pages]``, from a fresh page
+    on). Branch ``b`` has queries ``cu_q[b]:cu_q[b + 1]`` (int32 ``[B + 1]``,
+    ascending; default: one query per branch), the last tokens of its suffix:
+    query ``i`` of ``n`` sees the prefix and the first
+    ``suffix_tokens[b] - n + 1 + i`` tokens of the suffix. The prefix is read
+    once for all branches; any H.
+
+    Returns bf16 ``[T, H, 512]``, or writes it to ``out`` (contiguous), where
+    queries of no branch are left as they were. A query that sees no key gives
+    zeros; tokens on a page outside the cache are padding.
+    """
+    if q.ndim != 3 or q.shape[2] != QK_DIM or value_dim != V_DIM or not q.shape[1]:
+        raise ValueError("Expected q [T,H,576] with H >= 1 and value_dim 512")
+    if q.dtype != torch.bfloat16:
+        raise ValueError("shared prefix MLA requires BF16 queries")
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be positive and finite")
+    _check_paged(kv_cache, prefix_table, q.device)
+    if (type(prefix_tokens) is not int
+            or not 0 <= prefix_tokens <= prefix_table.numel() * PAGE_TOKENS):
+        raise ValueError("prefix_tokens must be covered by the prefix table")
+    if (not isinstance(suffix_tables, torch.Tensor) or suffix_tables.dtype != torch.int32
+            or suffix_tables.ndim != 2 or suffix_tables.device != q.device):
+        raise ValueError("suffix_tables must be int32 [branches, pages] on the query device")
+    branches = suffix_tables.shape[0]
+    if (not isinstance(suffix_tokens, torch.Tensor) or suffix_tokens.dtype != torch.int32
+            or tuple(suffix_tokens.shape) != (branches,) or suffix_tokens.device != q.device):
+        raise ValueError("suffix_tokens must be int32 [branches] on the query device")
+    if cu_q is not None:
+        cu_q = _check_starts(cu_q, q.device, "cu_q")
+        if cu_q.numel() != branches + 1:
+            raise ValueError("cu_q must be int32 [branches + 1]")
+    elif branches != q.shape[0]:
+        raise ValueError("without cu_q every branch has one query")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise ValueError("shared prefix MLA has no backward pass")
+    _native.require_gfx950(q.device, "shared prefix MLA")
+    shape = (*q.shape[:2], value_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != q.dtype
+          or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned [T, H, 512] tensor of q's "
+                         "dtype on q's device")
+    if not q.shape[0] or not branches:
+        return out
+    if not kv_cache.shape[0]:
+        raise ValueError("kv_cache must hold a page")
+    q, cache = _aligned(q), _aligned(kv_cache)
+    prefix_table, suffix_tables = prefix_table.contiguous(), suffix_tables.contiguous()
+    suffix_tokens = suffix_tokens.contiguous()
+    with _native.on_device(q.device):
+        needed = _native.size_of("dsa_shared_prefix_mla_workspace_bytes", q.device.index,
+                                 q.shape[0], q.shape[1], prefix_tokens, suffix_tables.shape[1])
+        workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
+        _native.call(
+            "dsa_shared_prefix_mla_fp8",
+            q.data_ptr(), q.shape[0], q.shape[1], cache.data_ptr(), cache.shape[0],
+            prefix_table.data_ptr(), prefix_tokens, suffix_tables.data_ptr(),
+            suffix_tables.shape[1], suffix_tokens.data_ptr(), _native.ptr(cu_q), branches,
+            float(scale), out.data_ptr(), _native.ptr(workspace), needed,
+            _native.raw_stream(q.device),
+        )
+    return out

@@ -150,7 +150,6 @@ __device__ __forceinline__ uint32_t opaque_address(uint32_t v) {
 // A row's keys may be split over work-groups: split s leaves its unscaled sum of
 // p v (fp32 [splits][rows][dim]) and (maximum, sum of p) pairs ([splits][rows];
 // split_stats). Their join is sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-// kDim / 8 lanes take a row, 8 dims each; what bounds it is reading the parts.
 
 // What a split leaves for a row: (-inf, 0) where nothing was visible (its values
 // are then neither written nor read), a NaN maximum where a score was NaN.
@@ -159,29 +158,28 @@ __device__ __forceinline__ float2 split_stats(float top, float sum) {
   return make_float2(sum == sum ? top : sum, sum);
 }
 
+// Joins them: four groups of kDim / 8 lanes take a row, a quarter of its splits
+// each, 8 dims a lane. What bounds it is reading the parts.
 template <typename E, int kDim>
 __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ parts, const float2* __restrict__ stats,
                                                    int64_t rows, int splits, const int32_t* __restrict__ cu,
                                                    int32_t sequences, int64_t heads, uint16_t* __restrict__ out) {
-  constexpr int kLanes = kDim / 8;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
+  constexpr int kLanes = kDim / 8, kWays = 4, kRows = 256 / (kLanes * kWays);
+  __shared__ float shared[kWays][kRows][kDim + 4];
+  const int local = threadIdx.x / (kLanes * kWays);
+  const int way = threadIdx.x / kLanes % kWays;
   const int d = (threadIdx.x % kLanes) * 8;
-  if (row >= rows) return;
+  const int64_t row = (int64_t)blockIdx.x * kRows + local;
   // Rows outside the sequences have no parts, and stay as they are.
-  if (cu != nullptr && (row < cu[0] * heads || row >= cu[sequences] * heads)) return;
-  float top = -__builtin_inff();
-  bool any = false;  // (a NaN maximum, of a split with NaN scores, counts and spreads)
-  for (int s = 0; s < splits; ++s) {
-    const float m = stats[s * rows + row].x;
-    any |= m != -__builtin_inff();
-    top = fmaxf(top, m);
-  }
+  const bool live = row < rows && (cu == nullptr || (row >= cu[0] * heads && row < cu[sequences] * heads));
   float acc[8] = {}, sum = 0.0f;
-  if (any) {
+  if (live) {
+    float top = -__builtin_inff();
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, stats[s * rows + row].x);
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+    for (int s = way; s < splits; s += kWays) {
       const float2 st = stats[s * rows + row];
-      if (st.x == -__builtin_inff()) continue;
+      if (st.x == -__builtin_inff()) continue;  // (a NaN maximum, of a split with NaN scores, spreads)
       const float w = __builtin_amdgcn_exp2f(st.x - top);
       sum += w * st.y;
       const float4* o = reinterpret_cast<const float4*>(parts + (s * rows + row) * kDim + d);
@@ -189,12 +187,33 @@ __global__ __launch_bounds__(256) void join_splits(const float* __restrict__ par
       acc[0] += w * a.x, acc[1] += w * a.y, acc[2] += w * a.z, acc[3] += w * a.w;
       acc[4] += w * b.x, acc[5] += w * b.y, acc[6] += w * b.z, acc[7] += w * b.w;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) shared[way][local][d + i] = acc[i];
+    if (d == 0) shared[way][local][kDim] = sum;
+  }
+  __syncthreads();
+  if (!live || way != 0) return;
+#pragma unroll
+  for (int w = 1; w < kWays; ++w) {
+    sum = w == 1 ? shared[0][local][kDim] + shared[w][local][kDim] : sum + shared[w][local][kDim];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += shared[w][local][d + i];
   }
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   v4u packed;
 #pragma unroll
   for (int i = 0; i < 4; ++i) packed[i] = E::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
   *reinterpret_cast<v4u*>(out + row * kDim + d) = packed;
+}
+
+template <typename E, int kDim>
+int launch_join(const float* parts, const float2* stats, int64_t rows, int splits, const int32_t* cu,
+                int32_t sequences, int64_t heads, uint16_t* out, hipStream_t stream) {
+  constexpr int kRows = 256 / (kDim / 8 * 4);
+  hipLaunchKernelGGL((join_splits<E, kDim>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, stream, parts,
+                     stats, rows, splits, cu, sequences, heads, out);
+  DSA_CHECK_LAUNCH("join of split keys");
+  return kOk;
 }
 
 }  // namespace

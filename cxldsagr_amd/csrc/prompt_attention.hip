@@ -417,12 +417,9 @@ int launch_prompt(const PromptArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((prompt_fwd<E, kQk, kV>), dim3((unsigned)((int64_t)a.slots * a.kv_heads * a.splits)), dim3(kThreads),
                      0, stream, a);
   DSA_CHECK_LAUNCH("prompt attention");
-  if (a.splits > 1) {
-    const int64_t rows = a.q_tokens * a.heads;
-    hipLaunchKernelGGL((join_splits<E, kV>), dim3((unsigned)((rows * (kV / 8) + 255) / 256)), dim3(256), 0, stream,
-                       a.parts, a.stats, rows, a.splits, a.cu_q, a.sequences, (int64_t)a.heads, a.out);
-    DSA_CHECK_LAUNCH("prompt attention join");
-  }
+  if (a.splits > 1)
+    return launch_join<E, kV>(a.parts, a.stats, a.q_tokens * a.heads, a.splits, a.cu_q, a.sequences, a.heads, a.out,
+                              stream);
   return kOk;
 }
 

@@ -1,0 +1,497 @@
+// MLA attention of branches that share a long prefix, over the fp8 paged cache
+// (656-byte records: 512 e4m3 latent values in 4 tiles, 4 fp32 tile scales, 64
+// bf16 RoPE values; 64 tokens a page).
+//
+// Every query (token t of branch b, head h) attends to the whole prefix and to
+// what it sees of its branch's suffix: out = sum_j p_j rec_j[:512] / sum_j p_j
+// with p = exp(scale q . rec_j), in fp32 from bf16 operands (e4m3 times a power
+// of two is exact in bf16; p is rounded to bf16 before the product with V).
+// 2 (576 + 512) flop per (row, key).
+//
+// All heads read the one record of a key and the prefix is unmasked, so over the
+// prefix the rows of all tokens and heads are one matrix. A work item has 128 of
+// its rows, whatever branches they belong to, and a range of the keys, each record
+// of which is read, converted and staged once for all 128; four waves (one per
+// SIMD) take 32 rows each. With a multiple of 128 heads an item's rows are of one
+// token, and its keys are the prefix and then the token's suffix; with other
+// counts the suffix has items of its own, up to 128 heads of one token. Where a
+// row's keys are in several items, a second launch joins their sums.
+//
+// A wave computes S^T = K Q^T (v_mfma_f32_32x32x16_bf16) for 32 keys and its 32
+// rows, and O^T += V^T P^T with the probabilities where the scores were (the keys
+// of V^T are read in the order in which a lane holds its scores). O^T takes 256 of
+// a lane's 512 registers and Q^T 112 (the last 8 of its 36 operands are read from
+// LDS). Per 32 keys a SIMD has 68 products of 32 cycles, 2.2k cycles, while the CU
+// reads 304 KB of LDS and writes 37 KB, about 3.4k cycles at the ~115 and ~49 bytes
+// a cycle that one wave per SIMD reaches: LDS is the bound, and a row tile of 32
+// per wave (each operand read feeds one product) is what registers allow.
+#include "attention_core.h"
+#include "../../include/dsa_gfx950.h"
+
+namespace dsa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kQkDim = 576, kVDim = 512;
+constexpr int kWaveRows = 32;
+constexpr int kTileRows = 4 * kWaveRows;
+constexpr int kBlockKeys = 32;
+constexpr int kPageTokens = 64;
+constexpr int kRecordBytes = 656;
+
+// bf16 rows of one block in LDS: 1168 bytes = 36 dwords (mod 64) apart, so that
+// 16 rows' chunks of 16 bytes, and rows r, r + 4, r + 8, r + 12 of 64 bytes, lie
+// on distinct banks.
+constexpr int kRowBytes = kQkDim * 2 + 16;
+constexpr int kBufBytes = kBlockKeys * kRowBytes;
+constexpr int kBuffers = 3;
+constexpr int kSteps = kQkDim / 16, kDims = kVDim / 32;
+// Q^T operands of the last kQLds steps stay in LDS, the others in registers:
+// with all 36 there, O^T (256 registers of a lane) leaves too few for the rest.
+constexpr int kQLds = 8;
+constexpr int kQReg = kSteps - kQLds;
+constexpr int kQBytes = kQLds * 4 * 1024;  // [wave][step][lane] 16 bytes
+
+// Source of keys past the end and pages outside the cache: zeros, so that what a
+// masked key's p = 0 multiplies is finite.
+__device__ __align__(16) uint8_t zero_record[kRecordBytes + 16];
+
+struct PrefixArgs {
+  const uint16_t* q;
+  const uint8_t* cache;
+  const int32_t* prefix_table;
+  const int32_t* suffix_tables;  // [branches][suffix_pages]
+  const int32_t* suffix_tokens;  // [branches]
+  const int32_t* cu_q;           // [branches + 1], or null: one query per branch
+  uint16_t* out;
+  float* parts;   // [splits][tokens * heads][512], with more than one split
+  float2* stats;  // [splits][tokens * heads]
+  int64_t tokens, pages, prefix;
+  int32_t heads, branches, suffix_pages;
+  int32_t joint;  // items have the prefix and the suffix
+  int32_t items, splits;                  // of the row tiles of all tokens
+  int32_t suffix_splits;                  // of the suffix's own items
+  float scale_log2;
+};
+
+// Key order of a score tile: row m = 16 t + 8 u + 4 h + jj holds key 16 t + 4 jj
+// + 2 u + h, so that the four keys of a transposing V read are 4 rows apart.
+__device__ __forceinline__ int tile_key(int m) {
+  return (m & 16) + 4 * (m & 3) + 2 * ((m >> 3) & 1) + ((m >> 2) & 1);
+}
+
+template <bool kHigh>
+__device__ __forceinline__ uint32_t dequant_pair(uint32_t word, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, kHigh));
+}
+
+__global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArgs a) {
+  using E = Bf16;
+  __shared__ __align__(1024) uint8_t lds[kBuffers * kBufBytes + kQBytes];
+  const uint32_t lds_base = (uint32_t)(uintptr_t)&lds[0];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int64_t all_rows = a.tokens * a.heads;
+
+  // ---- the item: its rows, how many keys of the prefix and of a suffix they
+  // see, and its range of their blocks. Items of one range are neighbours, and
+  // each XCD takes an eighth of the items in that order: they read the same
+  // records from its L2.
+  int64_t row0, row_end, prefix = 0, suffix = 0;
+  const int32_t* suffix_table = nullptr;
+  int split, splits, part;
+  int64_t token = -1;  // whose suffix the item has
+  if (blockIdx.x < (uint32_t)a.items) {
+    const int64_t tiles = (all_rows + kTileRows - 1) / kTileRows;
+    const int64_t item = (int64_t)(blockIdx.x & 7) * (a.items >> 3) + (blockIdx.x >> 3);
+    if (item >= tiles * a.splits) return;
+    split = part = (int)(item / tiles);
+    splits = a.splits;
+    row0 = (item % tiles) * kTileRows;
+    row_end = min(row0 + kTileRows, all_rows);
+    prefix = a.prefix;
+    if (a.joint) token = row0 / a.heads;
+  } else {
+    const int64_t item = blockIdx.x - (uint32_t)a.items;
+    const int groups = (a.heads + kTileRows - 1) / kTileRows;
+    splits = a.suffix_splits;
+    split = (int)(item % splits);
+    part = a.splits + split;
+    token = item / splits / groups;
+    const int head0 = (int)(item / splits % groups) * kTileRows;
+    row0 = token * a.heads + head0;
+    row_end = token * a.heads + min(head0 + kTileRows, (int)a.heads);
+  }
+  int64_t row_begin = row0;
+  if (a.cu_q != nullptr) {
+    // Rows of no branch are left alone.
+    row_begin = max(row0, a.cu_q[0] * (int64_t)a.heads);
+    row_end = min(row_end, a.cu_q[a.branches] * (int64_t)a.heads);
+    if (row_begin >= row_end) return;
+  }
+  if (token >= 0) {
+    int branch = (int)token;
+    int64_t left = 0;  // queries of the branch after this one
+    if (a.cu_q != nullptr) {
+      int lo = 0, hi = a.branches;  // the last branch that starts at or before it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu_q[mid] <= token) lo = mid; else hi = mid;
+      }
+      branch = lo;
+      left = max((int64_t)a.cu_q[lo + 1] - 1 - token, (int64_t)0);
+    }
+    const int64_t held = min((int64_t)a.suffix_tokens[branch], (int64_t)a.suffix_pages * kPageTokens);
+    suffix = max(held - left, (int64_t)0);
+    suffix_table = a.suffix_tables + (int64_t)branch * a.suffix_pages;
+  }
+  const int prefix_blocks = (int)((prefix + kBlockKeys - 1) / kBlockKeys);
+  const int all_blocks = prefix_blocks + (int)((suffix + kBlockKeys - 1) / kBlockKeys);
+  const int per_split = (all_blocks + splits - 1) / splits;
+  const int b0 = split * per_split;
+  const int b1 = min(b0 + per_split, all_blocks);
+
+  const int64_t wave_row = row0 + wave * kWaveRows;
+  const bool live = wave_row + n < row_end && wave_row + n >= row_begin;  // this lane's row, in both halves
+  const int64_t row_at = min(wave_row + n, row_end - 1);
+  const bool active = __builtin_amdgcn_readfirstlane(wave_row < row_end && b1 > b0);
+
+  v4u q_ops[kQReg];
+  const uint32_t q_lds = lds_base + kBuffers * kBufBytes + (uint32_t)wave * (kQLds * 1024) + 16 * lane;
+  {
+    const uint16_t* src = a.q + row_at * kQkDim + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
+#pragma unroll
+    for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
+#pragma unroll
+    for (int ks = 0; ks < kQLds; ++ks)
+      lds_store<v4u>(q_lds + 1024 * ks, *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks)));
+  }
+
+  // ---- staging: eight lanes a key. Lane j brings bytes 128 i + 16 j of the
+  // latent (a chunk of every tile), the scales, and bytes 16 j of the RoPE part.
+  const int kk = threadIdx.x >> 3, j8 = threadIdx.x & 7;
+  auto page_of = [&](int b) -> int {
+    if (b >= b1) return -1;
+    return b < prefix_blocks ? a.prefix_table[b >> 1] : suffix_table[(b - prefix_blocks) >> 1];
+  };
+  // Valid keys of block b on `page`, and its first record there.
+  auto keys_of = [&](int b, int page) -> int {
+    if (page < 0 || page >= a.pages) return 0;
+    const int64_t left = b < prefix_blocks ? prefix - (int64_t)b * kBlockKeys
+                                           : suffix - (int64_t)(b - prefix_blocks) * kBlockKeys;
+    return (int)min(left, (int64_t)kBlockKeys);
+  };
+  auto half_of = [&](int b) -> int { return (b < prefix_blocks ? b : b - prefix_blocks) & 1; };
+  v4u st[6];
+  auto fetch = [&](int b, int page) __attribute__((always_inline)) {
+    const uint8_t* rec =
+        kk < keys_of(b, page) ? a.cache + ((int64_t)page * kPageTokens + half_of(b) * kBlockKeys + kk) * kRecordBytes
+                              : zero_record;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(rec + 128 * i + 16 * j8);
+    st[4] = *reinterpret_cast<const v4u*>(rec + kVDim);
+    st[5] = *reinterpret_cast<const v4u*>(rec + kVDim + 16 + 16 * j8);
+  };
+  // Chunk i of the landed record (4: the RoPE part) as bf16 into the block's row.
+  auto unpack = [&](uint32_t to, int i) __attribute__((always_inline)) {
+    if (i == 4) {
+      lds_store<v4u>(to + 2 * kVDim - 16 * j8, st[5]);
+      return;
+    }
+    const float scale = __builtin_bit_cast(v4f, st[4])[i];
+    const v4u w = st[i];
+    lds_store<v4u>(to + 256 * i, v4u{dequant_pair<false>(w.x, scale), dequant_pair<true>(w.x, scale),
+                                     dequant_pair<false>(w.y, scale), dequant_pair<true>(w.y, scale)});
+    lds_store<v4u>(to + 256 * i + 16, v4u{dequant_pair<false>(w.z, scale), dequant_pair<true>(w.z, scale),
+                                          dequant_pair<false>(w.w, scale), dequant_pair<true>(w.w, scale)});
+  };
+  const uint32_t store_lane = (uint32_t)kk * kRowBytes + 32 * j8;
+  auto buf_of = [&](int b) -> uint32_t { return lds_base + (uint32_t)(b % kBuffers) * kBufBytes; };
+
+  v16f o[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = v16f{};
+  RowState row{-__builtin_inff(), 0.0f};
+
+  // LDS lane addresses. K: key tile_key(n), dims 16 ks + 8 h. V: lane 4 jj + qq
+  // of 16-lane group g reads key 16 t + 4 jj + 2 u + h, dims 32 d + 16 (g & 1) + 4 qq.
+  const uint32_t k_lane = (uint32_t)tile_key(n) * kRowBytes + 16 * h;
+  const uint32_t v_lane = (uint32_t)(4 * ((lane & 15) >> 2) + h) * kRowBytes + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  constexpr int kAhead = 3, kVops = 2 * kDims;
+
+  auto read_v = [&](uint32_t at, int i) __attribute__((always_inline)) -> v4u {
+    const int t = i & 1, d = i >> 1;
+    const v2u lo = lds_column(at + (16 * t) * kRowBytes + 64 * d);
+    const v2u hi = lds_column(at + (16 * t + 2) * kRowBytes + 64 * d);
+    return v4u{lo.x, lo.y, hi.x, hi.y};
+  };
+  auto scores = [&](int b, v16f& s, auto slice) __attribute__((always_inline)) {
+    const uint32_t at = opaque_address(buf_of(b) + k_lane);
+    v4u kop[kAhead], qop[2];
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at + 32 * ks);
+    s = v16f{};
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      s = E::mfma(kop[ks % kAhead], ks < kQReg ? q_ops[ks < kQReg ? ks : 0] : qop[ks & 1], s);
+      if (ks + kAhead < kSteps) kop[ks % kAhead] = lds_load<v4u>(at + 32 * (ks + kAhead));
+      if (ks + 2 >= kQReg && ks + 2 < kSteps) qop[ks & 1] = lds_load<v4u>(q_lds + 1024 * (ks + 2 - kQReg));
+      slice(ks);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto values = [&](uint32_t at, v4u (&vop)[kAhead], const v4u (&p)[2], auto slice) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kVops; ++i) {
+      o[i >> 1] = E::mfma(vop[i % kAhead], p[i & 1], o[i >> 1]);
+      if (i + kAhead < kVops) vop[i % kAhead] = read_v(at, i + kAhead);
+      slice(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto mask = [&](int b, int page, v16f& s) __attribute__((always_inline)) {
+    const int seen = keys_of(b, page);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = tile_key(8 * (i >> 2) + 4 * h + (i & 3)) < seen ? s[i] : -__builtin_inff();
+  };
+  auto needs_mask = [&](int b, int page) -> bool { return keys_of(b, page) < kBlockKeys; };
+
+  // ---- pipeline. Step b: scores of block b + 1 beside the probabilities of
+  // block b, then block b's product with V beside the conversion of block b + 2
+  // into LDS; block b + 3's records are on their way. One barrier per step; three
+  // buffers.
+  int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
+  if (b1 > b0) {
+    fetch(b0, page);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) unpack(buf_of(b0) + store_lane, i);
+    fetch(b0 + 1, page1);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) unpack(buf_of(b0 + 1) + store_lane, i);
+    fetch(b0 + 2, page2);
+  }
+  lds_barrier();
+  if (active) {
+    int b = b0;
+    v16f s, next;
+    v4u p[2];
+    float shift = 0.0f;
+    auto no_slice = [](int) {};
+    auto soften = [&](const v16f& from, int i, int of) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 8 * i / of; u < 8 * (i + 1) / of; ++u)
+        p[u >> 2][u & 3] = probability_pair<E>(from[2 * u], from[2 * u + 1], a.scale_log2, shift, row.sum);
+    };
+    enum { kGo, kBreak, kDone };
+    auto step = [&](const v16f& from, v16f& to) __attribute__((always_inline)) -> int {
+      if (b + 1 == b1) return kDone;
+      ++b;
+      const int page3 = page_of(b + 2);
+      const uint32_t at = opaque_address(buf_of(b - 1) + v_lane);
+      v4u vop[kAhead];
+      scores(b, to, [&](int i) __attribute__((always_inline)) {
+        soften(from, i, kSteps);
+        if (i >= kSteps - kAhead) vop[i - (kSteps - kAhead)] = read_v(at, i - (kSteps - kAhead));
+      });
+      const uint32_t store = opaque_address(buf_of(b + 1) + store_lane);
+      float top = -__builtin_inff();
+      values(at, vop, p, [&](int i) __attribute__((always_inline)) {
+        if (i % 4 == 0 && i < 20) unpack(store, i / 4);
+        if (i == 20) fetch(b + 2, page3);
+        if (i >= 8 && i < 16) top = fmaxf(fmaxf(top, to[2 * (i - 8)]), to[2 * (i - 8) + 1]);
+      });
+      lds_barrier();
+      const float mx = max_halves(top) * a.scale_log2;
+      page = page1;
+      page1 = page2;
+      page2 = page3;
+      return needs_mask(b, page) || __builtin_amdgcn_ballot_w64(must_raise(row, mx)) != 0 ? kBreak : kGo;
+    };
+    scores(b, s, no_slice);
+    for (bool more = true; more;) {
+      if (needs_mask(b, page)) mask(b, page, s);
+      const float factor = raise(row, row_max(s, a.scale_log2));
+      shift = shift_of(row);
+      if (__builtin_amdgcn_ballot_w64(factor != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[d] *= factor;
+      }
+      for (;;) {
+        int end = step(s, next);
+        if (end != kGo) {
+          more = end == kBreak;
+          if (more) s = next;
+          break;
+        }
+        end = step(next, s);
+        if (end != kGo) {
+          more = end == kBreak;
+          if (!more) s = next;
+          break;
+        }
+      }
+    }
+    const uint32_t at = opaque_address(buf_of(b) + v_lane);
+    v4u vop[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);
+    soften(s, 0, 1);
+    values(at, vop, p, no_slice);
+  } else {
+    // A wave without rows stages its keys all the same.
+    for (int b = b0 + 1; b < b1; ++b) {
+      const int page3 = page_of(b + 2);
+      const uint32_t store = buf_of(b + 1) + store_lane;
+#pragma unroll
+      for (int i = 0; i < 5; ++i) unpack(store, i);
+      fetch(b + 2, page3);
+      lds_barrier();
+    }
+  }
+
+  // ---- store (as in prompt attention: the halves trade to store 16 bytes).
+  const float sum = sum_halves(row.sum);
+  if (a.splits + a.suffix_splits > 1) {
+    const int64_t at = (int64_t)part * all_rows + row_at;
+    if (live && h == 0) a.stats[at] = split_stats(row.top, sum);
+    if (live && sum != 0.0f) {
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<v4f*>(a.parts + at * kVDim + 32 * d + 8 * c + 4 * h) =
+              v4f{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+    }
+    return;
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[u][e] = E::pack(o[d][4 * (c + u) + 2 * e] * inv, o[d][4 * (c + u) + 2 * e + 1] * inv);
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      if (live) *reinterpret_cast<v4u*>(a.out + row_at * kVDim + 32 * d + 8 * (c + h)) = v4u{x[0], y[0], x[1], y[1]};
+    }
+}
+
+// Key splits of `tiles` row tiles over `blocks` blocks of 32 keys: the count of
+// least time, by the rounds of work-groups (one per CU), their fixed part and their
+// steps, and what a part costs to write and read again.
+constexpr double kFixedUs = 14.0, kStepUs = 1.7, kPartUsPerRow = 0.001;
+
+int best_splits(int64_t tiles, int64_t blocks, int64_t rows, int64_t cus) {
+  int best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= 256 && s <= (blocks > 1 ? blocks : 1); ++s) {
+    const double rounds = (double)((tiles * s + cus - 1) / cus);
+    const double us = rounds * (kFixedUs + kStepUs * (double)((blocks + s - 1) / s)) +
+                      (s > 1 ? 4.0 + kPartUsPerRow * (double)(rows * s) : 0.0);
+    if (us < least) {
+      least = us;
+      best = (int)s;
+    }
+    if (rounds > 8) break;
+  }
+  return best;
+}
+
+struct PrefixPlan {
+  bool joint;
+  int64_t splits, suffix_splits, stats_at, bytes;
+};
+
+PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t suffix_pages) {
+  PrefixPlan p{};
+  const int64_t cus = device_cu_count();
+  const int64_t rows = tokens * heads;
+  const int64_t prefix_blocks = (prefix + kBlockKeys - 1) / kBlockKeys;
+  const int64_t suffix_blocks = suffix_pages * (kPageTokens / kBlockKeys);
+  p.joint = heads % kTileRows == 0;
+  if (p.joint || prefix > 0)
+    p.splits = best_splits((rows + kTileRows - 1) / kTileRows, prefix_blocks + (p.joint ? suffix_blocks : 0), rows, cus);
+  if (!p.joint && (suffix_pages > 0 || prefix == 0))
+    p.suffix_splits = best_splits(tokens * ((heads + kTileRows - 1) / kTileRows), suffix_blocks, rows, cus);
+  const int64_t parts = p.splits + p.suffix_splits;
+  if (parts > 1) {
+    p.stats_at = parts * rows * kVDim * 4;
+    p.bytes = p.stats_at + parts * rows * 8;
+  }
+  return p;
+}
+
+}  // namespace
+}  // namespace dsa
+
+extern "C" int dsa_shared_prefix_mla_workspace_bytes(int64_t tokens, int64_t heads, int64_t prefix_tokens,
+                                                     int64_t suffix_pages, int64_t* bytes) {
+  using namespace dsa;
+  DSA_CHECK_ARG(bytes != nullptr, "null pointer");
+  DSA_CHECK_ARG(tokens >= 0 && heads > 0 && prefix_tokens >= 0 && suffix_pages >= 0,
+                "invalid shared prefix MLA shape");
+  *bytes = prefix_plan(tokens, heads, prefix_tokens, suffix_pages).bytes;
+  return kOk;
+}
+
+extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t heads, const void* cache,
+                                         int64_t pages, const int32_t* prefix_table, int64_t prefix_tokens,
+                                         const int32_t* suffix_tables, int64_t suffix_pages,
+                                         const int32_t* suffix_tokens, const int32_t* cu_q, int64_t branches,
+                                         float scale, void* out, void* workspace, int64_t workspace_bytes,
+                                         hipStream_t stream) {
+  using namespace dsa;
+  DSA_CHECK_ARG(tokens >= 0 && heads > 0 && heads <= 65536 && branches >= 0 && branches < 0x7FFFFFFF,
+                "invalid shared prefix MLA shape");
+  DSA_CHECK_ARG(prefix_tokens >= 0 && prefix_tokens < 0x7FFFFFFF && suffix_pages >= 0 &&
+                    suffix_pages < 0x7FFFFFFF / kPageTokens,
+                "prefix and suffix lengths must fit int32");
+  DSA_CHECK_ARG(scale > 0.0f && __builtin_isfinite(scale), "scale must be positive and finite");
+  if (tokens == 0) return kOk;
+  DSA_CHECK_ARG(branches > 0 && (cu_q != nullptr || branches == tokens),
+                "without cu_q every branch has one query");
+  DSA_CHECK_ARG(pages >= 1 && pages < 0x7FFFFFFF / kPageTokens, "cache rows must fit int32");
+  DSA_CHECK_ARG(q && cache && out && suffix_tokens && (prefix_tokens == 0 || prefix_table) &&
+                    (suffix_pages == 0 || suffix_tables),
+                "null pointer");
+  DSA_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) %
+                        16 == 0,
+                "q, cache and out must be 16-byte aligned");
+  const PrefixPlan p = prefix_plan(tokens, heads, prefix_tokens, suffix_pages);
+  const int64_t tiles = (tokens * heads + kTileRows - 1) / kTileRows;
+  const int64_t items = p.splits > 0 ? (tiles * p.splits + 7) / 8 * 8 : 0;
+  const int64_t own = tokens * ((heads + kTileRows - 1) / kTileRows) * p.suffix_splits;
+  DSA_CHECK_ARG(items + own < 0x7FFFFFFF && tokens * heads < (1ll << 40), "too many query rows");
+  if (p.bytes > 0)
+    DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
+                  "shared prefix MLA workspace too small or misaligned");
+  PrefixArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.prefix_table = prefix_table;
+  a.suffix_tables = suffix_tables;
+  a.suffix_tokens = suffix_tokens;
+  a.cu_q = cu_q;
+  a.out = static_cast<uint16_t*>(out);
+  a.parts = static_cast<float*>(workspace);
+  a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.stats_at);
+  a.tokens = tokens, a.pages = pages, a.prefix = prefix_tokens;
+  a.heads = (int32_t)heads, a.branches = (int32_t)branches, a.suffix_pages = (int32_t)suffix_pages;
+  a.joint = p.joint, a.items = (int32_t)items, a.splits = (int32_t)p.splits;
+  a.suffix_splits = (int32_t)p.suffix_splits;
+  a.scale_log2 = scale * kLog2E;
+  hipLaunchKernelGGL(shared_prefix_fwd, dim3((unsigned)(items + own)), dim3(kThreads), 0, stream, a);
+  DSA_CHECK_LAUNCH("shared prefix MLA");
+  if (p.bytes > 0)
+    return launch_join<Bf16, kVDim>(a.parts, a.stats, tokens * heads, (int)(p.splits + p.suffix_splits), cu_q,
+                                    (int32_t)branches, heads, a.out, stream);
+  return kOk;
+}

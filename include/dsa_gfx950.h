@@ -482,6 +482,31 @@ int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          hipStream_t stream);
 
 /*
+ * MLA attention of branches that share a prefix, over the fp8 paged cache. No
+ * reference counterpart.
+ * q: bf16 [tokens, heads, 576] contiguous; cache: uint8 [pages, 64, 656];
+ * prefix_table: int32 [ceil(prefix_tokens / 64)], the pages of the shared prefix;
+ * suffix_tables: int32 [branches, suffix_pages], the pages of each branch's own
+ * tokens; suffix_tokens: int32 [branches], how many those are (at most 64 *
+ * suffix_pages count). Branch b has queries cu_q[b] .. cu_q[b + 1] - 1 (int32
+ * [branches + 1], ascending), the last tokens of its suffix: of n queries query i
+ * sees the prefix and the first suffix_tokens[b] - n + 1 + i of the suffix. cu_q
+ * null: one query per branch, tokens == branches. out: bf16 [tokens, heads, 512]
+ * contiguous = softmax(scale q . record) record[:512], zeros for a query that sees
+ * no key; queries of no branch are not written. q, cache and out 16-byte
+ * aligned; scale > 0. Tokens on a page outside the cache count as padding.
+ * `workspace`: as dsa_prompt_attention's, dsa_shared_prefix_mla_workspace_bytes.
+ */
+int dsa_shared_prefix_mla_workspace_bytes(int64_t tokens, int64_t heads, int64_t prefix_tokens,
+                                          int64_t suffix_pages, int64_t* bytes);
+int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t heads, const void* cache,
+                              int64_t pages, const int32_t* prefix_table, int64_t prefix_tokens,
+                              const int32_t* suffix_tables, int64_t suffix_pages,
+                              const int32_t* suffix_tokens, const int32_t* cu_q, int64_t branches,
+                              float scale, void* out, void* workspace, int64_t workspace_bytes,
+                              hipStream_t stream);
+
+/*
  * A11 - gather whole records from pinned host memory into device memory,
  * device[device_ids[r]] = host[host_ids[r]] for r < count, or for
  * r < *valid_count when valid_count (a device int64 or uint32 scalar, kind
