@@ -230,6 +230,118 @@ def pack_kv_fp8(kv, kv_cache, page_table, token_offset=0, status=None):
     return kv_cache
 
 
+def _check_slots(slots, tokens, device):
+    if (not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int32, torch.int64)
+            or tuple(slots.shape) != (tokens,) or slots.device != device):
+        raise ValueError("slots must be int32 or int64 [tokens] on the cache device")
+    return slots.contiguous()
+
+
+def _check_cache(cache, device):
+    if (not isinstance(cache, torch.Tensor) or cache.dtype != torch.uint8 or cache.ndim != 3
+            or cache.shape[1:] != (PAGE_TOKENS, RECORD_BYTES) or cache.device != device):
+        raise ValueError("kv_cache must be uint8 [pages, 64, 656] on the records' device")
+    if not cache.is_contiguous() or cache.data_ptr() % 16:
+        raise ValueError("kv_cache must be contiguous and 16-byte aligned")
+
+
+def _check_status(status, device):
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1
+                               or status.device != device):
+        raise ValueError("status must be int32 on the cache device")
+
+
+def write_kv_fp8(kv, kv_cache, slots, *, norm_weight=None, eps=1e-6, positions=None,
+                 frequencies=None, interleaved=True, magnitude=1.0, status=None):
+    """Write bf16 ``kv [T, 576]`` (512 latent + 64 RoPE values; any row stride)
+    into ``slots`` of the fp8 paged cache, as ``pack_kv_fp8`` writes records.
+
+    ``slots`` int32 / int64 ``[T]``: token ``t``'s place ``page * 64 + offset``,
+    any order, of any sequences, distinct; negative: not written. With
+    ``norm_weight`` (f32 ``[512]``) the latent goes through RMSNorm first, with
+    ``positions`` (int32 / int64 ``[T]``) and ``frequencies`` (f32 ``[32]``, as
+    ``projections.rotary_frequencies``) the RoPE part is rotated
+    (``projections.apply_rope_pair``); both round to bf16 as separate operators
+    would, so the record is that of norm, rotation and ``pack_kv_fp8`` in turn.
+    ``status`` (int32 [1], optional) gets bit 0 set if a slot lies past the cache
+    (that token is not written). Returns ``kv_cache``.
+    """
+    if kv.ndim != 2 or kv.shape[1] != QK_DIM or kv.dtype != torch.bfloat16:
+        raise ValueError("kv must be bf16 [tokens, 576]")
+    _native.require_gfx950(kv.device, "fp8 KV write")
+    tokens = kv.shape[0]
+    _check_cache(kv_cache, kv.device)
+    slots = _check_slots(slots, tokens, kv.device)
+    _check_status(status, kv.device)
+    if not math.isfinite(eps) or eps < 0 or not math.isfinite(magnitude):
+        raise ValueError("eps must be finite and nonnegative, magnitude finite")
+    if norm_weight is not None:
+        if (norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (V_DIM,)
+                or norm_weight.device != kv.device):
+            raise ValueError("norm_weight must be FP32 [512] on the cache device")
+        norm_weight = _aligned(norm_weight)
+    if (positions is None) != (frequencies is None):
+        raise ValueError("a rotation needs positions and frequencies")
+    if positions is not None:
+        if (positions.dtype not in (torch.int32, torch.int64)
+                or tuple(positions.shape) != (tokens,) or positions.device != kv.device):
+            raise ValueError("positions must be int32 or int64 [tokens] on the cache device")
+        if (frequencies.dtype != torch.float32
+                or tuple(frequencies.shape) != ((QK_DIM - V_DIM) // 2,)
+                or frequencies.device != kv.device):
+            raise ValueError("frequencies must be FP32 [32] on the cache device")
+        positions, frequencies = positions.contiguous(), frequencies.contiguous()
+    if tokens == 0:
+        return kv_cache
+    if kv.stride(1) != 1 or kv.stride(0) % 8 or kv.stride(0) < 0 or kv.data_ptr() % 16:
+        kv = kv.clone(memory_format=torch.contiguous_format)
+    with _native.on_device(kv.device):
+        _native.call(
+            "dsa_kv_write_fp8",
+            kv.data_ptr(), kv.stride(0), tokens, slots.data_ptr(), int(slots.dtype == torch.int64),
+            _native.ptr(norm_weight), float(eps),
+            _native.ptr(positions),
+            int(positions is not None and positions.dtype == torch.int64),
+            _native.ptr(frequencies), float(magnitude), int(interleaved),
+            kv_cache.shape[0], kv_cache.data_ptr(), _native.ptr(status),
+            _native.raw_stream(kv.device),
+        )
+    return kv_cache
+
+
+def read_kv_fp8(kv_cache, slots, *, out=None, status=None):
+    """Records of the fp8 paged cache back as bf16 ``[T, 576]`` (what they stand
+    for, exactly), e.g. a history to be projected up to a prompt's keys and values.
+
+    ``slots`` int32 / int64 ``[T]`` as in ``write_kv_fp8``, repeats allowed; a
+    negative slot gives zeros, one past the cache too, and sets bit 0 of
+    ``status`` (int32 [1], optional). ``out``: contiguous bf16 ``[T, 576]`` to
+    write to instead of a new tensor.
+    """
+    if not isinstance(kv_cache, torch.Tensor):
+        raise ValueError("kv_cache must be uint8 [pages, 64, 656] on the records' device")
+    device = kv_cache.device
+    _native.require_gfx950(device, "fp8 KV read")
+    _check_cache(kv_cache, device)
+    tokens = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.ndim == 1 else -1
+    slots = _check_slots(slots, tokens, device)
+    _check_status(status, device)
+    if out is None:
+        out = torch.empty((tokens, QK_DIM), dtype=torch.bfloat16, device=device)
+    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != (tokens, QK_DIM)
+          or out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned bf16 [T, 576] tensor on the "
+                         "cache device")
+    if tokens == 0:
+        return out
+    with _native.on_device(device):
+        _native.call("dsa_kv_read_fp8", kv_cache.data_ptr(), kv_cache.shape[0], slots.data_ptr(),
+                     int(slots.dtype == torch.int64), tokens, out.data_ptr(), _native.ptr(status),
+                     _native.raw_stream(device))
+    return out
+
+
 PROMPT_HEAD_DIMS = ((192, 128), (128, 128), (64, 64))
 
 

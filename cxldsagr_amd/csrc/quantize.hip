@@ -12,6 +12,7 @@
 // dtypes use one wave per row.
 #include "dsa_common.h"
 #include "logits_core.h"
+#include "rotary_core.h"
 #include "../../include/dsa_gfx950.h"
 
 namespace dsa {
@@ -602,6 +603,179 @@ extern "C" int dsa_kv_pack_fp8(const void* kv, int64_t tokens, int64_t token_off
                      static_cast<const uint16_t*>(kv), tokens, token_offset, page_table, pages,
                      static_cast<uint8_t*>(cache), status);
   DSA_CHECK_LAUNCH("fp8 KV pack");
+  return kOk;
+}
+
+namespace dsa {
+namespace {
+
+struct WriteArgs {
+  const uint16_t* kv;
+  int64_t kv_stride, tokens, rows;  // rows: 64 per page
+  const void* slots;
+  const float* norm_weight;  // null: no norm
+  float eps;
+  const void* positions;     // null: no rotation
+  const float* frequencies;
+  float magnitude;
+  int32_t wide_slots, wide_positions, interleaved;
+  uint8_t* cache;
+  int32_t* status;
+};
+
+// New tokens into any slots of the fp8 paged cache: the latent through RMSNorm
+// (fp32, x * rsqrt(mean x^2 + eps) * w, rounded to bf16, which is what a model's
+// norm hands on), the RoPE part rotated (fp32, rounded to bf16), then the record of
+// pack_tokens. One wave per token, lane l with 8 latent values; lanes 0 .. 31 have
+// a rotary pair each. Bound by memory: 1,152 B read and 656 B written per token.
+__global__ __launch_bounds__(256) void write_kv(const WriteArgs a) {
+  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (token >= a.tokens) return;
+  const int64_t slot = a.wide_slots ? static_cast<const int64_t*>(a.slots)[token]
+                                    : static_cast<const int32_t*>(a.slots)[token];
+  if (slot < 0) return;  // padding
+  if (slot >= a.rows) {
+    if (lane == 0 && a.status) atomicOr(a.status, 1);
+    return;
+  }
+  uint8_t* rec = a.cache + slot * 656;
+  const uint16_t* src = a.kv + token * a.kv_stride;
+  const uint4 raw = *reinterpret_cast<const uint4*>(src + lane * 8);
+  const int pair = lane & 31;
+  uint32_t ra, rb;  // the pair's bf16 bits
+  if (a.interleaved) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(src + 512 + 2 * pair);
+    ra = word & 0xFFFFu;
+    rb = word >> 16;
+  } else {
+    ra = src[512 + pair];
+    rb = src[544 + pair];
+  }
+  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_to_f32(words[i] & 0xFFFFu);
+    v[2 * i + 1] = bf16_to_f32(words[i] >> 16);
+  }
+  if (a.norm_weight != nullptr) {
+    const float4 w0 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane);
+    const float4 w1 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane + 4);
+    const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset, 64);
+    const float norm = 1.0f / __builtin_sqrtf(sum * (1.0f / 512.0f) + a.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(f32_to_bf16(v[i] * norm * w[i]));
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+    m = m > bits ? m : bits;
+  }
+  m = max_abs_bits_reduce<16>(m);
+  const float scale = scale_from_amax_bits(m, true);
+  uint32_t lo, hi;
+  quantize_eight(v, scale, true, lo, hi);
+  *reinterpret_cast<uint2*>(rec + lane * 8) = make_uint2(lo, hi);
+  if ((lane & 15) == 0) *reinterpret_cast<float*>(rec + 512 + 4 * (lane >> 4)) = scale;
+  if (lane < 32) {
+    if (a.positions != nullptr) {
+      const float2 cs = rotary_core::turn(rotary_core::position_at(a.positions, a.wide_positions, token),
+                                          a.frequencies[pair], a.magnitude);
+      const float x = bf16_to_f32(ra), y = bf16_to_f32(rb);
+      ra = f32_to_bf16(x * cs.x - y * cs.y);
+      rb = f32_to_bf16(y * cs.x + x * cs.y);
+    }
+    uint16_t* rope = reinterpret_cast<uint16_t*>(rec + 528);
+    if (a.interleaved) {
+      *reinterpret_cast<uint32_t*>(rope + 2 * pair) = ra | (rb << 16);
+    } else {
+      rope[pair] = (uint16_t)ra;
+      rope[32 + pair] = (uint16_t)rb;
+    }
+  }
+}
+
+// Records back as bf16 rows of 576 (e4m3 times a power of two is exact in bf16):
+// 32 lanes per token, 16 codes each, the first 8 of them also 16 bytes of the RoPE
+// part. A slot below 0 gives zeros, one past the cache too, with the status bit.
+// Bound by memory: 656 B read and 1,152 B written per token.
+__global__ __launch_bounds__(256) void read_kv(const uint8_t* __restrict__ cache, int64_t rows,
+                                               const void* __restrict__ slots, int wide_slots, int64_t tokens,
+                                               uint16_t* __restrict__ out, int32_t* __restrict__ status) {
+  const int64_t token = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (token >= tokens) return;
+  const int64_t slot = wide_slots ? static_cast<const int64_t*>(slots)[token]
+                                  : static_cast<const int32_t*>(slots)[token];
+  uint16_t* to = out + token * 576;
+  uint4 codes = make_uint4(0, 0, 0, 0), rope = make_uint4(0, 0, 0, 0);
+  float scale = 0.0f;
+  if (slot >= 0 && slot < rows) {
+    const uint8_t* rec = cache + slot * 656;
+    codes = *reinterpret_cast<const uint4*>(rec + 16 * lane);
+    scale = *reinterpret_cast<const float*>(rec + 512 + 4 * (lane >> 3));
+    if (lane < 8) rope = *reinterpret_cast<const uint4*>(rec + 528 + 16 * lane);
+  } else if (slot >= rows && lane == 0 && status) {
+    atomicOr(status, 1);
+  }
+  const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+  uint32_t pairs[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    pairs[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(words[i], scale, false));
+    pairs[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(words[i], scale, true));
+  }
+  *reinterpret_cast<uint4*>(to + 16 * lane) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+  *reinterpret_cast<uint4*>(to + 16 * lane + 8) = make_uint4(pairs[4], pairs[5], pairs[6], pairs[7]);
+  if (lane < 8) *reinterpret_cast<uint4*>(to + 512 + 8 * lane) = rope;
+}
+
+}  // namespace
+}  // namespace dsa
+
+extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t tokens, const void* slots,
+                                int wide_slots, const float* norm_weight, float norm_eps, const void* positions,
+                                int wide_positions, const float* frequencies, float magnitude, int interleaved,
+                                int64_t pages, void* cache, int32_t* status, hipStream_t stream) {
+  using namespace dsa;
+  DSA_CHECK_ARG(tokens >= 0 && pages >= 0 && kv_stride >= 0 && kv_stride % 8 == 0,
+                "invalid KV write shape (the row stride must be a multiple of 8 elements)");
+  DSA_CHECK_ARG(__builtin_isfinite(norm_eps) && norm_eps >= 0.0f && __builtin_isfinite(magnitude),
+                "eps must be finite and nonnegative, magnitude finite");
+  if (tokens == 0) return kOk;
+  DSA_CHECK_ARG(kv && slots && (cache || pages == 0) && (positions == nullptr || frequencies), "null pointer");
+  DSA_CHECK_ARG(reinterpret_cast<uintptr_t>(kv) % 16 == 0 && reinterpret_cast<uintptr_t>(cache) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(norm_weight) % 16 == 0,
+                "kv, cache and norm_weight must be 16-byte aligned");
+  DSA_CHECK_ARG((tokens + 3) / 4 < 0x7FFFFFFF, "too many tokens for one launch");
+  const WriteArgs a{static_cast<const uint16_t*>(kv), kv_stride, tokens, pages * 64, slots, norm_weight, norm_eps,
+                    positions, frequencies, magnitude, wide_slots != 0, wide_positions != 0, interleaved != 0,
+                    static_cast<uint8_t*>(cache), status};
+  hipLaunchKernelGGL(write_kv, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, stream, a);
+  DSA_CHECK_LAUNCH("fp8 KV write");
+  return kOk;
+}
+
+extern "C" int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slots, int wide_slots, int64_t tokens,
+                               void* out, int32_t* status, hipStream_t stream) {
+  using namespace dsa;
+  DSA_CHECK_ARG(tokens >= 0 && pages >= 0, "invalid KV read shape");
+  if (tokens == 0) return kOk;
+  DSA_CHECK_ARG(slots && out && (cache || pages == 0), "null pointer");
+  DSA_CHECK_ARG(reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(cache) % 16 == 0,
+                "cache and out must be 16-byte aligned");
+  DSA_CHECK_ARG((tokens + 7) / 8 < 0x7FFFFFFF, "too many tokens for one launch");
+  hipLaunchKernelGGL(read_kv, dim3((unsigned)((tokens + 7) / 8)), dim3(256), 0, stream,
+                     static_cast<const uint8_t*>(cache), pages * 64, slots, wide_slots != 0, tokens,
+                     static_cast<uint16_t*>(out), status);
+  DSA_CHECK_LAUNCH("fp8 KV read");
   return kOk;
 }
 

@@ -77,6 +77,84 @@ def rotary_table(positions, frequencies):
     return torch.cat((angles.cos(), angles.sin()), dim=-1).contiguous()
 
 
+def _check_heads(x, tokens, device, dtype, dim, name):
+    if (not isinstance(x, torch.Tensor) or x.ndim != 3 or x.shape[0] != tokens
+            or x.shape[2] != dim or x.dtype != dtype or x.device != device):
+        raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device}")
+
+
+def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False, magnitude=1.0,
+                    inverse=False, q_out=None, k_out=None):
+    """Rotary positions of queries and keys, in one launch.
+
+    The rotation of ``apply_rope_pair`` (``models/deepseek_v32/rotary.py:47-85``)
+    for any part of a head, with the angles formed in the kernel. ``q``
+    ``[T, H, D]`` and ``k`` ``[T, H_k, D]`` (or None) in bf16, fp16 or fp32, the
+    last dim contiguous, any other strides. ``positions`` int32 / int64 ``[T]``,
+    ``frequencies`` f32 ``[R / 2]`` (``rotary_frequencies``, or any other scaling
+    for long contexts): dims ``offset .. offset + R - 1`` of each head turn by
+    ``positions[t] * frequencies[i]``, pair ``i`` being dims ``(2 i, 2 i + 1)`` with
+    ``interleaved``, else ``(i, i + R / 2)``; cos and sin are multiplied by
+    ``magnitude`` (the attention factor of a stretched context). Angles are in 64
+    bits, values in 32, rounded once. ``inverse`` turns back (with
+    ``magnitude`` as given): the gradient's rotation.
+
+    Returns ``(q_out, k_out)``, new contiguous tensors unless given; the dims that
+    are not rotated are copied. ``q_out`` may be ``q`` itself (in place; then
+    ``k_out`` is ``k`` or new), else it must not overlap the inputs. ``R`` and
+    ``D - R`` are even.
+    """
+    if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in _native.DTYPE_CODES:
+        raise ValueError("q must be bf16, fp16 or fp32 [tokens, heads, dim]")
+    tokens, device, dtype, dim = q.shape[0], q.device, q.dtype, q.shape[2]
+    if k is not None:
+        _check_heads(k, tokens, device, dtype, dim, "k")
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    if (not isinstance(positions, torch.Tensor) or tuple(positions.shape) != (tokens,)
+            or positions.dtype not in (torch.int32, torch.int64) or positions.device != device):
+        raise ValueError("positions must be int32 or int64 [tokens] on the query device")
+    if (not isinstance(frequencies, torch.Tensor) or frequencies.ndim != 1
+            or frequencies.dtype != torch.float32 or frequencies.device != device):
+        raise ValueError("frequencies must be FP32 [rotated // 2] on the query device")
+    rotated = 2 * frequencies.numel()
+    if (type(offset) is not int or offset < 0 or not 2 <= rotated <= dim - offset
+            or (dim - rotated) % 2):
+        raise ValueError("the rotated part must lie within the head, with an even rest")
+    if not math.isfinite(magnitude):
+        raise ValueError("magnitude must be finite")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        raise ValueError("rotate gradients by a call with inverse=True")
+    _native.require_gfx950(device, "rotary positions")
+    outs = []
+    for x, out, name in ((q, q_out, "q_out"), (k, k_out, "k_out")):
+        if out is None and x is not None:
+            out = torch.empty(x.shape, dtype=dtype, device=device)
+        elif out is not None:
+            _check_heads(out, tokens, device, dtype, dim, name)
+            if out.shape != x.shape or (out.stride(2) != 1 and dim > 1):
+                raise ValueError(f"{name} must have its input's shape and a contiguous last dim")
+        outs.append(out)
+    if tokens == 0:
+        return tuple(outs)
+    sides = []
+    for x, out in zip((q, k), outs):
+        if x is None:
+            sides += [None, 0, 0, None, 0, 0, 0]
+            continue
+        if x.stride(2) != 1 and dim > 1:
+            x = x.contiguous()
+        sides += [x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
+                  out.stride(1), x.shape[1]]
+    positions, frequencies = positions.contiguous(), frequencies.contiguous()
+    with _native.on_device(device):
+        _native.call(
+            "dsa_rope_pair", *sides, _native.DTYPE_CODES[dtype], tokens, dim, offset, rotated,
+            positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(),
+            float(magnitude), int(interleaved), int(inverse), _native.raw_stream(device))
+    return tuple(outs)
+
+
 def index_producer(q_proj, k_proj, head_logits, norm_weight, norm_bias, eps, cos_sin,
                    rope_rows=None, *, index_keys=None, index_scales=None, q_fold=False,
                    kv=None, kv_cache=None, page_table=None, token_offset=0, status=None,

@@ -451,6 +451,53 @@ int dsa_sparse_mla_fp8_paged_ws(const void* q, int64_t rows, int64_t heads, cons
                                 void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Rotary positions of queries and keys in one launch (apply_rope_pair,
+ * models/deepseek_v32/rotary.py:47-85, with angles formed here).
+ * q: [tokens, q_heads, dim], k: [tokens, k_heads, dim] of `dtype`, the last dim
+ * contiguous, token and head strides in elements; q_heads or k_heads may be 0.
+ * Dims offset .. offset + rotated - 1 of each head turn by t = positions[token] *
+ * frequencies[i] (positions int32, or int64 with wide_positions != 0; frequencies
+ * f32 [rotated / 2]): a' = magnitude (a cos t - b sin t), b' = magnitude (b cos t
+ * + a sin t) for the pair (a, b) = dims (2 i, 2 i + 1) with interleaved != 0, else
+ * (i, i + rotated / 2); inverse != 0: -t. Angles in 64 bits, values in 32,
+ * rounded once. The other dims are copied. q_out / k_out may be q / k with the
+ * same strides (in place) or memory apart from them. rotated and dim - rotated
+ * even.
+ */
+int dsa_rope_pair(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                  int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_heads,
+                  const void* k, int64_t k_token_stride, int64_t k_head_stride, void* k_out,
+                  int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_heads,
+                  int dtype, int64_t tokens, int64_t dim, int64_t offset, int64_t rotated,
+                  const void* positions, int wide_positions, const float* frequencies,
+                  float magnitude, int interleaved, int inverse, hipStream_t stream);
+
+/*
+ * New tokens into any slots of the fp8 paged cache, as dsa_kv_pack_fp8 writes
+ * them, optionally through the latent's RMSNorm and the RoPE part's rotation.
+ * kv: bf16 rows of 576 (512 latent + 64 RoPE), kv_stride elements apart; slots
+ * (int32, or int64 with wide_slots != 0): token i's row page * 64 + place of
+ * cache uint8 [pages * 64, 656]; below 0: not written; at or past the cache: not
+ * written, and 1 is ORed into *status (may be NULL). Distinct tokens of a call
+ * need distinct slots. norm_weight (f32 [512], or null): latent = bf16(x *
+ * rsqrt(mean x^2 + eps) * w). positions / frequencies (f32 [32]; positions null:
+ * none): rotation as dsa_rope_pair's, rounded to bf16.
+ */
+int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t tokens, const void* slots,
+                     int wide_slots, const float* norm_weight, float norm_eps,
+                     const void* positions, int wide_positions, const float* frequencies,
+                     float magnitude, int interleaved, int64_t pages, void* cache,
+                     int32_t* status, hipStream_t stream);
+
+/*
+ * Records of any slots of the fp8 paged cache as bf16 out [tokens, 576]
+ * contiguous, the values they stand for. A slot below 0 gives zeros; at or past
+ * the cache too, and 1 is ORed into *status (may be NULL).
+ */
+int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slots, int wide_slots,
+                    int64_t tokens, void* out, int32_t* status, hipStream_t stream);
+
+/*
  * Causal attention over packed sequences with grouped heads. No reference
  * counterpart (operators/flashinfer.py adapts a library's).
  * q: [q_tokens, heads, qk_dim], k: [k_tokens, kv_heads, qk_dim], v: [k_tokens,
