@@ -13,9 +13,16 @@ padding semantics and validation messages):
   record (512 e4m3 + 4 fp32 tile scales + 64 bf16 RoPE, 64 tokens per page),
   which has no reference counterpart.
 * ``pack_kv_fp8``          - writes bf16 ``[T, 576]`` records into that cache
-  (quantise-on-append).
+  (quantise-on-append); ``write_kv_fp8`` does so for any slots of it, through
+  the latent's norm and the RoPE part's rotation, and ``read_kv_fp8`` reads
+  records back.
+* ``prompt_attention``     - dense causal attention of packed sequences with
+  grouped heads (the non-absorbed form of a prompt).
+* ``shared_prefix_mla``    - dense MLA of branches that share a prefix in the
+  fp8 paged cache.
 
-Kernels: ``csrc/sparse_mla.hip`` and ``csrc/quantize.hip``.
+Kernels: ``csrc/sparse_mla.hip``, ``csrc/quantize.hip``,
+``csrc/prompt_attention.hip`` and ``csrc/shared_prefix.hip``.
 """
 
 import math
@@ -268,7 +275,6 @@ def write_kv_fp8(kv, kv_cache, slots, *, norm_weight=None, eps=1e-6, positions=N
     """
     if kv.ndim != 2 or kv.shape[1] != QK_DIM or kv.dtype != torch.bfloat16:
         raise ValueError("kv must be bf16 [tokens, 576]")
-    _native.require_gfx950(kv.device, "fp8 KV write")
     tokens = kv.shape[0]
     _check_cache(kv_cache, kv.device)
     slots = _check_slots(slots, tokens, kv.device)
@@ -291,6 +297,7 @@ def write_kv_fp8(kv, kv_cache, slots, *, norm_weight=None, eps=1e-6, positions=N
                 or frequencies.device != kv.device):
             raise ValueError("frequencies must be FP32 [32] on the cache device")
         positions, frequencies = positions.contiguous(), frequencies.contiguous()
+    _native.require_gfx950(kv.device, "fp8 KV write")
     if tokens == 0:
         return kv_cache
     if kv.stride(1) != 1 or kv.stride(0) % 8 or kv.stride(0) < 0 or kv.data_ptr() % 16:
@@ -321,7 +328,6 @@ def read_kv_fp8(kv_cache, slots, *, out=None, status=None):
     if not isinstance(kv_cache, torch.Tensor):
         raise ValueError("kv_cache must be uint8 [pages, 64, 656] on the records' device")
     device = kv_cache.device
-    _native.require_gfx950(device, "fp8 KV read")
     _check_cache(kv_cache, device)
     tokens = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.ndim == 1 else -1
     slots = _check_slots(slots, tokens, device)
@@ -333,6 +339,7 @@ def read_kv_fp8(kv_cache, slots, *, out=None, status=None):
           or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned bf16 [T, 576] tensor on the "
                          "cache device")
+    _native.require_gfx950(device, "fp8 KV read")
     if tokens == 0:
         return out
     with _native.on_device(device):
@@ -399,11 +406,11 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
         raise ValueError("max_k must be a nonnegative integer")
     if any(t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
         raise ValueError("prompt attention has no backward pass")
-    _native.require_gfx950(q.device, "prompt attention")
     cu_q = _check_starts(cu_q, q.device, "cu_q")
     cu_k = cu_q if cu_k is None else _check_starts(cu_k, q.device, "cu_k")
     if cu_k.numel() != cu_q.numel():
         raise ValueError("cu_q and cu_k must describe the same sequences")
+    _native.require_gfx950(q.device, "prompt attention")
     shape = (*q.shape[:2], v.shape[2])
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=q.device)
