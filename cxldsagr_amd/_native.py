@@ -80,7 +80,7 @@ SIGNATURES = {
     "dsa_kv_write_fp8": [_ptr, _i64, _i64, _ptr, _int, _ptr, _f32, _ptr, _int, _ptr, _f32, _int,
                          _i64, _ptr, _ptr, _ptr],
     "dsa_kv_read_fp8": [_ptr, _i64, _ptr, _int, _i64, _ptr, _ptr, _ptr],
-    "dsa_prompt_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64,
+    "dsa_prompt_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                              ctypes.POINTER(ctypes.c_int64)],
     "dsa_prompt_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _int, _i64,
                              _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _int,

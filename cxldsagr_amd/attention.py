@@ -425,7 +425,8 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
     q, k, v = _heads_layout(q), _heads_layout(k), _heads_layout(v)
     with _native.on_device(q.device):
         needed = _native.size_of("dsa_prompt_attention_workspace_bytes", q.device.index,
-                                 q.shape[0], q.shape[1], k.shape[1], v.shape[2], sequences, max_k)
+                                 q.shape[0], q.shape[1], k.shape[1], v.shape[2], sequences,
+                                 k.shape[0], max_k)
         workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
         _native.call(
             "dsa_prompt_attention",

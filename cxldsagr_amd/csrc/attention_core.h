@@ -3,6 +3,8 @@
 // LDS access, and the join of partial results over split keys.
 #pragma once
 
+#include <type_traits>
+
 #include "dsa_common.h"
 
 namespace dsa {
@@ -78,10 +80,20 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOutstanding) : "memory");
 }
 
-// 16 bytes per lane from base + off into LDS at lds_base + 16 * lane.
+// 16 bytes per lane from base + off + kFrom into LDS at lds_base + kTo + 16 * lane.
+// (The instruction's offset counts on both sides.)
+template <int kFrom, int kTo>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               ::"s"(lds_base), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4"
+               ::"s"(lds_base), "v"(off), "s"(base), "n"(kTo - kFrom), "n"(kFrom) : "memory", "m0", "scc");
+}
+
+template <int kCount, int kAt = 0, typename F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (kAt < kCount) {
+    f(std::integral_constant<int, kAt>{});
+    static_for<kCount, kAt + 1>(f);
+  }
 }
 
 // The larger of a value in lane l and lane l ^ 32, in both.
@@ -126,24 +138,36 @@ __device__ __forceinline__ float raise(RowState& row, float mx) {
   return factor;
 }
 
-// One pair of probabilities, in log2 units against the row's running maximum
-// (shift = -top, or 0 with no visible key so far: every score is then -inf and
-// p = 0); the rounded values join the row's sum.
+// A row's probabilities in log2 units against its running maximum, p = 2^(scale s +
+// shift) with shift = -top (or 0 with no visible key so far: every score is then
+// -inf and p = 0), as packed pairs whose rounded values join the row's sum. Issued
+// in ticks of at most six instructions: tick t scales pair t, takes the powers of
+// pair t - 1 and packs pair t - 2, so that none waits for the one before it.
 template <typename E>
-__device__ __forceinline__ uint32_t probability_pair(float s0, float s1, float scale_log2, float shift, float& sum) {
-  const uint32_t p = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, scale_log2, shift)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(s1, scale_log2, shift)));
-  sum = E::add_pair(p, sum);
-  return p;
-}
+struct Softener {
+  float x[2][2], y[2][2];
+  template <typename Scores, typename Sum>
+  __device__ __forceinline__ void tick(int t, int pairs, float scale_log2, Scores score, const float* shift, Sum put) {
+    if (t >= 2) put(t - 2, E::pack(y[t & 1][0], y[t & 1][1]));
+    if (t >= 1 && t - 1 < pairs) {
+      y[(t - 1) & 1][0] = __builtin_amdgcn_exp2f(x[(t - 1) & 1][0]);
+      y[(t - 1) & 1][1] = __builtin_amdgcn_exp2f(x[(t - 1) & 1][1]);
+    }
+    if (t < pairs) {
+      x[t & 1][0] = __builtin_fmaf(score(2 * t), scale_log2, shift[t >> 3]);
+      x[t & 1][1] = __builtin_fmaf(score(2 * t + 1), scale_log2, shift[t >> 3]);
+    }
+  }
+};
 __device__ __forceinline__ float shift_of(const RowState& row) {
   return row.top == -__builtin_inff() ? 0.0f : -row.top;
 }
 
-// A per-lane LDS address formed once and hidden from the optimizer (an identity
-// lane move), so that reads at constant distances use the instruction's offset.
-__device__ __forceinline__ uint32_t opaque_address(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xE4, 0xF, 0xF, false);
+// A per-lane LDS address formed once and hidden from the optimizer, so that reads
+// at constant distances use the instruction's offset field.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // ------------------------------------------------- joining split keys --
@@ -158,60 +182,104 @@ __device__ __forceinline__ float2 split_stats(float top, float sum) {
   return make_float2(sum == sum ? top : sum, sum);
 }
 
-// Joins them: four groups of kDim / 8 lanes take a row, a quarter of its splits
-// each, 8 dims a lane. What bounds it is reading the parts.
-template <typename E, int kDim>
-__global__ __launch_bounds__(256) void join_splits(const float* __restrict__ parts, const float2* __restrict__ stats,
-                                                   int64_t rows, int splits, const int32_t* __restrict__ cu,
-                                                   int32_t sequences, int64_t heads, uint16_t* __restrict__ out) {
-  constexpr int kLanes = kDim / 8, kWays = 4, kRows = 256 / (kLanes * kWays);
-  __shared__ float shared[kWays][kRows][kDim + 4];
-  const int local = threadIdx.x / (kLanes * kWays);
-  const int way = threadIdx.x / kLanes % kWays;
-  const int d = (threadIdx.x % kLanes) * 8;
+// Joins them: kWays groups of kDim / 16 lanes take a row, 16 dims a lane (four
+// vectors, each of neighbouring lanes side by side) and every kWays-th split each,
+// against a running maximum of their own. What bounds it is reading the parts: many
+// parts of few rows want many loads in flight (120 parts of 128 rows of 512 dims,
+// 31 MB: 42 us with 4 ways of 8 dims a lane and all maxima looked at first).
+template <typename E, int kDim, int kWays>
+__global__ __launch_bounds__(kWays * kDim / 16 > 256 ? kWays * kDim / 16 : 256) void join_splits(
+    const float* __restrict__ parts, const float2* __restrict__ stats, int64_t rows, int splits,
+    const int32_t* __restrict__ cu, int32_t sequences, int64_t heads, uint16_t* __restrict__ out) {
+  constexpr int kLanes = kDim / 16, kGroup = kWays * kLanes;
+  constexpr int kThreads = kGroup > 256 ? kGroup : 256, kRows = kThreads / kGroup;
+  __shared__ float shared[kRows][kWays][kDim];
+  __shared__ float2 of_way[kRows][kWays];
+  const int local = threadIdx.x / kGroup, way = threadIdx.x % kGroup / kLanes, l = threadIdx.x % kLanes;
   const int64_t row = (int64_t)blockIdx.x * kRows + local;
+  const float none = -__builtin_inff();
   // Rows outside the sequences have no parts, and stay as they are.
   const bool live = row < rows && (cu == nullptr || (row >= cu[0] * heads && row < cu[sequences] * heads));
-  float acc[8] = {}, sum = 0.0f;
   if (live) {
-    float top = -__builtin_inff();
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, stats[s * rows + row].x);
-#pragma unroll 4
-    for (int s = way; s < splits; s += kWays) {
-      const float2 st = stats[s * rows + row];
-      if (st.x == -__builtin_inff()) continue;  // (a NaN maximum, of a split with NaN scores, spreads)
-      const float w = __builtin_amdgcn_exp2f(st.x - top);
-      sum += w * st.y;
-      const float4* o = reinterpret_cast<const float4*>(parts + (s * rows + row) * kDim + d);
-      const float4 a = o[0], b = o[1];
-      acc[0] += w * a.x, acc[1] += w * a.y, acc[2] += w * a.z, acc[3] += w * a.w;
-      acc[4] += w * b.x, acc[5] += w * b.y, acc[6] += w * b.z, acc[7] += w * b.w;
+    float4 acc[4] = {};
+    float top = none, sum = 0.0f;
+    constexpr int kAtOnce = 4;
+    for (int s0 = way; s0 < splits; s0 += kWays * kAtOnce) {
+      float2 st[kAtOnce];
+      float4 o[kAtOnce][4];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int s = s0 + i * kWays;
+        st[i] = s < splits ? stats[s * rows + row] : make_float2(none, 0.0f);
+        // (A split without a visible key has written no values.)
+        const float4* src = reinterpret_cast<const float4*>(parts + (s * rows + row) * kDim) + l;
+        const bool some = st[i].y != 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] = some ? src[c * kLanes] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      float up = top;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) up = fmaxf(up, st[i].x);
+      const float keep = top == none ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+      sum *= keep;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c].x *= keep, acc[c].y *= keep, acc[c].z *= keep, acc[c].w *= keep;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        // (A NaN maximum, of a split with a NaN score, spreads.)
+        const float w = st[i].y != 0.0f ? __builtin_amdgcn_exp2f(st[i].x - up) : 0.0f;
+        sum += w * st[i].y;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          acc[c].x += w * o[i][c].x;
+          acc[c].y += w * o[i][c].y;
+          acc[c].z += w * o[i][c].z;
+          acc[c].w += w * o[i][c].w;
+        }
+      }
+      top = up;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) shared[way][local][d + i] = acc[i];
-    if (d == 0) shared[way][local][kDim] = sum;
+    for (int c = 0; c < 4; ++c) reinterpret_cast<float4*>(&shared[local][way][0])[c * kLanes + l] = acc[c];
+    if (l == 0) of_way[local][way] = make_float2(top, sum);
   }
   __syncthreads();
-  if (!live || way != 0) return;
+  if (!live) return;
+  float top = none;
 #pragma unroll
-  for (int w = 1; w < kWays; ++w) {
-    sum = w == 1 ? shared[0][local][kDim] + shared[w][local][kDim] : sum + shared[w][local][kDim];
+  for (int w = 0; w < kWays; ++w) top = fmaxf(top, of_way[local][w].x);
+  float sum = 0.0f, factor[kWays];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] += shared[w][local][d + i];
+  for (int w = 0; w < kWays; ++w) {
+    const float2 st = of_way[local][w];
+    factor[w] = st.y != 0.0f ? (st.x == none ? st.y : __builtin_amdgcn_exp2f(st.x - top)) : 0.0f;
+    sum += factor[w] * st.y;
   }
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-  v4u packed;
+  for (int d = 2 * (threadIdx.x % kGroup); d < kDim; d += 2 * kGroup) {
+    float a = 0.0f, b = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) packed[i] = E::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-  *reinterpret_cast<v4u*>(out + row * kDim + d) = packed;
+    for (int w = 0; w < kWays; ++w) {
+      const float2 v = *reinterpret_cast<const float2*>(&shared[local][w][d]);
+      a += factor[w] * v.x;
+      b += factor[w] * v.y;
+    }
+    *reinterpret_cast<uint32_t*>(out + row * kDim + d) = E::pack(a * inv, b * inv);
+  }
 }
 
 template <typename E, int kDim>
 int launch_join(const float* parts, const float2* stats, int64_t rows, int splits, const int32_t* cu,
                 int32_t sequences, int64_t heads, uint16_t* out, hipStream_t stream) {
-  constexpr int kRows = 256 / (kDim / 8 * 4);
-  hipLaunchKernelGGL((join_splits<E, kDim>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, stream, parts,
-                     stats, rows, splits, cu, sequences, heads, out);
+  auto go = [&](auto kernel, int threads, int per_group) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per_group - 1) / per_group)), dim3(threads), 0, stream, parts,
+                       stats, rows, splits, cu, sequences, heads, out);
+  };
+  // Ways for the parts there are.
+  constexpr int kLanes = kDim / 16;
+  if (splits <= 4) go(join_splits<E, kDim, 2>, 256, 256 / (2 * kLanes));
+  else if (splits <= 32) go(join_splits<E, kDim, 8>, 256, 256 / (8 * kLanes));
+  else go(join_splits<E, kDim, 32>, kLanes * 32 > 256 ? kLanes * 32 : 256, kLanes * 32 > 256 ? 1 : 256 / (32 * kLanes));
   DSA_CHECK_LAUNCH("join of split keys");
   return kOk;
 }

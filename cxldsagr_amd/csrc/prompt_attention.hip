@@ -31,10 +31,18 @@
 namespace dsa {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaveRows = 64;
-constexpr int kTileRows = 4 * kWaveRows;
-constexpr int kStageKeys = 64;
+// Keys of a stage.
+constexpr int kStageKeys = 32;
+
+// How a kernel is cut: kWaves waves of 32 rows; a stage's loads are issued kDistance
+// stages before it is entered. K of a stage is read until the next is entered, V for
+// two stages more.
+template <int kWaves_, int kDistance_>
+struct Cut {
+  static constexpr int kWaves = kWaves_, kDistance = kDistance_;
+  static constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
+  static constexpr int kBufK = kDistance + 1, kBufV = kDistance + 3;
+};
 
 struct PromptArgs {
   const uint16_t* q;
@@ -47,26 +55,26 @@ struct PromptArgs {
   float2* stats;   // [splits][q_tokens * heads]
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides, elements
   int64_t q_tokens, k_tokens;
-  int32_t heads, kv_heads, sequences, slots, splits, causal;
+  int32_t heads, kv_heads, sequences, slots, splits, split_stages, causal;
   float scale_log2;
 };
 
-// Slots of row tiles: sequence b's tiles start at slot cu_q[b] G / 256 + b, which
+// Slots of row tiles: sequence b's tiles start at slot cu_q[b] G / tile + b, which
 // leaves room for a part-filled tile of every sequence before it: a closed form,
 // so a work-group finds its sequence by bisection, with no plan made beforehand.
-__host__ __device__ inline int64_t first_slot(int64_t start, int64_t group, int64_t b) {
-  return start * group / kTileRows + b;
+__host__ __device__ inline int64_t first_slot(int64_t start, int64_t group, int64_t b, int64_t tile) {
+  return start * group / tile + b;
 }
 
-template <typename E, int kQk, int kV>
-__global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
+template <typename E, int kQk, int kV, typename C>
+__global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) void prompt_fwd(const PromptArgs a) {
+  constexpr int kWaves = C::kWaves, kTileRows = C::kRows;
   constexpr int kQuadsK = kQk / 32, kQuadsV = kV / 32;  // 64-byte column blocks
   constexpr int kStageK = kStageKeys * kQk * 2, kStageV = kStageKeys * kV * 2;
-  constexpr int kBufK = 3, kBufV = 4;
   constexpr int kSteps = kQk / 16, kDims = kV / 32;
-  __shared__ __align__(1024) uint8_t lds[kBufK * kStageK + kBufV * kStageV];
-  const uint32_t lds_k = (uint32_t)(uintptr_t)&lds[0];
-  const uint32_t lds_v = lds_k + kBufK * kStageK;
+  __shared__ __align__(1024) uint8_t lds[C::kBufK * kStageK + C::kBufV * kStageV];
+  const uint32_t lds_k = (uint32_t)(uintptr_t)&lds[0], end_k = lds_k + C::kBufK * kStageK;
+  const uint32_t lds_v = end_k, end_v = lds_v + C::kBufV * kStageV;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
@@ -81,8 +89,9 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
   int slot, kv_head;
   if (a.splits == 1 && a.kv_heads % 8 == 0) {
     const int64_t in_xcd = unit >> 3;
-    kv_head = (int)(in_xcd / a.slots) * 8 + (int)(unit & 7);
-    slot = a.slots - 1 - (int)(in_xcd % a.slots);
+    const int per_xcd = a.kv_heads / 8;
+    kv_head = (int)(in_xcd % per_xcd) * 8 + (int)(unit & 7);
+    slot = a.slots - 1 - (int)(in_xcd / per_xcd);
   } else {
     kv_head = (int)(unit % a.kv_heads);
     slot = a.slots - 1 - (int)(unit / a.kv_heads);
@@ -90,7 +99,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
   int lo = 0, hi = a.sequences;  // the last sequence whose first slot is <= slot
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (first_slot(a.cu_q[mid], group, mid) <= slot) lo = mid; else hi = mid;
+    if (first_slot(a.cu_q[mid], group, mid, kTileRows) <= slot) lo = mid; else hi = mid;
   }
   // Lengths outside the tensors are cut to them.
   const int64_t q_begin = min(max((int64_t)a.cu_q[lo], (int64_t)0), a.q_tokens);
@@ -98,7 +107,7 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
   const int64_t k_begin = min(max((int64_t)a.cu_k[lo], (int64_t)0), a.k_tokens);
   const int64_t k_end = min(max((int64_t)a.cu_k[lo + 1], k_begin), a.k_tokens);
   const int n_q = (int)(q_end - q_begin), n_k = (int)(k_end - k_begin);
-  const int64_t tile_row = ((int64_t)slot - first_slot(a.cu_q[lo], group, lo)) * kTileRows;
+  const int64_t tile_row = ((int64_t)slot - first_slot(a.cu_q[lo], group, lo, kTileRows)) * kTileRows;
   const int64_t rows = (int64_t)n_q * group;
   if (tile_row < 0 || tile_row >= rows) return;
 
@@ -110,25 +119,18 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
   };
   const int64_t last_row = min(tile_row + kTileRows, rows) - 1;
   const int all_stages = (visible(last_row / group) + kStageKeys - 1) / kStageKeys;
-  const int per_split = (all_stages + a.splits - 1) / a.splits;
-  const int s0 = split * per_split;
-  const int s1 = min(s0 + per_split, all_stages);
+  const int s0 = a.splits > 1 ? min(split * a.split_stages, all_stages) : 0;
+  const int s1 = a.splits > 1 ? (split + 1 < a.splits ? min(s0 + a.split_stages, all_stages) : all_stages) : all_stages;
 
-  // ---- this wave's rows: two tiles of 32, this lane's rows n and 32 + n.
-  const int64_t wave_row = tile_row + wave * kWaveRows;
-  const int wave_rows = (int)min((int64_t)kWaveRows, rows - wave_row);  // may be <= 0
-  int64_t token[2];
-  int head[2], sees[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    // Rows past the end repeat the wave's last row; nothing of them is stored.
-    const int64_t row = wave_row + min(32 * t + n, max(wave_rows - 1, 0));
-    const int64_t r = min(row, rows - 1);
-    token[t] = r / group;
-    head[t] = kv_head * group + (int)(r - token[t] * group);
-    sees[t] = visible(token[t]);
-  }
-  // The stages this wave takes part in, and the first 32 keys that need a mask.
+  // ---- this wave's 32 rows; lanes n and 32 + n have row n.
+  const int64_t wave_row = tile_row + wave * 32;
+  const int wave_rows = (int)min((int64_t)32, rows - wave_row);  // may be <= 0
+  // Rows past the end repeat the wave's last row; nothing of them is stored.
+  const int64_t r = min(wave_row + min(n, max(wave_rows - 1, 0)), rows - 1);
+  const int64_t token = r / group;
+  const int head = kv_head * group + (int)(r - token * group);
+  const int sees = visible(token);
+  // The stages this wave takes part in, and the first key that needs a mask.
   int w1 = s0, clear = 0;
   if (wave_rows > 0) {
     w1 = min(s1, (visible((wave_row + wave_rows - 1) / group) + kStageKeys - 1) / kStageKeys);
@@ -137,273 +139,300 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_fwd(const PromptArgs a) {
   w1 = __builtin_amdgcn_readfirstlane(w1);
   clear = __builtin_amdgcn_readfirstlane(clear);
 
-  v4u q_ops[2][kSteps];
+  v4u q_ops[kSteps];
+  {
+    const uint16_t* src = a.q + (q_begin + token) * a.q_token + head * a.q_head + 8 * h;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const uint16_t* src = a.q + (q_begin + token[t]) * a.q_token + head[t] * a.q_head + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) q_ops[t][ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
-  }
-  // In AGPRs, from where the products read their second operand: VGPRs are left
-  // to the accumulators and the softmax.
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) asm volatile("" : "+a"(q_ops[t][ks]));
-
-  // ---- staging. Wave w brings rows 16 w .. + 15 of every column block.
-  const uint8_t* k_base = reinterpret_cast<const uint8_t*>(a.k + k_begin * a.k_token + kv_head * a.k_head);
-  const uint8_t* v_base = reinterpret_cast<const uint8_t*>(a.v + k_begin * a.v_token + kv_head * a.v_head);
-  const int load_row = 16 * wave + (lane >> 2);
-  const uint32_t load_chunk = 16u * ((lane & 3) ^ (lane >> 4));
-  auto issue = [&](int stage) {
-    if (stage >= s1) return;
-    // Rows past the sequence's end repeat its last one: their scores are
-    // masked, and what multiplies their zero probabilities is a row's own.
-    const int64_t key0 = (int64_t)stage * kStageKeys;
-    const uint32_t row = (uint32_t)min((int64_t)load_row, n_k - 1 - key0);
-    const uint8_t* kb = k_base + key0 * a.k_token * 2;
-    const uint8_t* vb = v_base + key0 * a.v_token * 2;
-    const uint32_t k_off = row * (uint32_t)(a.k_token * 2) + load_chunk;
-    const uint32_t v_off = row * (uint32_t)(a.v_token * 2) + load_chunk;
-    const uint32_t kl = lds_k + (uint32_t)(stage % kBufK) * kStageK + 1024 * wave;
-    const uint32_t vl = lds_v + (uint32_t)(stage % kBufV) * kStageV + 1024 * wave;
-#pragma unroll
-    for (int c = 0; c < kQuadsK; ++c) load_to_lds(kb + 64 * c, k_off, kl + 4096 * c);
-#pragma unroll
-    for (int c = 0; c < kQuadsV; ++c) load_to_lds(vb + 64 * c, v_off, vl + 4096 * c);
-  };
-  constexpr int kLoads = kQuadsK + kQuadsV;
-
-  // LDS address of a stage's operands. K: key 32 half + n, chunk 2 ks + h of its
-  // row; odd ks flip chunk bit 1. V: keys 16 t + 8 u + 4 h + jj, dims
-  // 32 d + 16 (g & 1) + 4 qq; u flips chunk bit 1.
-  uint32_t k_lane[2], v_lane[2];
-#pragma unroll
-  for (int o = 0; o < 2; ++o) {
-    k_lane[o] = (uint32_t)(n >> 4) * 1024 + 64 * (n & 15) + 16 * ((2 * o + h) ^ ((n & 15) >> 2));
-    const int jj = (lane & 15) >> 2, qq = lane & 3, g1 = (lane >> 4) & 1;
-    v_lane[o] = 64 * (8 * o + 4 * h + jj) + 16 * ((2 * g1 + (qq >> 1)) ^ (2 * o + h)) + 8 * (qq & 1);
+    for (int ks = 0; ks < kSteps; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
   }
 
-  v16f o[2][kDims];
+  // ---- staging. A stage is two blocks of 16 rows by 64 bytes per column block,
+  // dealt to the waves: four have one row block each and every other column block,
+  // one has all.
+  constexpr int kSpread = kWaves == 1 ? 2 : 1;  // row blocks of a wave
+  constexpr int kLoadsK = 2 * kQuadsK / kWaves, kLoadsV = 2 * kQuadsV / kWaves, kLoads = kLoadsK + kLoadsV;
+  static_assert(2 * kQuadsK % kWaves == 0 && 2 * kQuadsV % kWaves == 0, "blocks per wave");
+  const uint8_t* k_from = reinterpret_cast<const uint8_t*>(a.k + (k_begin + (int64_t)s0 * kStageKeys) * a.k_token + kv_head * a.k_head);
+  const uint8_t* v_from = reinterpret_cast<const uint8_t*>(a.v + (k_begin + (int64_t)s0 * kStageKeys) * a.v_token + kv_head * a.v_head);
+  const int64_t k_stage = kStageKeys * a.k_token * 2, v_stage = kStageKeys * a.v_token * 2;
+  const int load_row = 16 * (wave & 1) + (lane >> 2);
+  const uint32_t load_at = 16u * ((lane & 3) ^ (lane >> 4)) + 64u * (wave >> 1);
+  uint32_t k_off[kSpread], v_off[kSpread];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int i = 0; i < kSpread; ++i) {
+    k_off[i] = (uint32_t)(load_row + 16 * i) * (uint32_t)(a.k_token * 2) + load_at;
+    v_off[i] = (uint32_t)(load_row + 16 * i) * (uint32_t)(a.v_token * 2) + load_at;
+  }
+  int to_load = s0;
+  uint32_t k_to = lds_k, v_to = lds_v;
+  auto issue = [&]() __attribute__((always_inline)) {
+    if (to_load >= s1) return;
+    if ((to_load + 1) * kStageKeys > n_k) {
+      // Rows past the sequence's end repeat its last one: their scores are
+      // masked, and what multiplies their zero probabilities is a row's own.
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) o[t][d] = v16f{};
-  RowState row[2] = {{-__builtin_inff(), 0.0f}, {-__builtin_inff(), 0.0f}};
-
-  // Block j: keys 32 j .. + 31, half j % 2 of stage j / 2.
-  auto k_at = [&](int j, int odd) -> uint32_t {
-    return opaque_address(lds_k + (uint32_t)((j >> 1) % kBufK) * kStageK + 2048 * (j & 1) + k_lane[odd]);
-  };
-  auto v_at = [&](int j, int upper) -> uint32_t {
-    return opaque_address(lds_v + (uint32_t)((j >> 1) % kBufV) * kStageV + 2048 * (j & 1) + v_lane[upper]);
-  };
-  constexpr int kAhead = 4;  // operands read ahead of their product
-  constexpr int kVops = 2 * kDims;
-  // S of block j (both row tiles); `slice(i)`, i < 2 kSteps, is issued after
-  // product i: independent work that the matrix unit leaves room for.
-  auto scores = [&](int j, v16f (&s)[2], auto slice) __attribute__((always_inline)) {
-    const uint32_t at[2] = {k_at(j, 0), k_at(j, 1)};
-    v4u kop[kAhead];
-#pragma unroll
-    for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at[ks & 1] + 4096 * (ks >> 1));
-    s[0] = v16f{};
-    s[1] = v16f{};
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t] = E::mfma(kop[ks % kAhead], q_ops[t][ks], s[t]);
-        if (t == 1 && ks + kAhead < kSteps)
-          kop[ks % kAhead] = lds_load<v4u>(at[ks & 1] + 4096 * ((ks + kAhead) >> 1));
-        slice(2 * ks + t);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < kSpread; ++i) {
+        const uint32_t row = (uint32_t)min(load_row + 16 * i, n_k - 1 - to_load * kStageKeys);
+        k_off[i] = row * (uint32_t)(a.k_token * 2) + load_at;
+        v_off[i] = row * (uint32_t)(a.v_token * 2) + load_at;
       }
     }
+    // Column block c of a wave's i-th load; its place is 2048 bytes a column block
+    // and 1024 a row block on. (A wave of four has c = 2 i + wave / 2.)
+    static_for<kLoadsK>([&](auto i) {
+      constexpr int c = kWaves == 1 ? i / 2 : 2 * i;
+      load_to_lds<64 * c, 2048 * c + (kWaves == 1 ? 1024 * (i % 2) : 0)>(k_from, k_off[kWaves == 1 ? i % 2 : 0], k_to + 1024 * wave);
+    });
+    static_for<kLoadsV>([&](auto i) {
+      constexpr int c = kWaves == 1 ? i / 2 : 2 * i;
+      load_to_lds<64 * c, 2048 * c + (kWaves == 1 ? 1024 * (i % 2) : 0)>(v_from, v_off[kWaves == 1 ? i % 2 : 0], v_to + 1024 * wave);
+    });
+    ++to_load;
+    k_from += k_stage;
+    v_from += v_stage;
+    k_to = k_to + kStageK == end_k ? lds_k : k_to + kStageK;
+    v_to = v_to + kStageV == end_v ? lds_v : v_to + kStageV;
   };
-  auto read_v = [&](const uint32_t (&at)[2], int i) __attribute__((always_inline)) -> v4u {
+
+  // LDS address of a stage's operands. K: key n, chunk 2 ks + h of its row; odd ks
+  // flip chunk bit 1 (32 bytes). V: keys 16 t + 8 u + 4 h + jj, dims 32 d + 16 (g & 1)
+  // + 4 qq; u flips chunk bit 1 and is 8 rows (512 bytes) on.
+  const uint32_t k_lane = (uint32_t)(n >> 4) * 1024 + 64 * (n & 15) + 16 * (h ^ ((n & 15) >> 2));
+  const uint32_t v_lane = (uint32_t)(64 * (4 * h + ((lane & 15) >> 2)) +
+                                     16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ h) + 8 * (lane & 1));
+
+  v16f o[kDims];
+  RowState row{-__builtin_inff(), 0.0f};
+  float shift = 0.0f;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = v16f{};
+
+  // Operands are read kAhead products ahead (in 64 dims, where three waves share
+  // a SIMD, two).
+  constexpr int kAhead = kV == 64 ? 2 : 4;
+  constexpr int kVops = 2 * kDims;
+  v4u kop[kAhead], vop[kAhead];
+  auto read_k = [&](uint32_t at, int ks) __attribute__((always_inline)) {
+    kop[ks % kAhead] = lds_load<v4u>((ks & 1 ? at ^ 32 : at) + 2048 * (ks >> 1));
+  };
+  auto read_v = [&](uint32_t at, int i) __attribute__((always_inline)) {
     const int t = i / kDims, d = i % kDims;
-    const v2u lo = lds_column(at[0] + 1024 * t + 4096 * d);
-    const v2u hi = lds_column(at[1] + 1024 * t + 4096 * d);
-    return v4u{lo.x, lo.y, hi.x, hi.y};
+    const v2u lo = lds_column(at + 1024 * t + 2048 * d);
+    const v2u hi = lds_column((at ^ 32) + 512 + 1024 * t + 2048 * d);
+    vop[i % kAhead] = v4u{lo.x, lo.y, hi.x, hi.y};
   };
-  // O^T += V^T P^T of block j, whose first operands are in vop.
-  auto values = [&](const uint32_t (&at)[2], v4u (&vop)[kAhead], const v4u (&p)[2][2], auto slice)
-                    __attribute__((always_inline)) {
+  // S of a stage (its first kAhead operands are in kop); `slice(i)` is issued
+  // after product i: independent work that the matrix unit leaves room for.
+  auto scores = [&](uint32_t at, v16f& s, auto slice) __attribute__((always_inline)) {
+    s = v16f{};
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      s = E::mfma(kop[ks % kAhead], q_ops[ks], s);
+      if (ks + kAhead < kSteps) read_k(at, ks + kAhead);
+      slice(ks);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // O^T += V^T P^T of a stage (its first kAhead operands are in vop).
+  auto values = [&](uint32_t at, const v4u (&p)[2], auto slice) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kVops; ++i) {
-      const int t = i / kDims, d = i % kDims;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        o[r][d] = E::mfma(vop[i % kAhead], p[r][t], o[r][d]);
-        if (r == 1 && i + kAhead < kVops) vop[i % kAhead] = read_v(at, i + kAhead);
-        slice(2 * i + r);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      o[i % kDims] = E::mfma(vop[i % kAhead], p[i / kDims], o[i % kDims]);
+      if (i + kAhead < kVops) read_v(at, i + kAhead);
+      slice(i);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Keys a row does not see: -inf.
-  auto mask = [&](int j, v16f (&s)[2]) __attribute__((always_inline)) {
+  auto mask = [&](int j, v16f& s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[t][i] = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3) < sees[t] ? s[t][i] : -__builtin_inff();
+    for (int i = 0; i < 16; ++i)
+      s[i] = kStageKeys * j + 8 * (i >> 2) + 4 * h + (i & 3) < sees ? s[i] : -__builtin_inff();
   };
-  // The stage has landed for this wave (the loads of the next may be in flight),
-  // then for every wave, which are then also done with the stage before.
-  auto enter_stage = [&](int stage) {
-    if (stage + 1 < s1) wait_loads<kLoads>(); else wait_loads<0>();
+  // The next stage has landed for this wave (those after it may be in flight), then
+  // for every wave, which are then also done with the K of the stage before and the
+  // V of the two before that.
+  int entered = s0;  // stages entered so far end here
+  auto enter_stage = [&]() __attribute__((always_inline)) {
+    if (entered + C::kDistance <= s1) wait_loads<(C::kDistance - 1) * kLoads>(); else wait_loads<0>();
     lds_barrier();
-    issue(stage + 2);
+    issue();
+    ++entered;
   };
+  static_assert((C::kDistance - 1) * kLoads < 64, "outstanding loads");
 
-  issue(s0);
-  issue(s0 + 1);
+#pragma unroll
+  for (int i = 0; i < C::kDistance; ++i) issue();
   if (w1 > s0) {
-    const int j1 = 2 * w1;
-    int j = 2 * s0;
-    v16f s[2], next[2];
-    v4u p[2][2];
-    float shift[2];
+    int j = s0;
+    uint32_t k_at = lds_k + k_lane, v_at = lds_v + v_lane;  // of stage j
+    auto next_k = [&]() { k_at = opaque(k_at - k_lane + kStageK == end_k ? lds_k + k_lane : k_at + kStageK); };
+    auto next_v = [&]() { v_at = opaque(v_at - v_lane + kStageV == end_v ? lds_v + v_lane : v_at + kStageV); };
+    v16f s, next;
+    v4u p[2];
+    constexpr int kPairs = 8, kTicks = kPairs + 2;
     auto no_slice = [](int) {};
-    // Slice i of n: the 16 pairs of probabilities of both rows.
-    auto soften = [&](const v16f (&from)[2], int i, int n) __attribute__((always_inline)) {
+    Softener<E> softener;
+    // Slice i of `of` of the probabilities of the scores in `from`.
+    auto soften = [&](const v16f& from, int i, int of) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 16 * i / n; u < 16 * (i + 1) / n; ++u) {
-        const int t = u >> 3, w = u & 7;
-        p[t][w >> 2][w & 3] =
-            probability_pair<E>(from[t][2 * w], from[t][2 * w + 1], a.scale_log2, shift[t], row[t].sum);
-      }
+      for (int u = kTicks * i / of; u < kTicks * (i + 1) / of; ++u)
+        softener.tick(u, kPairs, a.scale_log2, [&](int e) { return from[e]; }, &shift, [&](int w, uint32_t pair) {
+          p[w >> 2][w & 3] = pair;
+          row.sum = E::add_pair(pair, row.sum);
+        });
     };
-    // One step: block j + 1's scores beside the probabilities of block j (scores
-    // in `from`, its rows' maxima raised), then block j's product with V beside
-    // the maxima of block j + 1 (into `to`). Says whether the inner loop ends: a
-    // row's maximum must rise, the block needs a mask (kBreak), or there was no
-    // block left (kDone, `to` not written).
+    // One step: stage j's scores beside the probabilities of stage j - 1 (scores in
+    // `from`, its rows' maxima raised), then stage j - 1's product with V beside the
+    // maxima of stage j (into `to`) and the first K reads of stage j + 1, which is
+    // entered between the two. Says whether the inner loop ends: a row's maximum
+    // must rise or the stage needs a mask (kBreak), or there was no stage left
+    // (kDone, `to` not written).
     enum { kGo, kBreak, kDone };
-    auto step = [&](const v16f (&from)[2], v16f (&to)[2]) __attribute__((always_inline)) -> int {
+    auto step = [&](const v16f& from, v16f& to) __attribute__((always_inline)) -> int {
+      if (j + 1 == w1) return kDone;
       ++j;
-      if (j == j1) return kDone;
-      if (!(j & 1)) enter_stage(j >> 1);
-      const uint32_t at[2] = {v_at(j - 1, 0), v_at(j - 1, 1)};
-      v4u vop[kAhead];
+      scores(k_at, to, [&](int i) __attribute__((always_inline)) {
+        soften(from, i, kSteps);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);
-      scores(j, to, [&](int i) __attribute__((always_inline)) { soften(from, i, 2 * kSteps); });
-      float top[2] = {-__builtin_inff(), -__builtin_inff()};
-      values(at, vop, p, [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 16 * i / (2 * kVops); u < 16 * (i + 1) / (2 * kVops); ++u)
-          top[u >> 3] = fmaxf(fmaxf(top[u >> 3], to[u >> 3][2 * (u & 7)]), to[u >> 3][2 * (u & 7) + 1]);
+        for (int u = 0; u < kAhead; ++u)
+          if (i == kSteps - 1 - kAhead + u || (kSteps < kAhead + 1 && i == kSteps - 1)) read_v(v_at, u);
       });
-      const float m0 = max_halves(top[0]) * a.scale_log2, m1 = max_halves(top[1]) * a.scale_log2;
-      const bool rise = must_raise(row[0], m0) || must_raise(row[1], m1);
-      return 32 * j + 32 > clear || __builtin_amdgcn_ballot_w64(rise) != 0 ? kBreak : kGo;
+      // Computed by here, beside the products, not where they are used.
+      asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(row.sum));
+      if (j + 1 < s1) enter_stage();
+      next_k();
+      float top;
+      uint64_t rise = 0;
+      values(v_at, p, [&](int i) __attribute__((always_inline)) {
+        // Pairs of scores over half of the products, the check, the reads.
+        constexpr int kPerSlot = kVops >= 8 ? 2 : 4;
+#pragma unroll
+        for (int u = kPerSlot * i; u < kPerSlot * (i + 1) && u < kPairs; ++u) {
+          const float m = fmaxf(to[2 * u], to[2 * u + 1]);
+          top = u == 0 ? m : fmaxf(top, m);
+        }
+        if (i == kPairs / kPerSlot)
+          rise = __builtin_amdgcn_ballot_w64(must_raise(row, max_halves(top) * a.scale_log2));
+        if (i >= kVops - kAhead) read_k(k_at, i - (kVops - kAhead));
+      });
+      next_v();
+      return kStageKeys * (j + 1) > clear || rise != 0 ? kBreak : kGo;
     };
-    enter_stage(s0);
-    scores(j, s, no_slice);
+    enter_stage();
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks) read_k(k_at, ks);
+    scores(k_at, s, no_slice);
+    if (s0 + 1 < s1) enter_stage();
+    next_k();
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks) read_k(k_at, ks);
     // Masks, and the rise of a row's maximum (by which what it summed so far is
     // rescaled), stay outside the inner loop: a multiply of the accumulators in
     // it makes the compiler keep a second copy of them and spill.
     for (bool more = true; more;) {
-      if (32 * j + 32 > clear) mask(j, s);
-      float factor[2];
+      if (kStageKeys * (j + 1) > clear) mask(j, s);
+      const float factor = raise(row, row_max(s, a.scale_log2));
+      shift = shift_of(row);
+      if (__builtin_amdgcn_ballot_w64(factor != 1.0f)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        factor[t] = raise(row[t], row_max(s[t], a.scale_log2));
-        shift[t] = shift_of(row[t]);
-      }
-      if (__builtin_amdgcn_ballot_w64(factor[0] != 1.0f || factor[1] != 1.0f)) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int d = 0; d < kDims; ++d) o[t][d] *= factor[t];
+        for (int d = 0; d < kDims; ++d) o[d] *= factor;
       }
       for (;;) {
         int end = step(s, next);
         if (end != kGo) {
           more = end == kBreak;
-          if (more) s[0] = next[0], s[1] = next[1];
+          if (more) s = next;
           break;
         }
         end = step(next, s);
         if (end != kGo) {
           more = end == kBreak;
-          if (!more) s[0] = next[0], s[1] = next[1];
+          if (!more) s = next;
           break;
         }
       }
     }
-    const uint32_t at[2] = {v_at(j1 - 1, 0), v_at(j1 - 1, 1)};
-    v4u vop[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);
+    for (int i = 0; i < kAhead; ++i) read_v(v_at, i);
     soften(s, 0, 1);
-    values(at, vop, p, no_slice);
+    values(v_at, p, no_slice);
   }
-  for (int stage = max(w1, s0); stage < s1; ++stage) enter_stage(stage);
+  while (entered < s1) enter_stage();
 
   // ---- store. A lane holds dims 32 d + 8 b + 4 h + 0 .. 3 of its row; the halves
   // trade so that each stores 16 bytes.
+  const float sum = sum_halves(row.sum);
+  const bool live = n < wave_rows;
+  const int64_t at = (q_begin + token) * a.heads + head;
+  if (a.splits > 1) {
+    const int64_t part = (int64_t)split * a.q_tokens * a.heads + at;
+    if (live && h == 0) a.stats[part] = split_stats(row.top, sum);
+    if (live && sum != 0.0f) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float sum = sum_halves(row[t].sum);
-    const bool live = 32 * t + n < wave_rows;
-    const int64_t at = (q_begin + token[t]) * a.heads + head[t];
-    if (a.splits > 1) {
-      const int64_t part = (int64_t)split * a.q_tokens * a.heads + at;
-      if (live && h == 0) a.stats[part] = split_stats(row[t].top, sum);
-      if (live && sum != 0.0f) {
+      for (int d = 0; d < kDims; ++d)
 #pragma unroll
-        for (int d = 0; d < kDims; ++d)
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<v4f*>(a.parts + part * kV + 32 * d + 8 * b + 4 * h) =
-                v4f{o[t][d][4 * b], o[t][d][4 * b + 1], o[t][d][4 * b + 2], o[t][d][4 * b + 3]};
-      }
-      continue;
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<v4f*>(a.parts + part * kV + 32 * d + 8 * b + 4 * h) =
+              v4f{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-#pragma unroll
-    for (int d = 0; d < kDims; ++d)
-#pragma unroll
-      for (int b = 0; b < 4; b += 2) {
-        uint32_t w[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            w[u][e] = E::pack(o[t][d][4 * (b + u) + 2 * e] * inv, o[t][d][4 * (b + u) + 2 * e + 1] * inv);
-        const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-        const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-        if (live)
-          *reinterpret_cast<v4u*>(a.out + at * kV + 32 * d + 8 * (b + h)) = v4u{x[0], y[0], x[1], y[1]};
-      }
+    return;
   }
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int b = 0; b < 4; b += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[u][e] = E::pack(o[d][4 * (b + u) + 2 * e] * inv, o[d][4 * (b + u) + 2 * e + 1] * inv);
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      if (live) *reinterpret_cast<v4u*>(a.out + at * kV + 32 * d + 8 * (b + h)) = v4u{x[0], y[0], x[1], y[1]};
+    }
 }
 
-// Key splits: enough work-groups for the chip where the row tiles are few, but at
-// least 256 keys to a split (a part costs 4 (d_v + 2) bytes a row, written and read).
+// The cut of a call. Rows of a sequence and KV head that fill a wave at most (single
+// tokens): work-groups of one wave, two of them per CU; a wave alone in a work-group
+// of eight would walk every key by itself, which bounds the call, not memory. Others:
+// eight waves, 256 rows.
+using FewRows = Cut<1, 2>;
+using ManyRows = Cut<4, 2>;
+
+// Key splits, where the row tiles are too few for the chip: ranges of the same
+// number of keys, so that sequences of different lengths make work-groups of the
+// same size, about `rounds` per CU if all keys are seen, of at least 256 keys (a part
+// costs 4 (d_v + 2) bytes a row, written and read).
+constexpr int64_t kMinSplitKeys = 256, kMaxSplits = 64;
+
 struct PromptPlan {
-  int64_t slots, splits, bytes, stats_at;
+  bool few;
+  int64_t slots, splits, split_stages, bytes, stats_at;
 };
 
 PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_t v_dim, int64_t sequences,
-                       int64_t max_k) {
+                       int64_t k_tokens, int64_t max_k) {
   PromptPlan p{};
-  p.slots = first_slot(q_tokens, heads / kv_heads, sequences);
+  const int64_t rows = q_tokens * (heads / kv_heads);
+  p.few = rows <= FewRows::kRows * sequences;
+  const int64_t tile = p.few ? FewRows::kRows : ManyRows::kRows, keys = kStageKeys;
+  const int64_t rounds = 4;
+  p.slots = first_slot(q_tokens, heads / kv_heads, sequences, tile);
   const int64_t units = p.slots * kv_heads;
-  const int64_t cus = device_cu_count();
+  const int64_t cus = device_cu_count() * 2;
   p.splits = 1;
-  if (units < cus) {
-    const int64_t most = (max_k + 255) / 256;
-    p.splits = (2 * cus + units - 1) / units;
-    if (p.splits > most) p.splits = most;
-    if (p.splits > 64) p.splits = 64;
-    if (p.splits < 1) p.splits = 1;
+  const int64_t stages = (max_k + keys - 1) / keys, least = kMinSplitKeys / keys;
+  if (units < cus && stages > least) {
+    // Stages of all row tiles: the sequences' keys, as often as a sequence has tiles.
+    const int64_t tiles = (rows + tile * sequences - 1) / (tile * sequences);
+    const int64_t all = kv_heads * tiles * (k_tokens / keys + sequences);
+    p.split_stages = (all + rounds * device_cu_count() - 1) / (rounds * device_cu_count());
+    if (p.split_stages < (stages + kMaxSplits - 1) / kMaxSplits) p.split_stages = (stages + kMaxSplits - 1) / kMaxSplits;
+    if (p.split_stages < least) p.split_stages = least;
+    p.splits = (stages + p.split_stages - 1) / p.split_stages;
   }
   if (p.splits > 1) {
     p.stats_at = p.splits * q_tokens * heads * v_dim * 4;
@@ -413,9 +442,12 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
 }
 
 template <typename E, int kQk, int kV>
-int launch_prompt(const PromptArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt_fwd<E, kQk, kV>), dim3((unsigned)((int64_t)a.slots * a.kv_heads * a.splits)), dim3(kThreads),
-                     0, stream, a);
+int launch_prompt(const PromptArgs& a, bool few, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.slots * a.kv_heads * a.splits));
+  if (few)
+    hipLaunchKernelGGL((prompt_fwd<E, kQk, kV, FewRows>), grid, dim3(FewRows::kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prompt_fwd<E, kQk, kV, ManyRows>), grid, dim3(ManyRows::kThreads), 0, stream, a);
   DSA_CHECK_LAUNCH("prompt attention");
   if (a.splits > 1)
     return launch_join<E, kV>(a.parts, a.stats, a.q_tokens * a.heads, a.splits, a.cu_q, a.sequences, a.heads, a.out,
@@ -424,23 +456,23 @@ int launch_prompt(const PromptArgs& a, hipStream_t stream) {
 }
 
 template <typename E>
-int launch_dims(const PromptArgs& a, int64_t qk_dim, int64_t v_dim, hipStream_t stream) {
-  if (qk_dim == 192 && v_dim == 128) return launch_prompt<E, 192, 128>(a, stream);
-  if (qk_dim == 128 && v_dim == 128) return launch_prompt<E, 128, 128>(a, stream);
-  return launch_prompt<E, 64, 64>(a, stream);
+int launch_dims(const PromptArgs& a, int64_t qk_dim, int64_t v_dim, bool few, hipStream_t stream) {
+  if (qk_dim == 192 && v_dim == 128) return launch_prompt<E, 192, 128>(a, few, stream);
+  if (qk_dim == 128 && v_dim == 128) return launch_prompt<E, 128, 128>(a, few, stream);
+  return launch_prompt<E, 64, 64>(a, few, stream);
 }
 
 }  // namespace
 }  // namespace dsa
 
 extern "C" int dsa_prompt_attention_workspace_bytes(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_t v_dim,
-                                                    int64_t sequences, int64_t max_k, int64_t* bytes) {
+                                                    int64_t sequences, int64_t k_tokens, int64_t max_k, int64_t* bytes) {
   using namespace dsa;
   DSA_CHECK_ARG(bytes != nullptr, "null pointer");
-  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && max_k >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
+  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && k_tokens >= 0 && max_k >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
                     v_dim > 0,
                 "invalid prompt attention shape");
-  *bytes = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, max_k).bytes;
+  *bytes = sequences == 0 ? 0 : prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k).bytes;
   return kOk;
 }
 
@@ -470,7 +502,7 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
   DSA_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                  reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                 "q, k, v and out must be 16-byte aligned");
-  const PromptPlan p = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, max_k);
+  const PromptPlan p = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k);
   DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF, "too many row tiles");
   if (p.splits > 1)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
@@ -490,8 +522,9 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
   a.q_tokens = q_tokens, a.k_tokens = k_tokens;
   a.heads = (int32_t)heads, a.kv_heads = (int32_t)kv_heads;
   a.sequences = (int32_t)sequences, a.slots = (int32_t)p.slots, a.splits = (int32_t)p.splits;
+  a.split_stages = (int32_t)p.split_stages;
   a.causal = causal != 0;
   a.scale_log2 = scale * kLog2E;
-  return dtype == DSA_DTYPE_BF16 ? launch_dims<Bf16>(a, qk_dim, v_dim, stream)
-                                 : launch_dims<F16>(a, qk_dim, v_dim, stream);
+  return dtype == DSA_DTYPE_BF16 ? launch_dims<Bf16>(a, qk_dim, v_dim, p.few, stream)
+                                 : launch_dims<F16>(a, qk_dim, v_dim, p.few, stream);
 }

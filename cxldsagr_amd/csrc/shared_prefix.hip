@@ -48,7 +48,7 @@ constexpr int kBuffers = 3;
 constexpr int kSteps = kQkDim / 16, kDims = kVDim / 32;
 // Q^T operands of the last kQLds steps stay in LDS, the others in registers:
 // with all 36 there, O^T (256 registers of a lane) leaves too few for the rest.
-constexpr int kQLds = 8;
+constexpr int kQLds = 12;
 constexpr int kQReg = kSteps - kQLds;
 constexpr int kQBytes = kQLds * 4 * 1024;  // [wave][step][lane] 16 bytes
 
@@ -157,18 +157,9 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   const int64_t row_at = min(wave_row + n, row_end - 1);
   const bool active = __builtin_amdgcn_readfirstlane(wave_row < row_end && b1 > b0);
 
+  // Q^T operands: in AGPRs, and the last in LDS.
   v4u q_ops[kQReg];
   const uint32_t q_lds = lds_base + kBuffers * kBufBytes + (uint32_t)wave * (kQLds * 1024) + 16 * lane;
-  {
-    const uint16_t* src = a.q + row_at * kQkDim + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
-#pragma unroll
-    for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
-#pragma unroll
-    for (int ks = 0; ks < kQLds; ++ks)
-      lds_store<v4u>(q_lds + 1024 * ks, *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks)));
-  }
 
   // ---- staging: eight lanes a key. Lane j brings bytes 128 i + 16 j of the
   // latent (a chunk of every tile), the scales, and bytes 16 j of the RoPE part.
@@ -228,11 +219,16 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     const v2u hi = lds_column(at + (16 * t + 2) * kRowBytes + 64 * d);
     return v4u{lo.x, lo.y, hi.x, hi.y};
   };
-  auto scores = [&](int b, v16f& s, auto slice) __attribute__((always_inline)) {
-    const uint32_t at = opaque_address(buf_of(b) + k_lane);
-    v4u kop[kAhead], qop[2];
+  v4u kop[kAhead];
+  auto read_first_k = [&](int b) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t at = opaque(buf_of(b) + k_lane);
 #pragma unroll
     for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at + 32 * ks);
+    return at;
+  };
+  // S of a block at `at`, whose first kAhead operands are in kop.
+  auto scores = [&](uint32_t at, v16f& s, auto slice) __attribute__((always_inline)) {
+    v4u qop[2];
     s = v16f{};
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
@@ -264,8 +260,17 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   // into LDS; block b + 3's records are on their way. One barrier per step; three
   // buffers.
   int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
+  fetch(b0, page);
+  // Q^T, on its way beside the first records.
+  v4u q_rest[kQLds];
+  {
+    const uint16_t* src = a.q + row_at * kQkDim + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
+#pragma unroll
+    for (int ks = 0; ks < kQLds; ++ks) q_rest[ks] = *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks));
+  }
   if (b1 > b0) {
-    fetch(b0, page);
 #pragma unroll
     for (int i = 0; i < 5; ++i) unpack(buf_of(b0) + store_lane, i);
     fetch(b0 + 1, page1);
@@ -273,6 +278,10 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     for (int i = 0; i < 5; ++i) unpack(buf_of(b0 + 1) + store_lane, i);
     fetch(b0 + 2, page2);
   }
+#pragma unroll
+  for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
+#pragma unroll
+  for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
   lds_barrier();
   if (active) {
     int b = b0;
@@ -280,23 +289,29 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     v4u p[2];
     float shift = 0.0f;
     auto no_slice = [](int) {};
+    Softener<E> softener;
+    constexpr int kPairs = 8, kTicks = kPairs + 2;
     auto soften = [&](const v16f& from, int i, int of) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 8 * i / of; u < 8 * (i + 1) / of; ++u)
-        p[u >> 2][u & 3] = probability_pair<E>(from[2 * u], from[2 * u + 1], a.scale_log2, shift, row.sum);
+      for (int u = kTicks * i / of; u < kTicks * (i + 1) / of; ++u)
+        softener.tick(u, kPairs, a.scale_log2, [&](int e) { return from[e]; }, &shift, [&](int w, uint32_t pair) {
+          p[w >> 2][w & 3] = pair;
+          row.sum = E::add_pair(pair, row.sum);
+        });
     };
     enum { kGo, kBreak, kDone };
+    uint32_t k_now = read_first_k(b);
     auto step = [&](const v16f& from, v16f& to) __attribute__((always_inline)) -> int {
       if (b + 1 == b1) return kDone;
       ++b;
       const int page3 = page_of(b + 2);
-      const uint32_t at = opaque_address(buf_of(b - 1) + v_lane);
+      const uint32_t at = opaque(buf_of(b - 1) + v_lane);
       v4u vop[kAhead];
-      scores(b, to, [&](int i) __attribute__((always_inline)) {
+      scores(k_now, to, [&](int i) __attribute__((always_inline)) {
         soften(from, i, kSteps);
         if (i >= kSteps - kAhead) vop[i - (kSteps - kAhead)] = read_v(at, i - (kSteps - kAhead));
       });
-      const uint32_t store = opaque_address(buf_of(b + 1) + store_lane);
+      const uint32_t store = opaque(buf_of(b + 1) + store_lane);
       float top = -__builtin_inff();
       values(at, vop, p, [&](int i) __attribute__((always_inline)) {
         if (i % 4 == 0 && i < 20) unpack(store, i / 4);
@@ -304,13 +319,15 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
         if (i >= 8 && i < 16) top = fmaxf(fmaxf(top, to[2 * (i - 8)]), to[2 * (i - 8) + 1]);
       });
       lds_barrier();
+      k_now = read_first_k(b + 1);
       const float mx = max_halves(top) * a.scale_log2;
       page = page1;
       page1 = page2;
       page2 = page3;
       return needs_mask(b, page) || __builtin_amdgcn_ballot_w64(must_raise(row, mx)) != 0 ? kBreak : kGo;
     };
-    scores(b, s, no_slice);
+    scores(k_now, s, no_slice);
+    k_now = read_first_k(b + 1);
     for (bool more = true; more;) {
       if (needs_mask(b, page)) mask(b, page, s);
       const float factor = raise(row, row_max(s, a.scale_log2));
@@ -334,7 +351,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
         }
       }
     }
-    const uint32_t at = opaque_address(buf_of(b) + v_lane);
+    const uint32_t at = opaque(buf_of(b) + v_lane);
     v4u vop[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);

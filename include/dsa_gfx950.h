@@ -517,8 +517,8 @@ int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slots, int wid
  * may run at the same time.
  */
 int dsa_prompt_attention_workspace_bytes(int64_t q_tokens, int64_t heads, int64_t kv_heads,
-                                         int64_t v_dim, int64_t sequences, int64_t max_k,
-                                         int64_t* bytes);
+                                         int64_t v_dim, int64_t sequences, int64_t k_tokens,
+                                         int64_t max_k, int64_t* bytes);
 int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
                          const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,

@@ -278,13 +278,13 @@ def test_rope_and_cache_abi():
 def test_workspace_queries():
     size = ctypes.c_int64()
     # Whole tiles for every CU: no split. One token over many keys: split.
-    _native.call("dsa_prompt_attention_workspace_bytes", 4096, 128, 128, 128, 1, 4096, ctypes.byref(size))
+    _native.call("dsa_prompt_attention_workspace_bytes", 4096, 128, 128, 128, 1, 4096, 4096, ctypes.byref(size))
     assert size.value == 0
-    _native.call("dsa_prompt_attention_workspace_bytes", 1, 8, 1, 128, 1, 65536, ctypes.byref(size))
+    _native.call("dsa_prompt_attention_workspace_bytes", 1, 8, 1, 128, 1, 65536, 65536, ctypes.byref(size))
     assert size.value > 0
     _native.call("dsa_shared_prefix_mla_workspace_bytes", 1, 128, 65536, 1, ctypes.byref(size))
     assert size.value > 0
-    for name, args in (("dsa_prompt_attention_workspace_bytes", (-1, 1, 1, 64, 1, 1)),
+    for name, args in (("dsa_prompt_attention_workspace_bytes", (-1, 1, 1, 64, 1, 1, 1)),
                        ("dsa_shared_prefix_mla_workspace_bytes", (1, 0, 1, 1))):
         with pytest.raises(ValueError, match="shape"):
             _native.call(name, *args, ctypes.byref(size))
