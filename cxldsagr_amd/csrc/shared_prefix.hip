@@ -48,7 +48,7 @@ constexpr int kBuffers = 3;
 constexpr int kSteps = kQkDim / 16, kDims = kVDim / 32;
 // Q^T operands of the last kQLds steps stay in LDS, the others in registers:
 // with all 36 there, O^T (256 registers of a lane) leaves too few for the rest.
-constexpr int kQLds = 12;
+constexpr int kQLds = 8;
 constexpr int kQReg = kSteps - kQLds;
 constexpr int kQBytes = kQLds * 4 * 1024;  // [wave][step][lane] 16 bytes
 
@@ -168,26 +168,35 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     if (b >= b1) return -1;
     return b < prefix_blocks ? a.prefix_table[b >> 1] : suffix_table[(b - prefix_blocks) >> 1];
   };
-  // Valid keys of block b on `page`, and its first record there.
+  // Valid keys of block b on `page`, and its half of the page.
+  const uint32_t pages = (uint32_t)a.pages;
   auto keys_of = [&](int b, int page) -> int {
-    if (page < 0 || page >= a.pages) return 0;
-    const int64_t left = b < prefix_blocks ? prefix - (int64_t)b * kBlockKeys
-                                           : suffix - (int64_t)(b - prefix_blocks) * kBlockKeys;
-    return (int)min(left, (int64_t)kBlockKeys);
+    const int left = b < prefix_blocks ? (int)prefix - b * kBlockKeys : (int)suffix - (b - prefix_blocks) * kBlockKeys;
+    return (uint32_t)page < pages ? min(left, kBlockKeys) : 0;
   };
-  auto half_of = [&](int b) -> int { return (b < prefix_blocks ? b : b - prefix_blocks) & 1; };
-  v4u st[6];
-  auto fetch = [&](int b, int page) __attribute__((always_inline)) {
-    const uint8_t* rec =
-        kk < keys_of(b, page) ? a.cache + ((int64_t)page * kPageTokens + half_of(b) * kBlockKeys + kk) * kRecordBytes
-                              : zero_record;
+  typedef v4u Staged[6];
+  const uint32_t fetch_lane = (uint32_t)kk * kRecordBytes + 16 * j8;
+  const uint32_t scale_lane = (uint32_t)kk * kRecordBytes + kVDim;
+  auto fetch = [&](Staged& st, int b, int page) __attribute__((always_inline)) {
+    const int keys = keys_of(b, page);
+    const int half = (b < prefix_blocks ? b : b - prefix_blocks) & 1;
+    // (A block without keys is on no page; its address is not used.)
+    const uint8_t* from = a.cache + (keys > 0 ? ((int64_t)page * kPageTokens + half * kBlockKeys) * kRecordBytes : 0);
+    if (keys == kBlockKeys) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(rec + 128 * i + 16 * j8);
-    st[4] = *reinterpret_cast<const v4u*>(rec + kVDim);
-    st[5] = *reinterpret_cast<const v4u*>(rec + kVDim + 16 + 16 * j8);
+      for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(from + (fetch_lane + 128 * i));
+      st[4] = *reinterpret_cast<const v4u*>(from + scale_lane);
+      st[5] = *reinterpret_cast<const v4u*>(from + (fetch_lane + (kVDim + 16)));
+    } else {
+      const uint8_t* rec = kk < keys ? from + kk * kRecordBytes : zero_record;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(rec + 128 * i + 16 * j8);
+      st[4] = *reinterpret_cast<const v4u*>(rec + kVDim);
+      st[5] = *reinterpret_cast<const v4u*>(rec + kVDim + 16 + 16 * j8);
+    }
   };
   // Chunk i of the landed record (4: the RoPE part) as bf16 into the block's row.
-  auto unpack = [&](uint32_t to, int i) __attribute__((always_inline)) {
+  auto unpack = [&](const Staged& st, uint32_t to, int i) __attribute__((always_inline)) {
     if (i == 4) {
       lds_store<v4u>(to + 2 * kVDim - 16 * j8, st[5]);
       return;
@@ -200,7 +209,10 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
                                           dequant_pair<false>(w.w, scale), dequant_pair<true>(w.w, scale)});
   };
   const uint32_t store_lane = (uint32_t)kk * kRowBytes + 32 * j8;
-  auto buf_of = [&](int b) -> uint32_t { return lds_base + (uint32_t)(b % kBuffers) * kBufBytes; };
+  // Buffers go round: the one after `at` (an address within it).
+  auto after = [&](uint32_t at) -> uint32_t {
+    return at + kBufBytes >= lds_base + kBuffers * kBufBytes ? at + kBufBytes - kBuffers * kBufBytes : at + kBufBytes;
+  };
 
   v16f o[kDims];
 #pragma unroll
@@ -220,8 +232,8 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     return v4u{lo.x, lo.y, hi.x, hi.y};
   };
   v4u kop[kAhead];
-  auto read_first_k = [&](int b) __attribute__((always_inline)) -> uint32_t {
-    const uint32_t at = opaque(buf_of(b) + k_lane);
+  auto read_first_k = [&](uint32_t buffer) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t at = opaque(buffer + k_lane);
 #pragma unroll
     for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at + 32 * ks);
     return at;
@@ -260,28 +272,28 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   // into LDS; block b + 3's records are on their way. One barrier per step; three
   // buffers.
   int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
-  fetch(b0, page);
-  // Q^T, on its way beside the first records.
-  v4u q_rest[kQLds];
+  Staged st;
   {
+    // The first two blocks and Q^T on their way together.
+    Staged first;
+    fetch(first, b0, page);
+    fetch(st, b0 + 1, page1);
     const uint16_t* src = a.q + row_at * kQkDim + 8 * h;
+    v4u q_rest[kQLds];
 #pragma unroll
     for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
 #pragma unroll
     for (int ks = 0; ks < kQLds; ++ks) q_rest[ks] = *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks));
-  }
-  if (b1 > b0) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) unpack(buf_of(b0) + store_lane, i);
-    fetch(b0 + 1, page1);
+    for (int i = 0; i < 5; ++i) unpack(first, lds_base + store_lane, i);
 #pragma unroll
-    for (int i = 0; i < 5; ++i) unpack(buf_of(b0 + 1) + store_lane, i);
-    fetch(b0 + 2, page2);
+    for (int i = 0; i < 5; ++i) unpack(st, lds_base + kBufBytes + store_lane, i);
+    fetch(st, b0 + 2, page2);
+#pragma unroll
+    for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
   }
 #pragma unroll
   for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
-#pragma unroll
-  for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
   lds_barrier();
   if (active) {
     int b = b0;
@@ -300,26 +312,29 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
         });
     };
     enum { kGo, kBreak, kDone };
-    uint32_t k_now = read_first_k(b);
+    uint32_t now = lds_base;  // block b's buffer
+    uint32_t k_now = read_first_k(now);
     auto step = [&](const v16f& from, v16f& to) __attribute__((always_inline)) -> int {
       if (b + 1 == b1) return kDone;
       ++b;
       const int page3 = page_of(b + 2);
-      const uint32_t at = opaque(buf_of(b - 1) + v_lane);
+      const uint32_t at = opaque(now + v_lane);
+      now = after(now);
       v4u vop[kAhead];
       scores(k_now, to, [&](int i) __attribute__((always_inline)) {
         soften(from, i, kSteps);
         if (i >= kSteps - kAhead) vop[i - (kSteps - kAhead)] = read_v(at, i - (kSteps - kAhead));
       });
-      const uint32_t store = opaque(buf_of(b + 1) + store_lane);
+      const uint32_t ahead = after(now);
+      const uint32_t store = opaque(ahead + store_lane);
       float top = -__builtin_inff();
       values(at, vop, p, [&](int i) __attribute__((always_inline)) {
-        if (i % 4 == 0 && i < 20) unpack(store, i / 4);
-        if (i == 20) fetch(b + 2, page3);
+        if (i % 4 == 0 && i < 20) unpack(st, store, i / 4);
+        if (i == 20) fetch(st, b + 2, page3);
         if (i >= 8 && i < 16) top = fmaxf(fmaxf(top, to[2 * (i - 8)]), to[2 * (i - 8) + 1]);
       });
       lds_barrier();
-      k_now = read_first_k(b + 1);
+      k_now = read_first_k(ahead);
       const float mx = max_halves(top) * a.scale_log2;
       page = page1;
       page1 = page2;
@@ -327,7 +342,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
       return needs_mask(b, page) || __builtin_amdgcn_ballot_w64(must_raise(row, mx)) != 0 ? kBreak : kGo;
     };
     scores(k_now, s, no_slice);
-    k_now = read_first_k(b + 1);
+    k_now = read_first_k(after(now));
     for (bool more = true; more;) {
       if (needs_mask(b, page)) mask(b, page, s);
       const float factor = raise(row, row_max(s, a.scale_log2));
@@ -351,7 +366,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
         }
       }
     }
-    const uint32_t at = opaque(buf_of(b) + v_lane);
+    const uint32_t at = opaque(now + v_lane);
     v4u vop[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);
@@ -359,12 +374,12 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     values(at, vop, p, no_slice);
   } else {
     // A wave without rows stages its keys all the same.
-    for (int b = b0 + 1; b < b1; ++b) {
+    uint32_t to = lds_base + 2 * kBufBytes;
+    for (int b = b0 + 1; b < b1; ++b, to = after(to)) {
       const int page3 = page_of(b + 2);
-      const uint32_t store = buf_of(b + 1) + store_lane;
 #pragma unroll
-      for (int i = 0; i < 5; ++i) unpack(store, i);
-      fetch(b + 2, page3);
+      for (int i = 0; i < 5; ++i) unpack(st, to + store_lane, i);
+      fetch(st, b + 2, page3);
       lds_barrier();
     }
   }
@@ -401,26 +416,11 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     }
 }
 
-// Key splits of `tiles` row tiles over `blocks` blocks of 32 keys: the count of
-// least time, by the rounds of work-groups (one per CU), their fixed part and their
-// steps, and what a part costs to write and read again.
-constexpr double kFixedUs = 14.0, kStepUs = 1.7, kPartUsPerRow = 0.001;
-
-int best_splits(int64_t tiles, int64_t blocks, int64_t rows, int64_t cus) {
-  int best = 1;
-  double least = 1e30;
-  for (int64_t s = 1; s <= 256 && s <= (blocks > 1 ? blocks : 1); ++s) {
-    const double rounds = (double)((tiles * s + cus - 1) / cus);
-    const double us = rounds * (kFixedUs + kStepUs * (double)((blocks + s - 1) / s)) +
-                      (s > 1 ? 4.0 + kPartUsPerRow * (double)(rows * s) : 0.0);
-    if (us < least) {
-      least = us;
-      best = (int)s;
-    }
-    if (rounds > 8) break;
-  }
-  return best;
-}
+// Key splits: the count of least time, by the rounds of work-groups (one per CU),
+// their fixed part (Q, the first records, the stores), the steps of the longest, and
+// what reading a row's parts again costs. Fitted to one token over 32,896 keys (s =
+// 114 .. 257) and 31 tokens of 64 heads over 4,099.
+constexpr double kFixedUs = 13.0, kStepUs = 2.0, kJoinUs = 3.0, kPartUsPerRow = 0.0005;
 
 struct PrefixPlan {
   bool joint;
@@ -434,10 +434,45 @@ PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t su
   const int64_t prefix_blocks = (prefix + kBlockKeys - 1) / kBlockKeys;
   const int64_t suffix_blocks = suffix_pages * (kPageTokens / kBlockKeys);
   p.joint = heads % kTileRows == 0;
-  if (p.joint || prefix > 0)
-    p.splits = best_splits((rows + kTileRows - 1) / kTileRows, prefix_blocks + (p.joint ? suffix_blocks : 0), rows, cus);
-  if (!p.joint && (suffix_pages > 0 || prefix == 0))
-    p.suffix_splits = best_splits(tokens * ((heads + kTileRows - 1) / kTileRows), suffix_blocks, rows, cus);
+  // Work-groups and blocks of a split of the first kind of items, and of the
+  // suffix's own.
+  const int64_t tiles = (rows + kTileRows - 1) / kTileRows;
+  const int64_t blocks = p.joint ? prefix_blocks + suffix_blocks : prefix_blocks;
+  const int64_t own_tiles = tokens * ((heads + kTileRows - 1) / kTileRows);
+  const bool first = p.joint || prefix > 0, own = !p.joint && (suffix_pages > 0 || prefix == 0);
+  double least = 1e30;
+  for (int64_t ss = own ? 1 : 0; ss <= (own ? 64 : 0) && (ss <= 1 || ss <= suffix_blocks); ss *= 2) {
+    static constexpr int kSteps1[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
+    for (int64_t r = 0; r <= 12 + 10; ++r) {
+      // One; or as many as some rounds hold, with or without the suffix's own items;
+      // or splits of a few blocks: at most one per block, and no more than give the
+      // same longest split.
+      int64_t s = first ? 1 : 0;
+      if (first && r > 0) {
+        s = r > 12 ? (blocks + kSteps1[r - 13] - 1) / kSteps1[r - 13]
+                   : r % 2 ? (r + 1) / 2 * cus / tiles : (r / 2 * cus - own_tiles * ss) / tiles;
+        if (s > 256) s = 256;
+        if (s > blocks) s = blocks;
+        if (s < 1) continue;
+        s = (blocks + (blocks + s - 1) / s - 1) / ((blocks + s - 1) / s);
+      }
+      // Rounds of the first kind, and of the suffix's own items, which come last, as
+      // far as the last of those rounds has no room for them.
+      const int64_t full = (tiles * s + cus - 1) / cus, room = full * cus - tiles * s;
+      const int64_t over = own_tiles * ss > room ? (own_tiles * ss - room + cus - 1) / cus : 0;
+      const double step = s > 0 ? kFixedUs + kStepUs * (double)((blocks + s - 1) / s) : 0.0;
+      const double own_step = ss > 0 ? kFixedUs + kStepUs * (double)((suffix_blocks + ss - 1) / ss) : 0.0;
+      double us = (double)full * step + (double)over * own_step;
+      if (us < own_step) us = own_step;
+      if (s + ss > 1) us += kJoinUs + kPartUsPerRow * (double)(rows * (s + ss));
+      if (us < least) {
+        least = us;
+        p.splits = s;
+        p.suffix_splits = ss;
+      }
+    }
+    if (ss == 0) break;
+  }
   const int64_t parts = p.splits + p.suffix_splits;
   if (parts > 1) {
     p.stats_at = parts * rows * kVDim * 4;
