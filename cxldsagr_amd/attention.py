@@ -239,9 +239,9 @@ def pack_kv_fp8(kv, kv_cache, page_table, token_offset=0, status=None):
 
 def _check_slots(slots, tokens, device):
     if (not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int32, torch.int64)
-            or tuple(slots.shape) != (tokens,) or slots.device != device):
+            or slots.shape != (tokens,) or slots.device != device):
         raise ValueError("slots must be int32 or int64 [tokens] on the cache device")
-    return slots.contiguous()
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
 def _check_cache(cache, device):
@@ -275,44 +275,41 @@ def write_kv_fp8(kv, kv_cache, slots, *, norm_weight=None, eps=1e-6, positions=N
     """
     if kv.ndim != 2 or kv.shape[1] != QK_DIM or kv.dtype != torch.bfloat16:
         raise ValueError("kv must be bf16 [tokens, 576]")
-    tokens = kv.shape[0]
-    _check_cache(kv_cache, kv.device)
-    slots = _check_slots(slots, tokens, kv.device)
-    _check_status(status, kv.device)
+    tokens, device = kv.shape[0], kv.device
+    _check_cache(kv_cache, device)
+    slots = _check_slots(slots, tokens, device)
+    _check_status(status, device)
     if not math.isfinite(eps) or eps < 0 or not math.isfinite(magnitude):
         raise ValueError("eps must be finite and nonnegative, magnitude finite")
     if norm_weight is not None:
-        if (norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (V_DIM,)
-                or norm_weight.device != kv.device):
+        if (norm_weight.dtype != torch.float32 or norm_weight.shape != (V_DIM,)
+                or norm_weight.device != device):
             raise ValueError("norm_weight must be FP32 [512] on the cache device")
         norm_weight = _aligned(norm_weight)
     if (positions is None) != (frequencies is None):
         raise ValueError("a rotation needs positions and frequencies")
     if positions is not None:
-        if (positions.dtype not in (torch.int32, torch.int64)
-                or tuple(positions.shape) != (tokens,) or positions.device != kv.device):
+        if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,)
+                or positions.device != device):
             raise ValueError("positions must be int32 or int64 [tokens] on the cache device")
         if (frequencies.dtype != torch.float32
-                or tuple(frequencies.shape) != ((QK_DIM - V_DIM) // 2,)
-                or frequencies.device != kv.device):
+                or frequencies.shape != ((QK_DIM - V_DIM) // 2,) or frequencies.device != device):
             raise ValueError("frequencies must be FP32 [32] on the cache device")
         positions, frequencies = positions.contiguous(), frequencies.contiguous()
-    _native.require_gfx950(kv.device, "fp8 KV write")
+    _native.require_gfx950(device, "fp8 KV write")
     if tokens == 0:
         return kv_cache
-    if kv.stride(1) != 1 or kv.stride(0) % 8 or kv.stride(0) < 0 or kv.data_ptr() % 16:
+    stride, unit = kv.stride()
+    if unit != 1 or stride % 8 or stride < 0 or kv.data_ptr() % 16:
         kv = kv.clone(memory_format=torch.contiguous_format)
-    with _native.on_device(kv.device):
+        stride = QK_DIM
+    with _native.on_device(device):
         _native.call(
-            "dsa_kv_write_fp8",
-            kv.data_ptr(), kv.stride(0), tokens, slots.data_ptr(), int(slots.dtype == torch.int64),
-            _native.ptr(norm_weight), float(eps),
-            _native.ptr(positions),
-            int(positions is not None and positions.dtype == torch.int64),
-            _native.ptr(frequencies), float(magnitude), int(interleaved),
-            kv_cache.shape[0], kv_cache.data_ptr(), _native.ptr(status),
-            _native.raw_stream(kv.device),
-        )
+            "dsa_kv_write_fp8", kv.data_ptr(), stride, tokens, slots.data_ptr(),
+            slots.dtype == torch.int64, _native.ptr(norm_weight), eps, _native.ptr(positions),
+            positions is not None and positions.dtype == torch.int64, _native.ptr(frequencies),
+            magnitude, bool(interleaved), kv_cache.shape[0], kv_cache.data_ptr(),
+            _native.ptr(status), _native.raw_stream(device))
     return kv_cache
 
 
@@ -344,7 +341,7 @@ def read_kv_fp8(kv_cache, slots, *, out=None, status=None):
         return out
     with _native.on_device(device):
         _native.call("dsa_kv_read_fp8", kv_cache.data_ptr(), kv_cache.shape[0], slots.data_ptr(),
-                     int(slots.dtype == torch.int64), tokens, out.data_ptr(), _native.ptr(status),
+                     slots.dtype == torch.int64, tokens, out.data_ptr(), _native.ptr(status),
                      _native.raw_stream(device))
     return out
 
@@ -356,17 +353,19 @@ def _check_starts(starts, device, what):
     if (not isinstance(starts, torch.Tensor) or starts.dtype != torch.int32 or starts.ndim != 1
             or starts.numel() < 1 or starts.device != device):
         raise ValueError(f"{what} must be int32 [sequences + 1] on the query device")
-    return starts.contiguous()
+    return starts if starts.is_contiguous() else starts.contiguous()
 
 
 def _heads_layout(tensor):
     """``tensor`` [tokens, heads, dim] as the kernels read it: the last dim
     contiguous, the other strides multiples of 16 bytes, aligned; else a copy."""
     token, head, dim = tensor.stride()
+    address = tensor.data_ptr()
     if (dim != 1 or token % 8 or head % 8 or not 0 <= token < 1 << 25 or not 0 <= head < 1 << 25
-            or tensor.data_ptr() % 16):
-        return tensor.clone(memory_format=torch.contiguous_format)
-    return tensor
+            or address % 16):
+        tensor = tensor.clone(memory_format=torch.contiguous_format)
+        return tensor, tensor.data_ptr(), *tensor.stride()[:2]
+    return tensor, address, token, head
 
 
 def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None, out=None):
@@ -390,53 +389,54 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
     """
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError("Expected q [Tq,H,Dqk], k [Tk,Hkv,Dqk], and v [Tk,Hkv,Dv]")
-    if k.shape[:2] != v.shape[:2] or q.shape[2] != k.shape[2]:
+    q_tokens, heads, qk_dim = q.shape
+    k_tokens, kv_heads, v_dim = v.shape
+    if k.shape != (k_tokens, kv_heads, qk_dim):
         raise ValueError("Query, key, and value dimensions do not agree")
-    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1]:
+    if not heads or not kv_heads or heads % kv_heads:
         raise ValueError("q's heads must be a positive multiple of k's")
-    if (q.shape[2], v.shape[2]) not in PROMPT_HEAD_DIMS:
+    if (qk_dim, v_dim) not in PROMPT_HEAD_DIMS:
         raise ValueError(f"(Dqk, Dv) must be one of {PROMPT_HEAD_DIMS}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype, device = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise ValueError("q, k, and v must share bf16 or fp16")
-    if k.device != q.device or v.device != q.device:
+    if k.device != device or v.device != device:
         raise ValueError("q, k, and v must be on the same device")
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be positive and finite")
     if max_k is not None and (type(max_k) is not int or max_k < 0):
         raise ValueError("max_k must be a nonnegative integer")
-    if any(t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError("prompt attention has no backward pass")
-    cu_q = _check_starts(cu_q, q.device, "cu_q")
-    cu_k = cu_q if cu_k is None else _check_starts(cu_k, q.device, "cu_k")
-    if cu_k.numel() != cu_q.numel():
+    cu_q = _check_starts(cu_q, device, "cu_q")
+    cu_k = cu_q if cu_k is None else _check_starts(cu_k, device, "cu_k")
+    sequences = cu_q.numel() - 1
+    if cu_k.numel() != sequences + 1:
         raise ValueError("cu_q and cu_k must describe the same sequences")
-    _native.require_gfx950(q.device, "prompt attention")
-    shape = (*q.shape[:2], v.shape[2])
+    _native.require_gfx950(device, "prompt attention")
+    shape = (q_tokens, heads, v_dim)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != q.dtype
-          or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != dtype
+          or out.device != device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned [Tq, H, Dv] tensor of q's "
                          "dtype on q's device")
-    sequences = cu_q.numel() - 1
-    if not q.shape[0] or not sequences:
+    if not q_tokens or not sequences:
         return out
-    max_k = k.shape[0] if max_k is None else min(max_k, k.shape[0])
-    q, k, v = _heads_layout(q), _heads_layout(k), _heads_layout(v)
-    with _native.on_device(q.device):
-        needed = _native.size_of("dsa_prompt_attention_workspace_bytes", q.device.index,
-                                 q.shape[0], q.shape[1], k.shape[1], v.shape[2], sequences,
-                                 k.shape[0], max_k)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
+    max_k = k_tokens if max_k is None else min(max_k, k_tokens)
+    # (The tensors are kept until the call: they may be copies.)
+    q, *q_at = _heads_layout(q)
+    k, *k_at = _heads_layout(k)
+    v, *v_at = _heads_layout(v)
+    with _native.on_device(device):
+        needed = _native.size_of("dsa_prompt_attention_workspace_bytes", device.index, q_tokens,
+                                 heads, kv_heads, v_dim, sequences, k_tokens, max_k)
+        workspace = torch.empty(needed, dtype=torch.uint8, device=device) if needed else None
         _native.call(
-            "dsa_prompt_attention",
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), _native.DTYPE_CODES[q.dtype],
-            q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-            cu_q.data_ptr(), cu_k.data_ptr(), sequences, q.shape[0], k.shape[0], max_k,
-            float(scale), int(causal), out.data_ptr(), _native.ptr(workspace), needed,
-            _native.raw_stream(q.device),
-        )
+            "dsa_prompt_attention", *q_at, *k_at, *v_at, _native.DTYPE_CODES[dtype], heads,
+            kv_heads, qk_dim, v_dim, cu_q.data_ptr(), cu_k.data_ptr(), sequences, q_tokens,
+            k_tokens, max_k, scale, bool(causal), out.data_ptr(), _native.ptr(workspace), needed,
+            _native.raw_stream(device))
     return out
 
 

@@ -623,81 +623,132 @@ struct WriteArgs {
   int32_t* status;
 };
 
+// Reductions within 16 lanes by lane moves (xor 1 and 2 in a quad, the other quad of
+// eight, the other eight), then over the four rows.
+template <typename Op>
+__device__ __forceinline__ uint32_t reduce_16(uint32_t v, Op op) {
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t add_bits(uint32_t x, uint32_t y) {
+  return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+}
+__device__ __forceinline__ float sum_64(float f) {
+  uint32_t v = reduce_16(__float_as_uint(f), add_bits);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = add_bits(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __uint_as_float(add_bits(b[0], b[1]));
+}
+
 // New tokens into any slots of the fp8 paged cache: the latent through RMSNorm
 // (fp32, x * rsqrt(mean x^2 + eps) * w, rounded to bf16, which is what a model's
 // norm hands on), the RoPE part rotated (fp32, rounded to bf16), then the record of
-// pack_tokens. One wave per token, lane l with 8 latent values; lanes 0 .. 31 have
-// a rotary pair each. Bound by memory: 1,152 B read and 656 B written per token.
+// pack_tokens. A wave takes kTokens tokens whose loads are all issued first: lane l
+// has 8 latent values of each, and a half wave the 32 rotary pairs of every other
+// one. Bound by memory, 1,152 B read and 656 B written per token, once enough loads
+// are in flight: 65,536 tokens took 35.6 us (3.3 TB/s) with one token per wave and
+// reductions through LDS permutes.
+template <int kTokens>
 __global__ __launch_bounds__(256) void write_kv(const WriteArgs a) {
-  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t token0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kTokens;
   const int lane = threadIdx.x & 63;
-  if (token >= a.tokens) return;
-  const int64_t slot = a.wide_slots ? static_cast<const int64_t*>(a.slots)[token]
-                                    : static_cast<const int32_t*>(a.slots)[token];
-  if (slot < 0) return;  // padding
-  if (slot >= a.rows) {
-    if (lane == 0 && a.status) atomicOr(a.status, 1);
-    return;
-  }
-  uint8_t* rec = a.cache + slot * 656;
-  const uint16_t* src = a.kv + token * a.kv_stride;
-  const uint4 raw = *reinterpret_cast<const uint4*>(src + lane * 8);
-  const int pair = lane & 31;
-  uint32_t ra, rb;  // the pair's bf16 bits
-  if (a.interleaved) {
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(src + 512 + 2 * pair);
-    ra = word & 0xFFFFu;
-    rb = word >> 16;
-  } else {
-    ra = src[512 + pair];
-    rb = src[544 + pair];
-  }
-  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-  float v[8];
+  if (token0 >= a.tokens) return;
+  constexpr int kTurns = (kTokens + 1) / 2;
+  const int pair = lane & 31, half = lane >> 5;
+  uint4 raw[kTokens];
+  int64_t slot[kTokens], turn_slot[kTurns], position[kTurns];
+  uint32_t ra[kTurns], rb[kTurns];  // the pairs' bf16 bits
+  // A token that is not written (past the end or without a slot) has slot -1; one
+  // past the end reads the last token's row.
+  auto slot_of = [&](int64_t token) -> int64_t {
+    if (token >= a.tokens) return -1;
+    return a.wide_slots ? static_cast<const int64_t*>(a.slots)[token] : static_cast<const int32_t*>(a.slots)[token];
+  };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = bf16_to_f32(words[i] & 0xFFFFu);
-    v[2 * i + 1] = bf16_to_f32(words[i] >> 16);
+  for (int t = 0; t < kTokens; ++t) {
+    const int64_t token = token0 + t;
+    slot[t] = slot_of(token);
+    raw[t] = *reinterpret_cast<const uint4*>(a.kv + (token < a.tokens ? token : a.tokens - 1) * a.kv_stride + lane * 8);
   }
-  if (a.norm_weight != nullptr) {
-    const float4 w0 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane);
-    const float4 w1 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane + 4);
-    const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
-#pragma unroll
-    for (int offset = 32; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset, 64);
-    const float norm = 1.0f / __builtin_sqrtf(sum * (1.0f / 512.0f) + a.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(f32_to_bf16(v[i] * norm * w[i]));
-  }
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-    m = m > bits ? m : bits;
-  }
-  m = max_abs_bits_reduce<16>(m);
-  const float scale = scale_from_amax_bits(m, true);
-  uint32_t lo, hi;
-  quantize_eight(v, scale, true, lo, hi);
-  *reinterpret_cast<uint2*>(rec + lane * 8) = make_uint2(lo, hi);
-  if ((lane & 15) == 0) *reinterpret_cast<float*>(rec + 512 + 4 * (lane >> 4)) = scale;
-  if (lane < 32) {
-    if (a.positions != nullptr) {
-      const float2 cs = rotary_core::turn(rotary_core::position_at(a.positions, a.wide_positions, token),
-                                          a.frequencies[pair], a.magnitude);
-      const float x = bf16_to_f32(ra), y = bf16_to_f32(rb);
-      ra = f32_to_bf16(x * cs.x - y * cs.y);
-      rb = f32_to_bf16(y * cs.x + x * cs.y);
-    }
-    uint16_t* rope = reinterpret_cast<uint16_t*>(rec + 528);
+  for (int u = 0; u < kTurns; ++u) {
+    const int64_t token = token0 + 2 * u + half, row = token < a.tokens ? token : a.tokens - 1;
+    const uint16_t* src = a.kv + row * a.kv_stride + 512;
+    turn_slot[u] = kTokens == 1 && half ? -1 : slot_of(token);
+    position[u] = a.positions != nullptr ? rotary_core::position_at(a.positions, a.wide_positions, row) : 0;
     if (a.interleaved) {
-      *reinterpret_cast<uint32_t*>(rope + 2 * pair) = ra | (rb << 16);
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(src + 2 * pair);
+      ra[u] = word & 0xFFFFu;
+      rb[u] = word >> 16;
     } else {
-      rope[pair] = (uint16_t)ra;
-      rope[32 + pair] = (uint16_t)rb;
+      ra[u] = src[pair];
+      rb[u] = src[32 + pair];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) {
+    const uint32_t words[4] = {raw[t].x, raw[t].y, raw[t].z, raw[t].w};
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf16_to_f32(words[i] & 0xFFFFu);
+      v[2 * i + 1] = bf16_to_f32(words[i] >> 16);
+    }
+    if (a.norm_weight != nullptr) {
+      const float4 w0 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane);
+      const float4 w1 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane + 4);
+      const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
+      const float norm = 1.0f / __builtin_sqrtf(sum_64(sum) * (1.0f / 512.0f) + a.eps);
+      // Rounded to nearest even by v_cvt_pk_bf16_f32 (a NaN stays one).
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+        typedef float Two __attribute__((ext_vector_type(2)));
+        const uint32_t two = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector((Two){v[2 * i] * norm * w[2 * i], v[2 * i + 1] * norm * w[2 * i + 1]}, Pair));
+        v[2 * i] = bf16_to_f32(two & 0xFFFFu);
+        v[2 * i + 1] = bf16_to_f32(two >> 16);
+      }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+      m = m > bits ? m : bits;
+    }
+    m = reduce_16(m, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+    const float scale = scale_from_amax_bits(m, true);
+    uint32_t lo, hi;
+    quantize_eight(v, scale, true, lo, hi);
+    if (slot[t] < 0 || slot[t] >= a.rows) {
+      if (slot[t] >= a.rows && lane == 0 && a.status) atomicOr(a.status, 1);
+      continue;
+    }
+    uint8_t* rec = a.cache + slot[t] * 656;
+    *reinterpret_cast<uint2*>(rec + lane * 8) = make_uint2(lo, hi);
+    if ((lane & 15) == 0) *reinterpret_cast<float*>(rec + 512 + 4 * (lane >> 4)) = scale;
+  }
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    if (a.positions != nullptr) {
+      const float2 cs = rotary_core::turn(position[u], a.frequencies[pair], a.magnitude);
+      const float x = bf16_to_f32(ra[u]), y = bf16_to_f32(rb[u]);
+      ra[u] = rotary_core::to_bf16(x * cs.x - y * cs.y);
+      rb[u] = rotary_core::to_bf16(y * cs.x + x * cs.y);
+    }
+    if (turn_slot[u] < 0 || turn_slot[u] >= a.rows) continue;
+    uint16_t* rope = reinterpret_cast<uint16_t*>(a.cache + turn_slot[u] * 656 + 528);
+    if (a.interleaved) {
+      *reinterpret_cast<uint32_t*>(rope + 2 * pair) = ra[u] | (rb[u] << 16);
+    } else {
+      rope[pair] = (uint16_t)ra[u];
+      rope[32 + pair] = (uint16_t)rb[u];
     }
   }
 }
@@ -758,7 +809,12 @@ extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t token
   const WriteArgs a{static_cast<const uint16_t*>(kv), kv_stride, tokens, pages * 64, slots, norm_weight, norm_eps,
                     positions, frequencies, magnitude, wide_slots != 0, wide_positions != 0, interleaved != 0,
                     static_cast<uint8_t*>(cache), status};
-  hipLaunchKernelGGL(write_kv, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, stream, a);
+  // One token per wave while waves are few, then two (65,536 tokens: one 29.6 us, two
+  // 26.9, four 30.4).
+  if (tokens <= 4096)
+    hipLaunchKernelGGL(write_kv<1>, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(write_kv<2>, dim3((unsigned)((tokens + 7) / 8)), dim3(256), 0, stream, a);
   DSA_CHECK_LAUNCH("fp8 KV write");
   return kOk;
 }

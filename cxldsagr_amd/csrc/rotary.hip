@@ -6,9 +6,12 @@
 // head are copied (or left, in place).
 //
 // Bound by memory: each value is read and written once. A work-group takes some
-// tokens (or a part of one token's heads), forms their cosines and sines once in
-// LDS (64-bit angles, shared by all heads), and then walks items of eight pairs,
-// two 16-byte vectors of 16-bit values, four items in flight per thread.
+// tokens (or a part of one token's heads) in items of eight pairs, two 16-byte
+// vectors of 16-bit values, one per thread (two or four of them were no faster in
+// 8,192 tokens of 128 heads, 55 us or 4.9 TB/s, and slower in small calls: 1,023
+// fp32 tokens 17.6 us, with four 20.0); while they are on their way it forms the
+// tokens' cosines and sines in LDS (64-bit angles, once for all heads; 16 tokens 6.6
+// -> 3.4 us against forming them first).
 // Types, offsets or strides that do not allow vectors take one pair at a time.
 #include "rotary_core.h"
 #include "../../include/dsa_gfx950.h"
@@ -17,9 +20,7 @@ namespace dsa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;              // in flight per thread
 constexpr int kTableEntries = 2048;    // (cos, sin) of a work-group
-constexpr int kGroupItems = kThreads * kItems;
 
 struct RopeSide {
   const void* in;
@@ -46,7 +47,7 @@ __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 template <>
-__device__ __forceinline__ uint16_t from_f32(float v) { return (uint16_t)f32_to_bf16(v); }
+__device__ __forceinline__ uint16_t from_f32(float v) { return (uint16_t)rotary_core::to_bf16(v); }
 
 // A vector of 8 elements, aligned to 16 bytes.
 template <typename T>
@@ -64,15 +65,6 @@ __global__ __launch_bounds__(kThreads) void rope_pair(const RopeArgs a) {
   const int64_t group = blockIdx.x - (second ? a.side[0].groups : 0);
   const int64_t token0 = group / side.groups_per_token * side.tokens_per_group;
   const int tokens = (int)min((int64_t)side.tokens_per_group, a.tokens - token0);
-  for (int e = threadIdx.x; e < tokens * a.half; e += kThreads) {
-    const int t = e / a.half;
-    float2 cs = rotary_core::turn(rotary_core::position_at(a.positions, a.wide_positions, token0 + t),
-                                  a.frequencies[e - t * a.half], a.magnitude);
-    cs.y *= a.sign;
-    table[e] = cs;
-  }
-  __syncthreads();
-
   constexpr int kPairs = kVector ? 8 : 1;
   constexpr int kSpan = kVector ? 8 : 1;
   const int turned = a.half / kPairs;                              // items that rotate, per head
@@ -81,83 +73,87 @@ __global__ __launch_bounds__(kThreads) void rope_pair(const RopeArgs a) {
   const int per_token = side.heads * per_head;
   // A part of one token's items, or all items of some tokens.
   const int part = (int)(group % side.groups_per_token);
-  const int begin = part * kGroupItems;
-  const int end = side.groups_per_token > 1 ? min(begin + kGroupItems, per_token) : tokens * per_token;
-  for (int base = begin; base < end; base += kGroupItems) {
-    T x[kItems][2 * kSpan];
-    T* to[kItems][2];
-    int pair[kItems];  // table entry of the first pair, -1: copied
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int item = base + i * kThreads + (int)threadIdx.x;
-      to[i][0] = nullptr;
-      if (item >= end) continue;
-      const int t = side.groups_per_token > 1 ? 0 : item / per_token;
-      const int rest = item - t * per_token;
-      const int head = rest / per_head, unit = rest - head * per_head;
-      int at0, at1;  // the two vectors' dims
-      if (unit < turned) {
-        pair[i] = t * a.half + unit * kPairs;
-        at0 = a.offset + (a.interleaved ? 2 * unit * kSpan : unit * kSpan);
-        at1 = at0 + (a.interleaved ? kSpan : a.half);
-      } else {
-        pair[i] = -1;
-        at0 = (unit - turned) * 2 * kSpan;
-        at1 = at0 + kSpan;
-        if (at0 >= a.offset) at0 += 2 * a.half;
-        if (at1 >= a.offset) at1 += 2 * a.half;
-      }
-      const T* in = static_cast<const T*>(side.in) + (token0 + t) * side.in_token + head * side.in_head;
-      T* out = static_cast<T*>(side.out) + (token0 + t) * side.out_token + head * side.out_head;
-      to[i][0] = out + at0;
-      to[i][1] = out + at1;
-      if constexpr (kVector) {
-        *reinterpret_cast<Eight<T>*>(&x[i][0]) = *reinterpret_cast<const Eight<T>*>(in + at0);
-        *reinterpret_cast<Eight<T>*>(&x[i][kSpan]) = *reinterpret_cast<const Eight<T>*>(in + at1);
-      } else {
-        x[i][0] = in[at0];
-        x[i][1] = in[at1];
-      }
+  const int begin = part * kThreads;
+  const int end = side.groups_per_token > 1 ? min(begin + kThreads, per_token) : tokens * per_token;
+  const int item = begin + (int)threadIdx.x;
+  const bool mine = item < end;
+  T x[2 * kSpan];
+  T *to0 = nullptr, *to1 = nullptr;
+  int pair = -1;  // table entry of the item's first pair, -1: copied
+  if (mine) {
+    const int t = side.groups_per_token > 1 ? 0 : item / per_token;
+    const int rest = item - t * per_token;
+    const int head = rest / per_head, unit = rest - head * per_head;
+    int at0, at1;  // the two vectors' dims
+    if (unit < turned) {
+      pair = t * a.half + unit * kPairs;
+      at0 = a.offset + (a.interleaved ? 2 * unit * kSpan : unit * kSpan);
+      at1 = at0 + (a.interleaved ? kSpan : a.half);
+    } else {
+      at0 = (unit - turned) * 2 * kSpan;
+      at1 = at0 + kSpan;
+      if (at0 >= a.offset) at0 += 2 * a.half;
+      if (at1 >= a.offset) at1 += 2 * a.half;
     }
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      if (to[i][0] == nullptr) continue;
-      if (pair[i] >= 0) {
-#pragma unroll
-        for (int p = 0; p < kPairs; ++p) {
-          const float2 cs = table[pair[i] + p];
-          T& xa = a.interleaved ? x[i][2 * p] : x[i][p];
-          T& xb = a.interleaved ? x[i][2 * p + 1] : x[i][kSpan + p];
-          const float u = to_f32(xa), v = to_f32(xb);
-          xa = from_f32<T>(u * cs.x - v * cs.y);
-          xb = from_f32<T>(v * cs.x + u * cs.y);
-        }
-      }
-      if constexpr (kVector) {
-        *reinterpret_cast<Eight<T>*>(to[i][0]) = *reinterpret_cast<Eight<T>*>(&x[i][0]);
-        *reinterpret_cast<Eight<T>*>(to[i][1]) = *reinterpret_cast<Eight<T>*>(&x[i][kSpan]);
-      } else {
-        *to[i][0] = x[i][0];
-        *to[i][1] = x[i][1];
-      }
+    const T* in = static_cast<const T*>(side.in) + (token0 + t) * side.in_token + head * side.in_head;
+    T* out = static_cast<T*>(side.out) + (token0 + t) * side.out_token + head * side.out_head;
+    to0 = out + at0;
+    to1 = out + at1;
+    if constexpr (kVector) {
+      *reinterpret_cast<Eight<T>*>(&x[0]) = *reinterpret_cast<const Eight<T>*>(in + at0);
+      *reinterpret_cast<Eight<T>*>(&x[kSpan]) = *reinterpret_cast<const Eight<T>*>(in + at1);
+    } else {
+      x[0] = in[at0];
+      x[1] = in[at1];
     }
+  }
+  for (int e = threadIdx.x; e < tokens * a.half; e += kThreads) {
+    const int t = e / a.half;
+    float2 cs = rotary_core::turn(rotary_core::position_at(a.positions, a.wide_positions, token0 + t),
+                                  a.frequencies[e - t * a.half], a.magnitude);
+    cs.y *= a.sign;
+    table[e] = cs;
+  }
+  __syncthreads();
+  if (!mine) return;
+  if (pair >= 0) {
+#pragma unroll
+    for (int p = 0; p < kPairs; ++p) {
+      const float2 cs = table[pair + p];
+      T& xa = a.interleaved ? x[2 * p] : x[p];
+      T& xb = a.interleaved ? x[2 * p + 1] : x[kSpan + p];
+      const float u = to_f32(xa), v = to_f32(xb);
+      xa = from_f32<T>(u * cs.x - v * cs.y);
+      xb = from_f32<T>(v * cs.x + u * cs.y);
+    }
+  }
+  if constexpr (kVector) {
+    *reinterpret_cast<Eight<T>*>(to0) = *reinterpret_cast<Eight<T>*>(&x[0]);
+    *reinterpret_cast<Eight<T>*>(to1) = *reinterpret_cast<Eight<T>*>(&x[kSpan]);
+  } else {
+    *to0 = x[0];
+    *to1 = x[1];
   }
 }
 
-template <typename T>
-int launch_rope(RopeArgs a, bool vector, hipStream_t stream) {
-  const int64_t per_head = vector ? a.half / 8 + (a.copy ? (a.dim - 2 * a.half) / 16 : 0)
-                                  : a.half + (a.copy ? (a.dim - 2 * a.half) / 2 : 0);
+int64_t items_per_head(const RopeArgs& a, bool vector) {
+  return vector ? a.half / 8 + (a.copy ? (a.dim - 2 * a.half) / 16 : 0)
+                : a.half + (a.copy ? (a.dim - 2 * a.half) / 2 : 0);
+}
+
+template <typename T, bool kVector>
+int launch_items(RopeArgs a, hipStream_t stream) {
+  const int64_t per_head = items_per_head(a, kVector);
   int64_t groups = 0;
   for (RopeSide& s : a.side) {
     const int64_t per_token = per_head * s.heads;
     s.tokens_per_group = s.groups_per_token = 1;
     s.groups = 0;
     if (per_token == 0) continue;
-    if (per_token >= kGroupItems) {
-      s.groups_per_token = (int32_t)((per_token + kGroupItems - 1) / kGroupItems);
+    if (per_token >= kThreads) {
+      s.groups_per_token = (int32_t)((per_token + kThreads - 1) / kThreads);
     } else {
-      int64_t t = kGroupItems / per_token;
+      int64_t t = kThreads / per_token;
       if (t * a.half > kTableEntries) t = kTableEntries / a.half;
       s.tokens_per_group = (int32_t)t;
     }
@@ -166,12 +162,14 @@ int launch_rope(RopeArgs a, bool vector, hipStream_t stream) {
   }
   DSA_CHECK_ARG(groups < 0x7FFFFFFF, "too many tokens for one launch");
   if (groups == 0) return kOk;
-  if (vector)
-    hipLaunchKernelGGL((rope_pair<T, true>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((rope_pair<T, false>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((rope_pair<T, kVector>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
   DSA_CHECK_LAUNCH("rope");
   return kOk;
+}
+
+template <typename T>
+int launch_rope(const RopeArgs& a, bool vector, hipStream_t stream) {
+  return vector ? launch_items<T, true>(a, stream) : launch_items<T, false>(a, stream);
 }
 
 }  // namespace

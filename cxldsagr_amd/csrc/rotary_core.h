@@ -19,6 +19,9 @@ __device__ __forceinline__ float2 turn(int64_t position, float frequency, float 
   return make_float2(c * magnitude, s * magnitude);
 }
 
+// float32 -> bf16 bits, to nearest even (v_cvt_pk_bf16_f32; a NaN stays one).
+__device__ __forceinline__ uint32_t to_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+
 // The position of a token: int32 or int64.
 __device__ __forceinline__ int64_t position_at(const void* positions, int wide, int64_t token) {
   return wide ? static_cast<const int64_t*>(positions)[token] : static_cast<const int32_t*>(positions)[token];

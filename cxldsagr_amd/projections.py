@@ -78,9 +78,16 @@ def rotary_table(positions, frequencies):
 
 
 def _check_heads(x, tokens, device, dtype, dim, name):
-    if (not isinstance(x, torch.Tensor) or x.ndim != 3 or x.shape[0] != tokens
-            or x.shape[2] != dim or x.dtype != dtype or x.device != device):
+    if (not isinstance(x, torch.Tensor) or x.ndim != 3 or x.dtype != dtype or x.device != device
+            or x.shape[::2] != (tokens, dim)):
         raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device}")
+
+
+def _check_rope_out(out, x, name):
+    if (not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != x.dtype
+            or out.device != x.device or (out.stride(2) != 1 and out.shape[2] > 1)):
+        raise ValueError(f"{name} must have its input's shape, type and device and a contiguous "
+                         "last dim")
 
 
 def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False, magnitude=1.0,
@@ -106,12 +113,13 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
     """
     if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in _native.DTYPE_CODES:
         raise ValueError("q must be bf16, fp16 or fp32 [tokens, heads, dim]")
-    tokens, device, dtype, dim = q.shape[0], q.device, q.dtype, q.shape[2]
+    shape, device, dtype = q.shape, q.device, q.dtype
+    tokens, heads, dim = shape
     if k is not None:
         _check_heads(k, tokens, device, dtype, dim, "k")
     elif k_out is not None:
         raise ValueError("k_out without k")
-    if (not isinstance(positions, torch.Tensor) or tuple(positions.shape) != (tokens,)
+    if (not isinstance(positions, torch.Tensor) or positions.shape != (tokens,)
             or positions.dtype not in (torch.int32, torch.int64) or positions.device != device):
         raise ValueError("positions must be int32 or int64 [tokens] on the query device")
     if (not isinstance(frequencies, torch.Tensor) or frequencies.ndim != 1
@@ -123,36 +131,44 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
         raise ValueError("the rotated part must lie within the head, with an even rest")
     if not math.isfinite(magnitude):
         raise ValueError("magnitude must be finite")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("rotate gradients by a call with inverse=True")
     _native.require_gfx950(device, "rotary positions")
-    outs = []
-    for x, out, name in ((q, q_out, "q_out"), (k, k_out, "k_out")):
-        if out is None and x is not None:
-            out = torch.empty(x.shape, dtype=dtype, device=device)
-        elif out is not None:
-            _check_heads(out, tokens, device, dtype, dim, name)
-            if out.shape != x.shape or (out.stride(2) != 1 and dim > 1):
-                raise ValueError(f"{name} must have its input's shape and a contiguous last dim")
-        outs.append(out)
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check_rope_out(q_out, q, "q_out")
+    if k is not None:
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=dtype, device=device)
+        else:
+            _check_rope_out(k_out, k, "k_out")
     if tokens == 0:
-        return tuple(outs)
-    sides = []
-    for x, out in zip((q, k), outs):
-        if x is None:
-            sides += [None, 0, 0, None, 0, 0, 0]
-            continue
-        if x.stride(2) != 1 and dim > 1:
-            x = x.contiguous()
-        sides += [x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
-                  out.stride(1), x.shape[1]]
-    positions, frequencies = positions.contiguous(), frequencies.contiguous()
+        return q_out, k_out
+    q_strides, to_strides = q.stride(), q_out.stride()
+    if q_strides[2] != 1 and dim > 1:
+        q = q.contiguous()
+        q_strides = q.stride()
+    sides = (q.data_ptr(), q_strides[0], q_strides[1], q_out.data_ptr(), to_strides[0], to_strides[1], heads)
+    if k is None:
+        sides += (None, 0, 0, None, 0, 0, 0)
+    else:
+        k_strides, to_strides = k.stride(), k_out.stride()
+        if k_strides[2] != 1 and dim > 1:
+            k = k.contiguous()
+            k_strides = k.stride()
+        sides += (k.data_ptr(), k_strides[0], k_strides[1], k_out.data_ptr(), to_strides[0], to_strides[1],
+                  k.shape[1])
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
     with _native.on_device(device):
         _native.call(
             "dsa_rope_pair", *sides, _native.DTYPE_CODES[dtype], tokens, dim, offset, rotated,
-            positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(),
-            float(magnitude), int(interleaved), int(inverse), _native.raw_stream(device))
-    return tuple(outs)
+            positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(),
+            magnitude, bool(interleaved), bool(inverse), _native.raw_stream(device))
+    return q_out, k_out
 
 
 def index_producer(q_proj, k_proj, head_logits, norm_weight, norm_bias, eps, cos_sin,
