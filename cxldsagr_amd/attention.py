@@ -330,7 +330,7 @@ def read_kv_fp8(kv_cache, slots, *, out=None, status=None):
     slots = _check_slots(slots, tokens, device)
     _check_status(status, device)
     if out is None:
-        out = torch.empty((tokens, QK_DIM), dtype=torch.bfloat16, device=device)
+        out = kv_cache.new_empty((tokens, QK_DIM), dtype=torch.bfloat16)
     elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != (tokens, QK_DIM)
           or out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous()
           or out.data_ptr() % 16):
@@ -382,8 +382,8 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
 
     Returns ``[Tq, H, d_v]`` in ``q``'s type, or writes it to ``out``
     (contiguous); queries outside the sequences (before ``cu_q[0]``, from
-    ``cu_q[-1]`` on) are left as they were in ``out``. ``max_k`` (default
-    ``Tk``): an upper bound of a sequence's keys, by which few queries' keys are
+    ``cu_q[-1]`` on) are left as they were in ``out``. ``max_k``: the longest
+    sequence's keys where the caller knows it, by which few queries' keys are
     split over the GPU; it does not change what is computed. Forward only. A
     key that some query of its sequence does not see must have finite values.
     """
@@ -416,14 +416,14 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
     _native.require_gfx950(device, "prompt attention")
     shape = (q_tokens, heads, v_dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = q.new_empty(shape)
     elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != dtype
           or out.device != device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned [Tq, H, Dv] tensor of q's "
                          "dtype on q's device")
     if not q_tokens or not sequences:
         return out
-    max_k = k_tokens if max_k is None else min(max_k, k_tokens)
+    max_k = -1 if max_k is None else min(max_k, k_tokens)
     # (The tensors are kept until the call: they may be copies.)
     q, *q_at = _heads_layout(q)
     k, *k_at = _heads_layout(k)
@@ -431,7 +431,7 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
     with _native.on_device(device):
         needed = _native.size_of("dsa_prompt_attention_workspace_bytes", device.index, q_tokens,
                                  heads, kv_heads, v_dim, sequences, k_tokens, max_k)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=device) if needed else None
+        workspace = q.new_empty(needed, dtype=torch.uint8) if needed else None
         _native.call(
             "dsa_prompt_attention", *q_at, *k_at, *v_at, _native.DTYPE_CODES[dtype], heads,
             kv_heads, qk_dim, v_dim, cu_q.data_ptr(), cu_k.data_ptr(), sequences, q_tokens,
@@ -488,7 +488,7 @@ def shared_prefix_mla(q, kv_cache, prefix_table, prefix_tokens, suffix_tables, s
     _native.require_gfx950(q.device, "shared prefix MLA")
     shape = (*q.shape[:2], value_dim)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != q.dtype
           or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned [T, H, 512] tensor of q's "
@@ -503,7 +503,7 @@ def shared_prefix_mla(q, kv_cache, prefix_table, prefix_tokens, suffix_tables, s
     with _native.on_device(q.device):
         needed = _native.size_of("dsa_shared_prefix_mla_workspace_bytes", q.device.index,
                                  q.shape[0], q.shape[1], prefix_tokens, suffix_tables.shape[1])
-        workspace = torch.empty(needed, dtype=torch.uint8, device=q.device) if needed else None
+        workspace = q.new_empty(needed, dtype=torch.uint8) if needed else None
         _native.call(
             "dsa_shared_prefix_mla_fp8",
             q.data_ptr(), q.shape[0], q.shape[1], cache.data_ptr(), cache.shape[0],

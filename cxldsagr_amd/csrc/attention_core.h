@@ -108,6 +108,26 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __uint_as_float(both[0]) + __uint_as_float(both[1]);
 }
 
+// A value's sum or largest over the wave, in every lane, by lane moves: xor 1 and 2 in
+// a quad, the other quad of eight, the other eight, the other rows.
+template <typename Op>
+__device__ __forceinline__ uint32_t reduce_lanes(uint32_t v, Op op) {
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(b[0], b[1]);
+}
+__device__ __forceinline__ uint32_t sum_lanes(uint32_t v) {
+  return reduce_lanes(v, [](uint32_t x, uint32_t y) { return x + y; });
+}
+__device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
+  return reduce_lanes(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+}
+
 // The running maximum and sum of one row of scores (held by lanes l and l ^ 32:
 // the maximum by both, of the sum a part each).
 struct RowState {

@@ -55,7 +55,7 @@ struct PromptArgs {
   float2* stats;   // [splits][q_tokens * heads]
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides, elements
   int64_t q_tokens, k_tokens;
-  int32_t heads, kv_heads, sequences, slots, splits, split_stages, causal;
+  int32_t heads, kv_heads, sequences, slots, splits, split_stages, causal, ranked;
   float scale_log2;
 };
 
@@ -64,6 +64,59 @@ struct PromptArgs {
 // so a work-group finds its sequence by bisection, with no plan made beforehand.
 __host__ __device__ inline int64_t first_slot(int64_t start, int64_t group, int64_t b, int64_t tile) {
   return start * group / tile + b;
+}
+
+// The row tile of a rank among all tiles of up to 64 sequences by the stages of keys
+// that their last row sees, most first: lane b looks at sequence b. The tiles of a
+// sequence see more the later they are, so the tiles that see more than x stages are
+// counted in closed form, a bisection over x finds how many the rank's tile sees, and a
+// scan which of the tiles that see as many it is. It costs about 1 us, and neighbours
+// are then of different sequences; without it a batch's longest sequences start when
+// others have run. See prompt_plan for where it is used.
+template <int kTileRows, typename Lookup>
+__device__ __forceinline__ bool tile_of_rank(int rank, int sequences, int group, int causal, Lookup sequence, int& which,
+                                             int64_t& tile_row) {
+  const int lane = threadIdx.x & 63;
+  int64_t rows = 0;
+  int n_k = 0, history = 0;
+  if (lane < sequences) {
+    const auto s = sequence(lane);
+    rows = (int64_t)s.n_q * group;
+    n_k = s.n_k;
+    history = s.n_k - s.n_q;
+  }
+  const int tiles = (int)((rows + kTileRows - 1) / kTileRows);
+  // This lane's tiles that see more than x stages (x = -1: all).
+  auto above = [&](int x) -> int {
+    const int64_t keys = (int64_t)x * kStageKeys;
+    if (x < 0) return tiles;
+    if (keys >= n_k) return 0;
+    const int64_t y = causal ? keys - history : 0;  // of its last row's token at least
+    return y <= 0 ? tiles : max(tiles - (int)(y * group / kTileRows), 0);
+  };
+  auto all = [&](int v) -> int { return __builtin_amdgcn_readfirstlane((int)sum_lanes((uint32_t)v)); };
+  if (rank >= all(tiles)) return false;
+  // The smallest x that at most `rank` tiles see more than.
+  int lo = -1, hi = __builtin_amdgcn_readfirstlane((int)(max_lanes((uint32_t)n_k) + kStageKeys - 1) / kStageKeys);
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (all(above(mid)) <= rank) hi = mid; else lo = mid;
+  }
+  const int more = above(hi), same = above(hi - 1) - more;
+  int before = same;  // of the lanes below, then
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(before, d, 64);
+    if (lane >= d) before += up;
+  }
+  before -= same;
+  const int place = rank - all(more) - before;
+  const uint64_t mine = __builtin_amdgcn_ballot_w64(place >= 0 && place < same);
+  if (mine == 0) return false;
+  which = __builtin_ctzll(mine);
+  const int tile = __builtin_amdgcn_readlane(tiles - more - 1 - place, which);
+  tile_row = (int64_t)tile * kTileRows;
+  return true;
 }
 
 template <typename E, int kQk, int kV, typename C>
@@ -81,33 +134,49 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
 
   // ---- which row tile, KV head and split. Work-groups go round the XCDs by
   // linear id: with a multiple of 8 KV heads each XCD takes whole heads, whose
-  // keys its L2 then holds. Later tiles first: under a causal mask they see the
-  // most keys.
+  // keys its L2 then holds. `rank` goes over the row tiles, longest first.
   const int group = a.heads / a.kv_heads;
-  int64_t unit = blockIdx.x / a.splits;
+  const int64_t unit = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x % a.splits);
-  int slot, kv_head;
+  int rank, kv_head;
   if (a.splits == 1 && a.kv_heads % 8 == 0) {
     const int64_t in_xcd = unit >> 3;
     const int per_xcd = a.kv_heads / 8;
     kv_head = (int)(in_xcd % per_xcd) * 8 + (int)(unit & 7);
-    slot = a.slots - 1 - (int)(in_xcd / per_xcd);
+    rank = (int)(in_xcd / per_xcd);
   } else {
     kv_head = (int)(unit % a.kv_heads);
-    slot = a.slots - 1 - (int)(unit / a.kv_heads);
-  }
-  int lo = 0, hi = a.sequences;  // the last sequence whose first slot is <= slot
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first_slot(a.cu_q[mid], group, mid, kTileRows) <= slot) lo = mid; else hi = mid;
+    rank = (int)(unit / a.kv_heads);
   }
   // Lengths outside the tensors are cut to them.
-  const int64_t q_begin = min(max((int64_t)a.cu_q[lo], (int64_t)0), a.q_tokens);
-  const int64_t q_end = min(max((int64_t)a.cu_q[lo + 1], q_begin), a.q_tokens);
-  const int64_t k_begin = min(max((int64_t)a.cu_k[lo], (int64_t)0), a.k_tokens);
-  const int64_t k_end = min(max((int64_t)a.cu_k[lo + 1], k_begin), a.k_tokens);
-  const int n_q = (int)(q_end - q_begin), n_k = (int)(k_end - k_begin);
-  const int64_t tile_row = ((int64_t)slot - first_slot(a.cu_q[lo], group, lo, kTileRows)) * kTileRows;
+  struct Sequence {
+    int64_t q_begin, k_begin;
+    int n_q, n_k;
+  };
+  auto sequence = [&](int b) -> Sequence {
+    const int64_t q_begin = min(max((int64_t)a.cu_q[b], (int64_t)0), a.q_tokens);
+    const int64_t q_end = min(max((int64_t)a.cu_q[b + 1], q_begin), a.q_tokens);
+    const int64_t k_begin = min(max((int64_t)a.cu_k[b], (int64_t)0), a.k_tokens);
+    const int64_t k_end = min(max((int64_t)a.cu_k[b + 1], k_begin), a.k_tokens);
+    return {q_begin, k_begin, (int)(q_end - q_begin), (int)(k_end - k_begin)};
+  };
+  int lo = 0;
+  int64_t tile_row;
+  if (kWaves > 1 && a.ranked) {
+    if (!tile_of_rank<kTileRows>(rank, a.sequences, group, a.causal, sequence, lo, tile_row)) return;
+  } else {
+    // Later slots first: within a sequence later tiles see the most keys.
+    const int slot = a.slots - 1 - rank;
+    int hi = a.sequences;  // the last sequence whose first slot is <= slot
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first_slot(a.cu_q[mid], group, mid, kTileRows) <= slot) lo = mid; else hi = mid;
+    }
+    tile_row = ((int64_t)slot - first_slot(a.cu_q[lo], group, lo, kTileRows)) * kTileRows;
+  }
+  const auto [q_begin_, k_begin_, n_q_, n_k_] = sequence(lo);
+  const int64_t q_begin = q_begin_, k_begin = k_begin_;
+  const int n_q = n_q_, n_k = n_k_;
   const int64_t rows = (int64_t)n_q * group;
   if (tile_row < 0 || tile_row >= rows) return;
 
@@ -403,13 +472,18 @@ using FewRows = Cut<1, 2>;
 using ManyRows = Cut<4, 2>;
 
 // Key splits, where the row tiles are too few for the chip: ranges of the same
-// number of keys, so that sequences of different lengths make work-groups of the
-// same size, about `rounds` per CU if all keys are seen, of at least 256 keys (a part
-// costs 4 (d_v + 2) bytes a row, written and read).
-constexpr int64_t kMinSplitKeys = 256, kMaxSplits = 64;
+// number of stages, so that sequences of different lengths make work-groups of the
+// same size.
+// Few rows: about two rounds of work-groups if all keys are seen, of at least 256
+// keys (eight single tokens over 40,000 keys of 8 heads 40.5 us, with one round 44.1,
+// three 39.9, four 39.9; over 16 heads of 192 / 128, 30,000 keys, 61.8, 67.4, 62.0, 64.6).
+// Many rows: where it pays by the rounds of work-groups, their fixed part and their
+// stages, against a join of 4 d_v bytes a row and split, written and read.
+constexpr int64_t kMinSplitStages = 8, kMaxSplits = 256;
+constexpr double kFixedUs = 5.0, kStageUs = 1.15, kJoinUs = 4.0, kJoinBytesPerUs = 4.0e6;
 
 struct PromptPlan {
-  bool few;
+  bool few, ranked;
   int64_t slots, splits, split_stages, bytes, stats_at;
 };
 
@@ -418,20 +492,40 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
   PromptPlan p{};
   const int64_t rows = q_tokens * (heads / kv_heads);
   p.few = rows <= FewRows::kRows * sequences;
-  const int64_t tile = p.few ? FewRows::kRows : ManyRows::kRows, keys = kStageKeys;
-  const int64_t rounds = 4;
-  p.slots = first_slot(q_tokens, heads / kv_heads, sequences, tile);
+  p.slots = first_slot(q_tokens, heads / kv_heads, sequences, p.few ? FewRows::kRows : ManyRows::kRows);
   const int64_t units = p.slots * kv_heads;
-  const int64_t cus = device_cu_count() * 2;
+  const int64_t round = 2 * device_cu_count();  // two work-groups per CU
+  // Tiles by rank where the work-groups are at most a round and a half: 8,140 tokens
+  // in 13 sequences, 8 heads of 64 dims (608 work-groups) 32.7 -> 26.1 us, 4,434 in 8,
+  // 16 heads of 192 / 128 (672) 40.1 -> 38.0; with 64 heads (2,688) 125.8 -> 134.3.
+  p.ranked = !p.few && sequences > 1 && sequences <= 64 && 2 * units <= 3 * round;
   p.splits = 1;
-  const int64_t stages = (max_k + keys - 1) / keys, least = kMinSplitKeys / keys;
-  if (units < cus && stages > least) {
-    // Stages of all row tiles: the sequences' keys, as often as a sequence has tiles.
-    const int64_t tiles = (rows + tile * sequences - 1) / (tile * sequences);
-    const int64_t all = kv_heads * tiles * (k_tokens / keys + sequences);
-    p.split_stages = (all + rounds * device_cu_count() - 1) / (rounds * device_cu_count());
+  // Stages of a row tile, if a sequence is as long as the others, and of the longest
+  // (taken for twice that, of single tokens four times, where it is not given).
+  const int64_t mean = k_tokens / kStageKeys / sequences + 1;
+  int64_t stages = ((max_k < 0 ? k_tokens : max_k) + kStageKeys - 1) / kStageKeys;
+  if (max_k < 0 && stages > (p.few ? 4 : 2) * mean) stages = (p.few ? 4 : 2) * mean;
+  const int64_t usual = mean < stages ? mean : stages;
+  if (units < round && stages > kMinSplitStages) {
+    if (p.few) {
+      p.split_stages = (units * usual + 2 * round - 1) / (2 * round);
+    } else {
+      double least = (double)stages * kStageUs + kFixedUs;
+      p.split_stages = stages;
+      for (int64_t s = 2; s <= kMaxSplits; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : s < 32 ? 8 : s < 64 ? 16 : 64) {
+        const int64_t of = (stages + s - 1) / s;
+        if (of < kMinSplitStages) break;
+        const double groups = (double)units * (double)((usual + of - 1) / of) / (double)round;
+        const double us = (groups > 1.0 ? groups : 1.0) * (kFixedUs + kStageUs * (double)of) + kJoinUs +
+                          (double)(rows * kv_heads * ((usual + of - 1) / of) * v_dim * 8) / kJoinBytesPerUs;
+        if (us < least) {
+          least = us;
+          p.split_stages = of;
+        }
+      }
+    }
     if (p.split_stages < (stages + kMaxSplits - 1) / kMaxSplits) p.split_stages = (stages + kMaxSplits - 1) / kMaxSplits;
-    if (p.split_stages < least) p.split_stages = least;
+    if (p.split_stages < kMinSplitStages) p.split_stages = kMinSplitStages;
     p.splits = (stages + p.split_stages - 1) / p.split_stages;
   }
   if (p.splits > 1) {
@@ -469,7 +563,7 @@ extern "C" int dsa_prompt_attention_workspace_bytes(int64_t q_tokens, int64_t he
                                                     int64_t sequences, int64_t k_tokens, int64_t max_k, int64_t* bytes) {
   using namespace dsa;
   DSA_CHECK_ARG(bytes != nullptr, "null pointer");
-  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && k_tokens >= 0 && max_k >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
+  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && k_tokens >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
                     v_dim > 0,
                 "invalid prompt attention shape");
   *bytes = sequences == 0 ? 0 : prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k).bytes;
@@ -490,7 +584,7 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
   DSA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
                 "heads must be a positive multiple of kv_heads");
   DSA_CHECK_ARG(q_tokens >= 0 && k_tokens >= 0 && q_tokens < 0x7FFFFFFF && k_tokens < 0x7FFFFFFF && sequences >= 0 &&
-                    sequences < 0x7FFFFFFF && max_k >= 0,
+                    sequences < 0x7FFFFFFF,
                 "token and sequence counts must be in [0, 2^31)");
   DSA_CHECK_ARG(scale > 0.0f && __builtin_isfinite(scale), "scale must be positive and finite");
   if (q_tokens == 0) return kOk;
@@ -523,7 +617,7 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
   a.heads = (int32_t)heads, a.kv_heads = (int32_t)kv_heads;
   a.sequences = (int32_t)sequences, a.slots = (int32_t)p.slots, a.splits = (int32_t)p.splits;
   a.split_stages = (int32_t)p.split_stages;
-  a.causal = causal != 0;
+  a.causal = causal != 0, a.ranked = p.ranked;
   a.scale_log2 = scale * kLog2E;
   return dtype == DSA_DTYPE_BF16 ? launch_dims<Bf16>(a, qk_dim, v_dim, p.few, stream)
                                  : launch_dims<F16>(a, qk_dim, v_dim, p.few, stream);

@@ -135,12 +135,12 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
         raise ValueError("rotate gradients by a call with inverse=True")
     _native.require_gfx950(device, "rotary positions")
     if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=device)
+        q_out = q.new_empty(shape)
     else:
         _check_rope_out(q_out, q, "q_out")
     if k is not None:
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=dtype, device=device)
+            k_out = k.new_empty(k.shape)
         else:
             _check_rope_out(k_out, k, "k_out")
     if tokens == 0:
