@@ -148,11 +148,12 @@ __device__ __forceinline__ bool must_raise(const RowState& row, float mx) {
   return mx > row.top + kLazyRescale || (row.top == none && mx != none);
 }
 
-// Raises it; returns the factor for what was summed before.
+// Raises it; returns the factor for what was summed before (1 with no visible key so
+// far: those sums are zeros, which are not worth a pass over the accumulators).
 __device__ __forceinline__ float raise(RowState& row, float mx) {
   if (!must_raise(row, mx)) return 1.0f;
   const float top = fmaxf(row.top, mx);
-  const float factor = __builtin_amdgcn_exp2f(row.top - top);
+  const float factor = row.top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(row.top - top);
   row.top = top;
   row.sum *= factor;
   return factor;

@@ -64,7 +64,7 @@ struct PrefixArgs {
   const int32_t* suffix_tokens;  // [branches]
   const int32_t* cu_q;           // [branches + 1], or null: one query per branch
   uint16_t* out;
-  float* parts;   // [splits][tokens * heads][512], with more than one split
+  float* parts;   // with more than one split: part_at()
   float2* stats;  // [splits][tokens * heads]
   int64_t tokens, pages, prefix;
   int32_t heads, branches, suffix_pages;
@@ -83,6 +83,15 @@ __device__ __forceinline__ int tile_key(int m) {
 template <bool kHigh>
 __device__ __forceinline__ uint32_t dequant_pair(uint32_t word, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, kHigh));
+}
+
+// Where four dims (of `dim4` fours) of a row's part begin: rows in groups of 32, a
+// group's [dim4][row] as the lanes of an accumulator have them, so that a store of
+// both halves is 1 KB in one piece (by rows, pieces of 32 bytes, the stores of 128
+// rows took 16k cycles; so 9k).
+__device__ __forceinline__ int64_t part_at(int64_t part, int64_t rows, int64_t row, int dim4) {
+  const int64_t groups = (rows + 31) >> 5;
+  return (((part * groups + (row >> 5)) * (kVDim / 4) + dim4) * 32 + (row & 31)) * 4;
 }
 
 __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArgs a) {
@@ -123,6 +132,20 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     row0 = token * a.heads + head0;
     row_end = token * a.heads + min(head0 + kTileRows, (int)a.heads);
   }
+  // Q^T operands, in AGPRs and the last in LDS, on their way while the keys of the
+  // item are looked up.
+  const int64_t wave_row = row0 + wave * kWaveRows;
+  v4u q_ops[kQReg], q_rest[kQLds];
+  {
+    const uint16_t* src = a.q + min(wave_row + n, all_rows - 1) * kQkDim + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
+#pragma unroll
+    for (int ks = 0; ks < kQLds; ++ks) q_rest[ks] = *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks));
+  }
+  const uint32_t q_lds = lds_base + kBuffers * kBufBytes + (uint32_t)wave * (kQLds * 1024) + 16 * lane;
+  __builtin_amdgcn_sched_barrier(0);
+
   int64_t row_begin = row0;
   if (a.cu_q != nullptr) {
     // Rows of no branch are left alone.
@@ -152,14 +175,9 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   const int b0 = split * per_split;
   const int b1 = min(b0 + per_split, all_blocks);
 
-  const int64_t wave_row = row0 + wave * kWaveRows;
   const bool live = wave_row + n < row_end && wave_row + n >= row_begin;  // this lane's row, in both halves
   const int64_t row_at = min(wave_row + n, row_end - 1);
   const bool active = __builtin_amdgcn_readfirstlane(wave_row < row_end && b1 > b0);
-
-  // Q^T operands: in AGPRs, and the last in LDS.
-  v4u q_ops[kQReg];
-  const uint32_t q_lds = lds_base + kBuffers * kBufBytes + (uint32_t)wave * (kQLds * 1024) + 16 * lane;
 
   // ---- staging: eight lanes a key. Lane j brings bytes 128 i + 16 j of the
   // latent (a chunk of every tile), the scales, and bytes 16 j of the RoPE part.
@@ -274,16 +292,10 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
   Staged st;
   {
-    // The first two blocks and Q^T on their way together.
+    // The first two blocks on their way together.
     Staged first;
     fetch(first, b0, page);
     fetch(st, b0 + 1, page1);
-    const uint16_t* src = a.q + row_at * kQkDim + 8 * h;
-    v4u q_rest[kQLds];
-#pragma unroll
-    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
-#pragma unroll
-    for (int ks = 0; ks < kQLds; ++ks) q_rest[ks] = *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks));
 #pragma unroll
     for (int i = 0; i < 5; ++i) unpack(first, lds_base + store_lane, i);
 #pragma unroll
@@ -387,14 +399,14 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   // ---- store (as in prompt attention: the halves trade to store 16 bytes).
   const float sum = sum_halves(row.sum);
   if (a.splits + a.suffix_splits > 1) {
-    const int64_t at = (int64_t)part * all_rows + row_at;
-    if (live && h == 0) a.stats[at] = split_stats(row.top, sum);
+    if (live && h == 0) a.stats[(int64_t)part * all_rows + row_at] = split_stats(row.top, sum);
     if (live && sum != 0.0f) {
+      float* to = a.parts + part_at(part, all_rows, row_at, h);
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          *reinterpret_cast<v4f*>(a.parts + at * kVDim + 32 * d + 8 * c + 4 * h) =
+          *reinterpret_cast<v4f*>(to + (8 * d + 2 * c) * 128) =
               v4f{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
     }
     return;
@@ -414,6 +426,91 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
       const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
       if (live) *reinterpret_cast<v4u*>(a.out + row_at * kVDim + 32 * d + 8 * (c + h)) = v4u{x[0], y[0], x[1], y[1]};
     }
+}
+
+// Joins the parts of the rows: a wave has four dims (a lane's 16 bytes) of 32 rows in
+// each half, kChunks waves neighbouring ones, and kWays of them every kWays-th part
+// each, four in flight at a time, against a running maximum of their own. What bounds it is
+// reading the parts.
+template <int kWays, int kChunks>
+__global__ __launch_bounds__(64 * kWays * kChunks) void join_parts(
+    const float* __restrict__ parts, const float2* __restrict__ stats, int64_t rows, int splits,
+    const int32_t* __restrict__ cu, int32_t branches, int64_t heads, uint16_t* __restrict__ out) {
+  __shared__ v4f shared[kWays][kChunks][64];
+  __shared__ float2 of_way[kWays][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int way = wave % kWays, chunk = wave / kWays;
+  constexpr int kPerGroup = kVDim / 8 / kChunks;  // work-groups of 32 rows
+  const int64_t row = (int64_t)(blockIdx.x / kPerGroup) * 32 + (lane & 31);
+  const int dim4 = 2 * ((int)(blockIdx.x % kPerGroup) * kChunks + chunk) + (lane >> 5);
+  const float none = -__builtin_inff();
+  // Rows outside the branches have no parts, and stay as they are.
+  const bool live = row < rows && (cu == nullptr || (row >= cu[0] * heads && row < cu[branches] * heads));
+  v4f acc = {};
+  float top = none, sum = 0.0f;
+  if (live) {
+    constexpr int kAtOnce = 4;
+    for (int s0 = way; s0 < splits; s0 += kWays * kAtOnce) {
+      float2 st[kAtOnce];
+      v4f o[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int s = s0 + i * kWays;
+        st[i] = s < splits ? stats[s * rows + row] : make_float2(none, 0.0f);
+        o[i] = *reinterpret_cast<const v4f*>(parts + part_at(min(s, splits - 1), rows, row, dim4));
+      }
+      float up = top;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) up = fmaxf(up, st[i].x);
+      const float keep = top == none ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+      sum *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        // (A part without a visible key has no values in memory. A NaN maximum, of
+        // one with a NaN score, spreads.)
+        if (st[i].y == 0.0f) continue;
+        const float w = __builtin_amdgcn_exp2f(st[i].x - up);
+        sum += w * st[i].y;
+        acc += w * o[i];
+      }
+      top = up;
+    }
+  }
+  if constexpr (kWays > 1) {
+    shared[way][chunk][lane] = acc;
+    if (chunk == 0 && lane < 32) of_way[way][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (way != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) top = fmaxf(top, of_way[w][lane & 31].x);
+    sum = 0.0f;
+    acc = v4f{};
+#pragma unroll
+    for (int w = 0; w < kWays; ++w) {
+      const float2 st = of_way[w][lane & 31];
+      if (st.y == 0.0f) continue;
+      const float factor = st.x == none ? st.y : __builtin_amdgcn_exp2f(st.x - top);
+      sum += factor * st.y;
+      acc += factor * shared[w][chunk][lane];
+    }
+  }
+  if (!live) return;
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+  *reinterpret_cast<v2u*>(out + row * kVDim + 4 * dim4) =
+      v2u{Bf16::pack(acc.x * inv, acc.y * inv), Bf16::pack(acc.z * inv, acc.w * inv)};
+}
+
+int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t stream) {
+  const auto go = [&](auto kernel, int ways, int chunks) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 31) / 32 * (kVDim / 8 / chunks))), dim3(64 * ways * chunks), 0,
+                       stream, a.parts, a.stats, rows, splits, a.cu_q, a.branches, (int64_t)a.heads, a.out);
+  };
+  if (splits <= 4) go(join_parts<1, 4>, 1, 4);
+  else if (splits <= 32) go(join_parts<4, 2>, 4, 2);
+  else go(join_parts<16, 1>, 16, 1);
+  DSA_CHECK_LAUNCH("join of the shared prefix's parts");
+  return kOk;
 }
 
 // Key splits: the count of least time, by the rounds of work-groups (one per CU),
@@ -475,7 +572,7 @@ PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t su
   }
   const int64_t parts = p.splits + p.suffix_splits;
   if (parts > 1) {
-    p.stats_at = parts * rows * kVDim * 4;
+    p.stats_at = parts * ((rows + 31) / 32 * 32) * kVDim * 4;
     p.bytes = p.stats_at + parts * rows * 8;
   }
   return p;
@@ -542,8 +639,6 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   a.scale_log2 = scale * kLog2E;
   hipLaunchKernelGGL(shared_prefix_fwd, dim3((unsigned)(items + own)), dim3(kThreads), 0, stream, a);
   DSA_CHECK_LAUNCH("shared prefix MLA");
-  if (p.bytes > 0)
-    return launch_join<Bf16, kVDim>(a.parts, a.stats, tokens * heads, (int)(p.splits + p.suffix_splits), cu_q,
-                                    (int32_t)branches, heads, a.out, stream);
+  if (p.bytes > 0) return launch_join_parts(a, tokens * heads, (int)(p.splits + p.suffix_splits), stream);
   return kOk;
 }
