@@ -206,8 +206,7 @@ __device__ __forceinline__ float2 split_stats(float top, float sum) {
 // Joins them: kWays groups of kDim / 16 lanes take a row, 16 dims a lane (four
 // vectors, each of neighbouring lanes side by side) and every kWays-th split each,
 // against a running maximum of their own. What bounds it is reading the parts: many
-// parts of few rows want many loads in flight (120 parts of 128 rows of 512 dims,
-// 31 MB: 42 us with 4 ways of 8 dims a lane and all maxima looked at first).
+// parts of few rows want many loads in flight.
 template <typename E, int kDim, int kWays>
 __global__ __launch_bounds__(kWays * kDim / 16 > 256 ? kWays * kDim / 16 : 256) void join_splits(
     const float* __restrict__ parts, const float2* __restrict__ stats, int64_t rows, int splits,

@@ -583,9 +583,11 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
                 "head dims must be (192, 128), (128, 128) or (64, 64)");
   DSA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
                 "heads must be a positive multiple of kv_heads");
-  DSA_CHECK_ARG(q_tokens >= 0 && k_tokens >= 0 && q_tokens < 0x7FFFFFFF && k_tokens < 0x7FFFFFFF && sequences >= 0 &&
-                    sequences < 0x7FFFFFFF,
-                "token and sequence counts must be in [0, 2^31)");
+  // (Rounding up to a stage must stay within int32.)
+  constexpr int64_t kMost = 0x7FFFFFFF - kStageKeys;
+  DSA_CHECK_ARG(q_tokens >= 0 && k_tokens >= 0 && q_tokens <= kMost && k_tokens <= kMost && sequences >= 0 &&
+                    sequences <= kMost,
+                "token and sequence counts must be in [0, 2^31 - 33]");
   DSA_CHECK_ARG(scale > 0.0f && __builtin_isfinite(scale), "scale must be positive and finite");
   if (q_tokens == 0) return kOk;
   DSA_CHECK_ARG(sequences > 0, "queries need a sequence");

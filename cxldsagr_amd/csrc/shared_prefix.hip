@@ -430,8 +430,8 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
 
 // Joins the parts of the rows: a wave has four dims (a lane's 16 bytes) of 32 rows in
 // each half, kChunks waves neighbouring ones, and kWays of them every kWays-th part
-// each, four in flight at a time, against a running maximum of their own. What bounds it is
-// reading the parts.
+// each, four in flight at a time, against a running maximum of their own. What bounds
+// it is reading the parts (171 of 128 rows, 45 MB: 9.9 us).
 template <int kWays, int kChunks>
 __global__ __launch_bounds__(64 * kWays * kChunks) void join_parts(
     const float* __restrict__ parts, const float2* __restrict__ stats, int64_t rows, int splits,
@@ -506,8 +506,11 @@ int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t
     hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 31) / 32 * (kVDim / 8 / chunks))), dim3(64 * ways * chunks), 0,
                        stream, a.parts, a.stats, rows, splits, a.cu_q, a.branches, (int64_t)a.heads, a.out);
   };
+  // Ways for the parts there are; 16 where the rows alone do not fill the chip (171
+  // parts of 128 rows: 9.9 us with 16, 12.3 with 4; 68 of 256: 9.2 and 9.0; 34 of 640:
+  // 11.8 and 9.3).
   if (splits <= 4) go(join_parts<1, 4>, 1, 4);
-  else if (splits <= 32) go(join_parts<4, 2>, 4, 2);
+  else if (splits <= 32 || rows >= 256) go(join_parts<4, 2>, 4, 2);
   else go(join_parts<16, 1>, 16, 1);
   DSA_CHECK_LAUNCH("join of the shared prefix's parts");
   return kOk;
@@ -515,9 +518,10 @@ int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t
 
 // Key splits: the count of least time, by the rounds of work-groups (one per CU),
 // their fixed part (Q, the first records, the stores), the steps of the longest, and
-// what reading a row's parts again costs. Fitted to one token over 32,896 keys (s =
-// 114 .. 257) and 31 tokens of 64 heads over 4,099.
-constexpr double kFixedUs = 13.0, kStepUs = 2.0, kJoinUs = 3.0, kPartUsPerRow = 0.0005;
+// what reading a row's parts again costs. Fitted to one token of 128 heads over 32,896
+// keys (64, 128, 206, 257 splits: 52, 40, 39, 54 us), 5 tokens over 8,333 (13, 25, 45,
+// 68: 59, 45, 44, 58) and 8 over 70,000 (16, 32, 64: 294, 186, 231).
+constexpr double kFixedUs = 17.0, kStepUs = 2.2, kJoinUs = 3.0, kPartUsPerRow = 0.0003;
 
 struct PrefixPlan {
   bool joint;
@@ -554,12 +558,12 @@ PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t su
         s = (blocks + (blocks + s - 1) / s - 1) / ((blocks + s - 1) / s);
       }
       // Rounds of the first kind, and of the suffix's own items, which come last, as
-      // far as the last of those rounds has no room for them.
+      // far as the CUs that the last of those rounds leaves free do not take them.
       const int64_t full = (tiles * s + cus - 1) / cus, room = full * cus - tiles * s;
-      const int64_t over = own_tiles * ss > room ? (own_tiles * ss - room + cus - 1) / cus : 0;
       const double step = s > 0 ? kFixedUs + kStepUs * (double)((blocks + s - 1) / s) : 0.0;
       const double own_step = ss > 0 ? kFixedUs + kStepUs * (double)((suffix_blocks + ss - 1) / ss) : 0.0;
-      double us = (double)full * step + (double)over * own_step;
+      const int64_t rest = ss > 0 ? own_tiles * ss - room * (int64_t)(step / own_step + 0.5) : 0;
+      double us = (double)full * step + (rest > 0 ? (double)((rest + cus - 1) / cus) * own_step : 0.0);
       if (us < own_step) us = own_step;
       if (s + ss > 1) us += kJoinUs + kPartUsPerRow * (double)(rows * (s + ss));
       if (us < least) {

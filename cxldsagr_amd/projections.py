@@ -88,6 +88,8 @@ def _check_rope_out(out, x, name):
             or out.device != x.device or (out.stride(2) != 1 and out.shape[2] > 1)):
         raise ValueError(f"{name} must have its input's shape, type and device and a contiguous "
                          "last dim")
+    if 0 in out.stride() and any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{name} must not be expanded: several values would share a place")
 
 
 def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False, magnitude=1.0,

@@ -288,3 +288,21 @@ def test_workspace_queries():
                        ("dsa_shared_prefix_mla_workspace_bytes", (1, 0, 1, 1))):
         with pytest.raises(ValueError, match="shape"):
             _native.call(name, *args, ctypes.byref(size))
+
+
+def test_prompt_keys_whose_stages_would_pass_int32():
+    for count in (0x7FFFFFFF - 31, 0x7FFFFFFF):
+        with pytest.raises(ValueError, match="counts"):
+            _c_prompt(k_tokens=count)
+        with pytest.raises(ValueError, match="counts"):
+            _c_prompt(q_tokens=count)
+
+
+def test_rope_refuses_expanded_outputs(monkeypatch):
+    from cxldsagr_amd import _native
+
+    # (The outputs' checks come after the device's.)
+    monkeypatch.setattr(_native, "require_gfx950", lambda *args: None)
+    for out in (z(1, 4, 64).expand(2, 4, 64), z(2, 1, 64).expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="expanded"):
+            apply_rope_pair(z(2, 4, 64), None, cu(0, 1), torch.ones(32), q_out=out)
