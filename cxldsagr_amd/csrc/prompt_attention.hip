@@ -48,56 +48,41 @@ struct PromptArgs {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;
-  const int32_t* cu_q;
-  const int32_t* cu_k;
   uint16_t* out;
   float* parts;    // [splits][q_tokens * heads][d_v], splits > 1 only
   float2* stats;   // [splits][q_tokens * heads]
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides, elements
-  int64_t q_tokens, k_tokens;
-  int32_t heads, kv_heads, sequences, slots, splits, split_stages, causal, ranked;
+  int32_t heads, split_stages, causal, ranked;
   float scale_log2;
 };
 
-// Slots of row tiles: sequence b's tiles start at slot cu_q[b] G / tile + b, which
-// leaves room for a part-filled tile of every sequence before it: a closed form,
-// so a work-group finds its sequence by bisection, with no plan made beforehand.
-__host__ __device__ inline int64_t first_slot(int64_t start, int64_t group, int64_t b, int64_t tile) {
-  return start * group / tile + b;
-}
-
 // The row tile of a rank among all tiles of up to 64 sequences by the stages of keys
-// that their last row sees, most first: lane b looks at sequence b. The tiles of a
-// sequence see more the later they are, so the tiles that see more than x stages are
-// counted in closed form, a bisection over x finds how many the rank's tile sees, and a
-// scan which of the tiles that see as many it is. It costs about 1 us, and neighbours
-// are then of different sequences; without it a batch's longest sequences start when
-// others have run. See prompt_plan for where it is used.
-template <int kTileRows, typename Lookup>
-__device__ __forceinline__ bool tile_of_rank(int rank, int sequences, int group, int causal, Lookup sequence, int& which,
-                                             int64_t& tile_row) {
+// that their last row sees, most first: lane b looks at sequence b, of n_q queries and
+// n_k keys (0 of both past the last). The tiles of a sequence see more the later they
+// are, so the tiles that see more than x stages are counted in closed form, a bisection
+// over x finds how many the rank's tile sees, and a scan which of the tiles that see as
+// many it is. It costs about 1 us, and neighbours are then of different sequences;
+// without it a batch's longest sequences start when others have run. See prompt_plan
+// for where it is used. `which` is -1 past the last tile.
+template <int kTileRows>
+__device__ __forceinline__ void tile_of_rank(int rank, uint32_t group, int causal, int n_q, int n_k, int& which,
+                                             uint32_t& tile_row) {
   const int lane = threadIdx.x & 63;
-  int64_t rows = 0;
-  int n_k = 0, history = 0;
-  if (lane < sequences) {
-    const auto s = sequence(lane);
-    rows = (int64_t)s.n_q * group;
-    n_k = s.n_k;
-    history = s.n_k - s.n_q;
-  }
-  const int tiles = (int)((rows + kTileRows - 1) / kTileRows);
+  const int history = n_k - n_q;
+  const int tiles = (int)(((uint32_t)n_q * group + kTileRows - 1) / kTileRows);
   // This lane's tiles that see more than x stages (x = -1: all).
   auto above = [&](int x) -> int {
-    const int64_t keys = (int64_t)x * kStageKeys;
+    const int keys = x * kStageKeys;
     if (x < 0) return tiles;
     if (keys >= n_k) return 0;
-    const int64_t y = causal ? keys - history : 0;  // of its last row's token at least
-    return y <= 0 ? tiles : max(tiles - (int)(y * group / kTileRows), 0);
+    const int y = causal ? keys - history : 0;  // of its last row's token at least
+    return y <= 0 ? tiles : max(tiles - (int)((uint32_t)y * group / kTileRows), 0);
   };
   auto all = [&](int v) -> int { return __builtin_amdgcn_readfirstlane((int)sum_lanes((uint32_t)v)); };
-  if (rank >= all(tiles)) return false;
+  which = -1;
+  if (rank >= all(tiles)) return;
   // The smallest x that at most `rank` tiles see more than.
-  int lo = -1, hi = __builtin_amdgcn_readfirstlane((int)(max_lanes((uint32_t)n_k) + kStageKeys - 1) / kStageKeys);
+  int lo = -1, hi = (__builtin_amdgcn_readfirstlane((int)max_lanes((uint32_t)n_k)) + kStageKeys - 1) / kStageKeys;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (all(above(mid)) <= rank) hi = mid; else lo = mid;
@@ -112,15 +97,16 @@ __device__ __forceinline__ bool tile_of_rank(int rank, int sequences, int group,
   before -= same;
   const int place = rank - all(more) - before;
   const uint64_t mine = __builtin_amdgcn_ballot_w64(place >= 0 && place < same);
-  if (mine == 0) return false;
+  if (mine == 0) return;
   which = __builtin_ctzll(mine);
   const int tile = __builtin_amdgcn_readlane(tiles - more - 1 - place, which);
-  tile_row = (int64_t)tile * kTileRows;
-  return true;
+  tile_row = (uint32_t)tile * kTileRows;
 }
 
 template <typename E, int kQk, int kV, typename C>
-__global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) void prompt_fwd(const PromptArgs a) {
+__global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) void prompt_fwd(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int32_t sequences, int32_t q_tokens,
+    int32_t k_tokens, int32_t slots, int32_t splits, int32_t kv_heads, int32_t group_, const PromptArgs a) {
   constexpr int kWaves = C::kWaves, kTileRows = C::kRows;
   constexpr int kQuadsK = kQk / 32, kQuadsV = kV / 32;  // 64-byte column blocks
   constexpr int kStageK = kStageKeys * kQk * 2, kStageV = kStageKeys * kV * 2;
@@ -135,69 +121,76 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
   // ---- which row tile, KV head and split. Work-groups go round the XCDs by
   // linear id: with a multiple of 8 KV heads each XCD takes whole heads, whose
   // keys its L2 then holds. `rank` goes over the row tiles, longest first.
-  const int group = a.heads / a.kv_heads;
-  const int64_t unit = blockIdx.x / a.splits;
-  const int split = (int)(blockIdx.x % a.splits);
+  // (All of this in 32 bits, which hold the rows of a call: divisions of 64 bits made
+  // the start of a work-group YYY.)
+  const uint32_t group = group_;
+  const uint32_t unit = splits == 1 ? blockIdx.x : blockIdx.x / (uint32_t)splits;
+  const int split = (int)(blockIdx.x - unit * (uint32_t)splits);
   int rank, kv_head;
-  if (a.splits == 1 && a.kv_heads % 8 == 0) {
-    const int64_t in_xcd = unit >> 3;
-    const int per_xcd = a.kv_heads / 8;
-    kv_head = (int)(in_xcd % per_xcd) * 8 + (int)(unit & 7);
+  if (splits == 1 && kv_heads % 8 == 0) {
+    const uint32_t in_xcd = unit >> 3, per_xcd = (uint32_t)kv_heads >> 3;
     rank = (int)(in_xcd / per_xcd);
+    kv_head = (int)(in_xcd - rank * per_xcd) * 8 + (int)(unit & 7);
   } else {
-    kv_head = (int)(unit % a.kv_heads);
-    rank = (int)(unit / a.kv_heads);
+    rank = (int)(unit / (uint32_t)kv_heads);
+    kv_head = (int)(unit - rank * (uint32_t)kv_heads);
   }
-  // Lengths outside the tensors are cut to them.
-  struct Sequence {
-    int64_t q_begin, k_begin;
-    int n_q, n_k;
-  };
-  auto sequence = [&](int b) -> Sequence {
-    const int64_t q_begin = min(max((int64_t)a.cu_q[b], (int64_t)0), a.q_tokens);
-    const int64_t q_end = min(max((int64_t)a.cu_q[b + 1], q_begin), a.q_tokens);
-    const int64_t k_begin = min(max((int64_t)a.cu_k[b], (int64_t)0), a.k_tokens);
-    const int64_t k_end = min(max((int64_t)a.cu_k[b + 1], k_begin), a.k_tokens);
-    return {q_begin, k_begin, (int)(q_end - q_begin), (int)(k_end - k_begin)};
-  };
+  // Lane b looks at sequence lo + b of the up to 64 that the tile may be of; starts
+  // outside the tensors are cut to them. Sequence b's tiles start at slot
+  // cu_q[b] G / tile + b, which leaves room for a part-filled tile of every sequence
+  // before it: a closed form, so a work-group finds its sequence with no plan made
+  // beforehand. Later slots first: within a sequence later tiles see the most keys.
+  const int slot = slots - 1 - rank;
+  auto cut = [](int start, int tokens) -> int { return min(max(start, 0), tokens); };
+  auto first_slot = [&](int start, int b) -> int { return (int)((uint32_t)start * group / kTileRows) + b; };
   int lo = 0;
-  int64_t tile_row;
-  if (kWaves > 1 && a.ranked) {
-    if (!tile_of_rank<kTileRows>(rank, a.sequences, group, a.causal, sequence, lo, tile_row)) return;
-  } else {
-    // Later slots first: within a sequence later tiles see the most keys.
-    const int slot = a.slots - 1 - rank;
-    int hi = a.sequences;  // the last sequence whose first slot is <= slot
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (first_slot(a.cu_q[mid], group, mid, kTileRows) <= slot) lo = mid; else hi = mid;
+  while (sequences > 64) {
+    const int half = sequences >> 1;
+    if (first_slot(cut(cu_q[lo + half], q_tokens), lo + half) <= slot) {
+      lo += half;
+      sequences -= half;
+    } else {
+      sequences = half;
     }
-    tile_row = ((int64_t)slot - first_slot(a.cu_q[lo], group, lo, kTileRows)) * kTileRows;
   }
-  const auto [q_begin_, k_begin_, n_q_, n_k_] = sequence(lo);
-  const int64_t q_begin = q_begin_, k_begin = k_begin_;
-  const int n_q = n_q_, n_k = n_k_;
-  const int64_t rows = (int64_t)n_q * group;
-  if (tile_row < 0 || tile_row >= rows) return;
+  const int b = lo + min(lane, sequences - 1);
+  const int lane_q = cut(cu_q[b], q_tokens), lane_k = cut(cu_k[b], k_tokens);
+  const int lane_nq = max(cut(cu_q[b + 1], q_tokens) - lane_q, 0);
+  const int lane_nk = max(cut(cu_k[b + 1], k_tokens) - lane_k, 0);
+  int which;
+  uint32_t tile_row = 0;
+  if (kWaves > 1 && a.ranked) {
+    const bool one = lane < sequences;
+    tile_of_rank<kTileRows>(rank, group, a.causal, one ? lane_nq : 0, one ? lane_nk : 0, which, tile_row);
+    if (which < 0) return;
+  } else {
+    // The last sequence whose first slot is <= slot.
+    const int first = first_slot(lane_q, b);
+    which = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < sequences && first <= slot)) - 1;
+    if (which < 0) return;
+    tile_row = (uint32_t)(slot - __builtin_amdgcn_readlane(first, which)) * kTileRows;
+  }
+  const int64_t q_begin = __builtin_amdgcn_readlane(lane_q, which), k_begin = __builtin_amdgcn_readlane(lane_k, which);
+  const int n_q = __builtin_amdgcn_readlane(lane_nq, which), n_k = __builtin_amdgcn_readlane(lane_nk, which);
+  const uint32_t rows = (uint32_t)n_q * group;
+  if (tile_row >= rows) return;
 
   // Keys that token i sees.
-  auto visible = [&](int64_t token) -> int {
-    if (!a.causal) return n_k;
-    const int64_t m = token + 1 + n_k - n_q;
-    return (int)min(max(m, (int64_t)0), (int64_t)n_k);
+  auto visible = [&](uint32_t token) -> int {
+    return a.causal ? max((int)token + 1 - n_q + n_k, 0) : n_k;
   };
-  const int64_t last_row = min(tile_row + kTileRows, rows) - 1;
+  const uint32_t last_row = min(tile_row + kTileRows, rows) - 1;
   const int all_stages = (visible(last_row / group) + kStageKeys - 1) / kStageKeys;
-  const int s0 = a.splits > 1 ? min(split * a.split_stages, all_stages) : 0;
-  const int s1 = a.splits > 1 ? (split + 1 < a.splits ? min(s0 + a.split_stages, all_stages) : all_stages) : all_stages;
+  const int s0 = splits > 1 ? min(split * a.split_stages, all_stages) : 0;
+  const int s1 = splits > 1 ? (split + 1 < splits ? min(s0 + a.split_stages, all_stages) : all_stages) : all_stages;
 
   // ---- this wave's 32 rows; lanes n and 32 + n have row n.
-  const int64_t wave_row = tile_row + wave * 32;
-  const int wave_rows = (int)min((int64_t)32, rows - wave_row);  // may be <= 0
-  // Rows past the end repeat the wave's last row; nothing of them is stored.
-  const int64_t r = min(wave_row + min(n, max(wave_rows - 1, 0)), rows - 1);
-  const int64_t token = r / group;
-  const int head = kv_head * group + (int)(r - token * group);
+  const uint32_t wave_row = tile_row + wave * 32;
+  const int wave_rows = wave_row < rows ? (int)min(32u, rows - wave_row) : 0;
+  // Rows past the end repeat the last row; nothing of them is stored.
+  const uint32_t r = min(wave_row + (uint32_t)n, rows - 1);
+  const uint32_t token = r / group;
+  const int head = (int)(kv_head * group + (r - token * group));
   const int sees = visible(token);
   // The stages this wave takes part in, and the first key that needs a mask.
   int w1 = s0, clear = 0;
@@ -434,8 +427,8 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
   const float sum = sum_halves(row.sum);
   const bool live = n < wave_rows;
   const int64_t at = (q_begin + token) * a.heads + head;
-  if (a.splits > 1) {
-    const int64_t part = (int64_t)split * a.q_tokens * a.heads + at;
+  if (splits > 1) {
+    const int64_t part = (int64_t)split * q_tokens * a.heads + at;
     if (live && h == 0) a.stats[part] = split_stats(row.top, sum);
     if (live && sum != 0.0f) {
 #pragma unroll
@@ -492,7 +485,7 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
   PromptPlan p{};
   const int64_t rows = q_tokens * (heads / kv_heads);
   p.few = rows <= FewRows::kRows * sequences;
-  p.slots = first_slot(q_tokens, heads / kv_heads, sequences, p.few ? FewRows::kRows : ManyRows::kRows);
+  p.slots = rows / (p.few ? FewRows::kRows : ManyRows::kRows) + sequences;
   const int64_t units = p.slots * kv_heads;
   const int64_t round = 2 * device_cu_count();  // two work-groups per CU
   // Tiles by rank where the work-groups are at most a round and a half: 8,140 tokens
@@ -535,25 +528,35 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
   return p;
 }
 
+struct PromptCall {
+  const int32_t *cu_q, *cu_k;
+  int64_t sequences, q_tokens, k_tokens, kv_heads;
+  PromptPlan plan;
+  PromptArgs args;
+};
+
 template <typename E, int kQk, int kV>
-int launch_prompt(const PromptArgs& a, bool few, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.slots * a.kv_heads * a.splits));
-  if (few)
-    hipLaunchKernelGGL((prompt_fwd<E, kQk, kV, FewRows>), grid, dim3(FewRows::kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((prompt_fwd<E, kQk, kV, ManyRows>), grid, dim3(ManyRows::kThreads), 0, stream, a);
+int launch_prompt(const PromptCall& c, hipStream_t stream) {
+  const auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.plan.slots * c.kv_heads * c.plan.splits)), dim3(threads), 0, stream,
+                       c.cu_q, c.cu_k, (int32_t)c.sequences, (int32_t)c.q_tokens, (int32_t)c.k_tokens,
+                       (int32_t)c.plan.slots, (int32_t)c.plan.splits, (int32_t)c.kv_heads,
+                       (int32_t)(c.args.heads / c.kv_heads), c.args);
+  };
+  if (c.plan.few) go(prompt_fwd<E, kQk, kV, FewRows>, FewRows::kThreads);
+  else go(prompt_fwd<E, kQk, kV, ManyRows>, ManyRows::kThreads);
   DSA_CHECK_LAUNCH("prompt attention");
-  if (a.splits > 1)
-    return launch_join<E, kV>(a.parts, a.stats, a.q_tokens * a.heads, a.splits, a.cu_q, a.sequences, a.heads, a.out,
-                              stream);
+  if (c.plan.splits > 1)
+    return launch_join<E, kV>(c.args.parts, c.args.stats, c.q_tokens * c.args.heads, (int)c.plan.splits, c.cu_q,
+                              (int32_t)c.sequences, c.args.heads, c.args.out, stream);
   return kOk;
 }
 
 template <typename E>
-int launch_dims(const PromptArgs& a, int64_t qk_dim, int64_t v_dim, bool few, hipStream_t stream) {
-  if (qk_dim == 192 && v_dim == 128) return launch_prompt<E, 192, 128>(a, few, stream);
-  if (qk_dim == 128 && v_dim == 128) return launch_prompt<E, 128, 128>(a, few, stream);
-  return launch_prompt<E, 64, 64>(a, few, stream);
+int launch_dims(const PromptCall& c, int64_t qk_dim, int64_t v_dim, hipStream_t stream) {
+  if (qk_dim == 192 && v_dim == 128) return launch_prompt<E, 192, 128>(c, stream);
+  if (qk_dim == 128 && v_dim == 128) return launch_prompt<E, 128, 128>(c, stream);
+  return launch_prompt<E, 64, 64>(c, stream);
 }
 
 }  // namespace
@@ -599,28 +602,24 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
                  reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                 "q, k, v and out must be 16-byte aligned");
   const PromptPlan p = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k);
-  DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF, "too many row tiles");
+  DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF && q_tokens * heads < 0x7FFFFF00, "too many query rows");
   if (p.splits > 1)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "prompt attention workspace too small or misaligned");
-  PromptArgs a{};
+  PromptCall c{cu_q, cu_k, sequences, q_tokens, k_tokens, kv_heads, p, {}};
+  PromptArgs& a = c.args;
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
-  a.cu_q = cu_q;
-  a.cu_k = cu_k;
   a.out = static_cast<uint16_t*>(out);
   a.parts = static_cast<float*>(workspace);
   a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.stats_at);
   a.q_token = q_token_stride, a.q_head = q_head_stride;
   a.k_token = k_token_stride, a.k_head = k_head_stride;
   a.v_token = v_token_stride, a.v_head = v_head_stride;
-  a.q_tokens = q_tokens, a.k_tokens = k_tokens;
-  a.heads = (int32_t)heads, a.kv_heads = (int32_t)kv_heads;
-  a.sequences = (int32_t)sequences, a.slots = (int32_t)p.slots, a.splits = (int32_t)p.splits;
-  a.split_stages = (int32_t)p.split_stages;
+  a.heads = (int32_t)heads, a.split_stages = (int32_t)p.split_stages;
   a.causal = causal != 0, a.ranked = p.ranked;
   a.scale_log2 = scale * kLog2E;
-  return dtype == DSA_DTYPE_BF16 ? launch_dims<Bf16>(a, qk_dim, v_dim, p.few, stream)
-                                 : launch_dims<F16>(a, qk_dim, v_dim, p.few, stream);
+  return dtype == DSA_DTYPE_BF16 ? launch_dims<Bf16>(c, qk_dim, v_dim, stream)
+                                 : launch_dims<F16>(c, qk_dim, v_dim, stream);
 }
