@@ -128,6 +128,19 @@ __device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
   return reduce_lanes(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
 }
 
+// The sum over the lanes below this one: within rows of 16, then of the rows before.
+__device__ __forceinline__ uint32_t sum_below(uint32_t v) {
+  const uint32_t own = v;
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+  const uint32_t row = (threadIdx.x & 63) >> 4;
+  const uint32_t r0 = __builtin_amdgcn_readlane((int)v, 15), r1 = __builtin_amdgcn_readlane((int)v, 31),
+                 r2 = __builtin_amdgcn_readlane((int)v, 47);
+  return v - own + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
+}
+
 // The running maximum and sum of one row of scores (held by lanes l and l ^ 32:
 // the maximum by both, of the sum a part each).
 struct RowState {

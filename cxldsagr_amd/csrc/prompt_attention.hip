@@ -58,44 +58,49 @@ struct PromptArgs {
 
 // The row tile of a rank among all tiles of up to 64 sequences by the stages of keys
 // that their last row sees, most first: lane b looks at sequence b, of n_q queries and
-// n_k keys (0 of both past the last). The tiles of a sequence see more the later they
-// are, so the tiles that see more than x stages are counted in closed form, a bisection
-// over x finds how many the rank's tile sees, and a scan which of the tiles that see as
-// many it is. It costs about 1 us, and neighbours are then of different sequences;
-// without it a batch's longest sequences start when others have run. See prompt_plan
-// for where it is used. `which` is -1 past the last tile.
+// n_k keys (0 of both past the last), less than 2^16 tiles in all. The tiles of a
+// sequence see more the later they are, so the tiles that see more than x stages are
+// counted in closed form, a search over x, four at a time, finds how many the rank's
+// tile sees, and a scan which of the tiles that see as many it is. Neighbours are then of
+// different sequences; without it a batch's longest sequences start when others have
+// run. See prompt_plan for where it is used. `which` is -1 past the last tile.
 template <int kTileRows>
 __device__ __forceinline__ void tile_of_rank(int rank, uint32_t group, int causal, int n_q, int n_k, int& which,
                                              uint32_t& tile_row) {
-  const int lane = threadIdx.x & 63;
   const int history = n_k - n_q;
   const int tiles = (int)(((uint32_t)n_q * group + kTileRows - 1) / kTileRows);
   // This lane's tiles that see more than x stages (x = -1: all).
-  auto above = [&](int x) -> int {
+  auto above = [&](int x) -> uint32_t {
     const int keys = x * kStageKeys;
-    if (x < 0) return tiles;
-    if (keys >= n_k) return 0;
     const int y = causal ? keys - history : 0;  // of its last row's token at least
-    return y <= 0 ? tiles : max(tiles - (int)((uint32_t)y * group / kTileRows), 0);
+    const int more = y <= 0 ? tiles : max(tiles - (int)((uint32_t)y * group / kTileRows), 0);
+    return x < 0 ? tiles : keys >= n_k ? 0 : more;
   };
-  auto all = [&](int v) -> int { return __builtin_amdgcn_readfirstlane((int)sum_lanes((uint32_t)v)); };
-  which = -1;
-  if (rank >= all(tiles)) return;
+  auto first = [](uint32_t v) -> int { return __builtin_amdgcn_readfirstlane((int)v); };
+  const int all = first(sum_lanes(tiles));
   // The smallest x that at most `rank` tiles see more than.
-  int lo = -1, hi = (__builtin_amdgcn_readfirstlane((int)max_lanes((uint32_t)n_k)) + kStageKeys - 1) / kStageKeys;
+  int lo = -1, hi = (first(max_lanes((uint32_t)n_k)) + kStageKeys - 1) / kStageKeys;
+  which = -1;
+  if (rank >= all) return;
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (all(above(mid)) <= rank) hi = mid; else lo = mid;
+    const int step = (hi - lo + 4) / 5;
+    int x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = min(lo + (i + 1) * step, hi);
+    const uint32_t low = first(sum_lanes(above(x[0]) | above(x[1]) << 16));
+    const uint32_t high = first(sum_lanes(above(x[2]) | above(x[3]) << 16));
+    const int counts[4] = {(int)(low & 0xFFFF), (int)(low >> 16), (int)(high & 0xFFFF), (int)(high >> 16)};
+    int below = lo;
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+      if (counts[i] <= rank) hi = x[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (counts[i] > rank) below = x[i];
+    lo = below;
   }
   const int more = above(hi), same = above(hi - 1) - more;
-  int before = same;  // of the lanes below, then
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(before, d, 64);
-    if (lane >= d) before += up;
-  }
-  before -= same;
-  const int place = rank - all(more) - before;
+  const int place = rank - first(sum_lanes(more)) - (int)sum_below((uint32_t)same);
   const uint64_t mine = __builtin_amdgcn_ballot_w64(place >= 0 && place < same);
   if (mine == 0) return;
   which = __builtin_ctzll(mine);
@@ -121,8 +126,9 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
   // ---- which row tile, KV head and split. Work-groups go round the XCDs by
   // linear id: with a multiple of 8 KV heads each XCD takes whole heads, whose
   // keys its L2 then holds. `rank` goes over the row tiles, longest first.
-  // (All of this in 32 bits, which hold the rows of a call: divisions of 64 bits made
-  // the start of a work-group YYY.)
+  // (All of this in 32 bits, which hold the rows of a call: with divisions of 64
+  // bits and sequences found by bisection the start of a work-group took 5.3k cycles,
+  // so 2.8k.)
   const uint32_t group = group_;
   const uint32_t unit = splits == 1 ? blockIdx.x : blockIdx.x / (uint32_t)splits;
   const int split = (int)(blockIdx.x - unit * (uint32_t)splits);
@@ -488,10 +494,11 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
   p.slots = rows / (p.few ? FewRows::kRows : ManyRows::kRows) + sequences;
   const int64_t units = p.slots * kv_heads;
   const int64_t round = 2 * device_cu_count();  // two work-groups per CU
-  // Tiles by rank where the work-groups are at most a round and a half: 8,140 tokens
-  // in 13 sequences, 8 heads of 64 dims (608 work-groups) 32.7 -> 26.1 us, 4,434 in 8,
-  // 16 heads of 192 / 128 (672) 40.1 -> 38.0; with 64 heads (2,688) 125.8 -> 134.3.
-  p.ranked = !p.few && sequences > 1 && sequences <= 64 && 2 * units <= 3 * round;
+  // Tiles by rank where the work-groups are at most two rounds: 4,434 tokens in 8
+  // sequences, 16 heads of 192 / 128 (672 work-groups) 34.7 -> 31.5 us, 3,000 in 3, 32
+  // heads of 128 (832) 46.9 -> 45.2. With more, neighbours of different sequences cost
+  // more in L2 than the order gives: 32 heads of the first (1,344) 52.7 -> 58.7.
+  p.ranked = !p.few && sequences > 1 && sequences <= 64 && units <= 2 * round;
   p.splits = 1;
   // Stages of a row tile, if a sequence is as long as the others, and of the longest
   // (taken for twice that, of single tokens four times, where it is not given).
