@@ -438,7 +438,7 @@ __global__ __launch_bounds__(64 * kWays * kChunks) void join_parts(
     const int32_t* __restrict__ cu, int32_t branches, int64_t heads, uint16_t* __restrict__ out) {
   __shared__ v4f shared[kWays][kChunks][64];
   __shared__ float2 of_way[kWays][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int way = wave % kWays, chunk = wave / kWays;
   constexpr int kPerGroup = kVDim / 8 / kChunks;  // work-groups of 32 rows
   const int64_t row = (int64_t)(blockIdx.x / kPerGroup) * 32 + (lane & 31);
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(64 * kWays * kChunks) void join_parts(
       for (int i = 0; i < kAtOnce; ++i) {
         const int s = s0 + i * kWays;
         st[i] = s < splits ? stats[s * rows + row] : make_float2(none, 0.0f);
-        o[i] = *reinterpret_cast<const v4f*>(parts + part_at(min(s, splits - 1), rows, row, dim4));
+        o[i] = s < splits ? *reinterpret_cast<const v4f*>(parts + part_at(s, rows, row, dim4)) : v4f{};
       }
       float up = top;
 #pragma unroll
@@ -506,11 +506,12 @@ int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t
     hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 31) / 32 * (kVDim / 8 / chunks))), dim3(64 * ways * chunks), 0,
                        stream, a.parts, a.stats, rows, splits, a.cu_q, a.branches, (int64_t)a.heads, a.out);
   };
-  // Ways for the parts there are; 16 where the rows alone do not fill the chip (171
-  // parts of 128 rows: 9.9 us with 16, 12.3 with 4; 68 of 256: 9.2 and 9.0; 34 of 640:
-  // 11.8 and 9.3).
+  // Ways for the parts there are (14 parts of 2,048 rows: 11.0 us with 2, 13.6 with 4;
+  // 91 of 256: 10.9 and 9.0); 16 where the rows alone do not fill the chip (171 of 128:
+  // 9.9 us, with 4 12.3).
   if (splits <= 4) go(join_parts<1, 4>, 1, 4);
-  else if (splits <= 32 || rows >= 256) go(join_parts<4, 2>, 4, 2);
+  else if (splits <= 32) go(join_parts<2, 4>, 2, 4);
+  else if (rows >= 256) go(join_parts<4, 2>, 4, 2);
   else go(join_parts<16, 1>, 16, 1);
   DSA_CHECK_LAUNCH("join of the shared prefix's parts");
   return kOk;
