@@ -155,11 +155,9 @@ __device__ __forceinline__ float row_max(const v16f& s, float scale_log2) {
   return max_halves(mx) * scale_log2;
 }
 
-// Whether a row's running maximum has to rise to take in scores up to mx.
-__device__ __forceinline__ bool must_raise(const RowState& row, float mx) {
-  const float none = -__builtin_inff();
-  return mx > row.top + kLazyRescale || (row.top == none && mx != none);
-}
+// Whether a row's running maximum (-inf: no visible key so far) has to rise to take in
+// scores up to mx.
+__device__ __forceinline__ bool must_raise(const RowState& row, float mx) { return mx > row.top + kLazyRescale; }
 
 // Raises it; returns the factor for what was summed before (1 with no visible key so
 // far: those sums are zeros, which are not worth a pass over the accumulators).

@@ -52,9 +52,8 @@ constexpr int kQLds = 8;
 constexpr int kQReg = kSteps - kQLds;
 constexpr int kQBytes = kQLds * 4 * 1024;  // [wave][step][lane] 16 bytes
 
-// Source of keys past the end and pages outside the cache: zeros, so that what a
-// masked key's p = 0 multiplies is finite.
-__device__ __align__(16) uint8_t zero_record[kRecordBytes + 16];
+// A buffer's last word: 32-bit words, no swizzle.
+constexpr int kRawBuffer = 0x00027000;
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -186,45 +185,43 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     if (b >= b1) return -1;
     return b < prefix_blocks ? a.prefix_table[b >> 1] : suffix_table[(b - prefix_blocks) >> 1];
   };
-  // Valid keys of block b on `page`, and its half of the page.
+  // Valid keys of block b on `page`.
   const uint32_t pages = (uint32_t)a.pages;
   auto keys_of = [&](int b, int page) -> int {
     const int left = b < prefix_blocks ? (int)prefix - b * kBlockKeys : (int)suffix - (b - prefix_blocks) * kBlockKeys;
     return (uint32_t)page < pages ? min(left, kBlockKeys) : 0;
   };
-  typedef v4u Staged[6];
-  const uint32_t fetch_lane = (uint32_t)kk * kRecordBytes + 16 * j8;
-  const uint32_t scale_lane = (uint32_t)kk * kRecordBytes + kVDim;
-  auto fetch = [&](Staged& st, int b, int page) __attribute__((always_inline)) {
-    const int keys = keys_of(b, page);
+  // Its records as a buffer that ends with them: what lies behind reads as zeros, so
+  // that what a masked key's p = 0 multiplies is finite. (A block without keys is on no
+  // page; its address is not used.)
+  auto records_of = [&](int b, int page, int keys) {
     const int half = (b < prefix_blocks ? b : b - prefix_blocks) & 1;
-    // (A block without keys is on no page; its address is not used.)
     const uint8_t* from = a.cache + (keys > 0 ? ((int64_t)page * kPageTokens + half * kBlockKeys) * kRecordBytes : 0);
-    if (keys == kBlockKeys) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(from + (fetch_lane + 128 * i));
-      st[4] = *reinterpret_cast<const v4u*>(from + scale_lane);
-      st[5] = *reinterpret_cast<const v4u*>(from + (fetch_lane + (kVDim + 16)));
-    } else {
-      const uint8_t* rec = kk < keys ? from + kk * kRecordBytes : zero_record;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const v4u*>(rec + 128 * i + 16 * j8);
-      st[4] = *reinterpret_cast<const v4u*>(rec + kVDim);
-      st[5] = *reinterpret_cast<const v4u*>(rec + kVDim + 16 + 16 * j8);
-    }
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, keys * kRecordBytes, kRawBuffer);
   };
-  // Chunk i of the landed record (4: the RoPE part) as bf16 into the block's row.
-  auto unpack = [&](const Staged& st, uint32_t to, int i) __attribute__((always_inline)) {
-    if (i == 4) {
+  typedef v4u Staged[6];
+  const int fetch_lane = kk * kRecordBytes + 16 * j8, scale_lane = kk * kRecordBytes + kVDim;
+  // Vector i of the staged ones: chunks 0 .. 3, the scales, the RoPE part.
+  auto fetch = [&](Staged& st, auto records, int i) __attribute__((always_inline)) {
+    st[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(
+        records, i == 4 ? scale_lane : fetch_lane + (i == 5 ? kVDim + 16 : 128 * i), 0, 0));
+  };
+  // Part u of the landed record: half u & 1 of chunk u / 2 as bf16 (word by word, of
+  // which `words` of one call are converted), from u = 8 on the RoPE part.
+  v4u converted;
+  auto unpack = [&](const Staged& st, uint32_t to, int u, int from, int words) __attribute__((always_inline)) {
+    if (u == 8) {
       lds_store<v4u>(to + 2 * kVDim - 16 * j8, st[5]);
       return;
     }
-    const float scale = __builtin_bit_cast(v4f, st[4])[i];
-    const v4u w = st[i];
-    lds_store<v4u>(to + 256 * i, v4u{dequant_pair<false>(w.x, scale), dequant_pair<true>(w.x, scale),
-                                     dequant_pair<false>(w.y, scale), dequant_pair<true>(w.y, scale)});
-    lds_store<v4u>(to + 256 * i + 16, v4u{dequant_pair<false>(w.z, scale), dequant_pair<true>(w.z, scale),
-                                          dequant_pair<false>(w.w, scale), dequant_pair<true>(w.w, scale)});
+    const float scale = __builtin_bit_cast(v4f, st[4])[u >> 1];
+#pragma unroll
+    for (int w = from; w < from + words; ++w) {
+      const uint32_t codes = st[u >> 1][2 * (u & 1) + w];
+      converted[2 * w] = dequant_pair<false>(codes, scale);
+      converted[2 * w + 1] = dequant_pair<true>(codes, scale);
+    }
+    if (from + words == 2) lds_store<v4u>(to + 256 * (u >> 1) + 16 * (u & 1), converted);
   };
   const uint32_t store_lane = (uint32_t)kk * kRowBytes + 32 * j8;
   // Buffers go round: the one after `at` (an address within it).
@@ -269,41 +266,57 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto values = [&](uint32_t at, v4u (&vop)[kAhead], const v4u (&p)[2], auto slice) __attribute__((always_inline)) {
+  // Products from .. to - 1 of the block at `at` with V.
+  auto values = [&](uint32_t at, v4u (&vop)[kAhead], const v4u (&p)[2], int from, int to, auto slice)
+                    __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kVops; ++i) {
+    for (int i = from; i < to; ++i) {
       o[i >> 1] = E::mfma(vop[i % kAhead], p[i & 1], o[i >> 1]);
       if (i + kAhead < kVops) vop[i % kAhead] = read_v(at, i + kAhead);
       slice(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto mask = [&](int b, int page, v16f& s) __attribute__((always_inline)) {
-    const int seen = keys_of(b, page);
+  auto mask = [&](int seen, v16f& s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = tile_key(8 * (i >> 2) + 4 * h + (i & 3)) < seen ? s[i] : -__builtin_inff();
   };
-  auto needs_mask = [&](int b, int page) -> bool { return keys_of(b, page) < kBlockKeys; };
 
   // ---- pipeline. Step b: scores of block b + 1 beside the probabilities of
   // block b, then block b's product with V beside the conversion of block b + 2
   // into LDS; block b + 3's records are on their way. One barrier per step; three
   // buffers.
-  int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
+  // Valid keys of blocks b, b + 1 and b + 2; the page of block b + 3.
+  int keys, keys1, keys2, page3 = page_of(b0 + 3);
   Staged st;
   {
     // The first two blocks on their way together.
+    const int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
+    keys = keys_of(b0, page), keys1 = keys_of(b0 + 1, page1), keys2 = keys_of(b0 + 2, page2);
     Staged first;
-    fetch(first, b0, page);
-    fetch(st, b0 + 1, page1);
+    const auto from = records_of(b0, page, keys), from1 = records_of(b0 + 1, page1, keys1),
+               from2 = records_of(b0 + 2, page2, keys2);
 #pragma unroll
-    for (int i = 0; i < 5; ++i) unpack(first, lds_base + store_lane, i);
+    for (int i = 0; i < 6; ++i) fetch(first, from, i);
 #pragma unroll
-    for (int i = 0; i < 5; ++i) unpack(st, lds_base + kBufBytes + store_lane, i);
-    fetch(st, b0 + 2, page2);
+    for (int i = 0; i < 6; ++i) fetch(st, from1, i);
+#pragma unroll
+    for (int u = 0; u < 9; ++u) unpack(first, lds_base + store_lane, u, 0, 2);
+#pragma unroll
+    for (int u = 0; u < 9; ++u) unpack(st, lds_base + kBufBytes + store_lane, u, 0, 2);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) fetch(st, from2, i);
 #pragma unroll
     for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
   }
+  // On to the next block: block b + 3's records, whose page is asked for a step ahead.
+  auto advance = [&](int b) {
+    const int keys3 = keys_of(b + 3, page3);
+    const auto from = records_of(b + 3, page3, keys3);
+    page3 = page_of(b + 4);
+    keys = keys1, keys1 = keys2, keys2 = keys3;
+    return from;
+  };
 #pragma unroll
   for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
   lds_barrier();
@@ -328,8 +341,8 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     uint32_t k_now = read_first_k(now);
     auto step = [&](const v16f& from, v16f& to) __attribute__((always_inline)) -> int {
       if (b + 1 == b1) return kDone;
+      const auto from3 = advance(b);
       ++b;
-      const int page3 = page_of(b + 2);
       const uint32_t at = opaque(now + v_lane);
       now = after(now);
       v4u vop[kAhead];
@@ -337,26 +350,33 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
         soften(from, i, kSteps);
         if (i >= kSteps - kAhead) vop[i - (kSteps - kAhead)] = read_v(at, i - (kSteps - kAhead));
       });
+      // Computed by here, beside the products, not where they are used.
+      asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(row.sum));
       const uint32_t ahead = after(now);
       const uint32_t store = opaque(ahead + store_lane);
       float top = -__builtin_inff();
-      values(at, vop, p, [&](int i) __attribute__((always_inline)) {
-        if (i % 4 == 0 && i < 20) unpack(st, store, i / 4);
-        if (i == 20) fetch(st, b + 2, page3);
+      // Two words of a record converted at a time, and its place taken by the next.
+      values(at, vop, p, 0, kVops - kAhead, [&](int i) __attribute__((always_inline)) {
+        if (i < 16) unpack(st, store, i >> 1, i & 1, 1);
+        if (i == 16) unpack(st, store, 8, 0, 2);
+        if (i % 4 == 0 && i > 0 && i <= 16) fetch(st, from3, i / 4 - 1);
+        if (i == 18) fetch(st, from3, 5);
+        if (i == 20) fetch(st, from3, 4);
         if (i >= 8 && i < 16) top = fmaxf(fmaxf(top, to[2 * (i - 8)]), to[2 * (i - 8) + 1]);
       });
+      // The last products' operands are in registers: the next block's first are read
+      // beside them.
       lds_barrier();
       k_now = read_first_k(ahead);
       const float mx = max_halves(top) * a.scale_log2;
-      page = page1;
-      page1 = page2;
-      page2 = page3;
-      return needs_mask(b, page) || __builtin_amdgcn_ballot_w64(must_raise(row, mx)) != 0 ? kBreak : kGo;
+      const uint64_t rise = __builtin_amdgcn_ballot_w64(must_raise(row, mx));
+      values(at, vop, p, kVops - kAhead, kVops, no_slice);
+      return keys < kBlockKeys || rise != 0 ? kBreak : kGo;
     };
     scores(k_now, s, no_slice);
     k_now = read_first_k(after(now));
     for (bool more = true; more;) {
-      if (needs_mask(b, page)) mask(b, page, s);
+      if (keys < kBlockKeys) mask(keys, s);
       const float factor = raise(row, row_max(s, a.scale_log2));
       shift = shift_of(row);
       if (__builtin_amdgcn_ballot_w64(factor != 1.0f)) {
@@ -383,15 +403,16 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) vop[i] = read_v(at, i);
     soften(s, 0, 1);
-    values(at, vop, p, no_slice);
+    values(at, vop, p, 0, kVops, no_slice);
   } else {
     // A wave without rows stages its keys all the same.
     uint32_t to = lds_base + 2 * kBufBytes;
-    for (int b = b0 + 1; b < b1; ++b, to = after(to)) {
-      const int page3 = page_of(b + 2);
+    for (int b = b0; b + 1 < b1; ++b, to = after(to)) {
+      const auto from3 = advance(b);
 #pragma unroll
-      for (int i = 0; i < 5; ++i) unpack(st, to + store_lane, i);
-      fetch(st, b + 2, page3);
+      for (int u = 0; u < 9; ++u) unpack(st, to + store_lane, u, 0, 2);
+#pragma unroll
+      for (int i = 0; i < 6; ++i) fetch(st, from3, i);
       lds_barrier();
     }
   }
