@@ -6,25 +6,30 @@
 // 16-bit inputs, probabilities rounded to 16 bits before the product with V;
 // a query without a visible key gives zeros. 2 (d_qk + d_v) flop per pair.
 //
-// Mapping (gfx950, wave64). The G heads that share a KV head are rows of one
-// problem: row r of a sequence is token r / G, head r % G, so that single tokens
-// of grouped heads fill a tile and K and V are staged once for all of them. A
-// work-group of four waves (one per SIMD) owns 256 rows, 64 per wave, and walks
-// the keys in stages of 64. A wave computes S^T = K Q^T (v_mfma_f32_32x32x16,
-// Q^T in registers) for 32 keys at a time and its two tiles of 32 rows: each
-// operand read from LDS feeds two products, which keeps LDS at half of what it
-// can deliver (64 of ~115 B a cycle with one wave per SIMD; with 32 rows per
-// wave it would be the bound). The result's layout - a lane holds 16 keys of one
-// row - is the operand layout of O^T += V^T P^T once the keys of V^T are read in
-// the same order, so probabilities never leave registers and a row's softmax
-// state and rescale factor belong to its lane.
-// Software pipeline: the products S of 32 keys run beside the softmax of the 32
-// keys before, then those keys' product with V.
+// Mapping (gfx950, wave64). The G heads that share a KV head are rows of one problem:
+// row r of a sequence is token r / G, head r % G, so that single tokens of grouped
+// heads fill a tile and K and V are staged once for all of them. A work-group has 128
+// rows, 32 per wave, two work-groups share a CU (one's start, masks and stores run
+// beside the other's products; 256 rows of one work-group took 285 us where these take
+// 200: 2,048 tokens, 128 heads of 192 / 128), and walks the keys in stages of 32. A
+// wave computes S^T = K Q^T (v_mfma_f32_32x32x16, Q^T in registers). The result's layout
+// - a lane holds 16 keys of one row - is the operand layout of O^T += V^T P^T once the
+// keys of V^T are read in the same order, so probabilities never leave registers and a
+// row's softmax state and rescale factor belong to its lane.
+// Software pipeline: the products S of a stage run beside the softmax of the stage
+// before, then that stage's product with V beside the maxima of the new one.
 //
-// Stages arrive by LDS DMA two ahead, in blocks of 16 rows by 64 bytes: lane l
-// brings chunk (l % 4) ^ (l / 16) (16 bytes) of row l / 4, which makes global
-// reads whole 64-byte segments and both the K reads (16 rows, one chunk) and the
-// transposing V reads (4 rows, 4 chunks) free of bank conflicts.
+// What bounds it: in long calls the matrix unit at the clock that the power limit leaves
+// (1.84 GHz in the call above, 860 TFLOP/s; 8,192 tokens 1.1 PFLOP/s, where a library
+// product of large matrices reaches 1.36); in batches of short sequences the start and end
+// of a work-group, 9k to 15k cycles (7 prompts of 4,001 tokens, 42 us); with few rows the
+// loads of K and V (8 single tokens over 40,000 keys, 31 us and 4 for the join, 4.7 TB/s).
+// Q loads and stores in pieces of 64 bytes, by lanes trading, took as long as they save.
+//
+// Stages arrive by LDS DMA two ahead, in blocks of 16 rows by 64 bytes: lane l brings
+// chunk (l % 4) ^ (l / 16) (16 bytes) of row l / 4, which makes global reads whole
+// 64-byte segments and both the K reads (16 rows, one chunk) and the transposing V
+// reads (4 rows, 4 chunks) free of bank conflicts.
 #include "attention_core.h"
 #include "../../include/dsa_gfx950.h"
 
@@ -465,8 +470,8 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
 
 // The cut of a call. Rows of a sequence and KV head that fill a wave at most (single
 // tokens): work-groups of one wave, two of them per CU; a wave alone in a work-group
-// of eight would walk every key by itself, which bounds the call, not memory. Others:
-// eight waves, 256 rows.
+// of several would walk every key by itself, which bounds the call, not memory (8 single
+// tokens over 40,000 keys 67 -> 44 us). Others: four waves, 128 rows.
 using FewRows = Cut<1, 2>;
 using ManyRows = Cut<4, 2>;
 

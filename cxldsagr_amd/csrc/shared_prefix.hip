@@ -21,10 +21,15 @@
 // rows, and O^T += V^T P^T with the probabilities where the scores were (the keys
 // of V^T are read in the order in which a lane holds its scores). O^T takes 256 of
 // a lane's 512 registers and Q^T 112 (the last 8 of its 36 operands are read from
-// LDS). Per 32 keys a SIMD has 68 products of 32 cycles, 2.2k cycles, while the CU
-// reads 304 KB of LDS and writes 37 KB, about 3.4k cycles at the ~115 and ~49 bytes
-// a cycle that one wave per SIMD reaches: LDS is the bound, and a row tile of 32
-// per wave (each operand read feeds one product) is what registers allow.
+// LDS); more rows per wave, for which an operand read would feed two products, do not
+// fit. Per 32 keys a SIMD has 68 products of 32 cycles, 2.2k cycles, while the CU
+// reads 304 KB of LDS and writes 37 KB, about 3.1k at 128 and 49 bytes a cycle; a step
+// takes 3.9k cycles. What bounds long calls is power: with steps of 4.5k cycles the
+// clock was 2.31 GHz and a step 1.95 us, with 3.9k it is 2.04 GHz and 1.92 us, and half
+// of the LDS reads left out would give 6 %. 64 tokens of 128 heads over 65,600 keys
+// take 996 us, 1.17 PFLOP/s, where a library product of large matrices reaches 1.36.
+// Short calls are bound by a work-group's start and end (17 us of a round) and by the
+// parts of split rows (one token over 32,896 keys: 27 us and 11 for the join).
 #include "attention_core.h"
 #include "../../include/dsa_gfx950.h"
 
@@ -86,8 +91,8 @@ __device__ __forceinline__ uint32_t dequant_pair(uint32_t word, float scale) {
 
 // Where four dims (of `dim4` fours) of a row's part begin: rows in groups of 32, a
 // group's [dim4][row] as the lanes of an accumulator have them, so that a store of
-// both halves is 1 KB in one piece (by rows, pieces of 32 bytes, the stores of 128
-// rows took 16k cycles; so 9k).
+// both halves is 1 KB in one piece (by rows, in pieces of 32 bytes, the stores of 128
+// rows took 16k cycles).
 __device__ __forceinline__ int64_t part_at(int64_t part, int64_t rows, int64_t row, int dim4) {
   const int64_t groups = (rows + 31) >> 5;
   return (((part * groups + (row >> 5)) * (kVDim / 4) + dim4) * 32 + (row & 31)) * 4;
@@ -311,8 +316,9 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   }
   // On to the next block: block b + 3's records, whose page is asked for a step ahead.
   auto advance = [&](int b) {
-    const int keys3 = keys_of(b + 3, page3);
-    const auto from = records_of(b + 3, page3, keys3);
+    const int page = __builtin_amdgcn_readfirstlane(page3);
+    const int keys3 = keys_of(b + 3, page);
+    const auto from = records_of(b + 3, page, keys3);
     page3 = page_of(b + 4);
     keys = keys1, keys1 = keys2, keys2 = keys3;
     return from;
