@@ -186,23 +186,26 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   // ---- staging: eight lanes a key. Lane j brings bytes 128 i + 16 j of the
   // latent (a chunk of every tile), the scales, and bytes 16 j of the RoPE part.
   const int kk = threadIdx.x >> 3, j8 = threadIdx.x & 7;
+  // (Selections, not branches, in what a step needs for a block to come; blocks from b1
+  // on have the last one's page, and no keys.)
   auto page_of = [&](int b) -> int {
-    if (b >= b1) return -1;
-    return b < prefix_blocks ? a.prefix_table[b >> 1] : suffix_table[(b - prefix_blocks) >> 1];
+    const int c = min(b, b1 - 1), own = c - prefix_blocks;
+    return (own < 0 ? a.prefix_table : suffix_table)[(own < 0 ? c : own) >> 1];
   };
   // Valid keys of block b on `page`.
   const uint32_t pages = (uint32_t)a.pages;
   auto keys_of = [&](int b, int page) -> int {
-    const int left = b < prefix_blocks ? (int)prefix - b * kBlockKeys : (int)suffix - (b - prefix_blocks) * kBlockKeys;
-    return (uint32_t)page < pages ? min(left, kBlockKeys) : 0;
+    const int own = b - prefix_blocks;
+    const int left = own < 0 ? (int)prefix - b * kBlockKeys : (int)suffix - own * kBlockKeys;
+    return (b < b1) & ((uint32_t)page < pages) ? min(left, kBlockKeys) : 0;
   };
   // Its records as a buffer that ends with them: what lies behind reads as zeros, so
-  // that what a masked key's p = 0 multiplies is finite. (A block without keys is on no
-  // page; its address is not used.)
+  // that what a masked key's p = 0 multiplies is finite.
   auto records_of = [&](int b, int page, int keys) {
     const int half = (b < prefix_blocks ? b : b - prefix_blocks) & 1;
-    const uint8_t* from = a.cache + (keys > 0 ? ((int64_t)page * kPageTokens + half * kBlockKeys) * kRecordBytes : 0);
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, keys * kRecordBytes, kRawBuffer);
+    const int64_t row = (int64_t)(keys > 0 ? page : 0) * kPageTokens + half * kBlockKeys;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.cache + row * kRecordBytes), 0,
+                                             keys * kRecordBytes, kRawBuffer);
   };
   typedef v4u Staged[6];
   const int fetch_lane = kk * kRecordBytes + 16 * j8, scale_lane = kk * kRecordBytes + kVDim;
@@ -292,11 +295,12 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   // into LDS; block b + 3's records are on their way. One barrier per step; three
   // buffers.
   // Valid keys of blocks b, b + 1 and b + 2; the page of block b + 3.
-  int keys, keys1, keys2, page3 = page_of(b0 + 3);
+  int keys, keys1, keys2, page3 = -1;
   Staged st;
   {
     // The first two blocks on their way together.
-    const int page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2);
+    int page = -1, page1 = -1, page2 = -1;
+    if (b1 > b0) page = page_of(b0), page1 = page_of(b0 + 1), page2 = page_of(b0 + 2), page3 = page_of(b0 + 3);
     keys = keys_of(b0, page), keys1 = keys_of(b0 + 1, page1), keys2 = keys_of(b0 + 2, page2);
     Staged first;
     const auto from = records_of(b0, page, keys), from1 = records_of(b0 + 1, page1, keys1),
