@@ -632,24 +632,40 @@ __device__ __forceinline__ uint32_t reduce_16(uint32_t v, Op op) {
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
   return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
 }
-__device__ __forceinline__ uint32_t add_bits(uint32_t x, uint32_t y) {
-  return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+// The sum of a 64-bit value over the wave, by the same moves and then over the rows.
+__device__ __forceinline__ double sum_64(double v) {
+  auto add = [&](auto move) {
+    const uint2 own = __builtin_bit_cast(uint2, v);
+    v += __builtin_bit_cast(double, make_uint2(move(own.x), move(own.y)));
+  };
+  add([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false); });
+  add([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false); });
+  add([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false); });
+  add([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, false); });
+  const uint2 row = __builtin_bit_cast(uint2, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(row.x, row.x, false, false);
+  const auto y = __builtin_amdgcn_permlane16_swap(row.y, row.y, false, false);
+  v = __builtin_bit_cast(double, make_uint2(x[0], y[0])) + __builtin_bit_cast(double, make_uint2(x[1], y[1]));
+  const uint2 both = __builtin_bit_cast(uint2, v);
+  const auto z = __builtin_amdgcn_permlane32_swap(both.x, both.x, false, false);
+  const auto w = __builtin_amdgcn_permlane32_swap(both.y, both.y, false, false);
+  return __builtin_bit_cast(double, make_uint2(z[0], w[0])) + __builtin_bit_cast(double, make_uint2(z[1], w[1]));
 }
-__device__ __forceinline__ float sum_64(float f) {
-  uint32_t v = reduce_16(__float_as_uint(f), add_bits);
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = add_bits(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return __uint_as_float(add_bits(b[0], b[1]));
+// x^-1/2: the instruction's estimate (to about 2^-23) and one Newton step, which an
+// estimate of 0 or infinity does not take.
+__device__ __forceinline__ double inverse_sqrt(double x) {
+  const double r = __builtin_amdgcn_rsq(x);
+  return r > 0.0 && r < __builtin_inf() ? r * (1.5 - 0.5 * x * r * r) : r;
 }
 
 // New tokens into any slots of the fp8 paged cache: the latent through RMSNorm
-// (fp32, x * rsqrt(mean x^2 + eps) * w, rounded to bf16, which is what a model's
-// norm hands on), the RoPE part rotated (fp32, rounded to bf16), then the record of
+// (x (mean x^2 + eps)^-1/2 w, the lanes' sums added in 64 bits, rounded to bf16, which is what a model's norm
+// hands on: with fp32 sums and products 13 to 24 of 33 million codes were not the
+// formula's, so 0 to 3, for 1.6 us of 65,536 tokens), the RoPE part rotated (fp32, rounded to bf16), then the record of
 // pack_tokens. A wave takes kTokens tokens whose loads are all issued first: lane l
 // has 8 latent values of each, and a half wave the 32 rotary pairs of every other
 // one. Bound by memory, 1,152 B read and 656 B written per token, once enough loads
-// are in flight: 65,536 tokens took 35.6 us (3.3 TB/s) with one token per wave and
+// are in flight: 65,536 tokens take 27.9 us (4.2 TB/s), 35.6 with one token per wave and
 // reductions through LDS permutes.
 template <int kTokens>
 __global__ __launch_bounds__(256) void write_kv(const WriteArgs a) {
@@ -701,17 +717,26 @@ __global__ __launch_bounds__(256) void write_kv(const WriteArgs a) {
       const float4 w0 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane);
       const float4 w1 = *reinterpret_cast<const float4*>(a.norm_weight + 8 * lane + 4);
       const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      float sum = 0.0f;
+      // (A lane's eight squares in 32 bits: over the lanes their roundings average out.)
+      float part = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
-      const float norm = 1.0f / __builtin_sqrtf(sum_64(sum) * (1.0f / 512.0f) + a.eps);
-      // Rounded to nearest even by v_cvt_pk_bf16_f32 (a NaN stays one).
+      for (int i = 0; i < 8; ++i) part = __builtin_fmaf(v[i], v[i], part);
+      const double norm = inverse_sqrt(sum_64((double)part) * (1.0 / 512.0) + (double)a.eps);
+      // The product v norm w rounded once, in 32 bits: norm as the sum of two floats,
+      // and what v norm lost to rounding added where it is multiplied by w. Then to bf16
+      // by v_cvt_pk_bf16_f32 (nearest even; a NaN stays one).
+      const float high = (float)norm, low = (float)(norm - (double)high);
+      auto normed_value = [&](int i) -> float {
+        const float p = v[i] * high;
+        const float rest = __builtin_fmaf(v[i], low, __builtin_fmaf(v[i], high, -p));
+        return __builtin_fmaf(p, w[i], rest * w[i]);
+      };
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         typedef __bf16 Pair __attribute__((ext_vector_type(2)));
         typedef float Two __attribute__((ext_vector_type(2)));
-        const uint32_t two = __builtin_bit_cast(
-            uint32_t, __builtin_convertvector((Two){v[2 * i] * norm * w[2 * i], v[2 * i + 1] * norm * w[2 * i + 1]}, Pair));
+        const Two normed = {normed_value(2 * i), normed_value(2 * i + 1)};
+        const uint32_t two = __builtin_bit_cast(uint32_t, __builtin_convertvector(normed, Pair));
         v[2 * i] = bf16_to_f32(two & 0xFFFFu);
         v[2 * i + 1] = bf16_to_f32(two >> 16);
       }
@@ -809,7 +834,7 @@ extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t token
   const WriteArgs a{static_cast<const uint16_t*>(kv), kv_stride, tokens, pages * 64, slots, norm_weight, norm_eps,
                     positions, frequencies, magnitude, wide_slots != 0, wide_positions != 0, interleaved != 0,
                     static_cast<uint8_t*>(cache), status};
-  // One token per wave while waves are few, then two (65,536 tokens: one 29.6 us, two
+  // One token per wave while waves are few, then two (65,536 tokens, norms in fp32: one 29.6 us, two
   // 26.9, four 30.4).
   if (tokens <= 4096)
     hipLaunchKernelGGL(write_kv<1>, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, stream, a);
