@@ -23,12 +23,11 @@
 // a lane's 512 registers and Q^T 112 (the last 8 of its 36 operands are read from
 // LDS); more rows per wave, for which an operand read would feed two products, do not
 // fit. Per 32 keys a SIMD has 68 products of 32 cycles, 2.2k cycles, while the CU
-// reads 304 KB of LDS and writes 37 KB, about 3.1k at 128 and 49 bytes a cycle; a step
-// takes 3.9k cycles. What bounds long calls is power: with steps of 4.5k cycles the
-// clock was 2.31 GHz and a step 1.95 us, with 3.9k it is 2.04 GHz and 1.92 us, and half
-// of the LDS reads left out would give 6 %. 64 tokens of 128 heads over 65,600 keys
-// take 996 us, 1.17 PFLOP/s, where a library product of large matrices reaches 1.36.
-// Short calls are bound by a work-group's start and end (17 us of a round) and by the
+// reads 304 KB of LDS and writes 37 KB, about 3.1k at 128 and 49 bytes a cycle. What
+// bounds long calls is that and power: steps of 4.5k cycles ran at 2.31 GHz in 1.95 us,
+// of 3.9k at 2.04 GHz in 1.92 us, and with fewer waits and scalar instructions 1.75; half
+// of the LDS reads left out gave 6 %. 64 tokens of 128 heads over 65,600 keys take 928
+// us, 1.26 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls are bound by a work-group's start and end (17 us of a round) and by the
 // parts of split rows (one token over 32,896 keys: 27 us and 11 for the join).
 #include "attention_core.h"
 #include "../../include/dsa_gfx950.h"
