@@ -27,8 +27,9 @@
 // bounds long calls is that and power: steps of 4.5k cycles ran at 2.31 GHz in 1.95 us,
 // of 3.9k at 2.04 GHz in 1.92 us, and with fewer waits and scalar instructions 1.75; half
 // of the LDS reads left out gave 6 %. 64 tokens of 128 heads over 65,600 keys take 928
-// us, 1.26 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls are bound by a work-group's start and end (17 us of a round) and by the
-// parts of split rows (one token over 32,896 keys: 27 us and 11 for the join).
+// us, 1.26 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls
+// are bound by a work-group's start and end (17 us of a round) and by the parts of split
+// rows (one token over 32,896 keys: 27 us and 11 for the join).
 #include "attention_core.h"
 #include "../../include/dsa_gfx950.h"
 
