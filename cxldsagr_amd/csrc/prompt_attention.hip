@@ -375,16 +375,14 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
       asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(row.sum));
       if (j + 1 < s1) enter_stage();
       next_k();
-      float top;
+      float top = -__builtin_inff();
       uint64_t rise = 0;
       values(v_at, p, [&](int i) __attribute__((always_inline)) {
         // Pairs of scores over half of the products, the check, the reads.
         constexpr int kPerSlot = kVops >= 8 ? 2 : 4;
 #pragma unroll
-        for (int u = kPerSlot * i; u < kPerSlot * (i + 1) && u < kPairs; ++u) {
-          const float m = fmaxf(to[2 * u], to[2 * u + 1]);
-          top = u == 0 ? m : fmaxf(top, m);
-        }
+        for (int u = kPerSlot * i; u < kPerSlot * (i + 1) && u < kPairs; ++u)
+          top = fmaxf(fmaxf(top, to[2 * u]), to[2 * u + 1]);
         if (i == kPairs / kPerSlot)
           rise = __builtin_amdgcn_ballot_w64(must_raise(row, max_halves(top) * a.scale_log2));
         if (i >= kVops - kAhead) read_k(k_at, i - (kVops - kAhead));
