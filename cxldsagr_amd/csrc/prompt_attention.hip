@@ -338,9 +338,16 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
   for (int i = 0; i < C::kDistance; ++i) issue();
   if (w1 > s0) {
     int j = s0;
-    uint32_t k_at = lds_k + k_lane, v_at = lds_v + v_lane;  // of stage j
-    auto next_k = [&]() { k_at = opaque(k_at - k_lane + kStageK == end_k ? lds_k + k_lane : k_at + kStageK); };
-    auto next_v = [&]() { v_at = opaque(v_at - v_lane + kStageV == end_v ? lds_v + v_lane : v_at + kStageV); };
+    uint32_t k_ring = lds_k, v_ring = lds_v;                // of stage j
+    uint32_t k_at = lds_k + k_lane, v_at = lds_v + v_lane;  // and this lane's place there
+    auto next_k = [&]() {
+      k_ring = __builtin_amdgcn_readfirstlane(k_ring + kStageK == end_k ? lds_k : k_ring + kStageK);
+      k_at = opaque(k_ring + k_lane);
+    };
+    auto next_v = [&]() {
+      v_ring = __builtin_amdgcn_readfirstlane(v_ring + kStageV == end_v ? lds_v : v_ring + kStageV);
+      v_at = opaque(v_ring + v_lane);
+    };
     v16f s, next;
     v4u p[2];
     constexpr int kPairs = 8, kTicks = kPairs + 2;
