@@ -202,6 +202,37 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
   return v;
 }
 
+// The value of lane J of a lane's quad (four neighbours).
+template <int J>
+__device__ __forceinline__ uint32_t quad_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, J * 0x55, 0xF, 0xF, true);
+}
+
+// x of the second of two lanes that kMove exchanges, and y of the first, trade places.
+template <int kMove>
+__device__ __forceinline__ void trade_lanes(uint32_t& x, uint32_t& y, bool second) {
+  const uint32_t other_x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kMove, 0xF, 0xF, true);
+  const uint32_t other_y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)y, kMove, 0xF, 0xF, true);
+  x = second ? other_y : x;
+  y = second ? y : other_x;
+}
+
+// Vector j of lane i of each quad and vector i of its lane j trade places.
+__device__ __forceinline__ void transpose_quad(v4u* w) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+  constexpr int kXor1 = 0xB1, kXor2 = 0x4E;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t v[4] = {w[0][e], w[1][e], w[2][e], w[3][e]};
+    trade_lanes<kXor1>(v[0], v[1], odd);
+    trade_lanes<kXor1>(v[2], v[3], odd);
+    trade_lanes<kXor2>(v[0], v[2], high);
+    trade_lanes<kXor2>(v[1], v[3], high);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j][e] = v[j];
+  }
+}
+
 // ------------------------------------------------- joining split keys --
 // A row's keys may be split over work-groups: split s leaves its unscaled sum of
 // p v (fp32 [splits][rows][dim]) and (maximum, sum of p) pairs ([splits][rows];

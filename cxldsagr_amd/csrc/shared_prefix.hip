@@ -20,14 +20,14 @@
 // A wave computes S^T = K Q^T (v_mfma_f32_32x32x16_bf16) for 32 keys and its 32
 // rows, and O^T += V^T P^T with the probabilities where the scores were (the keys
 // of V^T are read in the order in which a lane holds its scores). O^T takes 256 of
-// a lane's 512 registers and Q^T 112 (the last 8 of its 36 operands are read from
+// a lane's 512 registers and Q^T 96 (the last 12 of its 36 operands are read from
 // LDS); more rows per wave, for which an operand read would feed two products, do not
 // fit. Per 32 keys a SIMD has 68 products of 32 cycles, 2.2k cycles, while the CU
-// reads 304 KB of LDS and writes 37 KB, about 3.1k at 128 and 49 bytes a cycle. What
+// reads 320 KB of LDS and writes 37 KB, about 3.2k at 128 and 49 bytes a cycle. What
 // bounds long calls is that and power: steps of 4.5k cycles ran at 2.31 GHz in 1.95 us,
 // of 3.9k at 2.04 GHz in 1.92 us, and with fewer waits and scalar instructions 1.75; half
-// of the LDS reads left out gave 6 %. 64 tokens of 128 heads over 65,600 keys take 928
-// us, 1.26 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls
+// of the LDS reads left out gave 6 %. 64 tokens of 128 heads over 65,600 keys take 940
+// us, 1.24 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls
 // are bound by a work-group's start and end (17 us of a round) and by the parts of split
 // rows (one token over 32,896 keys: 27 us and 11 for the join).
 #include "attention_core.h"
@@ -52,8 +52,10 @@ constexpr int kBufBytes = kBlockKeys * kRowBytes;
 constexpr int kBuffers = 3;
 constexpr int kSteps = kQkDim / 16, kDims = kVDim / 32;
 // Q^T operands of the last kQLds steps stay in LDS, the others in registers:
-// with all 36 there, O^T (256 registers of a lane) leaves too few for the rest.
-constexpr int kQLds = 8;
+// with all 36 there, O^T (256 registers of a lane) leaves too few for the rest, and
+// with 28 the traded loads of Q spill some (loaded untraded they do not: long calls take
+// 0.8 % less, short ones 1.4 us more).
+constexpr int kQLds = 12;
 constexpr int kQReg = kSteps - kQLds;
 constexpr int kQBytes = kQLds * 4 * 1024;  // [wave][step][lane] 16 bytes
 
@@ -70,7 +72,8 @@ struct PrefixArgs {
   uint16_t* out;
   float* parts;   // with more than one split: part_at()
   float2* stats;  // [splits][tokens * heads]
-  int64_t tokens, pages, prefix;
+  int64_t pages, prefix;
+  int32_t rows, tiles;  // tokens * heads, and their tiles
   int32_t heads, branches, suffix_pages;
   int32_t joint;  // items have the prefix and the suffix
   int32_t items, splits;                  // of the row tiles of all tokens
@@ -105,60 +108,67 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
-  const int64_t all_rows = a.tokens * a.heads;
+  const int all_rows = a.rows;  // (all of this in 32 bits, which hold the rows of a call)
 
   // ---- the item: its rows, how many keys of the prefix and of a suffix they
   // see, and its range of their blocks. Items of one range are neighbours, and
   // each XCD takes an eighth of the items in that order: they read the same
   // records from its L2.
-  int64_t row0, row_end, prefix = 0, suffix = 0;
+  int row0, row_end;
+  int64_t prefix = 0, suffix = 0;
   const int32_t* suffix_table = nullptr;
   int split, splits, part;
-  int64_t token = -1;  // whose suffix the item has
+  int token = -1;  // whose suffix the item has
   if (blockIdx.x < (uint32_t)a.items) {
-    const int64_t tiles = (all_rows + kTileRows - 1) / kTileRows;
-    const int64_t item = (int64_t)(blockIdx.x & 7) * (a.items >> 3) + (blockIdx.x >> 3);
-    if (item >= tiles * a.splits) return;
-    split = part = (int)(item / tiles);
+    const uint32_t item = (blockIdx.x & 7) * ((uint32_t)a.items >> 3) + (blockIdx.x >> 3);
+    if (item >= (uint32_t)a.tiles * (uint32_t)a.splits) return;
+    split = part = (int)(item / (uint32_t)a.tiles);
     splits = a.splits;
-    row0 = (item % tiles) * kTileRows;
+    row0 = (int)(item - (uint32_t)split * (uint32_t)a.tiles) * kTileRows;
     row_end = min(row0 + kTileRows, all_rows);
     prefix = a.prefix;
-    if (a.joint) token = row0 / a.heads;
+    if (a.joint) token = (int)((uint32_t)row0 / (uint32_t)a.heads);
   } else {
-    const int64_t item = blockIdx.x - (uint32_t)a.items;
-    const int groups = (a.heads + kTileRows - 1) / kTileRows;
+    const uint32_t item = blockIdx.x - (uint32_t)a.items;
+    const uint32_t groups = ((uint32_t)a.heads + kTileRows - 1) / kTileRows;
     splits = a.suffix_splits;
-    split = (int)(item % splits);
+    const uint32_t unit = item / (uint32_t)splits;
+    split = (int)(item - unit * (uint32_t)splits);
     part = a.splits + split;
-    token = item / splits / groups;
-    const int head0 = (int)(item / splits % groups) * kTileRows;
+    token = (int)(unit / groups);
+    const int head0 = (int)(unit - (uint32_t)token * groups) * kTileRows;
     row0 = token * a.heads + head0;
     row_end = token * a.heads + min(head0 + kTileRows, (int)a.heads);
   }
   // Q^T operands, in AGPRs and the last in LDS, on their way while the keys of the
   // item are looked up.
-  const int64_t wave_row = row0 + wave * kWaveRows;
+  const int wave_row = row0 + wave * kWaveRows;
+  // Operands 4 g .. 4 g + 3 of half h are bytes 128 g + 64 h on of the lane's row, loaded
+  // as whole 64 bytes of each of its quad's rows and traded later. (With loads of 16 bytes
+  // of each of 32 rows, and divisions of 64 bits, 4.8 us went by before the first records
+  // were asked for; so 2.3. One token over 32,896 keys 38.8 -> 37.4 us.)
   v4u q_ops[kQReg], q_rest[kQLds];
-  {
-    const uint16_t* src = a.q + min(wave_row + n, all_rows - 1) * kQkDim + 8 * h;
+  static_for<4>([&](auto j) {
+    const uint32_t quad_row = quad_lane<j>((uint32_t)min(wave_row + n, all_rows - 1));
+    const uint16_t* src = a.q + (int64_t)quad_row * kQkDim + 32 * h + 8 * (lane & 3);
 #pragma unroll
-    for (int ks = 0; ks < kQReg; ++ks) q_ops[ks] = *reinterpret_cast<const v4u*>(src + 16 * ks);
+    for (int g = 0; g < kQReg / 4; ++g) q_ops[4 * g + j] = *reinterpret_cast<const v4u*>(src + 64 * g);
 #pragma unroll
-    for (int ks = 0; ks < kQLds; ++ks) q_rest[ks] = *reinterpret_cast<const v4u*>(src + 16 * (kQReg + ks));
-  }
+    for (int g = 0; g < kQLds / 4; ++g)
+      q_rest[4 * g + j] = *reinterpret_cast<const v4u*>(src + 64 * (kQReg / 4 + g));
+  });
   const uint32_t q_lds = lds_base + kBuffers * kBufBytes + (uint32_t)wave * (kQLds * 1024) + 16 * lane;
   __builtin_amdgcn_sched_barrier(0);
 
-  int64_t row_begin = row0;
+  int row_begin = row0;
   if (a.cu_q != nullptr) {
     // Rows of no branch are left alone.
-    row_begin = max(row0, a.cu_q[0] * (int64_t)a.heads);
-    row_end = min(row_end, a.cu_q[a.branches] * (int64_t)a.heads);
+    row_begin = (int)max((int64_t)row0, a.cu_q[0] * (int64_t)a.heads);
+    row_end = (int)min((int64_t)row_end, a.cu_q[a.branches] * (int64_t)a.heads);
     if (row_begin >= row_end) return;
   }
   if (token >= 0) {
-    int branch = (int)token;
+    int branch = token;
     int64_t left = 0;  // queries of the branch after this one
     if (a.cu_q != nullptr) {
       int lo = 0, hi = a.branches;  // the last branch that starts at or before it
@@ -180,7 +190,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   const int b1 = min(b0 + per_split, all_blocks);
 
   const bool live = wave_row + n < row_end && wave_row + n >= row_begin;  // this lane's row, in both halves
-  const int64_t row_at = min(wave_row + n, row_end - 1);
+  const int row_at = min(wave_row + n, row_end - 1);
   const bool active = __builtin_amdgcn_readfirstlane(wave_row < row_end && b1 > b0);
 
   // ---- staging: eight lanes a key. Lane j brings bytes 128 i + 16 j of the
@@ -238,13 +248,11 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
   };
 
   v16f o[kDims];
-#pragma unroll
-  for (int d = 0; d < kDims; ++d) o[d] = v16f{};
   RowState row{-__builtin_inff(), 0.0f};
 
-  // LDS lane addresses. K: key tile_key(n), dims 16 ks + 8 h. V: lane 4 jj + qq
+  // LDS lane addresses. K: key tile_key(n), dims 64 (ks / 4) + 32 h + 8 (ks % 4). V: lane 4 jj + qq
   // of 16-lane group g reads key 16 t + 4 jj + 2 u + h, dims 32 d + 16 (g & 1) + 4 qq.
-  const uint32_t k_lane = (uint32_t)tile_key(n) * kRowBytes + 16 * h;
+  const uint32_t k_lane = (uint32_t)tile_key(n) * kRowBytes + 64 * h;
   const uint32_t v_lane = (uint32_t)(4 * ((lane & 15) >> 2) + h) * kRowBytes + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
   constexpr int kAhead = 3, kVops = 2 * kDims;
 
@@ -254,11 +262,13 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     const v2u hi = lds_column(at + (16 * t + 2) * kRowBytes + 64 * d);
     return v4u{lo.x, lo.y, hi.x, hi.y};
   };
+  constexpr auto k_step = [](int ks) { return 128 * (ks >> 2) + 16 * (ks & 3); };
+  static_assert(kQReg % 4 == 0 && kQLds % 4 == 0, "operands in fours");
   v4u kop[kAhead];
   auto read_first_k = [&](uint32_t buffer) __attribute__((always_inline)) -> uint32_t {
     const uint32_t at = opaque(buffer + k_lane);
 #pragma unroll
-    for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at + 32 * ks);
+    for (int ks = 0; ks < kAhead; ++ks) kop[ks] = lds_load<v4u>(at + k_step(ks));
     return at;
   };
   // S of a block at `at`, whose first kAhead operands are in kop.
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
       s = E::mfma(kop[ks % kAhead], ks < kQReg ? q_ops[ks < kQReg ? ks : 0] : qop[ks & 1], s);
-      if (ks + kAhead < kSteps) kop[ks % kAhead] = lds_load<v4u>(at + 32 * (ks + kAhead));
+      if (ks + kAhead < kSteps) kop[ks % kAhead] = lds_load<v4u>(at + k_step(ks + kAhead));
       if (ks + 2 >= kQReg && ks + 2 < kSteps) qop[ks & 1] = lds_load<v4u>(q_lds + 1024 * (ks + 2 - kQReg));
       slice(ks);
       __builtin_amdgcn_sched_barrier(0);
@@ -310,13 +320,18 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
 #pragma unroll
     for (int i = 0; i < 6; ++i) fetch(st, from1, i);
 #pragma unroll
+    for (int g = 0; g < kQLds / 4; ++g) transpose_quad(&q_rest[4 * g]);
+#pragma unroll
+    for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
+#pragma unroll
+    for (int g = 0; g < kQReg / 4; ++g) transpose_quad(&q_ops[4 * g]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
     for (int u = 0; u < 9; ++u) unpack(first, lds_base + store_lane, u, 0, 2);
 #pragma unroll
     for (int u = 0; u < 9; ++u) unpack(st, lds_base + kBufBytes + store_lane, u, 0, 2);
 #pragma unroll
     for (int i = 0; i < 6; ++i) fetch(st, from2, i);
-#pragma unroll
-    for (int ks = 0; ks < kQLds; ++ks) lds_store<v4u>(q_lds + 1024 * ks, q_rest[ks]);
   }
   // On to the next block: block b + 3's records, whose page is asked for a step ahead.
   auto advance = [&](int b) {
@@ -330,6 +345,8 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
 #pragma unroll
   for (int ks = 0; ks < kQReg; ++ks) asm volatile("" : "+a"(q_ops[ks]));
   lds_barrier();
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = v16f{};
   if (active) {
     int b = b0;
     v16f s, next;
@@ -455,7 +472,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
           w[u][e] = E::pack(o[d][4 * (c + u) + 2 * e] * inv, o[d][4 * (c + u) + 2 * e + 1] * inv);
       const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
       const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-      if (live) *reinterpret_cast<v4u*>(a.out + row_at * kVDim + 32 * d + 8 * (c + h)) = v4u{x[0], y[0], x[1], y[1]};
+      if (live) *reinterpret_cast<v4u*>(a.out + (int64_t)row_at * kVDim + 32 * d + 8 * (c + h)) = v4u{x[0], y[0], x[1], y[1]};
     }
 }
 
@@ -654,7 +671,7 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   const int64_t tiles = (tokens * heads + kTileRows - 1) / kTileRows;
   const int64_t items = p.splits > 0 ? (tiles * p.splits + 7) / 8 * 8 : 0;
   const int64_t own = tokens * ((heads + kTileRows - 1) / kTileRows) * p.suffix_splits;
-  DSA_CHECK_ARG(items + own < 0x7FFFFFFF && tokens * heads < (1ll << 40), "too many query rows");
+  DSA_CHECK_ARG(items + own < 0x7FFFFFFF && tokens * heads < 0x7FFFFF00, "too many query rows");
   if (p.bytes > 0)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "shared prefix MLA workspace too small or misaligned");
@@ -668,7 +685,8 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   a.out = static_cast<uint16_t*>(out);
   a.parts = static_cast<float*>(workspace);
   a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.stats_at);
-  a.tokens = tokens, a.pages = pages, a.prefix = prefix_tokens;
+  a.rows = (int32_t)(tokens * heads), a.tiles = (int32_t)tiles;
+  a.pages = pages, a.prefix = prefix_tokens;
   a.heads = (int32_t)heads, a.branches = (int32_t)branches, a.suffix_pages = (int32_t)suffix_pages;
   a.joint = p.joint, a.items = (int32_t)items, a.splits = (int32_t)p.splits;
   a.suffix_splits = (int32_t)p.suffix_splits;
