@@ -566,11 +566,12 @@ int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t
 }
 
 // Key splits: the count of least time, by the rounds of work-groups (one per CU),
-// their fixed part (Q, the first records, the stores), the steps of the longest, and
-// what reading a row's parts again costs. Fitted to one token of 128 heads over 32,896
-// keys (64, 128, 206, 257 splits: 52, 40, 39, 54 us), 5 tokens over 8,333 (13, 25, 45,
-// 68: 59, 45, 44, 58) and 8 over 70,000 (16, 32, 64: 294, 186, 231).
-constexpr double kFixedUs = 17.0, kStepUs = 2.2, kJoinUs = 3.0, kPartUsPerRow = 0.0003;
+// their fixed part, the steps of the longest, and what writing a row's parts and
+// reading them again costs. Fitted to one token of 128 heads over 32,896 keys (103,
+// 147, 206 splits: 38.0, 36.6, 36.0 us), 18 over 10,330 (11, 14: 78, 75), 30 over 572 (1,
+// 2, 4, 6: 41, 34, 30, 34), 114 over 528 (1, 2, 3: 42, 51, 70) and 8 over 70,000 (16, 32,
+// 64: 294, 164, 231).
+constexpr double kFixedUs = 10.0, kStepUs = 1.75, kJoinUs = 3.0, kPartUsPerRow = 0.0007;
 
 struct PrefixPlan {
   bool joint;
