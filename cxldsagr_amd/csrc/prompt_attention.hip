@@ -486,15 +486,34 @@ using ManyRows = Cut<4, 2>;
 // Few rows: about two rounds of work-groups if all keys are seen, of at least 256
 // keys (eight single tokens over 40,000 keys of 8 heads 40.5 us, with one round 44.1,
 // three 39.9, four 39.9; over 16 heads of 192 / 128, 30,000 keys, 61.8, 67.4, 62.0, 64.6).
-// Many rows: where it pays by the rounds of work-groups, their fixed part and their
-// stages, against a join of 4 d_v bytes a row and split, written and read.
+// Many rows: the count of least time (many_rows_us), fitted to 12 calls of 64 to 3,000
+// queries over up to 65,600 keys, each with 1 to 48 splits.
 constexpr int64_t kMinSplitStages = 8, kMaxSplits = 256;
-constexpr double kFixedUs = 5.0, kStageUs = 1.15, kJoinUs = 4.0, kJoinBytesPerUs = 4.0e6;
 
 struct PromptPlan {
   bool few, ranked;
   int64_t slots, splits, split_stages, bytes, stats_at;
 };
+
+// Time of a call whose keys are split into ranges of `of` of at most `stages` stages
+// (about `seen` on average): a work-group takes 0.62 us a stage alone on its CU and
+// 1.15 where the CU has two, and 5 us beside them; reading K and V once bounds all
+// of them; the parts of each row are written and read again.
+double many_rows_us(double tiles, double seen, double stages, double of, double rows, double v_dim, double kv_bytes,
+                    double cus) {
+  const double scale = 0.5 + v_dim / 256, fixed = 5.0, alone = 0.62 * scale, shared = 1.15 * scale;
+  const double parts = of < stages ? __builtin_ceil((seen + stages) / 2 / of) : 1.0;
+  const double groups = tiles * parts, total = tiles * seen;
+  double us = fixed + alone * of;
+  if (groups > 2 * cus) {
+    us = (total * shared + groups * fixed) / (2 * cus) + 0.25 * (fixed + shared * of);
+  } else if (groups > cus) {
+    const double load = total / (2 * cus * of);
+    us += (shared - alone) * (load < 1.0 ? load : 1.0) * of;
+  }
+  if (us < kv_bytes / 5.5e6) us = kv_bytes / 5.5e6;
+  return of < stages ? us + 4.0 + rows * parts * v_dim * 8 / 3.4e6 : us;
+}
 
 PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_t v_dim, int64_t sequences,
                        int64_t k_tokens, int64_t max_k) {
@@ -520,16 +539,23 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
     if (p.few) {
       p.split_stages = (units * usual + 2 * round - 1) / (2 * round);
     } else {
-      double least = (double)stages * kStageUs + kFixedUs;
+      const double tiles = (double)(sequences * kv_heads) *
+                           (double)((rows + ManyRows::kRows * sequences - 1) / (ManyRows::kRows * sequences));
+      double seen = ((double)k_tokens - 0.5 * (double)q_tokens) / (double)(sequences * kStageKeys);
+      if (seen > (double)stages) seen = (double)stages;
+      if (seen < 1.0) seen = 1.0;
+      const double kv_bytes = 4.5 * (double)(k_tokens * kv_heads * v_dim);  // (its two dims together are about 2.25)
+      const auto us = [&](int64_t of) {
+        return many_rows_us(tiles, seen, (double)stages, (double)of, (double)(rows * kv_heads), (double)v_dim, kv_bytes,
+                            (double)device_cu_count());
+      };
       p.split_stages = stages;
+      double least = us(stages);
       for (int64_t s = 2; s <= kMaxSplits; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : s < 32 ? 8 : s < 64 ? 16 : 64) {
         const int64_t of = (stages + s - 1) / s;
         if (of < kMinSplitStages) break;
-        const double groups = (double)units * (double)((usual + of - 1) / of) / (double)round;
-        const double us = (groups > 1.0 ? groups : 1.0) * (kFixedUs + kStageUs * (double)of) + kJoinUs +
-                          (double)(rows * kv_heads * ((usual + of - 1) / of) * v_dim * 8) / kJoinBytesPerUs;
-        if (us < least) {
-          least = us;
+        if (const double t = us(of); t < least) {
+          least = t;
           p.split_stages = of;
         }
       }

@@ -153,3 +153,24 @@ def test_two_prefix_calls_at_once(gpu):
         again = _run(x, 3000)
         torch.cuda.synchronize()
         assert torch.equal(beside, want) and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("dims", [(192, 128), (128, 128), (64, 64)])
+@pytest.mark.parametrize(
+    ("queries", "keys", "heads", "kv_heads"),
+    [
+        ([100], [3000], 2, 2),
+        ([70, 40], [2500, 100], 5, 1),  # the shorter one's rows are in the first split only
+    ],
+)
+def test_chunks_whose_keys_are_split(gpu, dims, queries, keys, heads, kv_heads):
+    """More rows than a wave, few enough to be split over keys and joined."""
+    from cxldsagr_amd import _native
+    from cxldsagr_amd.attention import prompt_attention
+
+    x = _inputs(gpu, queries, keys, heads, kv_heads, dims, torch.bfloat16, 68)
+    assert _native.size_of("dsa_prompt_attention_workspace_bytes", 0, sum(queries), heads, kv_heads, dims[1],
+                           len(queries), sum(keys), max(keys)) > 0
+    for causal in (True, False):
+        got = prompt_attention(*x[:3], 0.1, *x[3:], max_k=max(keys), causal=causal)
+        check_prompt(got, *x[:3], 0.1, *x[3:], causal=causal)
