@@ -416,7 +416,8 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
     _native.require_gfx950(device, "prompt attention")
     shape = (q_tokens, heads, v_dim)
     if out is None:
-        out = q.new_empty(shape)
+        out = (torch.empty_like(q, memory_format=torch.contiguous_format) if v_dim == qk_dim
+               else q.new_empty(shape))
     elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != dtype
           or out.device != device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned [Tq, H, Dv] tensor of q's "
@@ -460,56 +461,61 @@ def shared_prefix_mla(q, kv_cache, prefix_table, prefix_tokens, suffix_tables, s
     queries of no branch are left as they were. A query that sees no key gives
     zeros; tokens on a page outside the cache are padding.
     """
-    if q.ndim != 3 or q.shape[2] != QK_DIM or value_dim != V_DIM or not q.shape[1]:
+    if q.ndim != 3 or value_dim != V_DIM:
         raise ValueError("Expected q [T,H,576] with H >= 1 and value_dim 512")
+    tokens, heads, dim = q.shape
+    if dim != QK_DIM or not heads:
+        raise ValueError("Expected q [T,H,576] with H >= 1 and value_dim 512")
+    device = q.device
     if q.dtype != torch.bfloat16:
         raise ValueError("shared prefix MLA requires BF16 queries")
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be positive and finite")
-    _check_paged(kv_cache, prefix_table, q.device)
+    _check_paged(kv_cache, prefix_table, device)
     if (type(prefix_tokens) is not int
             or not 0 <= prefix_tokens <= prefix_table.numel() * PAGE_TOKENS):
         raise ValueError("prefix_tokens must be covered by the prefix table")
     if (not isinstance(suffix_tables, torch.Tensor) or suffix_tables.dtype != torch.int32
-            or suffix_tables.ndim != 2 or suffix_tables.device != q.device):
+            or suffix_tables.ndim != 2 or suffix_tables.device != device):
         raise ValueError("suffix_tables must be int32 [branches, pages] on the query device")
-    branches = suffix_tables.shape[0]
+    branches, suffix_pages = suffix_tables.shape
     if (not isinstance(suffix_tokens, torch.Tensor) or suffix_tokens.dtype != torch.int32
-            or tuple(suffix_tokens.shape) != (branches,) or suffix_tokens.device != q.device):
+            or suffix_tokens.shape != (branches,) or suffix_tokens.device != device):
         raise ValueError("suffix_tokens must be int32 [branches] on the query device")
     if cu_q is not None:
-        cu_q = _check_starts(cu_q, q.device, "cu_q")
+        cu_q = _check_starts(cu_q, device, "cu_q")
         if cu_q.numel() != branches + 1:
             raise ValueError("cu_q must be int32 [branches + 1]")
-    elif branches != q.shape[0]:
+    elif branches != tokens:
         raise ValueError("without cu_q every branch has one query")
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("shared prefix MLA has no backward pass")
-    _native.require_gfx950(q.device, "shared prefix MLA")
-    shape = (*q.shape[:2], value_dim)
+    _native.require_gfx950(device, "shared prefix MLA")
+    shape = (tokens, heads, value_dim)
     if out is None:
         out = q.new_empty(shape)
-    elif (not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != q.dtype
-          or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
+    elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != q.dtype
+          or out.device != device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous, 16-byte aligned [T, H, 512] tensor of q's "
                          "dtype on q's device")
-    if not q.shape[0] or not branches:
+    if not tokens or not branches:
         return out
-    if not kv_cache.shape[0]:
+    pages = kv_cache.shape[0]
+    if not pages:
         raise ValueError("kv_cache must hold a page")
     q, cache = _aligned(q), _aligned(kv_cache)
     prefix_table, suffix_tables = prefix_table.contiguous(), suffix_tables.contiguous()
     suffix_tokens = suffix_tokens.contiguous()
-    with _native.on_device(q.device):
-        needed = _native.size_of("dsa_shared_prefix_mla_workspace_bytes", q.device.index,
-                                 q.shape[0], q.shape[1], prefix_tokens, suffix_tables.shape[1])
+    with _native.on_device(device):
+        needed = _native.size_of("dsa_shared_prefix_mla_workspace_bytes", device.index, tokens,
+                                 heads, prefix_tokens, suffix_pages)
         workspace = q.new_empty(needed, dtype=torch.uint8) if needed else None
         _native.call(
             "dsa_shared_prefix_mla_fp8",
-            q.data_ptr(), q.shape[0], q.shape[1], cache.data_ptr(), cache.shape[0],
+            q.data_ptr(), tokens, heads, cache.data_ptr(), pages,
             prefix_table.data_ptr(), prefix_tokens, suffix_tables.data_ptr(),
-            suffix_tables.shape[1], suffix_tokens.data_ptr(), _native.ptr(cu_q), branches,
+            suffix_pages, suffix_tokens.data_ptr(), _native.ptr(cu_q), branches,
             float(scale), out.data_ptr(), _native.ptr(workspace), needed,
-            _native.raw_stream(q.device),
+            _native.raw_stream(device),
         )
     return out

@@ -79,7 +79,7 @@ def rotary_table(positions, frequencies):
 
 def _check_heads(x, tokens, device, dtype, dim, name):
     if (not isinstance(x, torch.Tensor) or x.ndim != 3 or x.dtype != dtype or x.device != device
-            or x.shape[::2] != (tokens, dim)):
+            or x.shape != (tokens, x.shape[1], dim)):
         raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device}")
 
 
@@ -137,12 +137,12 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
         raise ValueError("rotate gradients by a call with inverse=True")
     _native.require_gfx950(device, "rotary positions")
     if q_out is None:
-        q_out = q.new_empty(shape)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rope_out(q_out, q, "q_out")
     if k is not None:
         if k_out is None:
-            k_out = k.new_empty(k.shape)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         else:
             _check_rope_out(k_out, k, "k_out")
     if tokens == 0:
