@@ -158,3 +158,22 @@ def test_captured_call_replays(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinities_and_nan_as_in_the_formula(gpu, dtype):
+    from cxldsagr_amd.projections import apply_rope_pair
+
+    gen = torch.Generator().manual_seed(47)
+    q = torch.randn(9, 4, 64, generator=gen).to(dtype)
+    q[1, 0, 3], q[2, 1, 40], q[3, 2, 7], q[0, 3, 5] = float("inf"), -float("inf"), float("nan"), float("inf")
+    q[4, 0, 8], q[4, 0, 9] = float("inf"), float("inf")
+    positions = torch.arange(9) * 1001
+    frequencies = _frequencies(64, gpu)
+    for interleaved in (True, False):
+        got, _ = apply_rope_pair(q.to(gpu), None, positions.to(gpu), frequencies, interleaved=interleaved)
+        want = dense.rope(q, positions, frequencies.cpu(), 0, interleaved, 1.0)
+        got = got.cpu().double()
+        assert torch.equal(got.isnan(), want.isnan())
+        infinite = want.isinf()
+        assert torch.equal(got.isinf(), infinite) and torch.equal(got[infinite], want[infinite])
