@@ -547,7 +547,7 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
       const double kv_bytes = 4.5 * (double)(k_tokens * kv_heads * v_dim);  // (its two dims together are about 2.25)
       const auto us = [&](int64_t of) {
         return many_rows_us(tiles, seen, (double)stages, (double)of, (double)(rows * kv_heads), (double)v_dim, kv_bytes,
-                            (double)device_cu_count());
+                            (double)(round / 2));
       };
       p.split_stages = stages;
       double least = us(stages);
