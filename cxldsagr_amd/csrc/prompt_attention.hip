@@ -483,11 +483,9 @@ using ManyRows = Cut<4, 2>;
 // Key splits, where the row tiles are too few for the chip: ranges of the same
 // number of stages, so that sequences of different lengths make work-groups of the
 // same size.
-// Few rows: about two rounds of work-groups if all keys are seen, of at least 256
-// keys (eight single tokens over 40,000 keys of 8 heads 40.5 us, with one round 44.1,
-// three 39.9, four 39.9; over 16 heads of 192 / 128, 30,000 keys, 61.8, 67.4, 62.0, 64.6).
-// Many rows: the count of least time (many_rows_us), fitted to 12 calls of 64 to 3,000
-// queries over up to 65,600 keys, each with 1 to 48 splits.
+// The count of least time (split_us), fitted to 11 calls of 1 to 24 single tokens over
+// 500 to 60,000 keys and 12 of 64 to 3,000 queries over up to 65,600, each with 1 to 48
+// splits.
 constexpr int64_t kMinSplitStages = 8, kMaxSplits = 256;
 
 struct PromptPlan {
@@ -496,22 +494,27 @@ struct PromptPlan {
 };
 
 // Time of a call whose keys are split into ranges of `of` of at most `stages` stages
-// (about `seen` on average): a work-group takes 0.62 us a stage alone on its CU and
-// 1.15 where the CU has two, and 5 us beside them; reading K and V once bounds all
-// of them; the parts of each row are written and read again.
-double many_rows_us(double tiles, double seen, double stages, double of, double rows, double v_dim, double kv_bytes,
-                    double cus) {
+// (about `seen` on average): a work-group takes 0.62 us a stage alone on its CU and, if
+// it has four waves, 1.15 where the CU has two, and 5 us beside them; reading K and V once
+// bounds all of them (`apart`: adds to their own time, as the root of the sum of both
+// squared: with few loads on their way neither hides the other); the parts of each row
+// are written and read again.
+double split_us(bool few, bool apart, double tiles, double seen, double stages, double of, double rows, double v_dim,
+                double kv_bytes, double cus) {
   const double scale = 0.5 + v_dim / 256, fixed = 5.0, alone = 0.62 * scale, shared = 1.15 * scale;
   const double parts = of < stages ? __builtin_ceil((seen + stages) / 2 / of) : 1.0;
   const double groups = tiles * parts, total = tiles * seen;
   double us = fixed + alone * of;
-  if (groups > 2 * cus) {
+  if (few) {
+    us *= __builtin_ceil(groups / (2 * cus));
+  } else if (groups > 2 * cus) {
     us = (total * shared + groups * fixed) / (2 * cus) + 0.25 * (fixed + shared * of);
   } else if (groups > cus) {
     const double load = total / (2 * cus * of);
     us += (shared - alone) * (load < 1.0 ? load : 1.0) * of;
   }
-  if (us < kv_bytes / 5.5e6) us = kv_bytes / 5.5e6;
+  const double read = kv_bytes / 5.5e6;
+  us = apart ? __builtin_sqrt(us * us + read * read) : us < read ? read : us;
   return of < stages ? us + 4.0 + rows * parts * v_dim * 8 / 3.4e6 : us;
 }
 
@@ -534,31 +537,33 @@ PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_
   const int64_t mean = k_tokens / kStageKeys / sequences + 1;
   int64_t stages = ((max_k < 0 ? k_tokens : max_k) + kStageKeys - 1) / kStageKeys;
   if (max_k < 0 && stages > (p.few ? 4 : 2) * mean) stages = (p.few ? 4 : 2) * mean;
-  const int64_t usual = mean < stages ? mean : stages;
   if (units < round && stages > kMinSplitStages) {
-    if (p.few) {
-      p.split_stages = (units * usual + 2 * round - 1) / (2 * round);
-    } else {
-      const double tiles = (double)(sequences * kv_heads) *
-                           (double)((rows + ManyRows::kRows * sequences - 1) / (ManyRows::kRows * sequences));
-      double seen = ((double)k_tokens - 0.5 * (double)q_tokens) / (double)(sequences * kStageKeys);
-      if (seen > (double)stages) seen = (double)stages;
-      if (seen < 1.0) seen = 1.0;
-      const double kv_bytes = 4.5 * (double)(k_tokens * kv_heads * v_dim);  // (its two dims together are about 2.25)
-      const auto us = [&](int64_t of) {
-        return many_rows_us(tiles, seen, (double)stages, (double)of, (double)(rows * kv_heads), (double)v_dim, kv_bytes,
-                            (double)(round / 2));
-      };
-      p.split_stages = stages;
-      double least = us(stages);
-      for (int64_t s = 2; s <= kMaxSplits; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : s < 32 ? 8 : s < 64 ? 16 : 64) {
-        const int64_t of = (stages + s - 1) / s;
-        if (of < kMinSplitStages) break;
-        if (const double t = us(of); t < least) {
-          least = t;
-          p.split_stages = of;
-        }
+    const int64_t tile = p.few ? FewRows::kRows : ManyRows::kRows;
+    const double tiles = (double)(sequences * kv_heads) * (double)((rows + tile * sequences - 1) / (tile * sequences));
+    double seen = ((double)k_tokens - 0.5 * (double)q_tokens) / (double)(sequences * kStageKeys);
+    if (seen > (double)stages) seen = (double)stages;
+    if (seen < 1.0) seen = 1.0;
+    const double kv_bytes = 4.5 * (double)(k_tokens * kv_heads * v_dim);  // (its two dims together are about 2.25)
+    const auto us = [&](int64_t of, bool apart) {
+      return split_us(p.few, apart, tiles, seen, (double)stages, (double)of, (double)(rows * kv_heads), (double)v_dim,
+                      kv_bytes, (double)(round / 2));
+    };
+    p.split_stages = stages;
+    double least = us(stages, false);
+    for (int64_t s = 2; s <= kMaxSplits; s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : s < 64 ? 8 : 32) {
+      const int64_t of = (stages + s - 1) / s;
+      if (of < kMinSplitStages) break;
+      if (const double t = us(of, false); t < least) {
+        least = t;
+        p.split_stages = of;
       }
+    }
+    // Single tokens: or two rounds of work-groups, which keep more loads on their way (4
+    // over 30,000 keys, 16 heads of 192 / 128: 63 us, with five splits 78).
+    if (p.few) {
+      int64_t of = (units * (mean < stages ? mean : stages) + 2 * round - 1) / (2 * round);
+      if (of < kMinSplitStages) of = kMinSplitStages;
+      if (us(of, true) < us(p.split_stages, true)) p.split_stages = of;
     }
     if (p.split_stages < (stages + kMaxSplits - 1) / kMaxSplits) p.split_stages = (stages + kMaxSplits - 1) / kMaxSplits;
     if (p.split_stages < kMinSplitStages) p.split_stages = kMinSplitStages;

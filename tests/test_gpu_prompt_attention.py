@@ -66,7 +66,7 @@ def test_few_queries_over_split_keys(gpu, keys, queries):
 
     x = _inputs(gpu, [queries, queries], [keys, 5], 4, 2, (128, 128), torch.bfloat16, 12)
     assert _native.size_of("dsa_prompt_attention_workspace_bytes", 0, 2 * queries, 4, 2, 128, 2,
-                           keys + 5, keys) > 0 or keys <= 256
+                           keys + 5, keys) > 0 or keys <= 257  # (so few are not worth a join)
     got = prompt_attention(*x[:3], 0.1, *x[3:], max_k=keys)
     _check(got, *x[:3], 0.1, *x[3:])
     # max_k only says how keys are split.
