@@ -1,8 +1,9 @@
 """Rotary pairs against the 64-bit formula. Tolerance: cos and sin are off by at most
-2^-20 m in all (the fraction of a turn rounded to 32 bits moves the angle by 2 pi 2^-25,
-their evaluation by 4 units of 2^-24, the magnitude's product by one more), so a
-result by 2^-20 m (|a| + |b|) and the fp32 products and sum by 2^-22 m (|a| + |b|); then it
-is rounded once, by at most half a step."""
+2^-20 m in all (derived for 32-bit functions of an angle in turns rounded to 32 bits: the
+rounding moves it by 2 pi 2^-25, their evaluation by 4 units of 2^-24, the magnitude's product
+by one more; formed in 64 bits and rounded once they are off by 2^-24 m), so a result by
+2^-20 m (|a| + |b|) and the fp32 products and sum by 2^-22 m (|a| + |b|); then it is rounded
+once, by at most half a step."""
 
 import pytest
 import torch
