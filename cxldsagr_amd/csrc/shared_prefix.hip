@@ -582,6 +582,7 @@ PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t su
   PrefixPlan p{};
   const int64_t cus = device_cu_count();
   const int64_t rows = tokens * heads;
+  if (rows == 0) return p;
   const int64_t prefix_blocks = (prefix + kBlockKeys - 1) / kBlockKeys;
   const int64_t suffix_blocks = suffix_pages * (kPageTokens / kBlockKeys);
   p.joint = heads % kTileRows == 0;

@@ -306,3 +306,17 @@ def test_rope_refuses_expanded_outputs(monkeypatch):
     for out in (z(1, 4, 64).expand(2, 4, 64), z(2, 1, 64).expand(2, 4, 64)):
         with pytest.raises(ValueError, match="expanded"):
             apply_rope_pair(z(2, 4, 64), None, cu(0, 1), torch.ones(32), q_out=out)
+
+
+@pytest.mark.parametrize("heads", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 1000])
+@pytest.mark.parametrize("suffix_pages", [0, 1])
+def test_a_workspace_for_no_tokens_is_empty(heads, prefix, suffix_pages):
+    """Calls without tokens are allowed, and so is asking for their workspace first."""
+    size = ctypes.c_int64(-1)
+    _native.call("dsa_shared_prefix_mla_workspace_bytes", 0, heads, prefix, suffix_pages, ctypes.byref(size))
+    assert size.value == 0
+    size = ctypes.c_int64(-1)
+    _native.call("dsa_prompt_attention_workspace_bytes", 0, heads, heads, 128, 1, prefix, prefix,
+                 ctypes.byref(size))
+    assert size.value == 0
