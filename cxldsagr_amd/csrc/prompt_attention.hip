@@ -521,6 +521,8 @@ double split_us(bool few, bool apart, double tiles, double seen, double stages, 
 PromptPlan prompt_plan(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_t v_dim, int64_t sequences,
                        int64_t k_tokens, int64_t max_k) {
   PromptPlan p{};
+  // (Stages of no more than k_tokens keys stay within the kernel's 32 bits.)
+  if (max_k > k_tokens) max_k = k_tokens;
   const int64_t rows = q_tokens * (heads / kv_heads);
   p.few = rows <= FewRows::kRows * sequences;
   p.slots = rows / (p.few ? FewRows::kRows : ManyRows::kRows) + sequences;

@@ -510,8 +510,8 @@ int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slots, int wid
  * keys j <= i + n_k - n_q, else every key. out: dtype [q_tokens, heads, v_dim]
  * contiguous, 16-byte aligned = softmax(scale q k^T) v, zeros for a query that
  * sees no key; queries outside the sequences are not written. scale > 0.
- * max_k: the longest sequence's keys, below 0: not known (it decides how keys are
- * split over work-groups, not what is computed). `workspace`: 16-byte aligned, at least
+ * max_k: the longest sequence's keys (more than k_tokens: k_tokens), below 0: not
+ * known (it decides how keys are split over work-groups, not what is computed). `workspace`: 16-byte aligned, at least
  * dsa_prompt_attention_workspace_bytes bytes (0: not used), no initialisation,
  * free again when the stream has passed the call; not to be shared by calls that
  * may run at the same time.

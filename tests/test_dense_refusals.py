@@ -320,3 +320,15 @@ def test_a_workspace_for_no_tokens_is_empty(heads, prefix, suffix_pages):
     _native.call("dsa_prompt_attention_workspace_bytes", 0, heads, heads, 128, 1, prefix, prefix,
                  ctypes.byref(size))
     assert size.value == 0
+
+
+def test_a_longest_sequence_past_the_keys_is_cut_to_them():
+    """(Key splits of so many stages would pass the 32 bits in which a work-group finds its own.)"""
+    for k_tokens in (5, 5000):
+        sizes = []
+        for longest in (k_tokens, k_tokens + 1, 1 << 31, 3 << 40, (1 << 63) - 1):
+            size = ctypes.c_int64()
+            _native.call("dsa_prompt_attention_workspace_bytes", 1, 8, 8, 128, 1, k_tokens, longest,
+                         ctypes.byref(size))
+            sizes.append(size.value)
+        assert sizes == sizes[:1] * 5
