@@ -609,6 +609,19 @@ int launch_dims(const PromptCall& c, int64_t qk_dim, int64_t v_dim, hipStream_t 
   return launch_prompt<E, 64, 64>(c, stream);
 }
 
+// What the plan's and the kernel's arithmetic is made for.
+int check_sizes(int64_t q_tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t k_tokens) {
+  DSA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
+                "heads must be a positive multiple of kv_heads");
+  // (Rounding up to a stage must stay within int32.)
+  constexpr int64_t kMost = 0x7FFFFFFF - kStageKeys;
+  DSA_CHECK_ARG(q_tokens >= 0 && k_tokens >= 0 && q_tokens <= kMost && k_tokens <= kMost && sequences >= 0 &&
+                    sequences <= kMost,
+                "token and sequence counts must be in [0, 2^31 - 33]");
+  DSA_CHECK_ARG(q_tokens * heads < 0x7FFFFF00, "too many query rows");
+  return kOk;
+}
+
 }  // namespace
 }  // namespace dsa
 
@@ -616,9 +629,9 @@ extern "C" int dsa_prompt_attention_workspace_bytes(int64_t q_tokens, int64_t he
                                                     int64_t sequences, int64_t k_tokens, int64_t max_k, int64_t* bytes) {
   using namespace dsa;
   DSA_CHECK_ARG(bytes != nullptr, "null pointer");
-  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && k_tokens >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
-                    v_dim > 0,
+  DSA_CHECK_ARG(q_tokens >= 0 && sequences >= 0 && k_tokens >= 0 && v_dim > 0 && v_dim <= 128,
                 "invalid prompt attention shape");
+  if (const int status = check_sizes(q_tokens, heads, kv_heads, sequences, k_tokens); status != kOk) return status;
   *bytes = sequences == 0 ? 0 : prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k).bytes;
   return kOk;
 }
@@ -634,13 +647,7 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
   DSA_CHECK_ARG(dtype == DSA_DTYPE_BF16 || dtype == DSA_DTYPE_F16, "prompt attention takes bf16 or fp16");
   DSA_CHECK_ARG((qk_dim == 192 && v_dim == 128) || (qk_dim == 128 && v_dim == 128) || (qk_dim == 64 && v_dim == 64),
                 "head dims must be (192, 128), (128, 128) or (64, 64)");
-  DSA_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536,
-                "heads must be a positive multiple of kv_heads");
-  // (Rounding up to a stage must stay within int32.)
-  constexpr int64_t kMost = 0x7FFFFFFF - kStageKeys;
-  DSA_CHECK_ARG(q_tokens >= 0 && k_tokens >= 0 && q_tokens <= kMost && k_tokens <= kMost && sequences >= 0 &&
-                    sequences <= kMost,
-                "token and sequence counts must be in [0, 2^31 - 33]");
+  if (const int status = check_sizes(q_tokens, heads, kv_heads, sequences, k_tokens); status != kOk) return status;
   DSA_CHECK_ARG(scale > 0.0f && __builtin_isfinite(scale), "scale must be positive and finite");
   if (q_tokens == 0) return kOk;
   DSA_CHECK_ARG(sequences > 0, "queries need a sequence");
@@ -652,7 +659,7 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
                  reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                 "q, k, v and out must be 16-byte aligned");
   const PromptPlan p = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k);
-  DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF && q_tokens * heads < 0x7FFFFF00, "too many query rows");
+  DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF, "too many query rows");
   if (p.splits > 1)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "prompt attention workspace too small or misaligned");

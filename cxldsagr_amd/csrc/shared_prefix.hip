@@ -633,6 +633,16 @@ PrefixPlan prefix_plan(int64_t tokens, int64_t heads, int64_t prefix, int64_t su
   return p;
 }
 
+// What the plan's and the kernel's arithmetic is made for.
+int check_sizes(int64_t tokens, int64_t heads, int64_t prefix_tokens, int64_t suffix_pages) {
+  DSA_CHECK_ARG(tokens >= 0 && heads > 0 && heads <= 65536, "invalid shared prefix MLA shape");
+  DSA_CHECK_ARG(prefix_tokens >= 0 && prefix_tokens < 0x7FFFFFFF && suffix_pages >= 0 &&
+                    suffix_pages < 0x7FFFFFFF / kPageTokens,
+                "prefix and suffix lengths must fit int32");
+  DSA_CHECK_ARG(tokens < (0x7FFFFF00 + heads - 1) / heads, "too many query rows");
+  return kOk;
+}
+
 }  // namespace
 }  // namespace dsa
 
@@ -640,8 +650,7 @@ extern "C" int dsa_shared_prefix_mla_workspace_bytes(int64_t tokens, int64_t hea
                                                      int64_t suffix_pages, int64_t* bytes) {
   using namespace dsa;
   DSA_CHECK_ARG(bytes != nullptr, "null pointer");
-  DSA_CHECK_ARG(tokens >= 0 && heads > 0 && prefix_tokens >= 0 && suffix_pages >= 0,
-                "invalid shared prefix MLA shape");
+  if (const int status = check_sizes(tokens, heads, prefix_tokens, suffix_pages); status != kOk) return status;
   *bytes = prefix_plan(tokens, heads, prefix_tokens, suffix_pages).bytes;
   return kOk;
 }
@@ -653,11 +662,8 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
                                          float scale, void* out, void* workspace, int64_t workspace_bytes,
                                          hipStream_t stream) {
   using namespace dsa;
-  DSA_CHECK_ARG(tokens >= 0 && heads > 0 && heads <= 65536 && branches >= 0 && branches < 0x7FFFFFFF,
-                "invalid shared prefix MLA shape");
-  DSA_CHECK_ARG(prefix_tokens >= 0 && prefix_tokens < 0x7FFFFFFF && suffix_pages >= 0 &&
-                    suffix_pages < 0x7FFFFFFF / kPageTokens,
-                "prefix and suffix lengths must fit int32");
+  DSA_CHECK_ARG(branches >= 0 && branches < 0x7FFFFFFF, "invalid shared prefix MLA shape");
+  if (const int status = check_sizes(tokens, heads, prefix_tokens, suffix_pages); status != kOk) return status;
   DSA_CHECK_ARG(scale > 0.0f && __builtin_isfinite(scale), "scale must be positive and finite");
   if (tokens == 0) return kOk;
   DSA_CHECK_ARG(branches > 0 && (cu_q != nullptr || branches == tokens),
@@ -673,7 +679,7 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   const int64_t tiles = (tokens * heads + kTileRows - 1) / kTileRows;
   const int64_t items = p.splits > 0 ? (tiles * p.splits + 7) / 8 * 8 : 0;
   const int64_t own = tokens * ((heads + kTileRows - 1) / kTileRows) * p.suffix_splits;
-  DSA_CHECK_ARG(items + own < 0x7FFFFFFF && tokens * heads < 0x7FFFFF00, "too many query rows");
+  DSA_CHECK_ARG(items + own < 0x7FFFFFFF, "too many query rows");
   if (p.bytes > 0)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "shared prefix MLA workspace too small or misaligned");

@@ -332,3 +332,29 @@ def test_a_longest_sequence_past_the_keys_is_cut_to_them():
                          ctypes.byref(size))
             sizes.append(size.value)
         assert sizes == sizes[:1] * 5
+
+
+@pytest.mark.parametrize(
+    ("name", "args", "message"),
+    [
+        ("dsa_shared_prefix_mla_workspace_bytes", (1 << 57, 128, 1000, 1), "too many"),
+        ("dsa_shared_prefix_mla_workspace_bytes", (1 << 50, 1 << 14, 1000, 1), "too many"),
+        ("dsa_shared_prefix_mla_workspace_bytes", (1 << 24, 128, 1000, 1), "too many"),
+        ("dsa_shared_prefix_mla_workspace_bytes", (1, 1 << 17, 1000, 1), "shape"),
+        ("dsa_shared_prefix_mla_workspace_bytes", (1, 128, (1 << 63) - 1, 1), "fit int32"),
+        ("dsa_shared_prefix_mla_workspace_bytes", (1, 128, 1000, 1 << 62), "fit int32"),
+        ("dsa_prompt_attention_workspace_bytes", (1, 32, 32, 128, 1 << 59, 1 << 62, 1 << 62), "counts"),
+        ("dsa_prompt_attention_workspace_bytes", (1 << 25, 128, 8, 128, 1, 64, 64), "too many"),
+        ("dsa_prompt_attention_workspace_bytes", (1, 1 << 17, 1, 128, 1, 64, 64), "multiple of kv_heads"),
+    ],
+)
+def test_sizes_past_what_a_call_takes_have_no_workspace(name, args, message):
+    """Refused as the call refuses them, before any arithmetic on them."""
+    with pytest.raises(ValueError, match=message):
+        _native.call(name, *args, ctypes.byref(ctypes.c_int64()))
+
+
+def test_row_counts_that_wrap_are_refused_before_the_plan():
+    for change in (dict(tokens=1 << 57), dict(tokens=1 << 50, heads=1 << 14), dict(tokens=1 << 24)):
+        with pytest.raises(ValueError, match="too many query rows"):
+            _c_shared(**{**change, "branches": change["tokens"] if change["tokens"] < 1 << 31 else 1, "cu_q": P})
