@@ -24,13 +24,15 @@ typedef v4s __attribute__((address_space(3))) * lds_v4s;
 
 constexpr float kLog2E = 1.4426950408889634f;
 // A row's running maximum is raised only when a block's exceeds it by more than
-// this, in log2 units: probabilities stay at or below 2^8 (exact in range for
-// both 16-bit types), and the accumulators are seldom rescaled.
+// this, in log2 units: probabilities stay at or below 2^(8 + kLift), and the
+// accumulators are seldom rescaled.
 constexpr float kLazyRescale = 8.0f;
 
 // The 16-bit element type of a kernel: its matrix product over 16 dims of 32
-// rows by 32 columns, and two floats rounded to nearest even into a pair.
+// rows by 32 columns, and two floats rounded to nearest even into a pair. kLift: the
+// log2 of the probability that a row's maximum has when it is raised.
 struct Bf16 {
+  static constexpr float kLift = 0.0f;
   static __device__ __forceinline__ v16f mfma(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   }
@@ -42,7 +44,11 @@ struct Bf16 {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), __builtin_bit_cast(v2bf, 0x3F803F80u), c, false);
   }
 };
+// fp16 holds 2^15 and loses bits below 2^-14: 2^7 at the maximum uses the range up to there,
+// and what is lost lies 7 binades lower (with 1 at the maximum 60,000 keys of 2^-26 each,
+// 9e-4 of the sum, went missing, and those of 2^-20 were off by up to 2^-6).
 struct F16 {
+  static constexpr float kLift = 7.0f;
   static __device__ __forceinline__ v16f mfma(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8hf, a), __builtin_bit_cast(v8hf, b), c, 0, 0, 0);
   }
@@ -141,8 +147,8 @@ __device__ __forceinline__ uint32_t sum_below(uint32_t v) {
   return v - own + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
 }
 
-// The running maximum and sum of one row of scores (held by lanes l and l ^ 32:
-// the maximum by both, of the sum a part each).
+// The running maximum, less the type's kLift, and sum of one row of scores (held by
+// lanes l and l ^ 32: the maximum by both, of the sum a part each).
 struct RowState {
   float top, sum;
 };
@@ -156,14 +162,21 @@ __device__ __forceinline__ float row_max(const v16f& s, float scale_log2) {
 }
 
 // Whether a row's running maximum (-inf: no visible key so far) has to rise to take in
-// scores up to mx.
-__device__ __forceinline__ bool must_raise(const RowState& row, float mx) { return mx > row.top + kLazyRescale; }
+// scores up to mx. (Far from zero a score's own steps may exceed what fp16 has left above
+// 2^15: there it rises earlier, from 2^24 on within 2^7 of the maximum.)
+template <typename E>
+__device__ __forceinline__ bool must_raise(const RowState& row, float mx) {
+  const float most = row.top + (E::kLift + kLazyRescale);
+  if constexpr (E::kLift > 0.0f) return mx > __builtin_fmaf(__builtin_fabsf(row.top), -0x1p-21f, most);
+  return mx > most;
+}
 
 // Raises it; returns the factor for what was summed before (1 with no visible key so
 // far: those sums are zeros, which are not worth a pass over the accumulators).
+template <typename E>
 __device__ __forceinline__ float raise(RowState& row, float mx) {
-  if (!must_raise(row, mx)) return 1.0f;
-  const float top = fmaxf(row.top, mx);
+  if (!must_raise<E>(row, mx)) return 1.0f;
+  const float top = fmaxf(row.top, mx - E::kLift);
   const float factor = row.top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(row.top - top);
   row.top = top;
   row.sum *= factor;

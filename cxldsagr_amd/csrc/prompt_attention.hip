@@ -391,7 +391,7 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
         for (int u = kPerSlot * i; u < kPerSlot * (i + 1) && u < kPairs; ++u)
           top = fmaxf(fmaxf(top, to[2 * u]), to[2 * u + 1]);
         if (i == kPairs / kPerSlot)
-          rise = __builtin_amdgcn_ballot_w64(must_raise(row, max_halves(top) * a.scale_log2));
+          rise = __builtin_amdgcn_ballot_w64(must_raise<E>(row, max_halves(top) * a.scale_log2));
         if (i >= kVops - kAhead) read_k(k_at, i - (kVops - kAhead));
       });
       next_v();
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(C::kThreads, kV == 64 && C::kWaves > 1 ? 3 : 1) voi
     // it makes the compiler keep a second copy of them and spill.
     for (bool more = true; more;) {
       if (kStageKeys * (j + 1) > clear) mask(j, s);
-      const float factor = raise(row, row_max(s, a.scale_log2));
+      const float factor = raise<E>(row, row_max(s, a.scale_log2));
       shift = shift_of(row);
       if (__builtin_amdgcn_ballot_w64(factor != 1.0f)) {
 #pragma unroll

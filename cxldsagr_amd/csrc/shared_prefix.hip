@@ -396,7 +396,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
       lds_barrier();
       k_now = read_first_k(ahead);
       const float mx = max_halves(top) * a.scale_log2;
-      const uint64_t rise = __builtin_amdgcn_ballot_w64(must_raise(row, mx));
+      const uint64_t rise = __builtin_amdgcn_ballot_w64(must_raise<E>(row, mx));
       values(at, vop, p, kVops - kAhead, kVops, no_slice);
       return keys < kBlockKeys || rise != 0 ? kBreak : kGo;
     };
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(kThreads, 1) void shared_prefix_fwd(const PrefixArg
     k_now = read_first_k(after(now));
     for (bool more = true; more;) {
       if (keys < kBlockKeys) mask(keys, s);
-      const float factor = raise(row, row_max(s, a.scale_log2));
+      const float factor = raise<E>(row, row_max(s, a.scale_log2));
       shift = shift_of(row);
       if (__builtin_amdgcn_ballot_w64(factor != 1.0f)) {
 #pragma unroll

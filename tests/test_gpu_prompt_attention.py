@@ -1,6 +1,8 @@
 """Prompt attention against the 64-bit formula, at the sizes and masks where it can go
 wrong. Tolerances: ``oracle.dense.attention_bound``, derived there."""
 
+import math
+
 import pytest
 import torch
 
@@ -189,3 +191,54 @@ def test_captured_call_replays_and_other_streams(gpu):
             assert torch.equal(call(), want)
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("drop", [15.7, 20.3, 25.3])
+@pytest.mark.parametrize(("queries", "keys"), [(1, 3000), (40, 900)])
+def test_many_low_scores_behind_one_peak(gpu, queries, keys, drop):
+    """fp16: the first key's probability is 1 and its value 0, every other's 2^-drop and 1,
+    which are then all of the result: small probabilities must not be lost, nor counted
+    otherwise in the sum than in the product. They are held against a maximum of at least 2^7, so
+    what the bound allows for subnormal ones is 2^7 less than for a maximum of 1."""
+    from cxldsagr_amd.attention import prompt_attention
+
+    q = torch.zeros(queries, 2, 64, dtype=torch.float16, device=gpu)
+    k = torch.zeros(keys, 1, 64, dtype=torch.float16, device=gpu)
+    v = torch.ones_like(k)
+    q[..., 0] = 1
+    k[1:, :, 0] = -drop * math.log(2)
+    v[0] = 0
+    cu_q, cu_k = _cu([queries], gpu), _cu([keys], gpu)
+    out, size, reach = dense.prompt_attention(q, k, v, 1.0, cu_q.tolist(), cu_k.tolist())
+    bound = dense.attention_bound(out, size, reach, keys, torch.finfo(q.dtype).eps, 64, 2.0 ** -7)
+    off = (prompt_attention(q, k, v, 1.0, cu_q, cu_k, max_k=keys).cpu().double() - out).abs()
+    assert (off <= bound).all(), (off / out).max()
+    # The peak last: what was summed before is scaled by 2^-drop in 32 bits.
+    k, v = k.flip(0), v.flip(0)
+    out, size, reach = dense.prompt_attention(q[:1], k, v, 1.0, [0, 1], [0, keys])
+    bound = dense.attention_bound(out, size, reach, keys, torch.finfo(q.dtype).eps, 64, 2.0 ** -7)
+    got = prompt_attention(q[:1], k, v, 1.0, _cu([1], gpu), cu_k, max_k=keys)
+    assert ((got.cpu().double() - out).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("power", [20, 24, 26])
+def test_fp16_scores_far_from_zero(gpu, power):
+    """Scores of up to 2^power in log2 units, whose 32-bit steps are then up to 4: the
+    probabilities, which are only as near to 1 as such steps let them be, stay within fp16."""
+    from cxldsagr_amd.attention import prompt_attention
+
+    gen = torch.Generator().manual_seed(21)
+    q = torch.zeros(3, 1, 64, dtype=torch.float16, device=gpu)
+    k = torch.zeros(400, 1, 64, dtype=torch.float16, device=gpu)
+    v = torch.randn(400, 1, 64, generator=gen).half().to(gpu)
+    q[..., 0] = 2.0 ** (power - 14)
+    k[..., 0] = 2.0 ** 13 * (1 + 2.0 ** -10 * torch.randint(16, (400, 1), generator=gen)).to(gpu)
+    cu_q, cu_k = _cu([3], gpu), _cu([400], gpu)
+    got = prompt_attention(q, k, v, 1.0, cu_q, cu_k)
+    assert got.isfinite().all()
+    # The keys of the largest score share the result equally, the others are at least 2^9 below
+    # it; what is off is fp32 sums and one rounding to fp16.
+    for i in range(3):
+        seen = k[:398 + i, 0, 0]
+        want = v[:398 + i, 0][seen == seen.max()].double().mean(0)
+        assert ((got[i, 0].double() - want).abs() <= 2.0 ** -10 * (want.abs() + 1)).all()
