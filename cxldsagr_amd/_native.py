@@ -13,12 +13,13 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libdsa_gfx950.so"
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _ptr = ctypes.c_void_p
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> argument types (restype is int for every entry point)
 SIGNATURES = {
@@ -75,9 +76,9 @@ SIGNATURES = {
     "dsa_sparse_mla_fp8_paged_ws": [_ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _f32,
                                     _ptr, _ptr, _i64, _ptr],
     "dsa_rope_pair": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64,
-                      _i64, _i64, _int, _i64, _i64, _i64, _i64, _ptr, _int, _ptr, _f32, _int,
+                      _i64, _i64, _int, _i64, _i64, _i64, _i64, _ptr, _int, _ptr, _f64, _int,
                       _int, _ptr],
-    "dsa_kv_write_fp8": [_ptr, _i64, _i64, _ptr, _int, _ptr, _f32, _ptr, _int, _ptr, _f32, _int,
+    "dsa_kv_write_fp8": [_ptr, _i64, _i64, _ptr, _int, _ptr, _f32, _ptr, _int, _ptr, _f64, _int,
                          _i64, _ptr, _ptr, _ptr],
     "dsa_kv_read_fp8": [_ptr, _i64, _ptr, _int, _i64, _ptr, _ptr, _ptr],
     "dsa_prompt_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64,

@@ -617,7 +617,7 @@ struct WriteArgs {
   float eps;
   const void* positions;     // null: no rotation
   const float* frequencies;
-  float magnitude;
+  double magnitude;
   int32_t wide_slots, wide_positions, interleaved;
   uint8_t* cache;
   int32_t* status;
@@ -818,12 +818,12 @@ __global__ __launch_bounds__(256) void read_kv(const uint8_t* __restrict__ cache
 
 extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t tokens, const void* slots,
                                 int wide_slots, const float* norm_weight, float norm_eps, const void* positions,
-                                int wide_positions, const float* frequencies, float magnitude, int interleaved,
+                                int wide_positions, const float* frequencies, double magnitude, int interleaved,
                                 int64_t pages, void* cache, int32_t* status, hipStream_t stream) {
   using namespace dsa;
   DSA_CHECK_ARG(tokens >= 0 && pages >= 0 && kv_stride >= 0 && kv_stride % 8 == 0,
                 "invalid KV write shape (the row stride must be a multiple of 8 elements)");
-  DSA_CHECK_ARG(__builtin_isfinite(norm_eps) && norm_eps >= 0.0f && __builtin_isfinite(magnitude),
+  DSA_CHECK_ARG(__builtin_isfinite(norm_eps) && norm_eps >= 0.0f && __builtin_isfinite((float)magnitude),
                 "eps must be finite and nonnegative, magnitude finite");
   if (tokens == 0) return kOk;
   DSA_CHECK_ARG(kv && slots && (cache || pages == 0) && (positions == nullptr || frequencies), "null pointer");

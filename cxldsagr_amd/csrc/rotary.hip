@@ -37,7 +37,8 @@ struct RopeArgs {
   const float* frequencies;
   int64_t tokens;
   int32_t wide_positions, dim, offset, half, interleaved, copy;
-  float magnitude, sign;
+  double magnitude;
+  float sign;
 };
 
 template <typename T>
@@ -180,7 +181,7 @@ extern "C" int dsa_rope_pair(const void* q, int64_t q_token_stride, int64_t q_he
                              int64_t k_token_stride, int64_t k_head_stride, void* k_out,
                              int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_heads, int dtype,
                              int64_t tokens, int64_t dim, int64_t offset, int64_t rotated, const void* positions,
-                             int wide_positions, const float* frequencies, float magnitude, int interleaved,
+                             int wide_positions, const float* frequencies, double magnitude, int interleaved,
                              int inverse, hipStream_t stream) {
   using namespace dsa;
   DSA_CHECK_ARG(dtype >= 0 && dtype <= 2, "unknown element type");
@@ -190,7 +191,7 @@ extern "C" int dsa_rope_pair(const void* q, int64_t q_token_stride, int64_t q_he
   DSA_CHECK_ARG(rotated >= 2 && rotated % 2 == 0 && rotated <= 2 * kTableEntries && offset >= 0 &&
                     offset + rotated <= dim && (dim - rotated) % 2 == 0,
                 "the rotated part must be an even number of dims within the head, the rest even too");
-  DSA_CHECK_ARG(__builtin_isfinite(magnitude), "magnitude must be finite");
+  DSA_CHECK_ARG(__builtin_isfinite((float)magnitude), "magnitude must be finite");
   if (tokens == 0 || q_heads + k_heads == 0) return kOk;
   DSA_CHECK_ARG((q_heads == 0 || (q && q_out)) && (k_heads == 0 || (k && k_out)) && positions && frequencies,
                 "null pointer");

@@ -6,12 +6,13 @@
 namespace dsa {
 namespace rotary_core {
 
-// cos and sin of position * frequency, times magnitude, in 64 bits and rounded once (in
-// 32, the angle of position 163,839 would be off by 2^-7). The angle in turns, less
+// cos and sin of position * frequency, times magnitude, in 64 bits and rounded once to 32
+// (in 32, the angle of position 163,839 would be off by 2^-7; a magnitude in 32 bits would
+// add a rounding of its own). The angle in turns, less
 // whole turns and quarters, leaves x within an eighth of a turn, where the power series
 // of sin to x^11 and of cos to x^10 are off by less than 2^-32: fewer instructions than
 // 32-bit functions of any angle take, whose results were off by up to 2^-23.
-__device__ __forceinline__ float2 turn(int64_t position, float frequency, float magnitude) {
+__device__ __forceinline__ float2 turn(int64_t position, float frequency, double magnitude) {
   constexpr double kInverseTurn = 0.15915494309189533577, kTurn = 6.28318530717958647693;  // 1 / (2 pi), 2 pi
   const double turns = (double)position * (double)frequency * kInverseTurn;
   const double part = turns - __builtin_rint(turns);
@@ -32,8 +33,8 @@ __device__ __forceinline__ float2 turn(int64_t position, float frequency, float 
   // By q quarters: (c, s), (-s, c), (-c, -s), (s, -c).
   const int q = (int)quarters & 3;
   const double cq = q & 1 ? s : c, sq = q & 1 ? c : s;
-  return make_float2((float)((q == 1 || q == 2 ? -cq : cq) * (double)magnitude),
-                     (float)((q & 2 ? -sq : sq) * (double)magnitude));
+  return make_float2((float)((q == 1 || q == 2 ? -cq : cq) * magnitude),
+                     (float)((q & 2 ? -sq : sq) * magnitude));
 }
 
 // float32 -> bf16 bits, to nearest even (v_cvt_pk_bf16_f32; a NaN stays one).

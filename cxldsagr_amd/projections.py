@@ -104,8 +104,9 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
     for long contexts): dims ``offset .. offset + R - 1`` of each head turn by
     ``positions[t] * frequencies[i]``, pair ``i`` being dims ``(2 i, 2 i + 1)`` with
     ``interleaved``, else ``(i, i + R / 2)``; cos and sin are multiplied by
-    ``magnitude`` (the attention factor of a stretched context). Angles are in 64
-    bits, values in 32, rounded once. ``inverse`` turns back (with
+    ``magnitude`` (the attention factor of a stretched context). Both are formed in
+    64 bits and rounded once to 32; products and sum are in 32 bits, and the
+    result is rounded once to ``q``'s type. ``inverse`` turns back (with
     ``magnitude`` as given): the gradient's rotation.
 
     Returns ``(q_out, k_out)``, new contiguous tensors unless given; the dims that

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 1
+#define DSA_ABI_VERSION 2
 
 /* Element types accepted by dsa_quantize_fp8_rows. */
 #define DSA_DTYPE_BF16 0
@@ -459,8 +459,9 @@ int dsa_sparse_mla_fp8_paged_ws(const void* q, int64_t rows, int64_t heads, cons
  * frequencies[i] (positions int32, or int64 with wide_positions != 0; frequencies
  * f32 [rotated / 2]): a' = magnitude (a cos t - b sin t), b' = magnitude (b cos t
  * + a sin t) for the pair (a, b) = dims (2 i, 2 i + 1) with interleaved != 0, else
- * (i, i + rotated / 2); inverse != 0: -t. Angles in 64 bits, values in 32,
- * rounded once. The other dims are copied. q_out / k_out may be q / k with the
+ * (i, i + rotated / 2); inverse != 0: -t. magnitude cos t and magnitude sin t are
+ * formed in 64 bits and rounded once to 32, the products and their sum are fp32, and
+ * the result is rounded once to `dtype`. The other dims are copied. q_out / k_out may be q / k with the
  * same strides (in place) or memory apart from them. rotated and dim - rotated
  * even.
  */
@@ -470,7 +471,7 @@ int dsa_rope_pair(const void* q, int64_t q_token_stride, int64_t q_head_stride, 
                   int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t k_heads,
                   int dtype, int64_t tokens, int64_t dim, int64_t offset, int64_t rotated,
                   const void* positions, int wide_positions, const float* frequencies,
-                  float magnitude, int interleaved, int inverse, hipStream_t stream);
+                  double magnitude, int interleaved, int inverse, hipStream_t stream);
 
 /*
  * New tokens into any slots of the fp8 paged cache, as dsa_kv_pack_fp8 writes
@@ -486,7 +487,7 @@ int dsa_rope_pair(const void* q, int64_t q_token_stride, int64_t q_head_stride, 
 int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t tokens, const void* slots,
                      int wide_slots, const float* norm_weight, float norm_eps,
                      const void* positions, int wide_positions, const float* frequencies,
-                     float magnitude, int interleaved, int64_t pages, void* cache,
+                     double magnitude, int interleaved, int64_t pages, void* cache,
                      int32_t* status, hipStream_t stream);
 
 /*

@@ -5,6 +5,8 @@ by one more; formed in 64 bits and rounded once they are off by 2^-24 m), so a r
 2^-20 m (|a| + |b|) and the fp32 products and sum by 2^-22 m (|a| + |b|); then it is rounded
 once, by at most half a step."""
 
+import math
+
 import pytest
 import torch
 
@@ -178,3 +180,66 @@ def test_infinities_and_nan_as_in_the_formula(gpu, dtype):
         assert torch.equal(got.isnan(), want.isnan())
         infinite = want.isinf()
         assert torch.equal(got.isinf(), infinite) and torch.equal(got[infinite], want[infinite])
+
+
+def _near(got, x, positions, frequencies, offset, interleaved, magnitude, inverse=False):
+    """cos and sin come from 64-bit angles and a 64-bit magnitude and are rounded once: off by
+    2^-24 of themselves and, for the series, less than 2^-31 m. The two products and the sum
+    round once each in fp32, the result once to its type (fp32: the sum's rounding). Each is at
+    most half a step."""
+    want = dense.rope(x, positions, frequencies, offset, interleaved, magnitude, inverse)
+    half = len(frequencies)
+    part = x.detach().cpu().double()[..., offset:offset + 2 * half].abs()
+    if interleaved:
+        both = (part[..., 0::2] + part[..., 1::2]).repeat_interleave(2, -1)
+    else:
+        both = (part[..., :half] + part[..., half:]).repeat(1, 1, 2)
+    turned = want[..., offset:offset + 2 * half].abs()
+    inner = (2 * 2.0 ** -24 + 2.0 ** -31 + 2.0 ** -47) * abs(magnitude) * both
+    inner += 2.0 ** -24 * (turned + inner)
+    if x.dtype != torch.float32:  # (fp16 has steps of 2^-24 below 2^-14)
+        inner += torch.finfo(x.dtype).eps / 2 * (turned + inner) + 2.0 ** -25
+    off = (got.cpu().double() - want)[..., offset:offset + 2 * half].abs()
+    assert (off <= inner).all(), (off - inner).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_as_near_as_the_roundings_allow(gpu, dtype, interleaved, inverse):
+    from cxldsagr_amd.projections import apply_rope_pair
+
+    gen = torch.Generator().manual_seed(48)
+    magnitude = 0.1 * math.log(40.0) + 1.0  # (not a value of 32 bits)
+    frequencies = _frequencies(64, gpu)
+    positions = torch.randint(163840, (200,), generator=gen).to(gpu)
+    positions[:3] = torch.tensor([0, 1, 163839])
+    kwargs = dict(offset=128, interleaved=interleaved, magnitude=magnitude, inverse=inverse)
+    x = torch.randn(200, 8, 192, generator=gen).to(dtype).to(gpu)
+    odd = torch.zeros(200, 8, 193, dtype=dtype, device=gpu)[..., 1:].copy_(x)  # (no vectors)
+    for part in (x, odd):
+        got, _ = apply_rope_pair(part, None, positions, frequencies, **kwargs)
+        _near(got, x, positions, frequencies, 128, interleaved, magnitude, inverse)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_cos_and_sin_are_rounded_once(gpu, interleaved, inverse):
+    """Pairs (1, 0) and (0, 1) give them as they are: off by half a step of fp32, 2^-24 of
+    themselves, and less than 2^-31 of the magnitude for the series."""
+    from cxldsagr_amd.projections import apply_rope_pair
+
+    gen = torch.Generator().manual_seed(49)
+    magnitude = 0.1 * math.log(40.0) + 1.0
+    frequencies = _frequencies(64, gpu)
+    positions = torch.randint(163840, (300,), generator=gen).to(gpu)
+    x = torch.zeros(300, 2, 64, device=gpu)
+    second = torch.arange(1, 64, 2) if interleaved else torch.arange(32, 64)
+    x[:, 0] = 1
+    x[:, 0, second] = 0
+    x[:, 1, second] = 1
+    got, _ = apply_rope_pair(x, None, positions, frequencies, interleaved=interleaved, magnitude=magnitude,
+                             inverse=inverse)
+    want = dense.rope(x, positions, frequencies, 0, interleaved, magnitude, inverse)
+    off = (got.cpu().double() - want).abs()
+    assert (off <= 2.0 ** -24 * want.abs() + 2.0 ** -31 * magnitude).all(), (off / want.abs()).max()
