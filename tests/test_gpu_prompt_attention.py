@@ -242,3 +242,50 @@ def test_fp16_scores_far_from_zero(gpu, power):
         seen = k[:398 + i, 0, 0]
         want = v[:398 + i, 0][seen == seen.max()].double().mean(0)
         assert ((got[i, 0].double() - want).abs() <= 2.0 ** -10 * (want.abs() + 1)).all()
+
+
+def _parts(queries, heads, kv_heads, v_dim, keys):
+    """Into how many ranges one sequence's keys are split (0: not)."""
+    from cxldsagr_amd import _native
+
+    size = _native.size_of("dsa_prompt_attention_workspace_bytes", 0, queries, heads, kv_heads, v_dim, 1,
+                           keys, keys)
+    return size // (queries * heads * (4 * v_dim + 8))
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize(
+    ("queries", "keys", "least", "most"),
+    [
+        (1, 700, 2, 4),         # each range of part counts is joined in its own way
+        (1, 2049, 5, 32),
+        (1, 33001, 33, 256),
+        (2, 33000, 33, 256),
+        (17, 703, 2, 4),        # more rows than one wave has
+        (17, 9001, 33, 256),
+    ],
+)
+def test_joins_of_few_and_many_parts(gpu, dims, dtype, queries, keys, least, most):
+    from cxldsagr_amd.attention import prompt_attention
+
+    assert least <= _parts(queries, 4, 2, dims[1], keys) <= most
+    q, k, v, cu_q, cu_k = _inputs(gpu, [queries], [keys], 4, 2, dims, dtype, 22)
+    # The largest scores in different parts for different rows, and one part that hardly counts.
+    k[keys // 3:keys // 2] *= 2
+    k[-100:-60] *= 0.125
+    got = prompt_attention(q, k, v, dims[0] ** -0.5, cu_q, cu_k, max_k=keys)
+    _check(got, q, k, v, dims[0] ** -0.5, cu_q, cu_k)
+    again = prompt_attention(q, k, v, dims[0] ** -0.5, cu_q, cu_k, max_k=keys)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("keys", [511, 512, 513, 767, 768, 769])
+@pytest.mark.parametrize("queries", [1, 3])
+def test_lengths_around_two_and_three_parts(gpu, keys, queries):
+    from cxldsagr_amd.attention import prompt_attention
+
+    q, k, v, cu_q, cu_k = _inputs(gpu, [queries], [keys], 4, 2, (128, 128), torch.bfloat16, 23)
+    assert _parts(queries, 4, 2, 128, keys) >= 2
+    got = prompt_attention(q, k, v, 0.1, cu_q, cu_k, max_k=keys)
+    _check(got, q, k, v, 0.1, cu_q, cu_k)

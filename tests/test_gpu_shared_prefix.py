@@ -146,3 +146,47 @@ def test_captured_call_replays(gpu):
             assert torch.equal(_run(x, 3000), want)
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+def _parts(tokens, heads, prefix, suffix_pages):
+    """Into how many parts a row's keys are split (0: not)."""
+    from cxldsagr_amd import _native
+
+    size = _native.size_of("dsa_shared_prefix_mla_workspace_bytes", 0, tokens, heads, prefix, suffix_pages)
+    rows = tokens * heads
+    return size // ((rows + 31) // 32 * 32 * 2048 + 8 * rows)
+
+
+@pytest.mark.parametrize(
+    ("prefix", "suffixes", "queries", "heads", "least", "most"),
+    [
+        # Each range of part counts is joined in its own way, more than 32 of them by rows too.
+        (96, [64, 3, 17] * 8, [1] * 24, 64, 2, 4),
+        (600, [5, 64], [1, 3], 128, 5, 32),
+        (8600, [40, 1], [1, 1], 128, 33, 256),
+        (8601, [7, 64], [2, 3], 64, 33, 256),
+        (8600, [70], [1], 128, 33, 256),
+        (8599, [3], [1], 16, 33, 256),
+    ],
+)
+def test_joins_of_few_and_many_parts(gpu, prefix, suffixes, queries, heads, least, most):
+    x, values = _case(gpu, prefix, suffixes, queries, heads, 38)
+    assert least <= _parts(sum(queries), heads, prefix, x["suffix_tables"].shape[1]) <= most
+    got = _run(x, prefix)
+    _check(got, x, values)
+    assert torch.equal(got, _run(x, prefix))
+
+
+@pytest.mark.parametrize("heads", [64, 128])
+def test_each_branch_alone_behind_the_prefix(gpu, heads):
+    """A branch called by itself, whose keys are split otherwise, and within the batch: both
+    are within the bound of the formula's values."""
+    lengths, queries = [9, 1, 70, 30], [2, 1, 1, 3]
+    x, values = _case(gpu, 5000, lengths, queries, heads, 39)
+    _check(_run(x, 5000), x, values)
+    starts = x["cu_q"].tolist()
+    for b, n in enumerate(queries):
+        one = dict(x, q=x["q"][starts[b]:starts[b + 1]].contiguous(),
+                   suffix_tables=x["suffix_tables"][b:b + 1], suffix_tokens=x["suffix_tokens"][b:b + 1],
+                   cu_q=torch.tensor([0, n], dtype=torch.int32, device=gpu))
+        _check(_run(one, 5000), one, (values[0], values[1][b:b + 1]))
