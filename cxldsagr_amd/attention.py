@@ -382,10 +382,19 @@ def prompt_attention(q, k, v, scale, cu_q, cu_k=None, *, causal=True, max_k=None
 
     Returns ``[Tq, H, d_v]`` in ``q``'s type, or writes it to ``out``
     (contiguous); queries outside the sequences (before ``cu_q[0]``, from
-    ``cu_q[-1]`` on) are left as they were in ``out``. ``max_k``: the longest
-    sequence's keys where the caller knows it, by which few queries' keys are
-    split over the GPU; it does not change what is computed. Forward only. A
-    key that some query of its sequence does not see must have finite values.
+    ``cu_q[-1]`` on) are left as they were in ``out``, and in a new tensor hold
+    anything. ``max_k``: the longest sequence's keys where the caller knows it,
+    by which few queries' keys are split over the GPU; it does not change what
+    is computed. Forward only. A key that some query of its sequence does not
+    see must have finite values.
+
+    Scores (up to 2^25 in magnitude once scaled), the softmax's maxima and all
+    sums are in 32 bits; probabilities are rounded to ``q``'s type before the
+    product with ``v`` and before they are summed. One cut into row tiles and
+    key ranges, chosen from the totals, serves all sequences of a call: single
+    tokens over long histories are faster in a call of their own than beside
+    prompts (2,048 tokens and one over 40,000 keys, 32 heads on 8: 672 us, apart
+    55 + 35).
     """
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError("Expected q [Tq,H,Dqk], k [Tk,Hkv,Dqk], and v [Tk,Hkv,Dv]")
@@ -458,8 +467,11 @@ def shared_prefix_mla(q, kv_cache, prefix_table, prefix_tokens, suffix_tables, s
     once for all branches; any H.
 
     Returns bf16 ``[T, H, 512]``, or writes it to ``out`` (contiguous), where
-    queries of no branch are left as they were. A query that sees no key gives
-    zeros; tokens on a page outside the cache are padding.
+    queries of no branch are left as they were (in a new tensor they hold
+    anything). A query that sees no key gives zeros; tokens on a page outside
+    the cache are padding. Scores, maxima and sums are in 32 bits; probabilities
+    are rounded to bf16 before the product with the latent and before they are
+    summed.
     """
     if q.ndim != 3 or value_dim != V_DIM:
         raise ValueError("Expected q [T,H,576] with H >= 1 and value_dim 512")

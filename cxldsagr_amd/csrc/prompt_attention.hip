@@ -11,7 +11,7 @@
 // heads fill a tile and K and V are staged once for all of them. A work-group has 128
 // rows, 32 per wave, two work-groups share a CU (one's start, masks and stores run
 // beside the other's products; 256 rows of one work-group took 285 us where these take
-// 200: 2,048 tokens, 128 heads of 192 / 128), and walks the keys in stages of 32. A
+// 185: 2,048 tokens, 128 heads of 192 / 128), and walks the keys in stages of 32. A
 // wave computes S^T = K Q^T (v_mfma_f32_32x32x16, Q^T in registers). The result's layout
 // - a lane holds 16 keys of one row - is the operand layout of O^T += V^T P^T once the
 // keys of V^T are read in the same order, so probabilities never leave registers and a
@@ -20,10 +20,12 @@
 // before, then that stage's product with V beside the maxima of the new one.
 //
 // What bounds it: in long calls the matrix unit at the clock that the power limit leaves
-// (1.84 GHz in the call above, 860 TFLOP/s; 8,192 tokens 1.1 PFLOP/s, where a library
-// product of large matrices reaches 1.36); in batches of short sequences the start and end
-// of a work-group, 9k to 15k cycles (7 prompts of 4,001 tokens, 42 us); with few rows the
-// loads of K and V (8 single tokens over 40,000 keys, 31 us and 4 for the join, 4.7 TB/s).
+// (1.84 GHz in the call above, 928 TFLOP/s) and its starts and ends; 8,192 tokens reach 1.0
+// PFLOP/s, where a library product of large matrices reaches 1.36. In batches of short
+// sequences the start and end of a work-group, 9k to 15k cycles (7 prompts of 4,001 tokens,
+// 37 us); with few rows the loads of K and V (8 single tokens over 40,000 keys, 30 us and 4
+// for the join, 4.9 TB/s). One cut serves a whole call: a prompt of 2,048 tokens beside one
+// token over 40,000 keys (32 heads on 8 of 128 dims) takes 672 us, apart 55 and 35.
 // Q loads and stores in pieces of 64 bytes, by lanes trading, took as long as they save.
 //
 // Stages arrive by LDS DMA two ahead, in blocks of 16 rows by 64 bytes: lane l brings

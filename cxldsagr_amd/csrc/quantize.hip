@@ -659,14 +659,14 @@ __device__ __forceinline__ double inverse_sqrt(double x) {
 }
 
 // New tokens into any slots of the fp8 paged cache: the latent through RMSNorm
-// (x (mean x^2 + eps)^-1/2 w, the lanes' sums added in 64 bits, rounded to bf16, which is what a model's norm
-// hands on: with fp32 sums and products 13 to 24 of 33 million codes were not the
-// formula's, so 0 to 3, for 1.6 us of 65,536 tokens), the RoPE part rotated (fp32, rounded to bf16), then the record of
-// pack_tokens. A wave takes kTokens tokens whose loads are all issued first: lane l
-// has 8 latent values of each, and a half wave the 32 rotary pairs of every other
-// one. Bound by memory, 1,152 B read and 656 B written per token, once enough loads
-// are in flight: 65,536 tokens take 27.9 us (4.2 TB/s), 35.6 with one token per wave and
-// reductions through LDS permutes.
+// (x (mean x^2 + eps)^-1/2 w, the lanes' sums added in 64 bits, rounded to bf16, which
+// is what a model's norm hands on: with fp32 sums and products 13 to 24 of 33 million
+// codes were not the formula's, so 0 to 3, for 1.6 us of 65,536 tokens), the RoPE part
+// rotated (fp32, rounded to bf16), then the record of pack_tokens. A wave takes kTokens
+// tokens whose loads are all issued first: lane l has 8 latent values of each, and a
+// half wave the 32 rotary pairs of every other one. Bound by memory, 1,152 B read and
+// 656 B written per token, once enough loads are in flight: 65,536 tokens take 26.8 us
+// (4.4 TB/s), 35.6 with one token per wave and reductions through LDS permutes.
 template <int kTokens>
 __global__ __launch_bounds__(256) void write_kv(const WriteArgs a) {
   const int64_t token0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kTokens;
@@ -834,8 +834,8 @@ extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t token
   const WriteArgs a{static_cast<const uint16_t*>(kv), kv_stride, tokens, pages * 64, slots, norm_weight, norm_eps,
                     positions, frequencies, magnitude, wide_slots != 0, wide_positions != 0, interleaved != 0,
                     static_cast<uint8_t*>(cache), status};
-  // One token per wave while waves are few, then two (65,536 tokens, norms in fp32: one 29.6 us, two
-  // 26.9, four 30.4).
+  // One token per wave while waves are few, then two (65,536 tokens, norms in fp32: one
+  // 29.6 us, two 26.9, four 30.4).
   if (tokens <= 4096)
     hipLaunchKernelGGL(write_kv<1>, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, stream, a);
   else

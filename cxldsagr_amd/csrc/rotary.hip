@@ -9,7 +9,7 @@
 // tokens (or a part of one token's heads) in items of eight pairs, two 16-byte
 // vectors of 16-bit values, one per thread (two or four of them were no faster in
 // 8,192 tokens of 128 heads, 55 us or 4.9 TB/s, and slower in small calls: 1,023
-// fp32 tokens 17.6 us, with four 20.0); while they are on their way it forms the
+// fp32 tokens 17.1 us, with four 20.0); while they are on their way it forms the
 // tokens' cosines and sines in LDS (64 bits, once for all heads; 16 tokens 6.6
 // -> 3.4 us against forming them first).
 // Types, offsets or strides that do not allow vectors take one pair at a time.

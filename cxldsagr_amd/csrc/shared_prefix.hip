@@ -29,7 +29,7 @@
 // of the LDS reads left out gave 6 %. 64 tokens of 128 heads over 65,600 keys take 940
 // us, 1.24 PFLOP/s, where a library product of large matrices reaches 1.36. Short calls
 // are bound by a work-group's start and end (10 us of a round) and by the parts of split
-// rows (one token over 32,896 keys: 27 us and 9 for the join).
+// rows (one token over 32,896 keys: 26 us and 9 for the join).
 #include "attention_core.h"
 #include "../../include/dsa_gfx950.h"
 

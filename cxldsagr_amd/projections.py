@@ -111,8 +111,8 @@ def apply_rope_pair(q, k, positions, frequencies, *, offset=0, interleaved=False
 
     Returns ``(q_out, k_out)``, new contiguous tensors unless given; the dims that
     are not rotated are copied. ``q_out`` may be ``q`` itself (in place; then
-    ``k_out`` is ``k`` or new), else it must not overlap the inputs. ``R`` and
-    ``D - R`` are even.
+    ``k_out`` is ``k`` or new), else it must not overlap the inputs. ``R`` (at most
+    4,096) and ``D - R`` are even.
     """
     if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in _native.DTYPE_CODES:
         raise ValueError("q must be bf16, fp16 or fp32 [tokens, heads, dim]")

@@ -26,6 +26,7 @@
 extern "C" {
 #endif
 
+/* 2: the magnitude of dsa_rope_pair and dsa_kv_write_fp8 is a double. */
 #define DSA_ABI_VERSION 2
 
 /* Element types accepted by dsa_quantize_fp8_rows. */
@@ -510,7 +511,9 @@ int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slots, int wid
  * what lies outside the tensors is cut off). With causal != 0 query i of n_q sees
  * keys j <= i + n_k - n_q, else every key. out: dtype [q_tokens, heads, v_dim]
  * contiguous, 16-byte aligned = softmax(scale q k^T) v, zeros for a query that
- * sees no key; queries outside the sequences are not written. scale > 0.
+ * sees no key; queries outside the sequences are not written. scale > 0. Scores (up to
+ * 2^25 in magnitude once scaled), maxima and sums are in 32 bits, probabilities are
+ * rounded to `dtype` before the product with v and before they are summed.
  * max_k: the longest sequence's keys (more than k_tokens: k_tokens), below 0: not
  * known (it decides how keys are split over work-groups, not what is computed). `workspace`: 16-byte aligned, at least
  * dsa_prompt_attention_workspace_bytes bytes (0: not used), no initialisation,
@@ -541,8 +544,8 @@ int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
  * sees the prefix and the first suffix_tokens[b] - n + 1 + i of the suffix. cu_q
  * null: one query per branch, tokens == branches. out: bf16 [tokens, heads, 512]
  * contiguous = softmax(scale q . record) record[:512], zeros for a query that sees
- * no key; queries of no branch are not written. q, cache and out 16-byte
- * aligned; scale > 0. Tokens on a page outside the cache count as padding.
+ * no key; queries of no branch are not written. Scores, maxima and sums are in 32
+ * bits, probabilities are rounded to bf16. q, cache and out 16-byte aligned; scale > 0. Tokens on a page outside the cache count as padding.
  * `workspace`: as dsa_prompt_attention's, dsa_shared_prefix_mla_workspace_bytes.
  */
 int dsa_shared_prefix_mla_workspace_bytes(int64_t tokens, int64_t heads, int64_t prefix_tokens,
