@@ -80,7 +80,8 @@ def attention_bound(out, size, reach, keys, eps, dim, tiny=0.0):
     eps / 2 of the result (2^-24 where it is tiny). ``tiny``: the largest |v| for a
     type whose probabilities may be subnormal (fp16: off by up to 2^-25 each, among
     probabilities that sum to at least 1), which moves the result by up to
-    2 keys 2^-25 tiny.
+    2 keys 2^-25 tiny. (Held against 2^7 at the maximum they sum to at least that: a
+    test that has to see small ones passes 2^-7 of it.)
     """
     score = (2 * (dim + 2) * 2.0 ** -24 + 2.0 ** -22) * reach + 2.0 ** -21
     d = (eps / 2 + score)[..., None]
