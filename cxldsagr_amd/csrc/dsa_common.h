@@ -42,6 +42,10 @@ void clear_error();
 
 int device_cu_count();
 
+// Whether a launch of so many work-groups (a count below 2^47) can be made: its work-items
+// are counted in 32 bits.
+constexpr bool grid_fits(int64_t groups, int64_t threads) { return groups * threads <= 0xFFFFFFFFll; }
+
 // The exact top-k of the fused indexer step from the candidate lists that the
 // logits kernel's candidate mode leaves (topk.hip; launched by logits.hip).
 int topk_from_candidates(const uint8_t* q, const uint8_t* k, const float* weights,

@@ -661,7 +661,10 @@ extern "C" int dsa_prompt_attention(const void* q, int64_t q_token_stride, int64
                  reinterpret_cast<uintptr_t>(out)) % 16 == 0,
                 "q, k, v and out must be 16-byte aligned");
   const PromptPlan p = prompt_plan(q_tokens, heads, kv_heads, v_dim, sequences, k_tokens, max_k);
-  DSA_CHECK_ARG(p.slots * kv_heads * p.splits < 0x7FFFFFFF, "too many query rows");
+  // (A call with splits has less than two rounds of row tiles, so its join is small.)
+  DSA_CHECK_ARG(p.slots <= 0xFFFFFFFFll / kv_heads / p.splits &&
+                    grid_fits(p.slots * kv_heads * p.splits, p.few ? FewRows::kThreads : ManyRows::kThreads),
+                "too many query rows or sequences");
   if (p.splits > 1)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "prompt attention workspace too small or misaligned");

@@ -830,7 +830,7 @@ extern "C" int dsa_kv_write_fp8(const void* kv, int64_t kv_stride, int64_t token
   DSA_CHECK_ARG(reinterpret_cast<uintptr_t>(kv) % 16 == 0 && reinterpret_cast<uintptr_t>(cache) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(norm_weight) % 16 == 0,
                 "kv, cache and norm_weight must be 16-byte aligned");
-  DSA_CHECK_ARG((tokens + 3) / 4 < 0x7FFFFFFF, "too many tokens for one launch");
+  DSA_CHECK_ARG(tokens < (int64_t)1 << 40 && grid_fits((tokens + 7) / 8, 256), "too many tokens for one launch");
   const WriteArgs a{static_cast<const uint16_t*>(kv), kv_stride, tokens, pages * 64, slots, norm_weight, norm_eps,
                     positions, frequencies, magnitude, wide_slots != 0, wide_positions != 0, interleaved != 0,
                     static_cast<uint8_t*>(cache), status};
@@ -852,7 +852,7 @@ extern "C" int dsa_kv_read_fp8(const void* cache, int64_t pages, const void* slo
   DSA_CHECK_ARG(slots && out && (cache || pages == 0), "null pointer");
   DSA_CHECK_ARG(reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(cache) % 16 == 0,
                 "cache and out must be 16-byte aligned");
-  DSA_CHECK_ARG((tokens + 7) / 8 < 0x7FFFFFFF, "too many tokens for one launch");
+  DSA_CHECK_ARG(tokens < (int64_t)1 << 40 && grid_fits((tokens + 7) / 8, 256), "too many tokens for one launch");
   hipLaunchKernelGGL(read_kv, dim3((unsigned)((tokens + 7) / 8)), dim3(256), 0, stream,
                      static_cast<const uint8_t*>(cache), pages * 64, slots, wide_slots != 0, tokens,
                      static_cast<uint16_t*>(out), status);

@@ -161,7 +161,7 @@ int launch_items(RopeArgs a, hipStream_t stream) {
     s.groups = (a.tokens + s.tokens_per_group - 1) / s.tokens_per_group * s.groups_per_token;
     groups += s.groups;
   }
-  DSA_CHECK_ARG(groups < 0x7FFFFFFF, "too many tokens for one launch");
+  DSA_CHECK_ARG(grid_fits(groups, kThreads), "too many tokens for one launch");
   if (groups == 0) return kOk;
   hipLaunchKernelGGL((rope_pair<T, kVector>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
   DSA_CHECK_LAUNCH("rope");

@@ -549,17 +549,20 @@ __global__ __launch_bounds__(64 * kWays * kChunks) void join_parts(
       v2u{Bf16::pack(acc.x * inv, acc.y * inv), Bf16::pack(acc.z * inv, acc.w * inv)};
 }
 
+// Ways for the parts there are (14 parts of 2,048 rows: 11.0 us with 2, 13.6 with 4; 91
+// of 256: 10.9 and 9.0); 16 where the rows alone do not fill the chip (171 of 128: 9.9 us,
+// with 4 12.3).
+int join_ways(int64_t rows, int64_t splits) { return splits <= 4 ? 1 : splits <= 32 ? 2 : rows >= 256 ? 4 : 16; }
+
 int launch_join_parts(const PrefixArgs& a, int64_t rows, int splits, hipStream_t stream) {
   const auto go = [&](auto kernel, int ways, int chunks) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 31) / 32 * (kVDim / 8 / chunks))), dim3(64 * ways * chunks), 0,
                        stream, a.parts, a.stats, rows, splits, a.cu_q, a.branches, (int64_t)a.heads, a.out);
   };
-  // Ways for the parts there are (14 parts of 2,048 rows: 11.0 us with 2, 13.6 with 4;
-  // 91 of 256: 10.9 and 9.0); 16 where the rows alone do not fill the chip (171 of 128:
-  // 9.9 us, with 4 12.3).
-  if (splits <= 4) go(join_parts<1, 4>, 1, 4);
-  else if (splits <= 32) go(join_parts<2, 4>, 2, 4);
-  else if (rows >= 256) go(join_parts<4, 2>, 4, 2);
+  const int ways = join_ways(rows, splits);
+  if (ways == 1) go(join_parts<1, 4>, 1, 4);
+  else if (ways == 2) go(join_parts<2, 4>, 2, 4);
+  else if (ways == 4) go(join_parts<4, 2>, 4, 2);
   else go(join_parts<16, 1>, 16, 1);
   DSA_CHECK_LAUNCH("join of the shared prefix's parts");
   return kOk;
@@ -679,7 +682,10 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   const int64_t tiles = (tokens * heads + kTileRows - 1) / kTileRows;
   const int64_t items = p.splits > 0 ? (tiles * p.splits + 7) / 8 * 8 : 0;
   const int64_t own = tokens * ((heads + kTileRows - 1) / kTileRows) * p.suffix_splits;
-  DSA_CHECK_ARG(items + own < 0x7FFFFFFF, "too many query rows");
+  // (The join has a wave for each way and eight dims of 32 rows.)
+  const int64_t rows = tokens * heads, joined = p.bytes > 0 ? join_ways(rows, p.splits + p.suffix_splits) : 0;
+  DSA_CHECK_ARG(grid_fits(items + own, kThreads) && grid_fits((rows + 31) / 32 * (kVDim / 8) * joined, 64),
+                "too many query rows");
   if (p.bytes > 0)
     DSA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
                   "shared prefix MLA workspace too small or misaligned");
@@ -701,6 +707,6 @@ extern "C" int dsa_shared_prefix_mla_fp8(const void* q, int64_t tokens, int64_t 
   a.scale_log2 = scale * kLog2E;
   hipLaunchKernelGGL(shared_prefix_fwd, dim3((unsigned)(items + own)), dim3(kThreads), 0, stream, a);
   DSA_CHECK_LAUNCH("shared prefix MLA");
-  if (p.bytes > 0) return launch_join_parts(a, tokens * heads, (int)(p.splits + p.suffix_splits), stream);
+  if (p.bytes > 0) return launch_join_parts(a, rows, (int)(p.splits + p.suffix_splits), stream);
   return kOk;
 }

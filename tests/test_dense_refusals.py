@@ -358,3 +358,19 @@ def test_row_counts_that_wrap_are_refused_before_the_plan():
     for change in (dict(tokens=1 << 57), dict(tokens=1 << 50, heads=1 << 14), dict(tokens=1 << 24)):
         with pytest.raises(ValueError, match="too many query rows"):
             _c_shared(**{**change, "branches": change["tokens"] if change["tokens"] < 1 << 31 else 1, "cu_q": P})
+
+
+def test_launches_past_32_bits_of_work_items():
+    """Refused with a message, before anything is launched."""
+    # 2^25 rows in two parts: the join's work-items.
+    with pytest.raises(ValueError, match="too many query rows"):
+        _c_shared(tokens=1 << 19, branches=1 << 19, heads=64)
+    with pytest.raises(ValueError, match="too many query rows"):
+        _c_prompt(sequences=1 << 21, heads=32, kv_heads=32, q_token=4096)
+    with pytest.raises(ValueError, match="too many tokens"):  # (33 dims: single pairs)
+        _native.call("dsa_rope_pair", P, 8448, 66, P, 8448, 66, 128, None, 0, 0, None, 0, 0, 0, 0, 1 << 24, 66,
+                     0, 66, P, 0, P, 1.0, 0, 0, None)
+    with pytest.raises(ValueError, match="too many tokens"):
+        _native.call("dsa_kv_write_fp8", P, 576, 1 << 27, P, 0, None, 0.0, None, 0, None, 1.0, 1, 1, P, None, None)
+    with pytest.raises(ValueError, match="too many tokens"):
+        _native.call("dsa_kv_read_fp8", P, 1, P, 0, 1 << 27, P, None, None)
