@@ -174,8 +174,7 @@ def prepare(case, seed):
             # The weights as the kernels read them, laid out once when a model is loaded.
             from cxldsagr_amd import feedforward
 
-            state["packed"] = feedforward.ExpertWeights(*state["parts"], first=first,
-                                                        total=total)
+            state["packed"] = feedforward.ExpertWeights(*state["parts"], first=first)
     return state
 
 
