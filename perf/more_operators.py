@@ -174,7 +174,8 @@ def prepare(case, seed):
             # The weights as the kernels read them, laid out once when a model is loaded.
             from cxldsagr_amd import feedforward
 
-            state["packed"] = feedforward.ExpertWeights(*state["parts"], first=first)
+            state["packed"] = feedforward.ExpertWeights(*state["parts"], first=first,
+                                                        total=total)
     return state
 
 
