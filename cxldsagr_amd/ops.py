@@ -15,11 +15,13 @@ the reference does not have: sparse_mla_fp8_paged and pack_kv_fp8, and those of
 the dense path around it: apply_rope_pair (rotary.py:47), write_kv_fp8 and
 read_kv_fp8 (records to and from any slots of the cache), prompt_attention
 (packed sequences, grouped heads) and shared_prefix_mla (branches over one
-prefix).
+prefix); and of the half of a layer behind the attention: residual_rms_norm,
+route_experts and expert_mlp over ExpertWeights.
 """
 
 from .attention import (pack_kv_fp8, prompt_attention, read_kv_fp8, shared_prefix_mla, sparse_mla,
                         sparse_mla_fp8_paged, sparse_mla_from_pool, write_kv_fp8)
+from .feedforward import ExpertWeights, expert_mlp, residual_rms_norm, route_experts
 from .indexer import exact_topk, logits, quantize_index
 from .kv_transfer import copy_host_records_async, gather_host_records
 from .projections import apply_rope_pair
@@ -39,4 +41,8 @@ __all__ = [
     "read_kv_fp8",
     "prompt_attention",
     "shared_prefix_mla",
+    "residual_rms_norm",
+    "route_experts",
+    "ExpertWeights",
+    "expert_mlp",
 ]

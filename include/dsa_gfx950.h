@@ -658,6 +658,62 @@ int dsa_pool_release_rows(const int32_t* page_table, int64_t pages, int64_t host
                           int32_t* h2d, int64_t* d2h, int64_t* priority, int64_t slots,
                           int32_t* status, hipStream_t stream);
 
+/*
+ * The half of a decoder layer behind the attention (no reference counterpart among the
+ * operators rebuilt here; forward only).
+ *
+ * dsa_residual_rms_norm: t = x + residual (32 bits), y = t * weight / sqrt(mean t^2 + eps).
+ * x, residual (or NULL): [tokens, dim] of `dtype` with row strides, dim 1 .. 16384; weight
+ * [dim] of weight_dtype (dtype or fp32). Outputs are contiguous, each or NULL: values y and
+ * residual_out t in `dtype`, rounded once; codes e4m3 [tokens, dim] of the rounded y with
+ * scales [tokens, dim / 128], the exponent bytes (e8m0) of a power of two per 128 values
+ * (amax * fl32(1/448) rounded up); both or neither, dim then in whole blocks of 128 and all
+ * rows 16-byte aligned. residual_out may be residual, values x.
+ */
+int dsa_residual_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                          int64_t residual_stride, int dtype, const void* weight,
+                          int weight_dtype, int64_t tokens, int64_t dim, double eps, void* values,
+                          void* residual_out, void* codes, void* scales, hipStream_t stream);
+
+/*
+ * Each token's k experts (1 .. 64) and their weights. logits: [tokens, experts] of `dtype`,
+ * row stride `stride`, experts 1 .. 1024. s = sigmoid (softmax == 0) or softmax of a row,
+ * formed in 64 bits and rounded to fp32; experts rank by s + bias (f32 [experts] or NULL),
+ * ties to the lower index, NaN above all, among the top_groups best of `groups` equal groups
+ * (1 .. 64; a group counts as its best expert, with a bias as its two best's sum).
+ * weights f32 and ids int32 [tokens, k], best first: s * scale, or with renormalize
+ * s / (the k's sum + 1e-20) * scale.
+ */
+int dsa_route_experts(const void* logits, int64_t stride, int dtype, int64_t tokens,
+                      int64_t experts, int64_t k, const float* bias, int softmax, int64_t groups,
+                      int64_t top_groups, int renormalize, double scale, float* weights,
+                      int32_t* ids, hipStream_t stream);
+
+/*
+ * out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j] - first,
+ * over the choices with 0 <= e < experts. x: e4m3 [tokens, dim], x_scale: exponent bytes
+ * [tokens, dim / 128]; ids int32, weights f32 [tokens, choices] (1 .. 64 choices); dim and
+ * inner in whole blocks of 128, tokens up to 2^22, experts 1 .. 1024 of the model's `total`
+ * (which only steers tiles). Weights are e4m3 in tiles of 16 rows by 128 columns, 2048 bytes,
+ * [experts][rows / 16][columns / 128][plane 2][g 4][row 16][16 bytes]: bytes 64 plane + 16 g ..
+ * of a row's 128. gate_up has 2 inner rows, tiles of 16 gate rows and of 16 up rows in turn;
+ * down has dim rows. Scales are exponent bytes per 128 by 128: gate_up_scale
+ * [experts, 2 inner / 128, dim / 128] (gate's blocks, then up's), down_scale
+ * [experts, dim / 128, inner / 128]. silu(gate) * up is rounded to e4m3 codes with a power of
+ * two per 128; sums are in 32 bits; an expert's result is held in 11 bits before it is
+ * weighted. out: [tokens, dim] of `dtype`. workspace: device memory of
+ * dsa_expert_mlp_workspace_bytes(...), 16-byte aligned, uninitialised; calls that overlap
+ * need different ones.
+ */
+int dsa_expert_mlp_workspace_bytes(int64_t tokens, int64_t choices, int64_t dim, int64_t inner,
+                                   int64_t experts, int64_t total, int64_t* bytes);
+int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t tokens, int64_t dim,
+                       int64_t inner, const void* gate_up, const void* gate_up_scale,
+                       const void* down, const void* down_scale, int64_t experts, int64_t first,
+                       int64_t total, const int32_t* ids, const float* weights, int64_t choices,
+                       void* out, int dtype, void* workspace, int64_t workspace_bytes,
+                       hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,8 @@ reference checkout):
                    ``attention/_validation.py:8-24``, ``device_only/mla.py:58-115``.
 * ``kv_fp8``     - the 656-byte paged fp8 KV record (no reference counterpart;
                    built from the A1 quantiser rule).
+* ``feedforward`` - the residual's RMSNorm, routing to experts and their MLP in
+                   64 bits (no reference counterpart).
 * ``recall``     - ``cache/sparse_token_cache.py:483-569`` and
                    ``operators/common/kv_transfer.py:21-68``.
 * ``layer``      - the CPU DSA layer in the order of

@@ -1,0 +1,146 @@
+"""The norm, the routing and the experts' MLP in 64 bits (TEST INFRASTRUCTURE ONLY).
+
+The formulas of ``feedforward.residual_rms_norm``, ``feedforward.route_experts`` and
+``feedforward.expert_mlp``; the last with what bounds a 32-bit kernel's error element
+by element. Pinned by ``tests/test_oracle_feedforward.py`` on closed forms.
+"""
+
+import math
+
+import torch
+
+BLOCK = 128
+
+
+def wide(tensor):
+    return tensor.detach().cpu().double()
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """``(y, t)``: the sum as one of 32 bits, its norm unrounded."""
+    t = x.detach().cpu().float()
+    if residual is not None:
+        t = t + residual.detach().cpu().float()
+    t = t.double()
+    return t / (t.square().mean(1, keepdim=True) + eps).sqrt() * wide(weight), t
+
+
+def scale_of(amax):
+    """The power of two at or above fl32(amax * fl32(1/448)), amax in 32 bits from 1e-4 on."""
+    part, power = math.frexp(float((torch.tensor(amax, dtype=torch.float32).clamp_min(1e-4)
+                                    * torch.tensor(1 / 448, dtype=torch.float32)).item()))
+    return 2.0 ** (power - (part == 0.5))
+
+
+def e4m3(values):
+    """``(nearest values that e4m3 holds, its step there, how far the next border is)``."""
+    size = values.abs().clamp_min(2.0 ** -6)
+    step = torch.exp2(torch.floor(torch.log2(size)) - 3)
+    units = values / step
+    whole = units.round()
+    border = (0.5 - (units - whole).abs()).clamp_min(0) * step
+    # (Below a power of two the steps are half as wide.)
+    edge = (whole.abs() == 8) & (values.abs() > 2.0 ** -6)
+    border = torch.where(edge, torch.minimum(border, (units.abs() - 7.75) * step), border)
+    border = torch.where(values.abs() > 464, values.abs() - 464 + 16, border)
+    return (whole * step).clamp(-448, 448), step, border
+
+
+def quantized(rows, off=None):
+    """``rows`` [n, m] in float64 as codes and scales stand for: ``(values, moved)``.
+    ``moved``: how far the result may move if each value is off by up to ``off``: a step
+    where a border is that near, the steps of both scales where the block's scale may
+    change."""
+    off = torch.zeros_like(rows) if off is None else off
+    out, moved = torch.empty_like(rows), torch.zeros_like(rows)
+    for i in range(len(rows)):
+        for b in range(0, rows.shape[1], BLOCK):
+            part, slack = rows[i, b:b + BLOCK], off[i, b:b + BLOCK]
+            # (2^-22: the products amax / 448 of 32 bits.)
+            low = float((part.abs() - slack).max().clamp_min(0)) * (1 - 2.0 ** -22)
+            high = float((part.abs() + slack).max()) * (1 + 2.0 ** -22)
+            scale, other = scale_of(low), scale_of(high)
+            own = scale_of(float(part.abs().max()))
+            code, step, border = e4m3(part / own)
+            out[i, b:b + BLOCK] = code * own
+            flip = torch.where((slack > 0) & (slack / own >= border), step * own + slack, torch.zeros_like(part))
+            if scale != other:
+                flip = e4m3(part / scale)[1] * scale + e4m3(part / other)[1] * other + slack
+            moved[i, b:b + BLOCK] = flip
+    return out, moved
+
+
+def route(logits, k, bias=None, scoring="sigmoid", groups=1, top_groups=None, renormalize=True,
+          scale=1.0):
+    """``(weights float64 [T, k], ids [T, k])``, one token after another."""
+    top_groups = groups if top_groups is None else top_groups
+    values = wide(logits)
+    exact = torch.sigmoid(values) if scoring == "sigmoid" else torch.softmax(values, 1)
+    scores = exact.float()
+    ranked = scores if bias is None else scores + bias.detach().cpu()
+    size = ranked.shape[1] // groups
+    order = lambda v: (0, 0.0) if math.isnan(v) else (1, -v)  # noqa: E731
+    weights, ids = [], []
+    for t in range(len(ranked)):
+        row = ranked[t]
+        of_group = []
+        for g in range(groups):
+            best = sorted(row[g * size:(g + 1) * size], key=lambda v: order(float(v)))[:2]
+            of_group.append(float(best[0] + best[1]) if bias is not None and size > 1 else float(best[0]))
+        kept = sorted(range(groups), key=lambda g: (order(of_group[g]), g))[:top_groups]
+        chosen = sorted((e for g in kept for e in range(g * size, (g + 1) * size)),
+                        key=lambda e: (order(float(row[e])), e))[:k]
+        w = exact[t, chosen]
+        weights.append((w / (w.sum() + 1e-20) if renormalize else w) * scale)
+        ids.append(chosen)
+    return torch.stack(weights), torch.tensor(ids, dtype=torch.int32)
+
+
+def weight_values(codes, scale):
+    """``[E, N, K]`` codes with a scale per 128 by 128, as the values they stand for."""
+    blocks = scale.detach().cpu().to(torch.float64)
+    return wide(codes) * blocks.repeat_interleave(BLOCK, 1).repeat_interleave(BLOCK, 2)
+
+
+def silu(g):
+    return g * torch.sigmoid(g)
+
+
+def expert_mlp(x, x_scale, gate_up, gate_up_scale, down, down_scale, ids, weights, first=0):
+    """``(out, bound)`` float64 [T, D]: ``bound`` is how far a kernel may be off before it
+    rounds the result, that sums products in 32 bits (in any order: n terms are off by at
+    most (n + 2) 2^-24 of their magnitudes' sum, taken twice as the unit's internal
+    rounding is its own), forms silu within 2^-16 of its value (an exponential and a
+    reciprocal of 32 bits; the former's argument, in log2 units 127 at most where it is a
+    normal number, is off by 2^-24 of that from its constant and as much from its product)
+    and holds an expert's result in 11 bits (half a step: 2^-11) against the largest of 64."""
+    rows = wide(x) * wide(x_scale).repeat_interleave(BLOCK, 1)
+    wg, wd = weight_values(gate_up, gate_up_scale), weight_values(down, down_scale)
+    inner, dim = wd.shape[2], wd.shape[1]
+    out, bound = torch.zeros(len(rows), dim, dtype=torch.float64), torch.zeros(len(rows), dim, dtype=torch.float64)
+    weights = wide(weights)
+
+    def sums(n):
+        return 2 * (n + 2) * 2.0 ** -24
+
+    for e in range(len(wg)):
+        token, choice = (ids.cpu() == e + first).nonzero(as_tuple=True)
+        if not len(token):
+            continue
+        both, size = rows[token] @ wg[e].t(), rows[token].abs() @ wg[e].abs().t()
+        gate, up = both[:, :inner], both[:, inner:]
+        off = sums(rows.shape[1]) * size
+        hidden = silu(gate) * up
+        # (silu's slope is at most 1.1.)
+        off = 1.1 * off[:, :inner] * (up.abs() + off[:, inner:]) + silu(gate).abs() * off[:, inner:]
+        off = off + hidden.abs() * 2.0 ** -16 + 2.0 ** -126 * (1 + up.abs())
+        hidden, moved = quantized(hidden, off)
+        y, reach = hidden @ wd[e].t(), (hidden.abs() + moved) @ wd[e].abs().t()
+        inexact = moved @ wd[e].abs().t() + sums(inner) * reach
+        held = (y.abs() + inexact).view(len(token), -1, 64)
+        held = (held * 2.0 ** -11 + held.amax(-1, keepdim=True) * 2.0 ** -38 + 2.0 ** -136).view(len(token), dim)
+        w = weights[token, choice][:, None]
+        out.index_add_(0, token, w * y)
+        # The weighted sum over up to 64 choices, in 32 bits.
+        bound.index_add_(0, token, w.abs() * (inexact + held + sums(64) * (y.abs() + inexact)))
+    return out, bound

@@ -1,0 +1,152 @@
+"""``feedforward.expert_mlp`` against the formula in 64 bits, within the bound that the oracle
+derives from the kernel's roundings element by element, plus the result's own."""
+
+import pytest
+import torch
+
+from oracle import feedforward as off
+
+pytestmark = pytest.mark.gpu
+
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def tokens_in_codes(gen, tokens, dim):
+    x = torch.randn(tokens, dim, generator=gen)
+    scale = torch.exp2(torch.randint(-3, 2, (tokens, dim // 128), generator=gen).float())
+    return (x * 60).to(F8), (scale / 64).to(E8)
+
+
+def matrix(gen, experts, rows, columns):
+    codes = (torch.randn(experts, rows, columns, generator=gen) * 60).to(F8)
+    scale = torch.exp2(torch.randint(-2, 2, (experts, rows // 128, columns // 128), generator=gen).float())
+    return codes, scale / 64 * 2.0 ** -round(torch.tensor(columns).double().log2().item() / 2)
+
+
+class Model:
+    def __init__(self, gpu, dim, inner, experts, first=0, total=None, seed=0):
+        from cxldsagr_amd.feedforward import ExpertWeights
+
+        gen = torch.Generator().manual_seed(seed + dim + inner)
+        self.parts = (*matrix(gen, experts, 2 * inner, dim), *matrix(gen, experts, dim, inner))
+        self.own = ExpertWeights(*(t.to(gpu) for t in self.parts), first=first, total=total)
+        self.first, self.gen, self.gpu, self.dim = first, gen, gpu, dim
+
+    def tokens(self, tokens, choices, low, high):
+        x, scale = tokens_in_codes(self.gen, tokens, self.dim)
+        ids = torch.randint(low, high, (tokens, choices), generator=self.gen, dtype=torch.int32)
+        return x, scale, ids, torch.randn(tokens, choices, generator=self.gen)
+
+    def run(self, x, scale, ids, weights, **how):
+        from cxldsagr_amd.feedforward import expert_mlp
+
+        return expert_mlp(x.to(self.gpu), scale.to(self.gpu), self.own, ids.to(self.gpu), weights.to(self.gpu), **how)
+
+    def check(self, x, scale, ids, weights, dtype=torch.bfloat16):
+        got = self.run(x, scale, ids, weights, dtype=dtype)
+        assert got.dtype == dtype and got.shape == x.shape
+        want, bound = off.expert_mlp(x, scale, *self.parts, ids, weights, self.first)
+        bound = bound + torch.finfo(dtype).eps / 2 * (want.abs() + bound) + 2.0 ** -25
+        far = (got.cpu().double() - want).abs()
+        assert (far <= bound).all(), (far / bound).max()
+        # The bound is one of roundings: most of it is the codes of silu(gate) * up.
+        assert bound.mean() < 0.2 * want.abs().mean().clamp_min(1e-3)
+        return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_types(gpu, dtype):
+    model = Model(gpu, 256, 128, 3)
+    model.check(*model.tokens(5, 2, 0, 3), dtype=dtype)
+
+
+@pytest.mark.parametrize(
+    ("tokens", "choices", "dim", "inner", "experts"),
+    [(1, 1, 128, 128, 1), (1, 8, 512, 256, 8), (2, 3, 384, 384, 5), (17, 4, 640, 128, 16), (31, 2, 256, 640, 4),
+     (33, 1, 896, 256, 1), (64, 8, 256, 256, 6), (129, 3, 384, 128, 2), (257, 2, 1152, 384, 3), (300, 6, 256, 128, 40),
+     (1, 64, 256, 128, 70)],
+)
+def test_sizes(gpu, tokens, choices, dim, inner, experts):
+    model = Model(gpu, dim, inner, experts, seed=tokens)
+    model.check(*model.tokens(tokens, choices, 0, experts))
+
+
+@pytest.mark.parametrize("rows", [15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 513])
+def test_rows_around_a_tile(gpu, rows):
+    """One expert with so many rows, one with a single one, one with none."""
+    model = Model(gpu, 256, 128, 3)
+    x, scale, ids, weights = model.tokens(rows + 1, 1, 1, 2)
+    ids[rows // 2] = 2
+    model.check(x, scale, ids, weights)
+
+
+def test_choices_of_other_ranks_none_and_twice(gpu):
+    """Slices of the experts sum to the whole; what is not here adds nothing."""
+    model = Model(gpu, 256, 128, 4, first=10, total=24)
+    x, scale, ids, weights = model.tokens(40, 4, 6, 18)
+    ids[0], ids[1], ids[2], ids[3] = -1, 12, 2 ** 31 - 1, -2 ** 31
+    weights[2] = float("nan")  # of choices that are not here
+    got = model.check(x, scale, ids, weights.nan_to_num())
+    assert not got[0].any() and not got[2].any() and not got[3].any()
+    assert torch.equal(model.run(x, scale, ids, weights), got)
+    nothing = model.run(x, scale, torch.full_like(ids, 9), weights)
+    assert nothing.shape == x.shape and not nothing.any()
+    assert model.run(x[:0], scale[:0], ids[:0], weights[:0]).shape == (0, 256)
+
+
+@pytest.mark.parametrize("tokens", [9, 200])
+def test_a_row_s_infinities_and_nan_stay_in_it(gpu, tokens):
+    model = Model(gpu, 256, 128, 2)
+    x, scale, ids, weights = model.tokens(tokens, 2, 0, 2)
+    clean = model.run(x, scale, ids, weights)
+    scale.view(torch.uint8)[2, 1] = 255  # NaN
+    x.view(torch.uint8)[4, 7] = 127  # NaN
+    weights[6, 0] = float("inf")
+    scale.view(torch.uint8)[7] = 254  # 2^127: products overflow
+    got = model.run(x, scale, ids, weights)
+    keep = [t for t in range(tokens) if t not in (2, 4, 6, 7)]
+    assert torch.equal(got[keep], clean[keep])
+    assert got[2].isnan().all() and got[4].isnan().all()
+    assert not got[6].isfinite().any() and not got[7].isfinite().any()
+
+
+@pytest.mark.parametrize("power", [-40, -20, 20, 40])
+def test_scales_far_from_one(gpu, power):
+    """Exponents of tokens and weights that cancel in part; results far below and above 1."""
+    model = Model(gpu, 256, 128, 2)
+    x, scale, ids, weights = model.tokens(6, 2, 0, 2)
+    scale = (scale.float() * 2.0 ** power).to(E8)
+    model.parts = (*model.parts[:2], model.parts[2], model.parts[3] * 2.0 ** (power // 2))
+    from cxldsagr_amd.feedforward import ExpertWeights
+
+    model.own = ExpertWeights(*(t.to(gpu) for t in model.parts))
+    got = model.run(x, scale, ids, weights, dtype=torch.float32)
+    want, bound = off.expert_mlp(x, scale, *model.parts, ids, weights)
+    bound = bound + 2.0 ** -24 * (want.abs() + bound) + 2.0 ** -149
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+def test_inputs_that_are_not_contiguous_and_an_output_given(gpu):
+    from cxldsagr_amd.feedforward import expert_mlp
+
+    model = Model(gpu, 256, 128, 3)
+    x, scale, ids, weights = (t.to(gpu) for t in model.tokens(12, 4, 0, 3))
+    want = model.run(x, scale, ids, weights)
+    wide = torch.zeros(12, 300, dtype=torch.uint8, device=gpu)
+    wide[:, 5:261] = x.view(torch.uint8)
+    out = torch.full((13, 256), 7.0, dtype=torch.bfloat16, device=gpu)
+    got = expert_mlp(wide.view(F8)[:, 5:261], scale.view(torch.uint8).t().contiguous().t().view(E8), model.own,
+                     ids.t().contiguous().t(), weights.repeat_interleave(2, 1)[:, ::2], out=out[:12])
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(out[:12], want) and (out[12] == 7).all()
+
+
+def test_many_rows_are_each_as_in_small_calls(gpu):
+    """A large batch against the formula on some of its tokens."""
+    model = Model(gpu, 512, 256, 4)
+    x, scale, ids, weights = model.tokens(3000, 3, 0, 4)
+    got = model.run(x, scale, ids, weights)
+    some = torch.tensor([0, 1, 511, 1500, 2047, 2998, 2999])
+    want, bound = off.expert_mlp(x[some], scale[some], *model.parts, ids[some], weights[some])
+    bound = bound + 2.0 ** -8 * (want.abs() + bound)
+    assert ((got[some.to(gpu)].cpu().double() - want).abs() <= bound).all()
