@@ -35,16 +35,22 @@ constexpr int kWaveCols = 64;               // weight rows (output columns) of a
 constexpr int kMaxExperts = 1024;
 constexpr int kGroupThreads = 1024;
 
-__device__ __forceinline__ v4f product(const v4u (&w)[2], const v4u (&x)[2], v4f c, int w_scale, int x_scale) {
-  v8i a, b;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a[i] = (int)w[0][i], a[4 + i] = (int)w[1][i], b[i] = (int)x[0][i], b[4 + i] = (int)x[1][i];
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, w_scale, 0, x_scale);
+// 32 codes of a lane from its 16 bytes of both planes.
+__device__ __forceinline__ v8i joined(v4u low, v4u high) {
+  return __builtin_bit_cast(v8i, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The scales are bytes kW and kX of their words.
+template <int kW = 0, int kX = 0>
+__device__ __forceinline__ v4f product(v8i w, v8i x, v4f c, uint32_t w_scale, uint32_t x_scale) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
 }
 
 // ------------------------------------------------------------ 1. groups --
 struct Tile {
-  int32_t expert, row, rows, unused;
+  int32_t expert, row, rows;
+  int32_t first, count;  // the expert's tiles
+  int32_t unused[3];
 };
 
 struct GroupArgs {
@@ -91,7 +97,8 @@ __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
   const uint32_t own = counts[expert], own_tiles = (own + a.tile_rows - 1) / a.tile_rows;
   for (uint32_t t = threadIdx.x; t < own_tiles; t += kGroupThreads) {
     const uint32_t at = t * a.tile_rows, left = own - at;
-    a.tiles[tile + t] = Tile{expert, (int32_t)(row + at), (int32_t)(left < (uint32_t)a.tile_rows ? left : a.tile_rows), 0};
+    a.tiles[tile + t] = Tile{expert, (int32_t)(row + at), (int32_t)(left < (uint32_t)a.tile_rows ? left : a.tile_rows),
+                             (int32_t)tile, (int32_t)own_tiles, {}};
   }
   if (expert == a.experts - 1 && threadIdx.x == 0) *a.tile_count = (int32_t)(tile + own_tiles);
   uint32_t next = row + before;
@@ -128,8 +135,113 @@ __device__ __forceinline__ float silu(float g) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -kLog2E));
 }
 
-// kRows 16-row tiles by 4 waves of 64 columns: every wave streams its own part of the weight
-// through registers.
+__device__ __forceinline__ uint32_t max_over_groups(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] > a[1] ? a[0] : a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return b[0] > b[1] ? b[0] : b[1];
+}
+
+// h of a work-group's rows and 128 columns (a wave's 32 of them in acc: tiles of gate and
+// up in turn), its codes and scales. amax: [4][16 kRows] words of LDS that no wave uses.
+template <int kRows>
+__device__ __forceinline__ void store_hidden(const ProductArgs& a, const Tile& tile, const v4f (&acc)[kRows][4], int block,
+                                             uint32_t* amax) {
+  const int wave = threadIdx.x >> 6, r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  const int64_t inner = a.columns / 2;
+  float h[kRows][8];
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[m][i] = silu(acc[m][i >> 2 << 1][i & 3]) * acc[m][(i >> 2 << 1) + 1][i & 3];
+      const uint32_t bits = __float_as_uint(h[m][i]) & 0x7FFFFFFFu;
+      top = top > bits ? top : bits;
+    }
+    top = max_over_groups(top);
+    if (g == 0) amax[(wave * kRows + m) * 16 + r] = top;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t of = amax[(w * kRows + m) * 16 + r];
+      top = top > of ? top : of;
+    }
+    const float scale = scale_from_amax_bits(top, true);
+    if (16 * m + r >= tile.rows) continue;
+    const int64_t row = tile.row + 16 * m + r;
+    uint32_t lo, hi;
+    quantize_eight(h[m], scale, true, lo, hi);
+    uint8_t* to = a.codes + row * inner + block * 128 + wave * 32 + 4 * g;
+    *reinterpret_cast<uint32_t*>(to) = lo;
+    *reinterpret_cast<uint32_t*>(to + 16) = hi;
+    if (wave == 0 && g == 0) a.scales[row * (inner / kBlock) + block] = (uint8_t)(__float_as_uint(scale) >> 23);
+  }
+}
+
+// y of a wave's rows and 64 columns from `column` on.
+template <int kRows>
+__device__ __forceinline__ void store_result(const ProductArgs& a, const Tile& tile, const v4f (&acc)[kRows][4], int column) {
+  const int r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) {
+    // The largest finite magnitude of the row's 64 values, its power of two.
+    uint32_t top = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t bits = __float_as_uint(acc[m][t][i]) & 0x7FFFFFFFu;
+        top = bits < 0x7F800000u && bits > top ? bits : top;
+      }
+    top = max_over_groups(top);
+    // (At least 2^-112: a smaller row of 64 keeps steps of 2^-136.)
+    const uint32_t power = (top >> 23) < 15u ? 15u : top >> 23;
+    const float factor = __uint_as_float((268u - power) << 23);
+    if (column >= a.columns || 16 * m + r >= tile.rows) continue;
+    const int64_t row = tile.row + 16 * m + r;
+    uint16_t* to = a.y + row * a.columns + column + 4 * g;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      *reinterpret_cast<uint2*>(to + 16 * t) =
+          make_uint2(F16::pack(acc[m][t][0] * factor, acc[m][t][1] * factor),
+                     F16::pack(acc[m][t][2] * factor, acc[m][t][3] * factor));
+    if (g == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power;
+  }
+}
+
+// The parts of the weight that a wave of `column` (past the end: of the last) reads.
+struct WaveWeight {
+  const uint8_t* codes;          // this lane's 16 bytes of the first tile
+  const uint8_t* scale[2];       // of even and odd tiles (up: gate's and up's), a byte a step
+};
+template <bool kUp>
+__device__ __forceinline__ WaveWeight weight_of(const ProductArgs& a, int expert, int block, int column, int steps) {
+  const int at = column < a.columns ? column : a.columns - kWaveCols;
+  WaveWeight w;
+  w.codes = a.w + ((int64_t)expert * (a.columns / 16) + at / 16) * steps * kTile + (threadIdx.x & 63) * 16;
+  const uint8_t* scale = a.w_scale + (int64_t)expert * (a.columns / kBlock) * steps;
+  w.scale[0] = scale + (int64_t)(kUp ? block : at / kBlock) * steps;
+  w.scale[1] = kUp ? w.scale[0] + (int64_t)(a.columns / 256) * steps : w.scale[0];
+  return w;
+}
+
+// The weight's 64 rows of one step.
+__device__ __forceinline__ void load_weight(v8i (&to)[4], const uint8_t* codes, int steps, int s) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const v4u* from = reinterpret_cast<const v4u*>(codes + ((int64_t)t * steps + s) * kTile);
+    to[t] = joined(from[0], from[64]);
+  }
+}
+
+// Few rows: kRows 16-row tiles by 4 waves of 64 columns, every wave streaming its own part
+// of the weight, and the tokens' codes, through registers. What bounds it is reading the
+// weight.
 template <int kRows, bool kUp>
 __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
   const int tile_at = blockIdx.x / a.column_blocks, block = blockIdx.x % a.column_blocks;
@@ -138,7 +250,7 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int column = block * 256 + wave * kWaveCols;  // of the packed weight
   const int steps = a.depth / kBlock;
-  __shared__ uint32_t amax[4][16 * kRows];
+  __shared__ uint32_t amax[kUp ? 4 * 16 * kRows : 1];
 
   const uint8_t* x[kRows];
   const uint8_t* xs[kRows];
@@ -150,101 +262,174 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
     x[m] = a.x + row * a.depth + g * 16;
     xs[m] = a.x_scale + row * steps;
   }
-  const bool some = column < a.columns;
-  const int64_t first = (int64_t)tile.expert * (a.columns / 16) + (some ? column : 0) / 16;
-  const uint8_t* w = a.w + first * steps * kTile + lane * 16;
-  // Up: gate's block of 128 and up's; down: the wave's 64 columns lie in one block.
-  const uint8_t* ws = a.w_scale + (int64_t)tile.expert * (a.columns / kBlock) * steps;
-  const uint8_t* ws0 = ws + (int64_t)(kUp ? block : (some ? column : 0) / kBlock) * steps;
-  const uint8_t* ws1 = kUp ? ws + (int64_t)(block + a.columns / 256) * steps : ws0;
+  const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
 
   v4f acc[kRows][4] = {};
   for (int s = 0; s < steps; ++s) {
-    v4u wv[4][2], xv[kRows][2];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        wv[t][p] = *reinterpret_cast<const v4u*>(w + ((int64_t)t * steps + s) * kTile + p * 1024);
-    const int s0 = ws0[s], s1 = ws1[s];
+    v8i wv[4];
+    load_weight(wv, w.codes, steps, s);
+    const int s0 = w.scale[0][s], s1 = w.scale[1][s];
 #pragma unroll
     for (int m = 0; m < kRows; ++m) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) xv[m][p] = *reinterpret_cast<const v4u*>(x[m] + s * kBlock + p * 64);
+      const v4u* from = reinterpret_cast<const v4u*>(x[m] + s * kBlock);
+      const v8i xv = joined(from[0], from[4]);
       const int sx = xs[m][s];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[m][t] = product(wv[t], xv[m], acc[m][t], kUp && (t & 1) ? s1 : s0, sx);
+      for (int t = 0; t < 4; ++t) acc[m][t] = product(wv[t], xv, acc[m][t], t & 1 ? s1 : s0, sx);
     }
   }
+  if constexpr (kUp) store_hidden<kRows>(a, tile, acc, block, amax);
+  else store_result<kRows>(a, tile, acc, column);
+}
+
+// Many rows: 16 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
+// registers, a step ahead; the rows' codes go into LDS straight from memory (two steps
+// ahead, four buffers), where all four waves read them, three 16-row tiles ahead of their
+// products. Half-way through a step the waves meet: from there on the next step's rows may
+// be read. A row's eight 16-byte parts are turned by its index, so that eight rows' reads of
+// one part fall on different banks.
+// Per step of 128 a CU's matrix units take 8 kRows 16 clocks, its LDS 10 kRows 8 (four waves'
+// reads and one write of 2 kRows KB at 128 bytes), its path to L2 half as many.
+constexpr int kMaxWideSteps = 120;
+template <int kRows>
+struct WideLds {
+  alignas(16) uint8_t rows[4][16 * kRows * kBlock];
+  alignas(16) uint8_t scales[kMaxWideSteps][16][kRows];  // a row's tile last: one read holds all
+  alignas(4) uint8_t weight_scales[kMaxWideSteps][2];
+};
+
+template <int kRows, bool kUp>
+__global__ __launch_bounds__(256, kRows <= 8 ? 2 : 1) void expert_product_wide(ProductArgs a) {
+  __shared__ WideLds<kRows> lds;
+  // Work-groups go round the eight XCDs: each takes a run of the work, in which an expert's
+  // row tiles are neighbours and read the same columns of its weight through one L2.
+  const int64_t all = (int64_t)*a.tile_count * a.column_blocks, each = (all + 7) / 8;
+  const int64_t at = (int64_t)(blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= each || at >= all) return;
+  Tile tile = a.tiles[at / a.column_blocks];
+  const int64_t within = at - (int64_t)tile.first * a.column_blocks;
+  const int block = (int)(within / tile.count);
+  tile = a.tiles[tile.first + within % tile.count];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int column = block * 256 + wave * kWaveCols;
+  const int steps = a.depth / kBlock;
+  const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
+
+  // This lane's parts of the rows that its wave fetches: 4 kRows rows, eight a load.
+  constexpr int kLoads = kRows / 2;
+  uint64_t from[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int in = (wave * kLoads + i) * 8 + (lane >> 3);
+    int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
+    if constexpr (kUp) row = a.order[row] / a.choices;
+    from[i] = (uint64_t)(a.x + row * a.depth + (((lane & 7) ^ (in & 7)) << 4));
+  }
+  const uint32_t lds_rows = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds.rows[0][0];
+  auto fetch = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t to = lds_rows + buffer * (16 * kRows * kBlock) + (wave * kLoads + i) * 1024;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                   ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from[i]) : "memory", "m0");
+    }
+  };
+  auto advance = [&](bool on) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) from[i] += on ? kBlock : 0;
+  };
+  fetch(0);
+  advance(steps > 1);
+  fetch(1);
+  v8i now[4];
+  load_weight(now, w.codes, steps, 0);
+
+  // The rows' and the weight's scales of all steps.
+  {
+    constexpr int kPer = 256 / (16 * kRows);  // threads of a row
+    const int in = threadIdx.x / kPer, part = threadIdx.x % kPer;
+    int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
+    if constexpr (kUp) row = a.order[row] / a.choices;
+    const uint8_t* xs = a.x_scale + row * steps;
+#pragma unroll 8
+    for (int s = part; s < steps; s += kPer) lds.scales[s][in & 15][in >> 4] = xs[s];
+    // (Down: of a block of 128 columns each pair of waves, up: of gate and up.)
+    const WaveWeight other = weight_of<kUp>(a, tile.expert, block, block * 256 + 128, steps);
+    const WaveWeight one = weight_of<kUp>(a, tile.expert, block, block * 256, steps);
+    for (int s = threadIdx.x; s < steps; s += 256) {
+      lds.weight_scales[s][0] = one.scale[0][s];
+      lds.weight_scales[s][1] = (kUp ? one.scale[1] : other.scale[0])[s];
+    }
+  }
+  wait_loads<0>();
+  lds_barrier();
+
+  const uint32_t lane_at = lds_rows + r * kBlock + ((g ^ (r & 7)) << 4);
+  // Tiles of rows in registers: those ahead of the products hide the LDS (with two waves a
+  // SIMD one is enough, and fits).
+  constexpr int kRing = kRows <= 8 ? 2 : 4, kAhead = kRing - 1;
+  v8i x[kRing];
+  auto read = [&](uint32_t buffer, int m) {
+    const uint32_t from = buffer * (16 * kRows * kBlock) + m * 16 * kBlock;
+    return joined(lds_load<v4u>(lane_at + from), lds_load<v4u>((lane_at ^ 64) + from));
+  };
+  typedef uint32_t RowScales __attribute__((ext_vector_type(kRows / 4)));
+  auto scales_of = [&](int s) { return *reinterpret_cast<const RowScales*>(&lds.scales[s][r][0]); };
+  auto weight_scales_of = [&](int s) {
+    const uint32_t both = *reinterpret_cast<const uint16_t*>(&lds.weight_scales[s][0]);
+    return kUp ? both : both >> (wave >> 1 << 3);
+  };
+#pragma unroll
+  for (int m = 0; m < kAhead; ++m) x[m] = read(0, m);
+  RowScales xs = scales_of(0);
+  uint32_t ws = weight_scales_of(0);
+
+  v4f acc[kRows][4] = {};
+#pragma unroll 1
+  for (int s = 0; s < steps; ++s) {
+    const int ahead = s + 1 < steps ? s + 1 : s;
+    v8i next[4];
+    const RowScales xs_next = scales_of(ahead);
+    const uint32_t ws_next = weight_scales_of(ahead);
+    static_for<kRows>([&](auto index) {
+      constexpr int m = decltype(index)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (m == 1) {
+        // Behind the first products, which wait for this step's weight: what is asked for
+        // here would be waited for there. (At the end the last rows come again, into buffers
+        // that are not read.)
+        advance(s + 2 < steps);
+        fetch((s + 2) & 3);
+        load_weight(next, w.codes, steps, ahead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (m == kRows / 2) {
+        // This wave's rows of the next step have come, and everyone's.
+        wait_loads<kLoads + 8>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      x[(m + kAhead) % kRing] = m + kAhead < kRows ? read(s & 3, m + kAhead) : read((s + 1) & 3, m + kAhead - kRows);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (kUp && (t & 1)) acc[m][t] = product<1, m & 3>(now[t], x[m % kRing], acc[m][t], ws, xs[m / 4]);
+        else acc[m][t] = product<0, m & 3>(now[t], x[m % kRing], acc[m][t], ws, xs[m / 4]);
+      }
+    });
+#pragma unroll
+    for (int t = 0; t < 4; ++t) now[t] = next[t];
+    xs = xs_next;
+    ws = ws_next;
+  }
+  // (What is still on its way into LDS has to land before the LDS is another's.)
+  wait_loads<0>();
 
   if constexpr (kUp) {
-    const int64_t inner = a.columns / 2;
-    float h[kRows][2][4];
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[m][t][i] = silu(acc[m][2 * t][i]) * acc[m][2 * t + 1][i];
-          const uint32_t bits = __float_as_uint(h[m][t][i]) & 0x7FFFFFFFu;
-          top = top > bits ? top : bits;
-        }
-      const uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
-      top = top > o ? top : o;
-      const uint32_t o2 = (uint32_t)__shfl_xor((int)top, 32);
-      top = top > o2 ? top : o2;
-      if (g == 0) amax[wave][16 * m + r] = top;
-    }
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) top = top > amax[v][16 * m + r] ? top : amax[v][16 * m + r];
-      const float scale = scale_from_amax_bits(top, true);
-      if (16 * m + r >= tile.rows) continue;
-      const int64_t row = tile.row + 16 * m + r;
-      uint32_t lo, hi;
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = h[m][0][i], v[4 + i] = h[m][1][i];
-      quantize_eight(v, scale, true, lo, hi);
-      uint8_t* to = a.codes + row * inner + column / 2 + 4 * g;
-      *reinterpret_cast<uint32_t*>(to) = lo;
-      *reinterpret_cast<uint32_t*>(to + 16) = hi;
-      if (wave == 0 && g == 0) a.scales[row * (inner / kBlock) + block] = (uint8_t)(__float_as_uint(scale) >> 23);
-    }
+    store_hidden<kRows>(a, tile, acc, block, reinterpret_cast<uint32_t*>(&lds.rows[0][0]));
   } else {
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      // The largest finite magnitude of the row's 64 values, its power of two.
-      uint32_t top = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t bits = __float_as_uint(acc[m][t][i]) & 0x7FFFFFFFu;
-          top = bits < 0x7F800000u && bits > top ? bits : top;
-        }
-      const uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
-      top = top > o ? top : o;
-      const uint32_t o2 = (uint32_t)__shfl_xor((int)top, 32);
-      top = top > o2 ? top : o2;
-      // (At least 2^-112: a smaller row of 64 keeps steps of 2^-136.)
-      const uint32_t power = (top >> 23) < 15u ? 15u : top >> 23;
-      const float factor = __uint_as_float((268u - power) << 23);
-      if (!some || 16 * m + r >= tile.rows) continue;
-      const int64_t row = tile.row + 16 * m + r;
-      uint16_t* to = a.y + row * a.columns + column + 4 * g;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        *reinterpret_cast<uint2*>(to + 16 * t) =
-            make_uint2(F16::pack(acc[m][t][0] * factor, acc[m][t][1] * factor),
-                       F16::pack(acc[m][t][2] * factor, acc[m][t][3] * factor));
-      if (g == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power;
-    }
+    store_result<kRows>(a, tile, acc, column);
   }
 }
 
@@ -307,7 +492,8 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   p.pairs = tokens * choices;
   // Rows of an expert, on average; tiles of about twice that.
   const int64_t mean = p.pairs / total;
-  p.rows = mean <= 6 ? 1 : mean <= 16 ? 2 : 4;
+  p.rows = mean <= 6 ? 1 : mean <= 16 ? 2 : mean <= 40 ? 4 : mean <= 128 ? 8 : 16;
+  if (dim > kMaxWideSteps * kBlock || inner > kMaxWideSteps * kBlock) p.rows = p.rows < 4 ? p.rows : 4;
   const int64_t size = 16 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;
@@ -339,20 +525,19 @@ int check_shape(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int
   return kOk;
 }
 
-template <int kRows, bool kUp>
-int launch_product(const ProductArgs& a, int64_t tiles, hipStream_t stream) {
-  const int64_t groups = tiles * a.column_blocks;
-  DSA_CHECK_ARG(grid_fits(groups, 256), "too many tokens for one launch");
-  hipLaunchKernelGGL((expert_product<kRows, kUp>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+template <bool kUp>
+int launch_product(const ProductArgs& a, const Plan& p, hipStream_t stream) {
+  auto go = [&](auto kernel, int64_t groups) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, a);
+  };
+  const int64_t groups = p.tiles * a.column_blocks;
+  if (p.rows == 1) go(expert_product<1, kUp>, groups);
+  else if (p.rows == 2) go(expert_product<2, kUp>, groups);
+  else if (p.rows == 4) go(expert_product<4, kUp>, groups);
+  else if (p.rows == 8) go(expert_product_wide<8, kUp>, (groups + 7) / 8 * 8);
+  else go(expert_product_wide<16, kUp>, (groups + 7) / 8 * 8);
   DSA_CHECK_LAUNCH("expert product");
   return kOk;
-}
-
-template <bool kUp>
-int product_of(const ProductArgs& a, const Plan& p, hipStream_t stream) {
-  if (p.rows == 1) return launch_product<1, kUp>(a, p.tiles, stream);
-  if (p.rows == 2) return launch_product<2, kUp>(a, p.tiles, stream);
-  return launch_product<4, kUp>(a, p.tiles, stream);
 }
 
 }  // namespace
@@ -408,15 +593,15 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   j.ids = ids, j.place = place, j.weights = weights, j.y = dn.y, j.powers = dn.powers, j.out = out;
   j.choices = (int32_t)choices, j.first = (int32_t)first, j.experts = (int32_t)experts, j.dim = (int32_t)dim;
   j.groups_per_token = (int32_t)((dim / 8 + 255) / 256);
-  DSA_CHECK_ARG(grid_fits(p.tiles * up.column_blocks, 256) && grid_fits(p.tiles * dn.column_blocks, 256) &&
+  DSA_CHECK_ARG(grid_fits(p.tiles * up.column_blocks + 7, 256) && grid_fits(p.tiles * dn.column_blocks + 7, 256) &&
                     grid_fits(tokens * j.groups_per_token, 256),
                 "too many tokens for one launch");
 
   const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 16 * p.rows};
   hipLaunchKernelGGL(group_pairs, dim3((unsigned)experts), dim3(kGroupThreads), 0, stream, group);
   DSA_CHECK_LAUNCH("grouping of pairs");
-  if (const int status = product_of<true>(up, p, stream)) return status;
-  if (const int status = product_of<false>(dn, p, stream)) return status;
+  if (const int status = launch_product<true>(up, p, stream)) return status;
+  if (const int status = launch_product<false>(dn, p, stream)) return status;
   auto join = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * j.groups_per_token)), dim3(256), 0, stream, j);
   };
