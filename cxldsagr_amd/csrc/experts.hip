@@ -4,8 +4,9 @@
 // x, q and the weights in e4m3 with a power-of-two scale (e8m0) for every 128 values of a
 // row, and every 128 by 128 of a weight.
 //
-// Four launches:
+// Four launches (five with wide tiles):
 //  1. group: the (token, choice) pairs of each expert, in token order, and row tiles of them;
+//     wide tiles: their rows' scales in the order of the products;
 //  2. up: row tiles times gate and up, h, its codes and scales;
 //  3. down: row tiles times down, y in 16 bits with a power of two for every 64 values of a
 //     row (its largest value just below 2^15 as fp16: 11 bits of each value; as bf16, 8, the
@@ -19,7 +20,9 @@
 // power of two per 32 values along K: the blocks of 128 cost nothing beyond that. Sums are
 // in 32 bits. Weights are laid out as the instruction reads them (ExpertWeights): a tile of
 // 16 rows by 128 is 2 KB, two planes of 16 bytes a lane, read by one wave straight into
-// registers; tiles of gate and up alternate, so that a lane holds g and u of the same h.
+// registers; tiles of gate and up alternate, so that a lane holds g and u of the same h; and
+// the rows of a wave's four tiles are dealt out so that a lane's results in all of them are
+// neighbours (16 of y, 8 of h) and four lanes fill a line.
 #include "attention_core.h"
 #include "quantize_core.h"
 #include "../../include/dsa_gfx950.h"
@@ -44,6 +47,14 @@ __device__ __forceinline__ v8i joined(v4u low, v4u high) {
 template <int kW = 0, int kX = 0>
 __device__ __forceinline__ v4f product(v8i w, v8i x, v4f c, uint32_t w_scale, uint32_t x_scale) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
+}
+
+// The wide kernels' form: 32 rows of a weight by 32 tokens, 64 values deep. Half as many
+// instructions for the same work: one wave a SIMD cannot keep the unit busy with the other
+// (45 clocks an instruction where the unit needs 32; 70 of 64 here).
+template <int kW, int kX>
+__device__ __forceinline__ v16f product32(v8i w, v8i x, v16f c, uint32_t w_scale, uint32_t x_scale) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
 }
 
 // ------------------------------------------------------------ 1. groups --
@@ -75,6 +86,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
   const int run = ((a.pairs + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t begin = (int64_t)wave * run, end = begin + run < a.pairs ? begin + run : a.pairs;
   uint32_t found = 0;
+#pragma unroll 8
   for (int64_t i = begin + lane; i < end; i += 64) {
     const uint32_t e = (uint32_t)a.ids[i] - (uint32_t)a.first;
     if (e < (uint32_t)a.experts) atomicAdd(&counts[e], 1u);
@@ -142,75 +154,43 @@ __device__ __forceinline__ uint32_t max_over_groups(uint32_t v) {
   return b[0] > b[1] ? b[0] : b[1];
 }
 
-// h of a work-group's rows and 128 columns (a wave's 32 of them in acc: tiles of gate and
-// up in turn), its codes and scales. amax: [4][16 kRows] words of LDS that no wave uses.
-template <int kRows>
-__device__ __forceinline__ void store_hidden(const ProductArgs& a, const Tile& tile, const v4f (&acc)[kRows][4], int block,
-                                             uint32_t* amax) {
-  const int wave = threadIdx.x >> 6, r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-  const int64_t inner = a.columns / 2;
-  float h[kRows][8];
+// h of kCount gates and ups of one row, and the largest magnitude's bits.
+template <int kCount, typename Gate, typename Up>
+__device__ __forceinline__ uint32_t hidden(float (&h)[kCount], Gate gate, Up up) {
+  uint32_t top = 0;
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[m][i] = silu(acc[m][i >> 2 << 1][i & 3]) * acc[m][(i >> 2 << 1) + 1][i & 3];
-      const uint32_t bits = __float_as_uint(h[m][i]) & 0x7FFFFFFFu;
-      top = top > bits ? top : bits;
-    }
-    top = max_over_groups(top);
-    if (g == 0) amax[(wave * kRows + m) * 16 + r] = top;
+  for (int i = 0; i < kCount; ++i) {
+    h[i] = silu(gate(i)) * up(i);
+    const uint32_t bits = __float_as_uint(h[i]) & 0x7FFFFFFFu;
+    top = top > bits ? top : bits;
   }
-  __syncthreads();
-#pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t of = amax[(w * kRows + m) * 16 + r];
-      top = top > of ? top : of;
-    }
-    const float scale = scale_from_amax_bits(top, true);
-    if (16 * m + r >= tile.rows) continue;
-    const int64_t row = tile.row + 16 * m + r;
-    uint32_t lo, hi;
-    quantize_eight(h[m], scale, true, lo, hi);
-    uint8_t* to = a.codes + row * inner + block * 128 + wave * 32 + 4 * g;
-    *reinterpret_cast<uint32_t*>(to) = lo;
-    *reinterpret_cast<uint32_t*>(to + 16) = hi;
-    if (wave == 0 && g == 0) a.scales[row * (inner / kBlock) + block] = (uint8_t)(__float_as_uint(scale) >> 23);
-  }
+  return top;
 }
 
-// y of a wave's rows and 64 columns from `column` on.
-template <int kRows>
-__device__ __forceinline__ void store_result(const ProductArgs& a, const Tile& tile, const v4f (&acc)[kRows][4], int column) {
-  const int r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+// The power of two of 64 values of a row by their largest finite magnitude's bits: its
+// exponent (at least 15: a smaller row of 64 keeps steps of 2^-136), and the factor that
+// takes that magnitude to 2^14 .. 2^15.
+struct Power {
+  uint32_t exponent;
+  float factor;
+};
+__device__ __forceinline__ Power power_of(uint32_t top) {
+  const uint32_t e = (top >> 23) < 15u ? 15u : top >> 23;
+  return Power{e, __uint_as_float((268u - e) << 23)};
+}
+__device__ __forceinline__ uint32_t finite_max(uint32_t top, float v) {
+  const uint32_t bits = __float_as_uint(v) & 0x7FFFFFFFu;
+  return bits < 0x7F800000u && bits > top ? bits : top;
+}
+// 16 neighbouring values of a row, as fp16.
+template <typename Value>
+__device__ __forceinline__ void store_sixteen(uint16_t* to, float factor, Value value) {
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    // The largest finite magnitude of the row's 64 values, its power of two.
-    uint32_t top = 0;
+  for (int half = 0; half < 2; ++half) {
+    v4u out;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = __float_as_uint(acc[m][t][i]) & 0x7FFFFFFFu;
-        top = bits < 0x7F800000u && bits > top ? bits : top;
-      }
-    top = max_over_groups(top);
-    // (At least 2^-112: a smaller row of 64 keeps steps of 2^-136.)
-    const uint32_t power = (top >> 23) < 15u ? 15u : top >> 23;
-    const float factor = __uint_as_float((268u - power) << 23);
-    if (column >= a.columns || 16 * m + r >= tile.rows) continue;
-    const int64_t row = tile.row + 16 * m + r;
-    uint16_t* to = a.y + row * a.columns + column + 4 * g;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      *reinterpret_cast<uint2*>(to + 16 * t) =
-          make_uint2(F16::pack(acc[m][t][0] * factor, acc[m][t][1] * factor),
-                     F16::pack(acc[m][t][2] * factor, acc[m][t][3] * factor));
-    if (g == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power;
+    for (int i = 0; i < 4; ++i) out[i] = F16::pack(value(8 * half + 2 * i) * factor, value(8 * half + 2 * i + 1) * factor);
+    reinterpret_cast<v4u*>(to)[half] = out;
   }
 }
 
@@ -230,13 +210,10 @@ __device__ __forceinline__ WaveWeight weight_of(const ProductArgs& a, int expert
   return w;
 }
 
-// The weight's 64 rows of one step.
-__device__ __forceinline__ void load_weight(v8i (&to)[4], const uint8_t* codes, int steps, int s) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const v4u* from = reinterpret_cast<const v4u*>(codes + ((int64_t)t * steps + s) * kTile);
-    to[t] = joined(from[0], from[64]);
-  }
+// Tile t of the wave's four, one step.
+__device__ __forceinline__ v8i load_weight(const uint8_t* codes, int steps, int t, int s) {
+  const v4u* from = reinterpret_cast<const v4u*>(codes + ((int64_t)t * steps + s) * kTile);
+  return joined(from[0], from[64]);
 }
 
 // Few rows: kRows 16-row tiles by 4 waves of 64 columns, every wave streaming its own part
@@ -267,7 +244,8 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
   v4f acc[kRows][4] = {};
   for (int s = 0; s < steps; ++s) {
     v8i wv[4];
-    load_weight(wv, w.codes, steps, s);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) wv[t] = load_weight(w.codes, steps, t, s);
     const int s0 = w.scale[0][s], s1 = w.scale[1][s];
 #pragma unroll
     for (int m = 0; m < kRows; ++m) {
@@ -278,46 +256,97 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
       for (int t = 0; t < 4; ++t) acc[m][t] = product(wv[t], xv, acc[m][t], t & 1 ? s1 : s0, sx);
     }
   }
-  if constexpr (kUp) store_hidden<kRows>(a, tile, acc, block, amax);
-  else store_result<kRows>(a, tile, acc, column);
+  if constexpr (kUp) {
+    const int64_t inner = a.columns / 2;
+    float h[kRows][8];
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      const uint32_t top = max_over_groups(hidden(h[m], [&](int i) { return acc[m][i >> 2 << 1][i & 3]; },
+                                                  [&](int i) { return acc[m][(i >> 2 << 1) + 1][i & 3]; }));
+      if (g == 0) amax[(wave * kRows + m) * 16 + r] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const uint32_t of = amax[(v * kRows + m) * 16 + r];
+        top = top > of ? top : of;
+      }
+      const float scale = scale_from_amax_bits(top, true);
+      if (16 * m + r >= tile.rows) continue;
+      const int64_t row = tile.row + 16 * m + r;
+      uint32_t lo, hi;
+      quantize_eight(h[m], scale, true, lo, hi);
+      *reinterpret_cast<uint2*>(a.codes + row * inner + block * 128 + wave * 32 + 8 * g) = make_uint2(lo, hi);
+      if (wave == 0 && g == 0) a.scales[row * (inner / kBlock) + block] = (uint8_t)(__float_as_uint(scale) >> 23);
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      auto value = [&](int i) { return acc[m][i >> 2][i & 3]; };
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = finite_max(top, value(i));
+      const Power power = power_of(max_over_groups(top));
+      if (column >= a.columns || 16 * m + r >= tile.rows) continue;
+      const int64_t row = tile.row + 16 * m + r;
+      store_sixteen(a.y + row * a.columns + column + 16 * g, power.factor, value);
+      if (g == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power.exponent;
+    }
+  }
 }
 
-// Many rows: 16 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
+// Many rows: 32 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
 // registers, a step ahead; the rows' codes go into LDS straight from memory (two steps
-// ahead, four buffers), where all four waves read them, three 16-row tiles ahead of their
+// ahead, four buffers), where all four waves read them, three operands ahead of their
 // products. Half-way through a step the waves meet: from there on the next step's rows may
 // be read. A row's eight 16-byte parts are turned by its index, so that eight rows' reads of
 // one part fall on different banks.
-// Per step of 128 a CU's matrix units take 8 kRows 16 clocks, its LDS 10 kRows 8 (four waves'
-// reads and one write of 2 kRows KB at 128 bytes), its path to L2 half as many.
-constexpr int kMaxWideSteps = 120;
+// Rows' scales come from memory a step ahead, laid out by tile.
+// Per step of 128 a CU's matrix units take 256 kRows clocks, its LDS 160 kRows (four waves'
+// reads and one write of 4 kRows KB at 128 bytes).
+constexpr int kMaxWideSteps = 256;
 template <int kRows>
 struct WideLds {
-  alignas(16) uint8_t rows[4][16 * kRows * kBlock];
-  alignas(16) uint8_t scales[kMaxWideSteps][16][kRows];  // a row's tile last: one read holds all
+  alignas(16) uint8_t rows[4][32 * kRows * kBlock];
   alignas(4) uint8_t weight_scales[kMaxWideSteps][2];
 };
 
+// The wave's weight tiles as two operands of 32 rows (up: gate's and up's), 64 deep: half k
+// of a step. Lane (r, h): rows r of tiles `first` and `second`, bytes 32 h .. of the half.
+__device__ __forceinline__ v8i load_weight32(const uint8_t* codes, int64_t tile, int k) {
+  const v4u* from = reinterpret_cast<const v4u*>(codes + tile + k * 1024);
+  return joined(from[0], from[16]);
+}
+
 template <int kRows, bool kUp>
-__global__ __launch_bounds__(256, kRows <= 8 ? 2 : 1) void expert_product_wide(ProductArgs a) {
+__global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(ProductArgs a) {
+  constexpr int kSize = 32 * kRows;  // rows of a tile
   __shared__ WideLds<kRows> lds;
   // Work-groups go round the eight XCDs: each takes a run of the work, in which an expert's
   // row tiles are neighbours and read the same columns of its weight through one L2.
-  const int64_t all = (int64_t)*a.tile_count * a.column_blocks, each = (all + 7) / 8;
-  const int64_t at = (int64_t)(blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  const uint32_t all = (uint32_t)(*a.tile_count * a.column_blocks), each = (all + 7) / 8;
+  const uint32_t at = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
   if ((blockIdx.x >> 3) >= each || at >= all) return;
-  Tile tile = a.tiles[at / a.column_blocks];
-  const int64_t within = at - (int64_t)tile.first * a.column_blocks;
-  const int block = (int)(within / tile.count);
-  tile = a.tiles[tile.first + within % tile.count];
+  Tile tile = a.tiles[at / (uint32_t)a.column_blocks];
+  const uint32_t within = at - (uint32_t)(tile.first * a.column_blocks);
+  const int block = (int)(within / (uint32_t)tile.count), tile_at = tile.first + (int)(within % (uint32_t)tile.count);
+  tile = a.tiles[tile_at];
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int column = block * 256 + wave * kWaveCols;
   const int steps = a.depth / kBlock;
   const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
+  // (weight_of gives the address of lane (g, r); here lanes 0 .. 15 and 16 .. 31 of a half
+  // take rows of the operand's two tiles.)
+  const int64_t tile_bytes = (int64_t)steps * kTile;
+  const uint8_t* codes = w.codes - lane * 16 + (r >> 4) * (kUp ? 2 : 1) * tile_bytes + (h * 32 + (r & 15)) * 16;
+  const int64_t second = (kUp ? 1 : 2) * tile_bytes;
 
-  // This lane's parts of the rows that its wave fetches: 4 kRows rows, eight a load.
-  constexpr int kLoads = kRows / 2;
+  // This lane's parts of the rows that its wave fetches: 8 kRows rows, eight a load.
+  constexpr int kLoads = kRows;
   uint64_t from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
@@ -327,110 +356,184 @@ __global__ __launch_bounds__(256, kRows <= 8 ? 2 : 1) void expert_product_wide(P
     from[i] = (uint64_t)(a.x + row * a.depth + (((lane & 7) ^ (in & 7)) << 4));
   }
   const uint32_t lds_rows = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds.rows[0][0];
-  auto fetch = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t to = lds_rows + buffer * (16 * kRows * kBlock) + (wave * kLoads + i) * 1024;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                   ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from[i]) : "memory", "m0");
-    }
+  auto fetch = [&](int buffer, int i) {
+    const uint32_t to = lds_rows + buffer * (kSize * kBlock) + (wave * kLoads + i) * 1024;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from[i]) : "memory", "m0");
   };
-  auto advance = [&](bool on) {
+  const uint32_t once = steps > 1 ? kBlock : 0;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) from[i] += on ? kBlock : 0;
-  };
-  fetch(0);
-  advance(steps > 1);
-  fetch(1);
-  v8i now[4];
-  load_weight(now, w.codes, steps, 0);
+  for (int i = 0; i < kLoads; ++i) fetch(0, i);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) from[i] += once, fetch(1, i);
+  v8i now[2][2];  // [half][operand]
+#pragma unroll
+  for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second, i >> 1);
 
-  // The rows' and the weight's scales of all steps.
+  // The weight's scales of all steps. (Down: of a block of 128 columns each pair of waves,
+  // up: of gate and up.)
   {
-    constexpr int kPer = 256 / (16 * kRows);  // threads of a row
-    const int in = threadIdx.x / kPer, part = threadIdx.x % kPer;
-    int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
-    if constexpr (kUp) row = a.order[row] / a.choices;
-    const uint8_t* xs = a.x_scale + row * steps;
-#pragma unroll 8
-    for (int s = part; s < steps; s += kPer) lds.scales[s][in & 15][in >> 4] = xs[s];
-    // (Down: of a block of 128 columns each pair of waves, up: of gate and up.)
-    const WaveWeight other = weight_of<kUp>(a, tile.expert, block, block * 256 + 128, steps);
     const WaveWeight one = weight_of<kUp>(a, tile.expert, block, block * 256, steps);
+    const WaveWeight other = weight_of<kUp>(a, tile.expert, block, block * 256 + 128, steps);
     for (int s = threadIdx.x; s < steps; s += 256) {
       lds.weight_scales[s][0] = one.scale[0][s];
       lds.weight_scales[s][1] = (kUp ? one.scale[1] : other.scale[0])[s];
     }
   }
+  // This lane's rows' scales: of row r of all 32-row parts, a step every 32 kRows bytes.
+  const uint8_t* row_scales = a.x_scale + (int64_t)tile_at * steps * kSize + r * kRows;
   wait_loads<0>();
   lds_barrier();
 
-  const uint32_t lane_at = lds_rows + r * kBlock + ((g ^ (r & 7)) << 4);
-  // Tiles of rows in registers: those ahead of the products hide the LDS (with two waves a
-  // SIMD one is enough, and fits).
-  constexpr int kRing = kRows <= 8 ? 2 : 4, kAhead = kRing - 1;
+  // Part m, half k of a step: a lane's two 16-byte parts of row r are 4 k + 2 h and the next.
+  const uint32_t lane_at = lds_rows + r * kBlock + (((2 * h) ^ (r & 7)) << 4);
+  // Operands in registers: those ahead of the products hide the LDS.
+  constexpr int kRing = kRows <= 4 ? 2 : 4, kAhead = kRing - 1, kParts = 2 * kRows;
   v8i x[kRing];
-  auto read = [&](uint32_t buffer, int m) {
-    const uint32_t from = buffer * (16 * kRows * kBlock) + m * 16 * kBlock;
-    return joined(lds_load<v4u>(lane_at + from), lds_load<v4u>((lane_at ^ 64) + from));
+  auto read = [&](uint32_t buffer, int q) {
+    const uint32_t from = buffer * (kSize * kBlock) + (q % kRows) * 32 * kBlock;
+    const uint32_t at = q < kRows ? lane_at : lane_at ^ 64;
+    return joined(lds_load<v4u>(at + from), lds_load<v4u>((at ^ 16) + from));
   };
   typedef uint32_t RowScales __attribute__((ext_vector_type(kRows / 4)));
-  auto scales_of = [&](int s) { return *reinterpret_cast<const RowScales*>(&lds.scales[s][r][0]); };
+  auto scales_of = [&](int s) { return *reinterpret_cast<const RowScales*>(row_scales + s * kSize); };
   auto weight_scales_of = [&](int s) {
     const uint32_t both = *reinterpret_cast<const uint16_t*>(&lds.weight_scales[s][0]);
     return kUp ? both : both >> (wave >> 1 << 3);
   };
 #pragma unroll
-  for (int m = 0; m < kAhead; ++m) x[m] = read(0, m);
+  for (int q = 0; q < kAhead; ++q) x[q] = read(0, q);
   RowScales xs = scales_of(0);
   uint32_t ws = weight_scales_of(0);
 
-  v4f acc[kRows][4] = {};
+  v16f acc[kRows][2] = {};
 #pragma unroll 1
   for (int s = 0; s < steps; ++s) {
     const int ahead = s + 1 < steps ? s + 1 : s;
-    v8i next[4];
-    const RowScales xs_next = scales_of(ahead);
-    const uint32_t ws_next = weight_scales_of(ahead);
-    static_for<kRows>([&](auto index) {
-      constexpr int m = decltype(index)::value;
+    const uint32_t on = s + 2 < steps ? kBlock : 0;
+    v8i next[2][2];
+    RowScales xs_next;
+    uint32_t ws_next;
+    static_for<kParts>([&](auto index) {
+      constexpr int q = decltype(index)::value, m = q % kRows, k = q / kRows;
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (m == 1) {
-        // Behind the first products, which wait for this step's weight: what is asked for
-        // here would be waited for there. (At the end the last rows come again, into buffers
-        // that are not read.)
-        advance(s + 2 < steps);
-        fetch((s + 2) & 3);
-        load_weight(next, w.codes, steps, ahead);
-        __builtin_amdgcn_sched_barrier(0);
+      // The next step's weight and scales and the rows of the one after are asked for in the
+      // first half, behind the first products, which wait for this step's (what is asked for
+      // before them would be waited for there), and a few at a time: a wave does not get on
+      // while the path to L2 is full. (At the end the last rows come again, into buffers that
+      // are not read.)
+      constexpr int kPer = kRows <= 4 ? 2 : 1;
+      if constexpr (q == 1) {
+        xs_next = scales_of(ahead);
+        ws_next = weight_scales_of(ahead);
       }
-      if constexpr (m == kRows / 2) {
+      if constexpr (q >= 1 && (q - 1) * kPer < kLoads) {
+#pragma unroll
+        for (int i = (q - 1) * kPer; i < q * kPer && i < kLoads; ++i) from[i] += on, fetch((s + 2) & 3, i);
+      }
+      if constexpr (q >= 1 && q <= 8 / kPer && q % (2 / kPer) == 0) {
+#pragma unroll
+        for (int i = (q * kPer - 2) / 2; i < q * kPer / 2; ++i)
+          next[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second + (int64_t)ahead * kTile, i >> 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (q == kRows) {
         // This wave's rows of the next step have come, and everyone's.
-        wait_loads<kLoads + 8>();
+        wait_loads<kLoads + 9>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       }
-      x[(m + kAhead) % kRing] = m + kAhead < kRows ? read(s & 3, m + kAhead) : read((s + 1) & 3, m + kAhead - kRows);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (kUp && (t & 1)) acc[m][t] = product<1, m & 3>(now[t], x[m % kRing], acc[m][t], ws, xs[m / 4]);
-        else acc[m][t] = product<0, m & 3>(now[t], x[m % kRing], acc[m][t], ws, xs[m / 4]);
-      }
+      x[(q + kAhead) % kRing] = q + kAhead < kParts ? read(s & 3, q + kAhead) : read((s + 1) & 3, q + kAhead - kParts);
+      acc[m][0] = product32<0, m & 3>(now[k][0], x[q % kRing], acc[m][0], ws, xs[m / 4]);
+      acc[m][1] = product32<kUp ? 1 : 0, m & 3>(now[k][1], x[q % kRing], acc[m][1], ws, xs[m / 4]);
     });
 #pragma unroll
-    for (int t = 0; t < 4; ++t) now[t] = next[t];
+    for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = next[i >> 1][i & 1];
     xs = xs_next;
     ws = ws_next;
   }
   // (What is still on its way into LDS has to land before the LDS is another's.)
   wait_loads<0>();
 
+  // Lane (r, h) holds of row r the results 8 (i / 4) + 4 h + i % 4 of each operand: of the
+  // tiles' dealt rows two runs, one for each p = (i / 4) % 2.
   if constexpr (kUp) {
     __syncthreads();
-    store_hidden<kRows>(a, tile, acc, block, reinterpret_cast<uint32_t*>(&lds.rows[0][0]));
+    const int64_t inner = a.columns / 2;
+    uint32_t* amax = reinterpret_cast<uint32_t*>(&lds.rows[0][0]);
+    float hid[kRows][2][8];
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t of = hidden(hid[m][p], [&](int i) { return acc[m][0][(i >> 2) * 8 + p * 4 + (i & 3)]; },
+                                   [&](int i) { return acc[m][1][(i >> 2) * 8 + p * 4 + (i & 3)]; });
+        top = top > of ? top : of;
+      }
+      const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      if (h == 0) amax[wave * kSize + m * 32 + r] = both[0] > both[1] ? both[0] : both[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      const int in = m * 32 + r;
+      uint32_t top = 0;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) top = top > amax[v * kSize + in] ? top : amax[v * kSize + in];
+      const float scale = scale_from_amax_bits(top, true);
+      if (in >= tile.rows) continue;
+      uint8_t* to = a.codes + (tile.row + in) * inner + block * 128 + wave * 32 + 8 * h;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t lo, hi;
+        quantize_eight(hid[m][p], scale, true, lo, hi);
+        *reinterpret_cast<uint2*>(to + 16 * p) = make_uint2(lo, hi);
+      }
+      if (wave == 0 && h == 0)
+        a.scales[((int64_t)tile_at * (inner / kBlock) + block) * kSize + r * kRows + m] = (uint8_t)(__float_as_uint(scale) >> 23);
+    }
   } else {
-    store_result<kRows>(a, tile, acc, column);
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      const int in = m * 32 + r;
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = finite_max(top, acc[m][i >> 4][i & 15]);
+      const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      const Power power = power_of(both[0] > both[1] ? both[0] : both[1]);
+      if (column >= a.columns || in >= tile.rows) continue;
+      const int64_t row = tile.row + in;
+      uint16_t* to = a.y + row * a.columns + column + 16 * h;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        store_sixteen(to + 32 * p, power.factor, [&](int i) { return acc[m][i >> 3][(i >> 2 & 1) * 8 + p * 4 + (i & 3)]; });
+      if (h == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power.exponent;
+    }
   }
+}
+
+// The scales of up's rows as the wide kernel reads them: [tile][step][32][kRows], a row's
+// part of 32 last, so that a lane's are one read. (What a work-group of it would fetch into
+// LDS byte by byte before its first product.)
+template <int kRows>
+__global__ __launch_bounds__(256) void tile_scales(ProductArgs a, uint8_t* out, int steps, int chunks) {
+  constexpr int kSize = 32 * kRows, kSteps = 16;
+  __shared__ __align__(16) uint8_t part[kSteps][kSize];
+  const int tile_at = blockIdx.x / chunks, first = (int)(blockIdx.x % chunks) * kSteps;
+  if (tile_at >= *a.tile_count) return;
+  const Tile tile = a.tiles[tile_at];
+  const int in = threadIdx.x % kSize;
+  const int64_t row = a.order[tile.row + (in < tile.rows ? in : tile.rows - 1)] / a.choices;
+  const uint8_t* from = a.x_scale + row * steps + first;
+#pragma unroll
+  for (int k = threadIdx.x / kSize; k < kSteps; k += 256 / kSize)
+    if (first + k < steps) part[k][(in & 31) * kRows + (in >> 5)] = from[k];
+  __syncthreads();
+  const int at = threadIdx.x * 16;
+  if (at < kSteps * kSize && first + at / kSize < steps)
+    *reinterpret_cast<uint4*>(out + ((int64_t)tile_at * steps + first) * kSize + at) =
+        *reinterpret_cast<const uint4*>(&part[0][0] + at);
 }
 
 // --------------------------------------------------------------- 4. join --
@@ -484,7 +587,7 @@ struct Plan {
   int64_t pairs, tiles;       // of the longest call, and its row tiles at most
   int rows;                   // 16-row parts of a tile
   // Offsets of the workspace's parts.
-  int64_t count, list, order, place, codes, scales, y, powers, bytes;
+  int64_t count, list, order, place, row_scales, codes, scales, y, powers, bytes;
 };
 
 Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_t experts, int64_t total) {
@@ -493,7 +596,6 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   // Rows of an expert, on average; tiles of about twice that.
   const int64_t mean = p.pairs / total;
   p.rows = mean <= 6 ? 1 : mean <= 16 ? 2 : mean <= 40 ? 4 : mean <= 128 ? 8 : 16;
-  if (dim > kMaxWideSteps * kBlock || inner > kMaxWideSteps * kBlock) p.rows = p.rows < 4 ? p.rows : 4;
   const int64_t size = 16 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;
@@ -508,7 +610,10 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   p.order = part(p.pairs * 4);
   p.place = part(p.pairs * 4);
   p.codes = part(p.pairs * inner);
-  p.scales = part(p.pairs * (inner / kBlock));
+  // Scales of rows; of tiles in the wide kernels.
+  const int64_t rows = p.rows >= 8 ? p.tiles * size : p.pairs;
+  p.row_scales = part(p.rows >= 8 ? rows * (dim / kBlock) : 0);
+  p.scales = part(rows * (inner / kBlock));
   p.y = part(p.pairs * dim * 2);
   p.powers = part(p.pairs * (dim / kWaveCols));
   p.bytes = at;
@@ -534,8 +639,8 @@ int launch_product(const ProductArgs& a, const Plan& p, hipStream_t stream) {
   if (p.rows == 1) go(expert_product<1, kUp>, groups);
   else if (p.rows == 2) go(expert_product<2, kUp>, groups);
   else if (p.rows == 4) go(expert_product<4, kUp>, groups);
-  else if (p.rows == 8) go(expert_product_wide<8, kUp>, (groups + 7) / 8 * 8);
-  else go(expert_product_wide<16, kUp>, (groups + 7) / 8 * 8);
+  else if (p.rows == 8) go(expert_product_wide<4, kUp>, (groups + 7) / 8 * 8);
+  else go(expert_product_wide<8, kUp>, (groups + 7) / 8 * 8);
   DSA_CHECK_LAUNCH("expert product");
   return kOk;
 }
@@ -600,6 +705,18 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 16 * p.rows};
   hipLaunchKernelGGL(group_pairs, dim3((unsigned)experts), dim3(kGroupThreads), 0, stream, group);
   DSA_CHECK_LAUNCH("grouping of pairs");
+  if (p.rows >= 8) {
+    uint8_t* tiled = ws + p.row_scales;
+    const int steps = (int)(dim / kBlock), chunks = (steps + 15) / 16;
+    DSA_CHECK_ARG(grid_fits(p.tiles * chunks, 256), "too many tokens for one launch");
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * chunks)), dim3(256), 0, stream, up, tiled, steps, chunks);
+    };
+    if (p.rows == 8) go(tile_scales<4>);
+    else go(tile_scales<8>);
+    DSA_CHECK_LAUNCH("scales of tiles");
+    up.x_scale = tiled;
+  }
   if (const int status = launch_product<true>(up, p, stream)) return status;
   if (const int status = launch_product<false>(dn, p, stream)) return status;
   auto join = [&](auto kernel) {

@@ -200,13 +200,17 @@ def _exponents(scale, shape, what):
 def _tiles(weight, parts):
     """``[E, N, K]`` codes as tiles of 16 rows by 128 in the order in which a wave reads
     them: ``[E, N / 16, K / 128, 2, 4, 16, 16 bytes]``, lane (g, r) of plane p holding bytes
-    64 p + 16 g .. of row r; tiles of the rows' ``parts`` equal parts in turn."""
+    64 p + 16 g .. of row r. A wave takes four tiles: 64 / ``parts`` neighbouring rows of
+    each of the ``parts`` equal parts of N, so dealt out that four lanes' results are
+    neighbours: with n = 4 / ``parts`` tiles of a part, row 4 a + i of its tile t is row
+    4 n a + 4 t + i of the 16 n; the parts' tiles in turn."""
     experts, rows, columns = weight.shape
     if weight.data_ptr() % 16 or weight.storage_offset() % 16:
         weight = weight.clone()
     units = weight.view(torch.uint8).view(torch.complex128)  # 16 bytes each
-    units = units.view(experts, parts, rows // parts // 16, 16, columns // SCALE_BLOCK, 2, 4)
-    return units.permute(0, 2, 1, 4, 5, 6, 3).contiguous().view(torch.uint8)
+    each = 4 // parts
+    units = units.view(experts, parts, rows // 64, 4, each, 4, columns // SCALE_BLOCK, 2, 4)
+    return units.permute(0, 2, 4, 1, 6, 7, 8, 3, 5).contiguous().view(torch.uint8)
 
 
 class ExpertWeights:

@@ -125,9 +125,16 @@ def test_tiles_hold_what_the_layout_says():
     flat = torch.empty(parts["gate_up"].numel() + 3, dtype=torch.uint8)
     flat[3:] = codes.flatten()
     parts["gate_up"] = flat[3:].view(codes.shape).view(F8)
-    got = ExpertWeights(**parts).gate_up.view(2, 32, 3, 2, 4, 16, 16)
-    for tile, k, plane, g, r in [(0, 0, 0, 0, 0), (1, 2, 1, 3, 15), (30, 1, 0, 2, 7), (31, 2, 1, 1, 5)]:
-        row = (tile % 2) * 256 + tile // 2 * 16 + r
+    own = ExpertWeights(**parts)
+    got = own.gate_up.view(2, 32, 3, 2, 4, 16, 16)
+    for tile, k, plane, g, r in [(0, 0, 0, 0, 0), (1, 2, 1, 3, 15), (30, 1, 0, 2, 7), (31, 2, 1, 1, 5), (14, 0, 1, 0, 9)]:
+        # Tiles of gate and up in turn; two of each make 32 neighbouring columns.
+        row = (tile % 2) * 256 + tile // 4 * 32 + r // 4 * 8 + tile // 2 % 2 * 4 + r % 4
+        at = 128 * k + 64 * plane + 16 * g
+        assert torch.equal(got[1, tile, k, plane, g, r], codes[1, row, at:at + 16])
+    got = own.down.view(2, 24, 2, 2, 4, 16, 16)
+    for tile, k, plane, g, r in [(0, 0, 0, 0, 0), (1, 1, 1, 3, 15), (23, 1, 0, 2, 7), (14, 0, 1, 0, 9)]:
+        row = tile // 4 * 64 + r // 4 * 16 + tile % 4 * 4 + r % 4
         at = 128 * k + 64 * plane + 16 * g
         assert torch.equal(got[1, tile, k, plane, g, r], codes[1, row, at:at + 16])
 
