@@ -302,8 +302,8 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
 // registers, a step ahead; the rows' codes go into LDS straight from memory (two steps
 // ahead, four buffers), where all four waves read them, three operands ahead of their
 // products. Half-way through a step the waves meet: from there on the next step's rows may
-// be read. A row's eight 16-byte parts are turned by its index, so that eight rows' reads of
-// one part fall on different banks.
+// be read. A row's eight 16-byte parts are turned by its index, so that the rows' reads of one
+// part fall on different banks.
 // Rows' scales come from memory a step ahead, laid out by tile.
 // Per step of 128 a CU's matrix units take 256 kRows clocks, its LDS 160 kRows (four waves'
 // reads and one write of 4 kRows KB at 128 bytes).
@@ -320,6 +320,12 @@ __device__ __forceinline__ v8i load_weight32(const uint8_t* codes, int64_t tile,
   const v4u* from = reinterpret_cast<const v4u*>(codes + tile + k * 1024);
   return joined(from[0], from[16]);
 }
+
+// How a row's parts are turned: two rows and their eight parts are all 64 banks. 16 lanes are
+// served at once, 0 .. 3 with 12 .. 15 and 20 .. 27, the other 16 of 32 together: eight of the
+// first 16 rows and eight of the others, which must not fall on the same banks. (Turned by
+// row % 8 alone half of the LDS's time went to conflicts.)
+__device__ __forceinline__ uint32_t turn_of(uint32_t row) { return (row & 7) ^ (row >> 4 & 1); }
 
 template <int kRows, bool kUp>
 __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(ProductArgs a) {
@@ -353,7 +359,7 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
     const int in = (wave * kLoads + i) * 8 + (lane >> 3);
     int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
     if constexpr (kUp) row = a.order[row] / a.choices;
-    from[i] = (uint64_t)(a.x + row * a.depth + (((lane & 7) ^ (in & 7)) << 4));
+    from[i] = (uint64_t)(a.x + row * a.depth + (((lane & 7) ^ turn_of(in)) << 4));
   }
   const uint32_t lds_rows = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds.rows[0][0];
   auto fetch = [&](int buffer, int i) {
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
   lds_barrier();
 
   // Part m, half k of a step: a lane's two 16-byte parts of row r are 4 k + 2 h and the next.
-  const uint32_t lane_at = lds_rows + r * kBlock + (((2 * h) ^ (r & 7)) << 4);
+  const uint32_t lane_at = lds_rows + r * kBlock + (((2 * h) ^ turn_of(r)) << 4);
   // Operands in registers: those ahead of the products hide the LDS.
   constexpr int kRing = kRows <= 4 ? 2 : 4, kAhead = kRing - 1, kParts = 2 * kRows;
   v8i x[kRing];
