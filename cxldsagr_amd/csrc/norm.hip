@@ -3,7 +3,7 @@
 // y rounded once to the element type, t too; and, where wanted, the e4m3 codes of the
 // rounded y with a power-of-two scale for every 128 values, as its exponent (e8m0).
 //
-// The sum of squares and y are in 64 bits, so that y and its codes are the formula's
+// The sum of squares is in 64 bits, y in 46 or more, so that y and its codes are the formula's
 // (a y of 32 bits lies on the other side of a rounding border in one of some 30,000 values,
 // and of a scale's border now and then, which doubles a whole block's step).
 //
@@ -16,7 +16,6 @@ namespace {
 
 constexpr int kMaxDim = 16384;
 constexpr int kThreads = 512;            // of a work-group at most
-constexpr int kMaxRowsAtOnce = 1 << 20;  // work-groups of a launch; each goes on to further rows
 
 struct NormArgs {
   const void* x;
@@ -28,7 +27,7 @@ struct NormArgs {
   uint8_t* scales;
   int64_t x_stride, residual_stride, tokens;
   int32_t dim, wide_weight;  // wide: fp32, else the rows' type
-  double eps;
+  double eps, per_dim;       // per_dim: 1 / dim
 };
 
 struct Bf16Bits {
@@ -63,25 +62,52 @@ __device__ __forceinline__ double sum_group(double v, double* shared) {
   return v;
 }
 
+// 1 / sqrt(v) in 64 bits: the unit's estimate and a step of the third order. (0 and infinity
+// give the estimate's infinity and 0.)
+__device__ __forceinline__ double reciprocal_root(double v) {
+  const double y = __builtin_amdgcn_rsq(v), r = __builtin_fma(-v * y, y, 1.0);
+  const double better = __builtin_fma(y * r, __builtin_fma(0.375, r, 0.5), y);
+  return r == r ? better : y;
+}
+
 // Items of 8 elements, kItems a thread at most: item i is thread i % threads' item
-// i / threads.
+// i / threads. A work-group goes from row to row with the weight in registers and the next
+// row on its way.
 template <typename T, int kItems>
-__global__ __launch_bounds__(kThreads) void residual_rms_norm(NormArgs a) {
+__global__ __launch_bounds__(kThreads, kItems <= 2 ? 4 : 2) void residual_rms_norm(NormArgs a) {
   using Item = Pack<T, 8>;
   __shared__ double shared[2][kThreads / 64];
   const int threads = blockDim.x, items = a.dim / 8;
-  int turn = 0;
-  for (int64_t row = blockIdx.x; row < a.tokens; row += gridDim.x, turn ^= 1) {
+  float w[kItems][8];
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    const int i = threadIdx.x + j * threads;
+    if (i >= items) continue;
+    if (a.wide_weight) {
+      const auto p = reinterpret_cast<const Pack<float, 8>*>(a.weight)[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[j][e] = p.v[e];
+    } else {
+      const Item p = reinterpret_cast<const Item*>(a.weight)[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[j][e] = value_of(p.v[e]);
+    }
+  }
+  Item in[kItems], add[kItems];
+  auto load = [&](int64_t row) {
     const Item* x = reinterpret_cast<const Item*>(static_cast<const T*>(a.x) + row * a.x_stride);
     const Item* r = reinterpret_cast<const Item*>(static_cast<const T*>(a.residual) + row * a.residual_stride);
-    float t[kItems][8];
-    Item in[kItems], add[kItems];
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
       const int i = threadIdx.x + j * threads;
       if (i < items) in[j] = x[i];
       if (i < items && a.residual) add[j] = r[i];
     }
+  };
+  load(blockIdx.x);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.tokens; row += gridDim.x, turn ^= 1) {
+    float t[kItems][8];
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
@@ -93,31 +119,34 @@ __global__ __launch_bounds__(kThreads) void residual_rms_norm(NormArgs a) {
         sum = __builtin_fma((double)t[j][e], (double)t[j][e], sum);
       }
     }
-    const double inverse = 1.0 / sqrt(sum_group(sum, shared[turn]) / a.dim + a.eps);
+    if (row + gridDim.x < a.tokens) load(row + gridDim.x);
+    const double mean = __builtin_fma(sum_group(sum, shared[turn]), a.per_dim, a.eps);
+    const double inverse = reciprocal_root(mean);
+    // t inverse w to 46 bits in pairs of 32 (a third of the time of 64-bit products); where
+    // the inverse does not fit a pair, in 64.
+    const bool pairs = mean > 0x1p-100 && mean < 0x1p100;
+    const float high = (float)inverse, low = (float)(inverse - high);
+    auto normed = [&](float v, float weight) {
+// (A product that becomes part of the sum would count its rounding twice.)
+#pragma clang fp contract(off)
+      if (!pairs) return (float)((double)v * inverse * weight);
+      const float u = v * high, u_low = __builtin_fmaf(v, low, __builtin_fmaf(v, high, -u));
+      const float y = u * weight, both = y + __builtin_fmaf(u_low, weight, __builtin_fmaf(u, weight, -y));
+      return both == both ? both : y;  // (an infinity less itself)
+    };
     const int64_t base = row * a.dim;
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
       const int i = threadIdx.x + j * threads;
       if (i >= items) continue;
+      Item out;
       if (a.residual_out) {
-        Item out;
 #pragma unroll
         for (int e = 0; e < 8; ++e) out.v[e] = rounded<T>(t[j][e]);
         reinterpret_cast<Item*>(static_cast<T*>(a.residual_out) + base)[i] = out;
       }
-      float w[8];
-      if (a.wide_weight) {
-        const auto p = reinterpret_cast<const Pack<float, 8>*>(a.weight)[i];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = p.v[e];
-      } else {
-        const Item p = reinterpret_cast<const Item*>(a.weight)[i];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = value_of(p.v[e]);
-      }
-      Item out;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out.v[e] = rounded<T>((float)((double)t[j][e] * w[e] * inverse));
+      for (int e = 0; e < 8; ++e) out.v[e] = rounded<T>(normed(t[j][e], w[j][e]));
       if (a.values) reinterpret_cast<Item*>(static_cast<T*>(a.values) + base)[i] = out;
       if (a.codes) {
         // 16 lanes hold a block of 128 values (the dims are whole blocks).
@@ -154,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void residual_rms_norm_scalar(NormArgs a)
       const double t = total(i);
       sum = __builtin_fma(t, t, sum);
     }
-    const double inverse = 1.0 / sqrt(sum_group(sum, shared[turn]) / a.dim + a.eps);
+    const double inverse = reciprocal_root(__builtin_fma(sum_group(sum, shared[turn]), a.per_dim, a.eps));
     const int64_t base = row * a.dim;
     for (int i = threadIdx.x; i < a.dim; i += blockDim.x) {
       const float t = total(i);
@@ -167,11 +196,13 @@ __global__ __launch_bounds__(kThreads) void residual_rms_norm_scalar(NormArgs a)
 
 template <typename T>
 int launch_norm(const NormArgs& a, bool vector, hipStream_t stream) {
-  const int groups = (int)(a.tokens < kMaxRowsAtOnce ? a.tokens : kMaxRowsAtOnce);
   const int items = vector ? a.dim / 8 : a.dim;
   auto go = [&](auto kernel, int per) {
-    const int threads = ((items + per - 1) / per + 63) / 64 * 64;
-    hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads < kThreads ? threads : kThreads), 0, stream, a);
+    int threads = ((items + per - 1) / per + 63) / 64 * 64;
+    if (threads > kThreads) threads = kThreads;
+    // As many work-groups as the CUs hold at once, 16 waves a CU; each goes on to further rows.
+    const int64_t most = (int64_t)device_cu_count() * (16 * 64 / threads);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tokens < most ? a.tokens : most)), dim3(threads), 0, stream, a);
   };
   if (!vector) go(residual_rms_norm_scalar<T>, 1);
   else if (items <= kThreads) go(residual_rms_norm<T, 1>, 1);
@@ -203,7 +234,7 @@ extern "C" int dsa_residual_rms_norm(const void* x, int64_t x_stride, const void
   a.codes = static_cast<uint8_t*>(codes), a.scales = static_cast<uint8_t*>(scales);
   a.x_stride = x_stride, a.residual_stride = residual_stride, a.tokens = tokens;
   a.dim = (int32_t)dim, a.wide_weight = weight_dtype == DSA_DTYPE_F32;
-  a.eps = eps;
+  a.eps = eps, a.per_dim = 1.0 / (double)dim;
   const int64_t align = dtype == DSA_DTYPE_F32 ? 4 : 8;
   bool vector = dim % 8 == 0 && x_stride % align == 0 && (!residual || residual_stride % align == 0);
   for (const void* p : {x, residual, weight, (const void*)values, (const void*)residual_out})
