@@ -188,7 +188,9 @@ _CURRENT = nullcontext()
 
 def on_device(device):
     """``torch.cuda.device(device)``, or nothing when it is current already."""
-    if device.index is not None and torch.cuda.current_device() == device.index:
+    index = device.index
+    # (Tensors of a device are there only once torch has initialised it.)
+    if index is not None and torch._C._cuda_getDevice() == index:
         return _CURRENT
     return torch.cuda.device(device)
 

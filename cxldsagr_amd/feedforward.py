@@ -41,11 +41,18 @@ class Normed(NamedTuple):
     residual: Optional[torch.Tensor]  # [T, D], x's type: x + residual
 
 
-def _rows(tensor):
-    """``tensor`` [T, D] with contiguous rows (any row stride), else a copy."""
-    if tensor.stride(1) != 1 or tensor.stride(0) < 0:
-        return tensor.contiguous()
-    return tensor
+_CODES = _native.DTYPE_CODES
+
+
+def _rows(tensor, aligned=False):
+    """``tensor`` [T, D] with contiguous rows (any row stride; ``aligned``: to 16 bytes), or
+    a copy, and its address and row stride."""
+    stride, unit = tensor.stride()
+    address = tensor.data_ptr()
+    if unit != 1 or stride < 0 or (aligned and (address % 16 or stride * tensor.element_size() % 16)):
+        tensor = tensor.clone(memory_format=torch.contiguous_format)
+        return tensor, tensor.data_ptr(), tensor.shape[1]
+    return tensor, address, stride
 
 
 def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quantize=False,
@@ -63,14 +70,14 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
     tensor or in ``residual_out`` (contiguous; it may be ``residual`` itself). Forward
     only.
     """
-    if x.ndim != 2 or weight.shape != (x.shape[1],):
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) != 2 or weight.shape != shape[1:]:
         raise ValueError("Expected x [T, D] and weight [D]")
-    tokens, dim = x.shape
-    dtype, device = x.dtype, x.device
-    code = _native.DTYPE_CODES.get(dtype)
+    tokens, dim = shape
+    code, weight_code = _CODES.get(dtype), _CODES.get(weight.dtype)
     if code is None:
         raise ValueError("x must be bf16, fp16 or fp32")
-    if weight.dtype != dtype and weight.dtype != torch.float32:
+    if weight_code != code and weight_code != 2:
         raise ValueError("weight must be fp32 or of x's type")
     if not 1 <= dim <= MAX_NORM_DIM:
         raise ValueError(f"x must have 1 to {MAX_NORM_DIM} dims")
@@ -81,14 +88,14 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
     if weight.device != device:
         raise ValueError("x and weight must be on the same device")
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != dtype or residual.device != device:
+        if residual.shape != shape or residual.dtype != dtype or residual.device != device:
             raise ValueError("residual must have x's shape, type and device")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    if not values and not quantize and residual is None:
+    elif not values and not quantize:
         raise ValueError("nothing to return: ask for values, codes or a residual's sum")
     if residual_out is not None and (
-            residual_out.shape != x.shape or residual_out.dtype != dtype
+            residual_out.shape != shape or residual_out.dtype != dtype
             or residual_out.device != device or not residual_out.is_contiguous()
             or residual_out.data_ptr() % 16):
         raise ValueError("residual_out must be a contiguous, 16-byte aligned tensor of x's shape, "
@@ -97,34 +104,29 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
                                     or (residual is not None and residual.requires_grad)):
         raise ValueError("residual RMS norm has no backward pass")
     _native.require_gfx950(device, "residual RMS norm")
-    x = _rows(x)
-    weight = weight if weight.is_contiguous() else weight.contiguous()
-    stride = x.stride(0)
-    residual_stride = 0
+    # (Codes are written by lanes of 8 values; the tensors are kept until the call: they may
+    # be copies.)
+    x, x_at, x_stride = _rows(x, quantize)
+    residual_at = residual_stride = 0
     if residual is not None:
-        residual = _rows(residual)
-        residual_stride = residual.stride(0)
+        residual, residual_at, residual_stride = _rows(residual, quantize)
         if residual_out is None:
-            residual_out = x.new_empty((tokens, dim))
+            residual_out = x.new_empty(shape)
+    if not weight.is_contiguous() or (quantize and weight.data_ptr() % 16):
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    out = x.new_empty(shape) if values else None
+    codes = scales = None
     if quantize:
-        # (Codes are written by lanes of 8 values.)
-        align = 16 // x.element_size()
-        if stride % align or x.data_ptr() % 16:
-            x, stride = x.clone(memory_format=torch.contiguous_format), dim
-        if residual is not None and (residual_stride % align or residual.data_ptr() % 16):
-            residual, residual_stride = residual.clone(memory_format=torch.contiguous_format), dim
-        if weight.data_ptr() % 16:
-            weight = weight.clone()
-    out = x.new_empty((tokens, dim)) if values else None
-    codes = x.new_empty((tokens, dim), dtype=CODES) if quantize else None
-    scales = x.new_empty((tokens, dim // SCALE_BLOCK), dtype=SCALES) if quantize else None
+        codes = x.new_empty(shape, dtype=CODES)
+        scales = x.new_empty((tokens, dim // SCALE_BLOCK), dtype=SCALES)
     if tokens:
         with _native.on_device(device):
             _native.call(
-                "dsa_residual_rms_norm", x.data_ptr(), stride, _native.ptr(residual),
-                residual_stride, code, weight.data_ptr(), _native.DTYPE_CODES[weight.dtype],
-                tokens, dim, eps, _native.ptr(out), _native.ptr(residual_out),
-                _native.ptr(codes), _native.ptr(scales), _native.raw_stream(device))
+                "dsa_residual_rms_norm", x_at, x_stride, residual_at, residual_stride, code,
+                weight.data_ptr(), weight_code, tokens, dim, eps,
+                out.data_ptr() if values else 0, _native.ptr(residual_out),
+                codes.data_ptr() if quantize else 0, scales.data_ptr() if quantize else 0,
+                _native.raw_stream(device))
     return Normed(out, codes, scales, residual_out)
 
 
@@ -144,11 +146,11 @@ def route_experts(logits, k, *, bias=None, scoring="sigmoid", groups=1, top_grou
     ``s * scale``, with ``renormalize`` ``s / (sum of the k + 1e-20) * scale``. Forward
     only.
     """
-    if logits.ndim != 2 or not 1 <= logits.shape[1] <= MAX_EXPERTS:
+    shape, device = logits.shape, logits.device
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_EXPERTS:
         raise ValueError(f"Expected logits [T, E] of 1 to {MAX_EXPERTS} experts")
-    tokens, experts = logits.shape
-    device = logits.device
-    code = _native.DTYPE_CODES.get(logits.dtype)
+    tokens, experts = shape
+    code = _CODES.get(logits.dtype)
     if code is None:
         raise ValueError("logits must be fp32, bf16 or fp16")
     if scoring not in ("sigmoid", "softmax"):
@@ -159,24 +161,25 @@ def route_experts(logits, k, *, bias=None, scoring="sigmoid", groups=1, top_grou
             or experts % groups or not 1 <= top_groups <= groups):
         raise ValueError(f"groups (1 to {MAX_GROUPS}) must divide the experts, top_groups be 1 to "
                          "groups")
-    if type(k) is not int or not 1 <= k <= min(MAX_CHOICES, top_groups * (experts // groups)):
+    if type(k) is not int or not 1 <= k <= MAX_CHOICES or k > top_groups * (experts // groups):
         raise ValueError(f"k must be 1 to {MAX_CHOICES} and within the experts of top_groups groups")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (experts,) or bias.device != device:
+        if bias.dtype != torch.float32 or bias.shape != shape[1:] or bias.device != device:
             raise ValueError("bias must be FP32 [E] on the logits' device")
-        bias = bias if bias.is_contiguous() else bias.contiguous()
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("routing to experts has no backward pass")
     _native.require_gfx950(device, "routing to experts")
-    logits = _rows(logits)
+    logits, logits_at, stride = _rows(logits)
     weights = logits.new_empty((tokens, k), dtype=torch.float32)
     ids = logits.new_empty((tokens, k), dtype=torch.int32)
     if tokens:
         with _native.on_device(device):
             _native.call(
-                "dsa_route_experts", logits.data_ptr(), logits.stride(0), code, tokens, experts, k,
+                "dsa_route_experts", logits_at, stride, code, tokens, experts, k,
                 _native.ptr(bias), scoring == "softmax", groups, top_groups, bool(renormalize),
                 scale, weights.data_ptr(), ids.data_ptr(), _native.raw_stream(device))
     return weights, ids
