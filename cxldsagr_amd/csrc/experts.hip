@@ -4,9 +4,8 @@
 // x, q and the weights in e4m3 with a power-of-two scale (e8m0) for every 128 values of a
 // row, and every 128 by 128 of a weight.
 //
-// Four launches (five with wide tiles):
+// Four launches:
 //  1. group: the (token, choice) pairs of each expert, in token order, and row tiles of them;
-//     wide tiles: their rows' scales in the order of the products;
 //  2. up: row tiles times gate and up, h, its codes and scales;
 //  3. down: row tiles times down, y in 16 bits with a power of two for every 64 values of a
 //     row (its largest value just below 2^15 as fp16: 11 bits of each value; as bf16, 8, the
@@ -75,55 +74,83 @@ struct GroupArgs {
 
 // Work-group e lists expert e's pairs. Each counts all experts' (in LDS), so that none waits
 // for another: rows and tiles of the experts before e are sums over the counts. A wave takes
-// a run of the pairs, so that a pair's row is the sum of what was found before it.
+// a run of the pairs, so that a pair's row is the sum of what was found before it, kAtOnce of
+// a lane's on their way at once: what bounds it is the way to memory and back (65,536 pairs
+// of 32 experts with eight at once: 43 us).
+template <int kAtOnce>
 __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
-  __shared__ uint32_t counts[kMaxExperts];
+  // (Behind the last: pairs of other experts, a place for each lane, as one for all would
+  // take them one after another.)
+  __shared__ uint32_t counts[kMaxExperts + 64];
   __shared__ uint32_t of_wave[kGroupThreads / 64][3];
-  const int expert = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  constexpr int kWaves = kGroupThreads / 64;
-  for (int i = threadIdx.x; i < a.experts; i += kGroupThreads) counts[i] = 0;
+  const uint32_t expert = blockIdx.x, experts = a.experts;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  constexpr int kPart = 64 * kAtOnce;
+  const int run = ((a.pairs + waves - 1) / waves + 63) / 64 * 64;
+  const int begin = wave * run < a.pairs ? wave * run : a.pairs, end = a.pairs - begin < run ? a.pairs : begin + run;
+  // Experts of pairs base + lane, base + 64 + lane, ... (past the end: others).
+  uint32_t e[kAtOnce];
+  auto load = [&](int base) {
+    int32_t id[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int p = base + 64 * i + lane;
+      id[i] = a.ids[p < end ? p : end - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t of = (uint32_t)id[i] - (uint32_t)a.first;
+      e[i] = base + 64 * i + lane < end ? min(of, experts) : experts;
+    }
+  };
+  if (begin < end) load(begin);
+  for (uint32_t i = threadIdx.x; i < experts; i += blockDim.x) counts[i] = 0;
   __syncthreads();
-  const int run = ((a.pairs + kWaves - 1) / kWaves + 63) / 64 * 64;
-  const int64_t begin = (int64_t)wave * run, end = begin + run < a.pairs ? begin + run : a.pairs;
   uint32_t found = 0;
-#pragma unroll 8
-  for (int64_t i = begin + lane; i < end; i += 64) {
-    const uint32_t e = (uint32_t)a.ids[i] - (uint32_t)a.first;
-    if (e < (uint32_t)a.experts) atomicAdd(&counts[e], 1u);
-    found += e == (uint32_t)expert;
+  for (int base = begin; base < end; base += kPart) {
+    if (base > begin) load(base);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      atomicAdd(&counts[e[i] < experts ? e[i] : experts + lane], 1u);
+      found += e[i] == expert;
+    }
   }
   found = sum_lanes(found);
   __syncthreads();
-  // Rows and tiles before this expert's, this thread's expert being i.
-  const int i = threadIdx.x;
-  const uint32_t n = i < a.experts ? counts[i] : 0u;
-  const uint32_t tiles_of = (n + a.tile_rows - 1) / a.tile_rows;
-  const uint32_t rows = sum_lanes(i < expert ? n : 0u), tiles = sum_lanes(i < expert ? tiles_of : 0u);
+  // Rows and tiles of the experts before this one.
+  uint32_t rows = 0, tiles = 0;
+  for (uint32_t i = threadIdx.x; i < expert; i += blockDim.x)
+    rows += counts[i], tiles += (counts[i] + a.tile_rows - 1) / a.tile_rows;
+  rows = sum_lanes(rows), tiles = sum_lanes(tiles);
   if (lane == 0) of_wave[wave][0] = rows, of_wave[wave][1] = tiles, of_wave[wave][2] = found;
   __syncthreads();
   uint32_t row = 0, tile = 0, before = 0;
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < waves; ++w) {
     row += of_wave[w][0], tile += of_wave[w][1];
     if (w < wave) before += of_wave[w][2];
   }
   const uint32_t own = counts[expert], own_tiles = (own + a.tile_rows - 1) / a.tile_rows;
-  for (uint32_t t = threadIdx.x; t < own_tiles; t += kGroupThreads) {
+  for (uint32_t t = threadIdx.x; t < own_tiles; t += blockDim.x) {
     const uint32_t at = t * a.tile_rows, left = own - at;
-    a.tiles[tile + t] = Tile{expert, (int32_t)(row + at), (int32_t)(left < (uint32_t)a.tile_rows ? left : a.tile_rows),
+    a.tiles[tile + t] = Tile{(int32_t)expert, (int32_t)(row + at), (int32_t)(left < (uint32_t)a.tile_rows ? left : a.tile_rows),
                              (int32_t)tile, (int32_t)own_tiles, {}};
   }
-  if (expert == a.experts - 1 && threadIdx.x == 0) *a.tile_count = (int32_t)(tile + own_tiles);
+  if (expert == experts - 1 && threadIdx.x == 0) *a.tile_count = (int32_t)(tile + own_tiles);
   uint32_t next = row + before;
-  for (int64_t base = begin; base < end; base += 64) {
-    const int64_t p = base + lane;
-    const bool mine = p < end && (uint32_t)a.ids[p] - (uint32_t)a.first == (uint32_t)expert;
-    const uint64_t all = __ballot(mine);
-    if (mine) {
-      const uint32_t to = next + (uint32_t)__popcll(all & ((1ull << lane) - 1));
-      a.order[to] = (int32_t)p;
-      a.place[p] = (int32_t)to;
+  for (int base = begin; base < end; base += kPart) {
+    if (run > kPart) load(base);  // (else they are here still)
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint64_t all = __ballot(e[i] == expert);
+      if (all == 0) continue;
+      if (e[i] == expert) {
+        const uint32_t to = next + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+        const int p = base + 64 * i + lane;
+        a.order[to] = p;
+        a.place[p] = (int32_t)to;
+      }
+      next += (uint32_t)__popcll(all);
     }
-    next += (uint32_t)__popcll(all);
   }
 }
 
@@ -216,11 +243,20 @@ __device__ __forceinline__ v8i load_weight(const uint8_t* codes, int steps, int 
   return joined(from[0], from[64]);
 }
 
+// What a wave's products of one step need: 64 rows of a weight, kRows 16-row tiles of codes,
+// and their scales.
+template <int kRows>
+struct Step {
+  v8i w[4], x[kRows];
+  uint32_t w_scale[2], x_scale[kRows];
+};
+
 // Few rows: kRows 16-row tiles by 4 waves of 64 columns, every wave streaming its own part
-// of the weight, and the tokens' codes, through registers. What bounds it is reading the
-// weight.
+// of the weight, and the tokens' codes, through registers, kDepth steps at once. What bounds
+// it is reading the weight: 8 KB a step, and a CU wants some 40 KB under way.
 template <int kRows, bool kUp>
-__global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
+__global__ __launch_bounds__(256, 2) void expert_product(ProductArgs a) {
+  constexpr int kDepth = kRows <= 2 ? 3 : 2;
   const int tile_at = blockIdx.x / a.column_blocks, block = blockIdx.x % a.column_blocks;
   if (tile_at >= *a.tile_count) return;
   const Tile tile = a.tiles[tile_at];
@@ -229,8 +265,27 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
   const int steps = a.depth / kBlock;
   __shared__ uint32_t amax[kUp ? 4 * 16 * kRows : 1];
 
+  const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
   const uint8_t* x[kRows];
   const uint8_t* xs[kRows];
+  Step<kRows> ring[kDepth];
+  auto load_w = [&](Step<kRows>& to, int s) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) to.w[t] = load_weight(w.codes, steps, t, s);
+    to.w_scale[0] = w.scale[0][s];
+    if constexpr (kUp) to.w_scale[1] = w.scale[1][s];
+  };
+  auto load_x = [&](Step<kRows>& to, int s) {
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      const v4u* from = reinterpret_cast<const v4u*>(x[m] + s * kBlock);
+      to.x[m] = joined(from[0], from[4]);
+      to.x_scale[m] = xs[m][s];
+    }
+  };
+  // (The weight first: its rows do not wait for the tokens' indices.)
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) load_w(ring[d], d < steps ? d : steps - 1);
 #pragma unroll
   for (int m = 0; m < kRows; ++m) {
     const int in = 16 * m + r;
@@ -239,23 +294,31 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
     x[m] = a.x + row * a.depth + g * 16;
     xs[m] = a.x_scale + row * steps;
   }
-  const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) load_x(ring[d], d < steps ? d : steps - 1);
 
   v4f acc[kRows][4] = {};
-  for (int s = 0; s < steps; ++s) {
-    v8i wv[4];
+  auto multiply = [&](const Step<kRows>& of) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wv[t] = load_weight(w.codes, steps, t, s);
-    const int s0 = w.scale[0][s], s1 = w.scale[1][s];
+    for (int m = 0; m < kRows; ++m)
 #pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      const v4u* from = reinterpret_cast<const v4u*>(x[m] + s * kBlock);
-      const v8i xv = joined(from[0], from[4]);
-      const int sx = xs[m][s];
+      for (int t = 0; t < 4; ++t)
+        acc[m][t] = product(of.w[t], of.x[m], acc[m][t], of.w_scale[kUp ? t & 1 : 0], of.x_scale[m]);
+  };
+  int s = 0;
+  for (; s + kDepth <= steps; s += kDepth) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[m][t] = product(wv[t], xv, acc[m][t], t & 1 ? s1 : s0, sx);
+    for (int d = 0; d < kDepth; ++d) {
+      multiply(ring[d]);
+      // (At the end the last step comes again, from the nearest cache.)
+      const int next = s + d + kDepth < steps ? s + d + kDepth : steps - 1;
+      load_w(ring[d], next);
+      load_x(ring[d], next);
     }
   }
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d)
+    if (s + d < steps) multiply(ring[d]);
   if constexpr (kUp) {
     const int64_t inner = a.columns / 2;
     float h[kRows][8];
@@ -304,14 +367,16 @@ __global__ __launch_bounds__(256) void expert_product(ProductArgs a) {
 // products. Half-way through a step the waves meet: from there on the next step's rows may
 // be read. A row's eight 16-byte parts are turned by its index, so that the rows' reads of one
 // part fall on different banks.
-// Rows' scales come from memory a step ahead, laid out by tile.
+// Rows' scales: up lays those of all steps out in LDS before the first; the scales of h come
+// from memory a step ahead, where up has put them by tile.
 // Per step of 128 a CU's matrix units take 256 kRows clocks, its LDS 160 kRows (four waves'
 // reads and one write of 4 kRows KB at 128 bytes).
-constexpr int kMaxWideSteps = 256;
-template <int kRows>
+constexpr int kMaxWideSteps = 256, kMaxWideUp = 124;  // steps; steps of up, whose scales LDS holds
+template <int kRows, bool kUp>
 struct WideLds {
   alignas(16) uint8_t rows[4][32 * kRows * kBlock];
-  alignas(4) uint8_t weight_scales[kMaxWideSteps][2];
+  alignas(16) uint8_t scales[kUp ? kMaxWideUp : 1][32][kRows];  // (a row's part of 32 last: one read holds all)
+  alignas(4) uint8_t weight_scales[kUp ? kMaxWideUp : kMaxWideSteps][2];
 };
 
 // The wave's weight tiles as two operands of 32 rows (up: gate's and up's), 64 deep: half k
@@ -330,7 +395,7 @@ __device__ __forceinline__ uint32_t turn_of(uint32_t row) { return (row & 7) ^ (
 template <int kRows, bool kUp>
 __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(ProductArgs a) {
   constexpr int kSize = 32 * kRows;  // rows of a tile
-  __shared__ WideLds<kRows> lds;
+  __shared__ WideLds<kRows, kUp> lds;
   // Work-groups go round the eight XCDs: each takes a run of the work, in which an expert's
   // row tiles are neighbours and read the same columns of its weight through one L2.
   const uint32_t all = (uint32_t)(*a.tile_count * a.column_blocks), each = (all + 7) / 8;
@@ -386,7 +451,36 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
       lds.weight_scales[s][1] = (kUp ? one.scale[1] : other.scale[0])[s];
     }
   }
-  // This lane's rows' scales: of row r of all 32-row parts, a step every 32 kRows bytes.
+  if constexpr (kUp) {
+    // The rows' scales of all steps, kPer threads a row, four steps at once where they are
+    // aligned.
+    constexpr int kPer = 256 / kSize;
+    const int in = threadIdx.x / kPer;
+    const int64_t row = a.order[tile.row + (in < tile.rows ? in : tile.rows - 1)] / a.choices;
+    const uint8_t* xs = a.x_scale + row * steps;
+    uint8_t* to = &lds.scales[0][in & 31][in >> 5];
+    if ((steps & 3) == 0 && ((uintptr_t)a.x_scale & 3) == 0) {
+      uint32_t four[kMaxWideUp / 4 / kPer + 1];
+      const int part = threadIdx.x % kPer;
+#pragma unroll
+      for (int i = 0; i < kMaxWideUp / 4 / kPer + 1; ++i)
+        if (4 * kPer * i < steps) {
+          const int s = 4 * (kPer * i + part);
+          four[i] = *reinterpret_cast<const uint32_t*>(xs + (s < steps ? s : 0));
+        }
+#pragma unroll
+      for (int i = 0; i < kMaxWideUp / 4 / kPer + 1; ++i) {
+        const int s = 4 * (kPer * i + part);
+        if (4 * kPer * i < steps && s < steps) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) to[(s + k) * kSize] = (uint8_t)(four[i] >> (8 * k));
+        }
+      }
+    } else {
+      for (int s = threadIdx.x % kPer; s < steps; s += kPer) to[s * kSize] = xs[s];
+    }
+  }
+  // Down: this lane's rows' scales, of row r of all 32-row parts, a step every 32 kRows bytes.
   const uint8_t* row_scales = a.x_scale + (int64_t)tile_at * steps * kSize + r * kRows;
   wait_loads<0>();
   lds_barrier();
@@ -402,7 +496,10 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
     return joined(lds_load<v4u>(at + from), lds_load<v4u>((at ^ 16) + from));
   };
   typedef uint32_t RowScales __attribute__((ext_vector_type(kRows / 4)));
-  auto scales_of = [&](int s) { return *reinterpret_cast<const RowScales*>(row_scales + s * kSize); };
+  auto scales_of = [&](int s) {
+    if constexpr (kUp) return *reinterpret_cast<const RowScales*>(&lds.scales[s][r][0]);
+    else return *reinterpret_cast<const RowScales*>(row_scales + s * kSize);
+  };
   auto weight_scales_of = [&](int s) {
     const uint32_t both = *reinterpret_cast<const uint16_t*>(&lds.weight_scales[s][0]);
     return kUp ? both : both >> (wave >> 1 << 3);
@@ -445,7 +542,7 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (q == kRows) {
         // This wave's rows of the next step have come, and everyone's.
-        wait_loads<kLoads + 9>();
+        wait_loads<kLoads + (kUp ? 8 : 9)>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -519,29 +616,6 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
   }
 }
 
-// The scales of up's rows as the wide kernel reads them: [tile][step][32][kRows], a row's
-// part of 32 last, so that a lane's are one read. (What a work-group of it would fetch into
-// LDS byte by byte before its first product.)
-template <int kRows>
-__global__ __launch_bounds__(256) void tile_scales(ProductArgs a, uint8_t* out, int steps, int chunks) {
-  constexpr int kSize = 32 * kRows, kSteps = 16;
-  __shared__ __align__(16) uint8_t part[kSteps][kSize];
-  const int tile_at = blockIdx.x / chunks, first = (int)(blockIdx.x % chunks) * kSteps;
-  if (tile_at >= *a.tile_count) return;
-  const Tile tile = a.tiles[tile_at];
-  const int in = threadIdx.x % kSize;
-  const int64_t row = a.order[tile.row + (in < tile.rows ? in : tile.rows - 1)] / a.choices;
-  const uint8_t* from = a.x_scale + row * steps + first;
-#pragma unroll
-  for (int k = threadIdx.x / kSize; k < kSteps; k += 256 / kSize)
-    if (first + k < steps) part[k][(in & 31) * kRows + (in >> 5)] = from[k];
-  __syncthreads();
-  const int at = threadIdx.x * 16;
-  if (at < kSteps * kSize && first + at / kSize < steps)
-    *reinterpret_cast<uint4*>(out + ((int64_t)tile_at * steps + first) * kSize + at) =
-        *reinterpret_cast<const uint4*>(&part[0][0] + at);
-}
-
 // --------------------------------------------------------------- 4. join --
 struct JoinArgs {
   const int32_t* ids;
@@ -571,16 +645,32 @@ __global__ __launch_bounds__(256) void join_choices(JoinArgs a) {
   const int column = ((int)(blockIdx.x % a.groups_per_token) * 256 + (int)threadIdx.x) * 8;
   if (column >= a.dim) return;
   float sum[8] = {};
-  for (int c = 0; c < a.choices; ++c) {
-    const int64_t pair = token * a.choices + c;
-    if ((uint32_t)a.ids[pair] - (uint32_t)a.first >= (uint32_t)a.experts) continue;
-    const int64_t row = a.place[pair];
-    const float weight = a.weights[pair];
-    const v8hf y = *reinterpret_cast<const v8hf*>(a.y + row * a.dim + column);
-    const uint32_t power = a.powers[row * (a.dim / kWaveCols) + column / kWaveCols];
-    const float unit = __uint_as_float((power - 14u) << 23);
+  // (All loads of a few choices are on their way before the first is used.)
+  constexpr int kAtOnce = 8;
+  for (int c0 = 0; c0 < a.choices; c0 += kAtOnce) {
+    v8hf y[kAtOnce];
+    float weight[kAtOnce];
+    uint32_t power[kAtOnce];
+    bool here[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += (float)y[i] * unit * weight;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int c = c0 + i < a.choices ? c0 + i : a.choices - 1;
+      const int64_t pair = token * a.choices + c;
+      here[i] = c0 + i < a.choices && (uint32_t)a.ids[pair] - (uint32_t)a.first < (uint32_t)a.experts;
+      weight[i] = a.weights[pair];
+      if (here[i]) {
+        const int64_t row = a.place[pair];
+        y[i] = *reinterpret_cast<const v8hf*>(a.y + row * a.dim + column);
+        power[i] = a.powers[row * (a.dim / kWaveCols) + column / kWaveCols];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (!here[i]) continue;
+      const float unit = __uint_as_float((power[i] - 14u) << 23);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += (float)y[i][j] * unit * weight[i];
+    }
   }
   Eight out;
 #pragma unroll
@@ -588,20 +678,197 @@ __global__ __launch_bounds__(256) void join_choices(JoinArgs a) {
   *reinterpret_cast<Eight*>(static_cast<T*>(a.out) + token * a.dim + column) = out;
 }
 
+// ------------------------------------------------------------- one by one --
+// With so few tokens that an expert seldom has two, each pair by itself: no groups, and the
+// results weighted and summed where they are formed. Two launches instead of four.
+struct PairArgs {
+  const uint8_t* x;
+  const uint8_t* x_scale;
+  const int32_t* ids;
+  const float* weights;
+  const uint8_t* w;        // gate and up; down
+  const uint8_t* w_scale;
+  float* hidden;           // [pairs, inner]
+  void* out;
+  int32_t dim, inner, choices, first, experts, blocks, parts;
+};
+
+// up: a work-group takes 32 columns of h, a quarter of the depth a wave.
+__global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
+  constexpr int kDepth = 3;
+  __shared__ float part[4][4][16];
+  const int pair = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+  const uint32_t expert = (uint32_t)a.ids[pair] - (uint32_t)a.first;
+  if (expert >= (uint32_t)a.experts) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
+  const int steps = a.dim / kBlock, begin = steps * wave / 4, end = steps * (wave + 1) / 4;
+  const int64_t token = pair / a.choices;
+  const uint8_t* w = a.w + ((int64_t)expert * (a.inner / 8) + block * 4) * steps * kTile + lane * 16;
+  const uint8_t* gate = a.w_scale + ((int64_t)expert * (a.inner / 64) + block / 4) * steps;
+  const uint8_t* up = gate + (int64_t)(a.inner / kBlock) * steps;
+  const uint8_t* x = a.x + token * a.dim + g * 16;
+  const uint8_t* xs = a.x_scale + token * steps;
+  Step<1> ring[kDepth];
+  auto load = [&](Step<1>& to, int s) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) to.w[t] = load_weight(w, steps, t, s);
+    to.w_scale[0] = gate[s], to.w_scale[1] = up[s];
+    const v4u* from = reinterpret_cast<const v4u*>(x + s * kBlock);
+    to.x[0] = joined(from[0], from[4]);
+    to.x_scale[0] = xs[s];
+  };
+  v4f acc[4] = {};
+  if (begin < end) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) load(ring[d], begin + d < end ? begin + d : end - 1);
+    auto multiply = [&](const Step<1>& of) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[t] = product(of.w[t], of.x[0], acc[t], of.w_scale[t & 1], of.x_scale[0]);
+    };
+    int s = begin;
+    for (; s + kDepth <= end; s += kDepth) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        multiply(ring[d]);
+        load(ring[d], s + d + kDepth < end ? s + d + kDepth : end - 1);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDepth - 1; ++d)
+      if (s + d < end) multiply(ring[d]);
+  }
+  // (All 16 columns of the product are the token's.)
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) *reinterpret_cast<v4f*>(&part[wave][t][4 * g]) = acc[t];
+  }
+  __syncthreads();
+  const int c = threadIdx.x;  // column 8 g + 4 j + i of h: results 4 g + i of the tiles 2 j and 2 j + 1
+  if (c >= 32) return;
+  const int j = c >> 2 & 1, at = c >> 3 << 2 | (c & 3);
+  float gated = 0.0f, upped = 0.0f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) gated += part[v][2 * j][at], upped += part[v][2 * j + 1][at];
+  a.hidden[(int64_t)pair * a.inner + block * 32 + c] = silu(gated) * upped;
+}
+
+// down: a work-group takes a token's 32 columns: while the first weights are on their way
+// it forms the codes of all choices' h, then a wave takes a choice's part of the depth after
+// another: the products, and the weight.
+constexpr int kPairCodes = 65536;
+template <typename T>
+__global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
+  constexpr int kDepth = 4;
+  __shared__ __align__(16) uint8_t codes[kPairCodes];
+  __shared__ uint8_t scales[kPairCodes / kBlock];
+  __shared__ float part[16][2][16];
+  const int64_t token = blockIdx.x / a.blocks;
+  const int block = blockIdx.x % a.blocks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
+  const int steps = a.inner / kBlock, units = a.choices * a.parts, waves = blockDim.x >> 6;
+  struct {
+    v8i w[2];
+    uint32_t scale;
+  } ring[kDepth];
+  const uint8_t* w = nullptr;
+  const uint8_t* ws = nullptr;
+  auto load = [&](auto& to, int s) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) to.w[t] = load_weight(w, steps, t, s);
+    to.scale = ws[s];
+  };
+  // A unit's expert (past the last: none) and its first weights.
+  int begin = 0, end = 0;
+  auto start = [&](int u) {
+    if (u >= units) return false;
+    const uint32_t expert = (uint32_t)a.ids[token * a.choices + u / a.parts] - (uint32_t)a.first;
+    if (expert >= (uint32_t)a.experts) return false;
+    const int at = u % a.parts;
+    begin = steps * at / a.parts, end = steps * (at + 1) / a.parts;
+    w = a.w + ((int64_t)expert * (a.dim / 16) + block * 2) * steps * kTile + lane * 16;
+    ws = a.w_scale + ((int64_t)expert * (a.dim / kBlock) + block / 4) * steps;
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) load(ring[d], begin + d < end ? begin + d : end - 1);
+    return true;
+  };
+  bool some = start(wave);
+
+  // 16 lanes a block of 128. (Of choices that are not here: what memory held, and not used.)
+  for (int i = threadIdx.x >> 4; i < a.choices * steps; i += blockDim.x >> 4) {
+    const float4* from = reinterpret_cast<const float4*>(a.hidden + token * a.choices * a.inner + i * kBlock + (threadIdx.x & 15) * 8);
+    const float4 one = from[0], two = from[1];
+    const float v[8] = {one.x, one.y, one.z, one.w, two.x, two.y, two.z, two.w};
+    uint32_t top = 0, lo, hi;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    const float scale = scale_from_amax_bits(max_abs_bits_reduce<16>(top), true);
+    quantize_eight(v, scale, true, lo, hi);
+    *reinterpret_cast<uint2*>(&codes[i * kBlock + (threadIdx.x & 15) * 8]) = make_uint2(lo, hi);
+    if ((threadIdx.x & 15) == 0) scales[i] = (uint8_t)(__float_as_uint(scale) >> 23);
+  }
+  __syncthreads();
+
+  v4f total[2] = {};
+  for (int u = wave; u < units; u += waves) {
+    if (u > wave) some = start(u);
+    if (!some) continue;
+    const int choice = u / a.parts;
+    v4f acc[2] = {};
+    for (int s = begin; s < end; s += kDepth) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        if (s + d >= end) break;
+        const v4u* x = reinterpret_cast<const v4u*>(&codes[(choice * steps + s + d) * kBlock + g * 16]);
+        const v8i of = joined(x[0], x[4]);
+        const uint32_t x_scale = scales[choice * steps + s + d];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[t] = product(ring[d].w[t], of, acc[t], ring[d].scale, x_scale);
+        load(ring[d], s + d + kDepth < end ? s + d + kDepth : end - 1);
+      }
+    }
+    const float weight = a.weights[token * a.choices + choice];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[t][i] += acc[t][i] * weight;
+  }
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) *reinterpret_cast<v4f*>(&part[wave][t][4 * g]) = total[t];
+  }
+  __syncthreads();
+  const int c = threadIdx.x;  // result 4 g + i of tile t: column 16 g + 4 t + i of 64, t 0 and 1 or 2 and 3
+  if (c >= 32) return;
+  const int t = c >> 2 & 1, at = c >> 3 << 2 | (c & 3);
+  float sum = 0.0f;
+  for (int v = 0; v < waves; ++v) sum += part[v][t][at];
+  static_cast<T*>(a.out)[token * a.dim + block / 2 * 64 + (c >> 3) * 16 + (block & 1) * 8 + t * 4 + (c & 3)] = rounded<T>(sum);
+}
+
 // ----------------------------------------------------------------- calls --
 struct Plan {
   int64_t pairs, tiles;       // of the longest call, and its row tiles at most
-  int rows;                   // 16-row parts of a tile
+  int rows;                   // 16-row parts of a tile; 0: each pair by itself
+  int parts;                  // of the depth of a pair's down
   // Offsets of the workspace's parts.
-  int64_t count, list, order, place, row_scales, codes, scales, y, powers, bytes;
+  int64_t count, list, order, place, codes, scales, y, powers, bytes;
 };
 
 Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_t experts, int64_t total) {
   Plan p{};
   p.pairs = tokens * choices;
+  // Pair by pair up to three quarters as many pairs as experts (32 experts, 8 choices: 1 token
+  // 80 -> 68 us, 3 182 -> 172, 4 would be 187 -> 219), where a token's codes fit into LDS.
+  if (p.pairs <= (total * 3 / 4 > choices ? total * 3 / 4 : choices) && choices * inner <= kPairCodes) {
+    p.parts = (int)(choices >= 16 ? 1 : 16 / choices);
+    if (p.parts > inner / kBlock) p.parts = (int)(inner / kBlock);
+    p.bytes = p.pairs * inner * 4;
+    return p;
+  }
   // Rows of an expert, on average; tiles of about twice that.
   const int64_t mean = p.pairs / total;
   p.rows = mean <= 6 ? 1 : mean <= 16 ? 2 : mean <= 40 ? 4 : mean <= 128 ? 8 : 16;
+  if (dim > kMaxWideUp * kBlock && p.rows > 4) p.rows = 4;
   const int64_t size = 16 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;
@@ -616,9 +883,8 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   p.order = part(p.pairs * 4);
   p.place = part(p.pairs * 4);
   p.codes = part(p.pairs * inner);
-  // Scales of rows; of tiles in the wide kernels.
+  // (Scales of rows; of whole tiles in the wide kernels.)
   const int64_t rows = p.rows >= 8 ? p.tiles * size : p.pairs;
-  p.row_scales = part(p.rows >= 8 ? rows * (dim / kBlock) : 0);
   p.scales = part(rows * (inner / kBlock));
   p.y = part(p.pairs * dim * 2);
   p.powers = part(p.pairs * (dim / kWaveCols));
@@ -680,6 +946,28 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   const Plan p = plan_of(tokens, choices, dim, inner, experts, total);
   DSA_CHECK_ARG(workspace_bytes >= p.bytes, "workspace of %lld bytes is smaller than the %lld needed",
                 (long long)workspace_bytes, (long long)p.bytes);
+  if (p.rows == 0) {
+    PairArgs one{};
+    one.x = static_cast<const uint8_t*>(x), one.x_scale = static_cast<const uint8_t*>(x_scale);
+    one.ids = ids, one.weights = weights, one.hidden = static_cast<float*>(workspace), one.out = out;
+    one.dim = (int32_t)dim, one.inner = (int32_t)inner, one.choices = (int32_t)choices;
+    one.first = (int32_t)first, one.experts = (int32_t)experts, one.parts = p.parts;
+    one.w = static_cast<const uint8_t*>(gate_up), one.w_scale = static_cast<const uint8_t*>(gate_up_scale);
+    one.blocks = (int32_t)(inner / 32);
+    hipLaunchKernelGGL(pair_hidden, dim3((unsigned)(p.pairs * one.blocks)), dim3(256), 0, stream, one);
+    DSA_CHECK_LAUNCH("hidden values of pairs");
+    one.w = static_cast<const uint8_t*>(down), one.w_scale = static_cast<const uint8_t*>(down_scale);
+    one.blocks = (int32_t)(dim / 32);
+    const int units = (int)choices * p.parts, threads = 64 * (units < 16 ? units : 16);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * one.blocks)), dim3(threads), 0, stream, one);
+    };
+    if (dtype == DSA_DTYPE_BF16) go(pair_result<Bf16Bits>);
+    else if (dtype == DSA_DTYPE_F16) go(pair_result<_Float16>);
+    else go(pair_result<float>);
+    DSA_CHECK_LAUNCH("results of pairs");
+    return kOk;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Tile* tiles = reinterpret_cast<Tile*>(ws + p.list);
   int32_t* count = reinterpret_cast<int32_t*>(ws + p.count);
@@ -709,20 +997,16 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
                 "too many tokens for one launch");
 
   const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 16 * p.rows};
-  hipLaunchKernelGGL(group_pairs, dim3((unsigned)experts), dim3(kGroupThreads), 0, stream, group);
+  // (A wave for every 256 pairs, up to 16: with fewer the work-groups start and meet sooner.)
+  const int64_t waves = (p.pairs + 255) / 256;
+  auto list = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)experts), dim3((unsigned)(waves < 16 ? 64 * waves : (int64_t)kGroupThreads)), 0,
+                       stream, group);
+  };
+  if (waves <= 16) list(group_pairs<4>);
+  else if (waves <= 32) list(group_pairs<8>);
+  else list(group_pairs<32>);
   DSA_CHECK_LAUNCH("grouping of pairs");
-  if (p.rows >= 8) {
-    uint8_t* tiled = ws + p.row_scales;
-    const int steps = (int)(dim / kBlock), chunks = (steps + 15) / 16;
-    DSA_CHECK_ARG(grid_fits(p.tiles * chunks, 256), "too many tokens for one launch");
-    auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * chunks)), dim3(256), 0, stream, up, tiled, steps, chunks);
-    };
-    if (p.rows == 8) go(tile_scales<4>);
-    else go(tile_scales<8>);
-    DSA_CHECK_LAUNCH("scales of tiles");
-    up.x_scale = tiled;
-  }
   if (const int status = launch_product<true>(up, p, stream)) return status;
   if (const int status = launch_product<false>(dn, p, stream)) return status;
   auto join = [&](auto kernel) {
