@@ -48,9 +48,9 @@ __device__ __forceinline__ v4f product(v8i w, v8i x, v4f c, uint32_t w_scale, ui
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
 }
 
-// The wide kernels' form: 32 rows of a weight by 32 tokens, 64 values deep. Half as many
-// instructions for the same work: one wave a SIMD cannot keep the unit busy with the other
-// (45 clocks an instruction where the unit needs 32; 70 of 64 here).
+// Row tiles take the form of 32 rows of a weight by 32 tokens, 64 values deep: half as many
+// instructions for the same work (one wave a SIMD issues the other in 45 clocks where the
+// unit needs 32, this in 70 of 64).
 template <int kW, int kX>
 __device__ __forceinline__ v16f product32(v8i w, v8i x, v16f c, uint32_t w_scale, uint32_t x_scale) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
@@ -243,125 +243,7 @@ __device__ __forceinline__ v8i load_weight(const uint8_t* codes, int steps, int 
   return joined(from[0], from[64]);
 }
 
-// What a wave's products of one step need: 64 rows of a weight, kRows 16-row tiles of codes,
-// and their scales.
-template <int kRows>
-struct Step {
-  v8i w[4], x[kRows];
-  uint32_t w_scale[2], x_scale[kRows];
-};
-
-// Few rows: kRows 16-row tiles by 4 waves of 64 columns, every wave streaming its own part
-// of the weight, and the tokens' codes, through registers, kDepth steps at once. What bounds
-// it is reading the weight: 8 KB a step, and a CU wants some 40 KB under way.
-template <int kRows, bool kUp>
-__global__ __launch_bounds__(256, 2) void expert_product(ProductArgs a) {
-  constexpr int kDepth = kRows <= 2 ? 3 : 2;
-  const int tile_at = blockIdx.x / a.column_blocks, block = blockIdx.x % a.column_blocks;
-  if (tile_at >= *a.tile_count) return;
-  const Tile tile = a.tiles[tile_at];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int column = block * 256 + wave * kWaveCols;  // of the packed weight
-  const int steps = a.depth / kBlock;
-  __shared__ uint32_t amax[kUp ? 4 * 16 * kRows : 1];
-
-  const WaveWeight w = weight_of<kUp>(a, tile.expert, block, column, steps);
-  const uint8_t* x[kRows];
-  const uint8_t* xs[kRows];
-  Step<kRows> ring[kDepth];
-  auto load_w = [&](Step<kRows>& to, int s) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) to.w[t] = load_weight(w.codes, steps, t, s);
-    to.w_scale[0] = w.scale[0][s];
-    if constexpr (kUp) to.w_scale[1] = w.scale[1][s];
-  };
-  auto load_x = [&](Step<kRows>& to, int s) {
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      const v4u* from = reinterpret_cast<const v4u*>(x[m] + s * kBlock);
-      to.x[m] = joined(from[0], from[4]);
-      to.x_scale[m] = xs[m][s];
-    }
-  };
-  // (The weight first: its rows do not wait for the tokens' indices.)
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) load_w(ring[d], d < steps ? d : steps - 1);
-#pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    const int in = 16 * m + r;
-    int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
-    if constexpr (kUp) row = a.order[row] / a.choices;
-    x[m] = a.x + row * a.depth + g * 16;
-    xs[m] = a.x_scale + row * steps;
-  }
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) load_x(ring[d], d < steps ? d : steps - 1);
-
-  v4f acc[kRows][4] = {};
-  auto multiply = [&](const Step<kRows>& of) {
-#pragma unroll
-    for (int m = 0; m < kRows; ++m)
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        acc[m][t] = product(of.w[t], of.x[m], acc[m][t], of.w_scale[kUp ? t & 1 : 0], of.x_scale[m]);
-  };
-  int s = 0;
-  for (; s + kDepth <= steps; s += kDepth) {
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      multiply(ring[d]);
-      // (At the end the last step comes again, from the nearest cache.)
-      const int next = s + d + kDepth < steps ? s + d + kDepth : steps - 1;
-      load_w(ring[d], next);
-      load_x(ring[d], next);
-    }
-  }
-#pragma unroll
-  for (int d = 0; d < kDepth - 1; ++d)
-    if (s + d < steps) multiply(ring[d]);
-  if constexpr (kUp) {
-    const int64_t inner = a.columns / 2;
-    float h[kRows][8];
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      const uint32_t top = max_over_groups(hidden(h[m], [&](int i) { return acc[m][i >> 2 << 1][i & 3]; },
-                                                  [&](int i) { return acc[m][(i >> 2 << 1) + 1][i & 3]; }));
-      if (g == 0) amax[(wave * kRows + m) * 16 + r] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const uint32_t of = amax[(v * kRows + m) * 16 + r];
-        top = top > of ? top : of;
-      }
-      const float scale = scale_from_amax_bits(top, true);
-      if (16 * m + r >= tile.rows) continue;
-      const int64_t row = tile.row + 16 * m + r;
-      uint32_t lo, hi;
-      quantize_eight(h[m], scale, true, lo, hi);
-      *reinterpret_cast<uint2*>(a.codes + row * inner + block * 128 + wave * 32 + 8 * g) = make_uint2(lo, hi);
-      if (wave == 0 && g == 0) a.scales[row * (inner / kBlock) + block] = (uint8_t)(__float_as_uint(scale) >> 23);
-    }
-  } else {
-#pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-      auto value = [&](int i) { return acc[m][i >> 2][i & 3]; };
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = finite_max(top, value(i));
-      const Power power = power_of(max_over_groups(top));
-      if (column >= a.columns || 16 * m + r >= tile.rows) continue;
-      const int64_t row = tile.row + 16 * m + r;
-      store_sixteen(a.y + row * a.columns + column + 16 * g, power.factor, value);
-      if (g == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power.exponent;
-    }
-  }
-}
-
-// Many rows: 32 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
+// Row tiles: 32 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
 // registers, a step ahead; the rows' codes go into LDS straight from memory (two steps
 // ahead, four buffers), where all four waves read them, three operands ahead of their
 // products. Half-way through a step the waves meet: from there on the next step's rows may
@@ -371,12 +253,14 @@ __global__ __launch_bounds__(256, 2) void expert_product(ProductArgs a) {
 // from memory a step ahead, where up has put them by tile.
 // Per step of 128 a CU's matrix units take 256 kRows clocks, its LDS 160 kRows (four waves'
 // reads and one write of 4 kRows KB at 128 bytes).
-constexpr int kMaxWideSteps = 256, kMaxWideUp = 124;  // steps; steps of up, whose scales LDS holds
+constexpr int kMaxSteps = 256;
+// Steps of up whose rows' scales LDS holds (of 128 rows with two work-groups a CU).
+constexpr int max_up_steps(int rows) { return rows <= 2 ? kMaxSteps : 124; }
 template <int kRows, bool kUp>
-struct WideLds {
+struct TileLds {
   alignas(16) uint8_t rows[4][32 * kRows * kBlock];
-  alignas(16) uint8_t scales[kUp ? kMaxWideUp : 1][32][kRows];  // (a row's part of 32 last: one read holds all)
-  alignas(4) uint8_t weight_scales[kUp ? kMaxWideUp : kMaxWideSteps][2];
+  alignas(16) uint8_t scales[kUp ? max_up_steps(kRows) : 1][32][kRows];  // (a row's part of 32 last: one read holds all)
+  alignas(4) uint8_t weight_scales[kUp ? max_up_steps(kRows) : kMaxSteps][2];
 };
 
 // The wave's weight tiles as two operands of 32 rows (up: gate's and up's), 64 deep: half k
@@ -393,9 +277,9 @@ __device__ __forceinline__ v8i load_weight32(const uint8_t* codes, int64_t tile,
 __device__ __forceinline__ uint32_t turn_of(uint32_t row) { return (row & 7) ^ (row >> 4 & 1); }
 
 template <int kRows, bool kUp>
-__global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(ProductArgs a) {
+__global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expert_product(ProductArgs a) {
   constexpr int kSize = 32 * kRows;  // rows of a tile
-  __shared__ WideLds<kRows, kUp> lds;
+  __shared__ TileLds<kRows, kUp> lds;
   // Work-groups go round the eight XCDs: each takes a run of the work, in which an expert's
   // row tiles are neighbours and read the same columns of its weight through one L2.
   const uint32_t all = (uint32_t)(*a.tile_count * a.column_blocks), each = (all + 7) / 8;
@@ -460,16 +344,16 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
     const uint8_t* xs = a.x_scale + row * steps;
     uint8_t* to = &lds.scales[0][in & 31][in >> 5];
     if ((steps & 3) == 0 && ((uintptr_t)a.x_scale & 3) == 0) {
-      uint32_t four[kMaxWideUp / 4 / kPer + 1];
+      uint32_t four[max_up_steps(kRows) / 4 / kPer + 1];
       const int part = threadIdx.x % kPer;
 #pragma unroll
-      for (int i = 0; i < kMaxWideUp / 4 / kPer + 1; ++i)
+      for (int i = 0; i < max_up_steps(kRows) / 4 / kPer + 1; ++i)
         if (4 * kPer * i < steps) {
           const int s = 4 * (kPer * i + part);
           four[i] = *reinterpret_cast<const uint32_t*>(xs + (s < steps ? s : 0));
         }
 #pragma unroll
-      for (int i = 0; i < kMaxWideUp / 4 / kPer + 1; ++i) {
+      for (int i = 0; i < max_up_steps(kRows) / 4 / kPer + 1; ++i) {
         const int s = 4 * (kPer * i + part);
         if (4 * kPer * i < steps && s < steps) {
 #pragma unroll
@@ -487,18 +371,19 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
 
   // Part m, half k of a step: a lane's two 16-byte parts of row r are 4 k + 2 h and the next.
   const uint32_t lane_at = lds_rows + r * kBlock + (((2 * h) ^ turn_of(r)) << 4);
-  // Operands in registers: those ahead of the products hide the LDS.
-  constexpr int kRing = kRows <= 4 ? 2 : 4, kAhead = kRing - 1, kParts = 2 * kRows;
+  // Operands in registers: the one ahead of the products, with the SIMD's other waves, hides
+  // the LDS.
+  constexpr int kRing = 2, kAhead = 1, kParts = 2 * kRows;
   v8i x[kRing];
   auto read = [&](uint32_t buffer, int q) {
     const uint32_t from = buffer * (kSize * kBlock) + (q % kRows) * 32 * kBlock;
     const uint32_t at = q < kRows ? lane_at : lane_at ^ 64;
     return joined(lds_load<v4u>(at + from), lds_load<v4u>((at ^ 16) + from));
   };
-  typedef uint32_t RowScales __attribute__((ext_vector_type(kRows / 4)));
+  using RowScales = std::conditional_t<kRows == 1, uint8_t, std::conditional_t<kRows == 2, uint16_t, uint32_t>>;
   auto scales_of = [&](int s) {
-    if constexpr (kUp) return *reinterpret_cast<const RowScales*>(&lds.scales[s][r][0]);
-    else return *reinterpret_cast<const RowScales*>(row_scales + s * kSize);
+    const uint8_t* at = kUp ? &lds.scales[kUp ? s : 0][r][0] : row_scales + s * kSize;
+    return (uint32_t)*reinterpret_cast<const RowScales*>(at);
   };
   auto weight_scales_of = [&](int s) {
     const uint32_t both = *reinterpret_cast<const uint16_t*>(&lds.weight_scales[s][0]);
@@ -506,7 +391,7 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
   };
 #pragma unroll
   for (int q = 0; q < kAhead; ++q) x[q] = read(0, q);
-  RowScales xs = scales_of(0);
+  uint32_t xs = scales_of(0);
   uint32_t ws = weight_scales_of(0);
 
   v16f acc[kRows][2] = {};
@@ -515,7 +400,7 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
     const int ahead = s + 1 < steps ? s + 1 : s;
     const uint32_t on = s + 2 < steps ? kBlock : 0;
     v8i next[2][2];
-    RowScales xs_next;
+    uint32_t xs_next;
     uint32_t ws_next;
     static_for<kParts>([&](auto index) {
       constexpr int q = decltype(index)::value, m = q % kRows, k = q / kRows;
@@ -525,19 +410,20 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
       // before them would be waited for there), and a few at a time: a wave does not get on
       // while the path to L2 is full. (At the end the last rows come again, into buffers that
       // are not read.)
-      constexpr int kPer = kRows <= 4 ? 2 : 1;
       if constexpr (q == 1) {
         xs_next = scales_of(ahead);
         ws_next = weight_scales_of(ahead);
       }
-      if constexpr (q >= 1 && (q - 1) * kPer < kLoads) {
-#pragma unroll
-        for (int i = (q - 1) * kPer; i < q * kPer && i < kLoads; ++i) from[i] += on, fetch((s + 2) & 3, i);
-      }
-      if constexpr (q >= 1 && q <= 8 / kPer && q % (2 / kPer) == 0) {
-#pragma unroll
-        for (int i = (q * kPer - 2) / 2; i < q * kPer / 2; ++i)
-          next[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second + (int64_t)ahead * kTile, i >> 1);
+      constexpr int kOps = kLoads + 4, kPer = (kOps + kRows - 1) / kRows;
+      if constexpr (q >= 1 && q <= kRows) {
+        static_for<kPer>([&](auto which) {
+          constexpr int op = (q - 1) * kPer + decltype(which)::value;
+          // Rows and weights in turn while there are rows.
+          constexpr bool fetches = op < 2 * kLoads && op % 2 == 0;
+          constexpr int i = op < 2 * kLoads ? op / 2 : op - kLoads;
+          if constexpr (fetches) from[i] += on, fetch((s + 2) & 3, i);
+          else if constexpr (op < kOps) next[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second + (int64_t)ahead * kTile, i >> 1);
+        });
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (q == kRows) {
@@ -547,8 +433,8 @@ __global__ __launch_bounds__(256, kRows <= 4 ? 2 : 1) void expert_product_wide(P
         __builtin_amdgcn_sched_barrier(0);
       }
       x[(q + kAhead) % kRing] = q + kAhead < kParts ? read(s & 3, q + kAhead) : read((s + 1) & 3, q + kAhead - kParts);
-      acc[m][0] = product32<0, m & 3>(now[k][0], x[q % kRing], acc[m][0], ws, xs[m / 4]);
-      acc[m][1] = product32<kUp ? 1 : 0, m & 3>(now[k][1], x[q % kRing], acc[m][1], ws, xs[m / 4]);
+      acc[m][0] = product32<0, m>(now[k][0], x[q % kRing], acc[m][0], ws, xs);
+      acc[m][1] = product32<kUp ? 1 : 0, m>(now[k][1], x[q % kRing], acc[m][1], ws, xs);
     });
 #pragma unroll
     for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = next[i >> 1][i & 1];
@@ -693,7 +579,14 @@ struct PairArgs {
   int32_t dim, inner, choices, first, experts, blocks, parts;
 };
 
-// up: a work-group takes 32 columns of h, a quarter of the depth a wave.
+// What a wave's products of one step need: 64 rows of a weight, a token's codes, their scales.
+struct Step {
+  v8i w[4], x;
+  uint32_t w_scale[2], x_scale;
+};
+
+// up: a work-group takes 32 columns of h, a quarter of the depth a wave, three steps at once
+// (what bounds it is reading the weight: 8 KB a step, of which a CU wants some 40 under way).
 __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
   constexpr int kDepth = 3;
   __shared__ float part[4][4][16];
@@ -708,22 +601,22 @@ __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
   const uint8_t* up = gate + (int64_t)(a.inner / kBlock) * steps;
   const uint8_t* x = a.x + token * a.dim + g * 16;
   const uint8_t* xs = a.x_scale + token * steps;
-  Step<1> ring[kDepth];
-  auto load = [&](Step<1>& to, int s) {
+  Step ring[kDepth];
+  auto load = [&](Step& to, int s) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) to.w[t] = load_weight(w, steps, t, s);
     to.w_scale[0] = gate[s], to.w_scale[1] = up[s];
     const v4u* from = reinterpret_cast<const v4u*>(x + s * kBlock);
-    to.x[0] = joined(from[0], from[4]);
-    to.x_scale[0] = xs[s];
+    to.x = joined(from[0], from[4]);
+    to.x_scale = xs[s];
   };
   v4f acc[4] = {};
   if (begin < end) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) load(ring[d], begin + d < end ? begin + d : end - 1);
-    auto multiply = [&](const Step<1>& of) {
+    auto multiply = [&](const Step& of) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = product(of.w[t], of.x[0], acc[t], of.w_scale[t & 1], of.x_scale[0]);
+      for (int t = 0; t < 4; ++t) acc[t] = product(of.w[t], of.x, acc[t], of.w_scale[t & 1], of.x_scale);
     };
     int s = begin;
     for (; s + kDepth <= end; s += kDepth) {
@@ -848,7 +741,7 @@ __global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
 // ----------------------------------------------------------------- calls --
 struct Plan {
   int64_t pairs, tiles;       // of the longest call, and its row tiles at most
-  int rows;                   // 16-row parts of a tile; 0: each pair by itself
+  int rows;                   // 32-row parts of a tile; 0: each pair by itself
   int parts;                  // of the depth of a pair's down
   // Offsets of the workspace's parts.
   int64_t count, list, order, place, codes, scales, y, powers, bytes;
@@ -865,11 +758,13 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
     p.bytes = p.pairs * inner * 4;
     return p;
   }
-  // Rows of an expert, on average; tiles of about twice that.
+  // Rows of an expert, on average: tiles that most experts fill once, as long as reading the
+  // weights is what takes time (32 experts of 7,168 by 2,048 dims: 16 rows 250, 251, 254 us in
+  // tiles of 32, 64, 128; 24 rows 274, 253, 258; 48 rows 287, 261, 267; 64 rows 338, 301, 274).
   const int64_t mean = p.pairs / total;
-  p.rows = mean <= 6 ? 1 : mean <= 16 ? 2 : mean <= 40 ? 4 : mean <= 128 ? 8 : 16;
-  if (dim > kMaxWideUp * kBlock && p.rows > 4) p.rows = 4;
-  const int64_t size = 16 * p.rows;
+  p.rows = mean <= 16 ? 1 : mean <= 48 ? 2 : 4;
+  if (dim > max_up_steps(4) * kBlock && p.rows > 2) p.rows = 2;
+  const int64_t size = 32 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;
   int64_t at = 0;
@@ -883,9 +778,7 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   p.order = part(p.pairs * 4);
   p.place = part(p.pairs * 4);
   p.codes = part(p.pairs * inner);
-  // (Scales of rows; of whole tiles in the wide kernels.)
-  const int64_t rows = p.rows >= 8 ? p.tiles * size : p.pairs;
-  p.scales = part(rows * (inner / kBlock));
+  p.scales = part(p.tiles * size * (inner / kBlock));  // (of whole tiles)
   p.y = part(p.pairs * dim * 2);
   p.powers = part(p.pairs * (dim / kWaveCols));
   p.bytes = at;
@@ -907,12 +800,10 @@ int launch_product(const ProductArgs& a, const Plan& p, hipStream_t stream) {
   auto go = [&](auto kernel, int64_t groups) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, a);
   };
-  const int64_t groups = p.tiles * a.column_blocks;
+  const int64_t groups = (p.tiles * a.column_blocks + 7) / 8 * 8;
   if (p.rows == 1) go(expert_product<1, kUp>, groups);
   else if (p.rows == 2) go(expert_product<2, kUp>, groups);
-  else if (p.rows == 4) go(expert_product<4, kUp>, groups);
-  else if (p.rows == 8) go(expert_product_wide<4, kUp>, (groups + 7) / 8 * 8);
-  else go(expert_product_wide<8, kUp>, (groups + 7) / 8 * 8);
+  else go(expert_product<4, kUp>, groups);
   DSA_CHECK_LAUNCH("expert product");
   return kOk;
 }
@@ -996,7 +887,7 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
                     grid_fits(tokens * j.groups_per_token, 256),
                 "too many tokens for one launch");
 
-  const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 16 * p.rows};
+  const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 32 * p.rows};
   // (A wave for every 256 pairs, up to 16: with fewer the work-groups start and meet sooner.)
   const int64_t waves = (p.pairs + 255) / 256;
   auto list = [&](auto kernel) {
