@@ -209,18 +209,6 @@ __device__ __forceinline__ uint32_t finite_max(uint32_t top, float v) {
   const uint32_t bits = __float_as_uint(v) & 0x7FFFFFFFu;
   return bits < 0x7F800000u && bits > top ? bits : top;
 }
-// 16 neighbouring values of a row, as fp16.
-template <typename Value>
-__device__ __forceinline__ void store_sixteen(uint16_t* to, float factor, Value value) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    v4u out;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = F16::pack(value(8 * half + 2 * i) * factor, value(8 * half + 2 * i + 1) * factor);
-    reinterpret_cast<v4u*>(to)[half] = out;
-  }
-}
-
 // The parts of the weight that a wave of `column` (past the end: of the last) reads.
 struct WaveWeight {
   const uint8_t* codes;          // this lane's 16 bytes of the first tile
@@ -445,11 +433,14 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
   wait_loads<0>();
 
   // Lane (r, h) holds of row r the results 8 (i / 4) + 4 h + i % 4 of each operand: of the
-  // tiles' dealt rows two runs, one for each p = (i / 4) % 2.
+  // tiles' dealt rows two runs, one for each p = (i / 4) % 2. Results go out through LDS, so
+  // that an instruction writes whole lines (16 or 32 bytes of many rows at a time, a step's
+  // time went by at each end). Parts of 16 bytes are turned by their row again.
+  __syncthreads();
   if constexpr (kUp) {
-    __syncthreads();
     const int64_t inner = a.columns / 2;
     uint32_t* amax = reinterpret_cast<uint32_t*>(&lds.rows[0][0]);
+    const uint32_t staged = lds_rows + 4 * kSize * sizeof(uint32_t);
     float hid[kRows][2][8];
 #pragma unroll
     for (int m = 0; m < kRows; ++m) {
@@ -471,16 +462,23 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
 #pragma unroll
       for (int v = 0; v < 4; ++v) top = top > amax[v * kSize + in] ? top : amax[v * kSize + in];
       const float scale = scale_from_amax_bits(top, true);
-      if (in >= tile.rows) continue;
-      uint8_t* to = a.codes + (tile.row + in) * inner + block * 128 + wave * 32 + 8 * h;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
+        v2u out;
         uint32_t lo, hi;
         quantize_eight(hid[m][p], scale, true, lo, hi);
-        *reinterpret_cast<uint2*>(to + 16 * p) = make_uint2(lo, hi);
+        out[0] = lo, out[1] = hi;
+        lds_store(staged + in * kBlock + (((wave * 2 + p) ^ (in & 7)) << 4) + 8 * h, out);
       }
-      if (wave == 0 && h == 0)
+      if (wave == 0 && h == 0 && in < tile.rows)
         a.scales[((int64_t)tile_at * (inner / kBlock) + block) * kSize + r * kRows + m] = (uint8_t)(__float_as_uint(scale) >> 23);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int row = i * 32 + wave * 8 + (lane >> 3), part = lane & 7;
+      const v4u out = lds_load<v4u>(staged + row * kBlock + ((part ^ (row & 7)) << 4));
+      if (row < tile.rows) *reinterpret_cast<v4u*>(a.codes + (tile.row + row) * inner + block * kBlock + part * 16) = out;
     }
   } else {
 #pragma unroll
@@ -491,13 +489,30 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
       for (int i = 0; i < 32; ++i) top = finite_max(top, acc[m][i >> 4][i & 15]);
       const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
       const Power power = power_of(both[0] > both[1] ? both[0] : both[1]);
-      if (column >= a.columns || in >= tile.rows) continue;
-      const int64_t row = tile.row + in;
-      uint16_t* to = a.y + row * a.columns + column + 16 * h;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
-        store_sixteen(to + 32 * p, power.factor, [&](int i) { return acc[m][i >> 3][(i >> 2 & 1) * 8 + p * 4 + (i & 3)]; });
-      if (h == 0) a.powers[row * (a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power.exponent;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // Eight neighbours: columns 32 p + 16 h + 8 half .. of the wave's 64.
+          v4u out;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 8 * half + 2 * i, of = (at >> 2 & 1) * 8 + p * 4 + (at & 3);
+            out[i] = F16::pack(acc[m][at >> 3][of] * power.factor, acc[m][at >> 3][of + 1] * power.factor);
+          }
+          lds_store(lds_rows + in * 512 + (((wave * 8 + 4 * p + 2 * h + half) ^ r) << 4), out);
+        }
+      if (h == 0 && column < a.columns && in < tile.rows)
+        a.powers[(tile.row + in) * (int64_t)(a.columns / kWaveCols) + column / kWaveCols] = (uint8_t)power.exponent;
+    }
+    __syncthreads();
+    const int part = lane & 31;
+#pragma unroll
+    for (int i = 0; i < kSize / 8; ++i) {
+      const int row = i * 8 + wave * 2 + (lane >> 5);
+      const v4u out = lds_load<v4u>(lds_rows + row * 512 + ((part ^ (row & 31)) << 4));
+      if (row < tile.rows && block * 256 + part * 8 < a.columns)
+        *reinterpret_cast<v4u*>(a.y + (tile.row + row) * (int64_t)a.columns + block * 256 + part * 8) = out;
     }
   }
 }
