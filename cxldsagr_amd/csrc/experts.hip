@@ -57,19 +57,20 @@ __device__ __forceinline__ v16f product32(v8i w, v8i x, v16f c, uint32_t w_scale
 }
 
 // ------------------------------------------------------------ 1. groups --
+// What every tile of an expert holds alike, so that a work-group finds its own in one look.
 struct Tile {
-  int32_t expert, row, rows;
-  int32_t first, count;  // the expert's tiles
+  int32_t expert, row, rows;  // the expert's rows
+  int32_t first, count;       // and its tiles
   int32_t unused[3];
 };
 
 struct GroupArgs {
   const int32_t* ids;   // [pairs]
-  int32_t* order;       // [pairs]: the pair of a row
+  int32_t* tokens;      // [pairs]: the token of a row
   int32_t* place;       // [pairs]: the row of a pair (of this call's experts)
   Tile* tiles;
   int32_t* tile_count;
-  int32_t pairs, first, experts, tile_rows;
+  int32_t pairs, choices, first, experts, tile_rows;
 };
 
 // Work-group e lists expert e's pairs. Each counts all experts' (in LDS), so that none waits
@@ -130,11 +131,8 @@ __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
     if (w < wave) before += of_wave[w][2];
   }
   const uint32_t own = counts[expert], own_tiles = (own + a.tile_rows - 1) / a.tile_rows;
-  for (uint32_t t = threadIdx.x; t < own_tiles; t += blockDim.x) {
-    const uint32_t at = t * a.tile_rows, left = own - at;
-    a.tiles[tile + t] = Tile{(int32_t)expert, (int32_t)(row + at), (int32_t)(left < (uint32_t)a.tile_rows ? left : a.tile_rows),
-                             (int32_t)tile, (int32_t)own_tiles, {}};
-  }
+  for (uint32_t t = threadIdx.x; t < own_tiles; t += blockDim.x)
+    a.tiles[tile + t] = Tile{(int32_t)expert, (int32_t)row, (int32_t)own, (int32_t)tile, (int32_t)own_tiles, {}};
   if (expert == experts - 1 && threadIdx.x == 0) *a.tile_count = (int32_t)(tile + own_tiles);
   uint32_t next = row + before;
   for (int base = begin; base < end; base += kPart) {
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
       if (e[i] == expert) {
         const uint32_t to = next + (uint32_t)__popcll(all & ((1ull << lane) - 1));
         const int p = base + 64 * i + lane;
-        a.order[to] = p;
+        a.tokens[to] = p / a.choices;
         a.place[p] = (int32_t)to;
       }
       next += (uint32_t)__popcll(all);
@@ -158,7 +156,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_pairs(GroupArgs a) {
 struct ProductArgs {
   const uint8_t* x;        // rows of `depth` codes: tokens (up), pairs in order (down)
   const uint8_t* x_scale;  // [rows, depth / 128]
-  const int32_t* order;
+  const int32_t* tokens;   // up: of the rows
   const uint8_t* w;        // [experts][columns / 16][depth / 128][2048]
   const uint8_t* w_scale;  // [experts][columns / 128][depth / 128]
   const Tile* tiles;
@@ -167,7 +165,7 @@ struct ProductArgs {
   uint8_t* scales;
   uint16_t* y;             // down: [pairs, columns] fp16, and its powers [pairs, columns / 64]
   uint8_t* powers;
-  int32_t depth, columns, choices, column_blocks;
+  int32_t depth, columns, column_blocks;
 };
 
 __device__ __forceinline__ float silu(float g) {
@@ -275,8 +273,10 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
   if ((blockIdx.x >> 3) >= each || at >= all) return;
   Tile tile = a.tiles[at / (uint32_t)a.column_blocks];
   const uint32_t within = at - (uint32_t)(tile.first * a.column_blocks);
-  const int block = (int)(within / (uint32_t)tile.count), tile_at = tile.first + (int)(within % (uint32_t)tile.count);
-  tile = a.tiles[tile_at];
+  const int block = (int)(within / (uint32_t)tile.count), nth = (int)(within % (uint32_t)tile.count);
+  const int tile_at = tile.first + nth;
+  tile.row += nth * kSize;
+  tile.rows = min(tile.rows - nth * kSize, kSize);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int column = block * 256 + wave * kWaveCols;
@@ -288,16 +288,23 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
   const uint8_t* codes = w.codes - lane * 16 + (r >> 4) * (kUp ? 2 : 1) * tile_bytes + (h * 32 + (r & 15)) * 16;
   const int64_t second = (kUp ? 1 : 2) * tile_bytes;
 
-  // This lane's parts of the rows that its wave fetches: 8 kRows rows, eight a load.
-  constexpr int kLoads = kRows;
+  // This lane's parts of the rows that its wave fetches: 8 kRows rows, eight a load; and, of
+  // up, the row whose scales this thread lays out, kPer threads a row. (Tokens' numbers first:
+  // one way to memory and back for all.)
+  constexpr int kLoads = kRows, kPer = 256 / kSize;
+  auto row_of = [&](int in) -> int64_t {
+    const int row = tile.row + min(in, tile.rows - 1);
+    return kUp ? a.tokens[row] : row;
+  };
+  int64_t rows[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) rows[i] = row_of((wave * kLoads + i) * 8 + (lane >> 3));
+  const int scale_row = threadIdx.x / kPer;
+  const uint8_t* xs_row = kUp ? a.x_scale + row_of(scale_row) * steps : nullptr;
   uint64_t from[kLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int in = (wave * kLoads + i) * 8 + (lane >> 3);
-    int64_t row = tile.row + (in < tile.rows ? in : tile.rows - 1);
-    if constexpr (kUp) row = a.order[row] / a.choices;
-    from[i] = (uint64_t)(a.x + row * a.depth + (((lane & 7) ^ turn_of(in)) << 4));
-  }
+  for (int i = 0; i < kLoads; ++i)
+    from[i] = (uint64_t)(a.x + rows[i] * a.depth + (((lane & 7) ^ turn_of((wave * kLoads + i) * 8 + (lane >> 3))) << 4));
   const uint32_t lds_rows = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds.rows[0][0];
   auto fetch = [&](int buffer, int i) {
     const uint32_t to = lds_rows + buffer * (kSize * kBlock) + (wave * kLoads + i) * 1024;
@@ -324,13 +331,8 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
     }
   }
   if constexpr (kUp) {
-    // The rows' scales of all steps, kPer threads a row, four steps at once where they are
-    // aligned.
-    constexpr int kPer = 256 / kSize;
-    const int in = threadIdx.x / kPer;
-    const int64_t row = a.order[tile.row + (in < tile.rows ? in : tile.rows - 1)] / a.choices;
-    const uint8_t* xs = a.x_scale + row * steps;
-    uint8_t* to = &lds.scales[0][in & 31][in >> 5];
+    // The rows' scales of all steps, four at once where they are aligned.
+    uint8_t* to = &lds.scales[0][scale_row & 31][scale_row >> 5];
     if ((steps & 3) == 0 && ((uintptr_t)a.x_scale & 3) == 0) {
       uint32_t four[max_up_steps(kRows) / 4 / kPer + 1];
       const int part = threadIdx.x % kPer;
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
       for (int i = 0; i < max_up_steps(kRows) / 4 / kPer + 1; ++i)
         if (4 * kPer * i < steps) {
           const int s = 4 * (kPer * i + part);
-          four[i] = *reinterpret_cast<const uint32_t*>(xs + (s < steps ? s : 0));
+          four[i] = *reinterpret_cast<const uint32_t*>(xs_row + (s < steps ? s : 0));
         }
 #pragma unroll
       for (int i = 0; i < max_up_steps(kRows) / 4 / kPer + 1; ++i) {
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
         }
       }
     } else {
-      for (int s = threadIdx.x % kPer; s < steps; s += kPer) to[s * kSize] = xs[s];
+      for (int s = threadIdx.x % kPer; s < steps; s += kPer) to[s * kSize] = xs_row[s];
     }
   }
   // Down: this lane's rows' scales, of row r of all 32-row parts, a step every 32 kRows bytes.
@@ -759,7 +761,7 @@ struct Plan {
   int rows;                   // 32-row parts of a tile; 0: each pair by itself
   int parts;                  // of the depth of a pair's down
   // Offsets of the workspace's parts.
-  int64_t count, list, order, place, codes, scales, y, powers, bytes;
+  int64_t count, list, tokens, place, codes, scales, y, powers, bytes;
 };
 
 Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_t experts, int64_t total) {
@@ -790,7 +792,7 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   };
   p.count = part(4);
   p.list = part(p.tiles * (int64_t)sizeof(Tile));
-  p.order = part(p.pairs * 4);
+  p.tokens = part(p.pairs * 4);
   p.place = part(p.pairs * 4);
   p.codes = part(p.pairs * inner);
   p.scales = part(p.tiles * size * (inner / kBlock));  // (of whole tiles)
@@ -877,22 +879,22 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Tile* tiles = reinterpret_cast<Tile*>(ws + p.list);
   int32_t* count = reinterpret_cast<int32_t*>(ws + p.count);
-  int32_t* order = reinterpret_cast<int32_t*>(ws + p.order);
+  int32_t* row_tokens = reinterpret_cast<int32_t*>(ws + p.tokens);
   int32_t* place = reinterpret_cast<int32_t*>(ws + p.place);
 
   ProductArgs up{};
-  up.x = static_cast<const uint8_t*>(x), up.x_scale = static_cast<const uint8_t*>(x_scale), up.order = order;
+  up.x = static_cast<const uint8_t*>(x), up.x_scale = static_cast<const uint8_t*>(x_scale), up.tokens = row_tokens;
   up.w = static_cast<const uint8_t*>(gate_up), up.w_scale = static_cast<const uint8_t*>(gate_up_scale);
   up.tiles = tiles, up.tile_count = count;
   up.codes = ws + p.codes, up.scales = ws + p.scales;
-  up.depth = (int32_t)dim, up.columns = (int32_t)(2 * inner), up.choices = (int32_t)choices;
+  up.depth = (int32_t)dim, up.columns = (int32_t)(2 * inner);
   up.column_blocks = (int32_t)(inner / kBlock);
   ProductArgs dn{};
-  dn.x = up.codes, dn.x_scale = up.scales, dn.order = order;
+  dn.x = up.codes, dn.x_scale = up.scales;
   dn.w = static_cast<const uint8_t*>(down), dn.w_scale = static_cast<const uint8_t*>(down_scale);
   dn.tiles = tiles, dn.tile_count = count;
   dn.y = reinterpret_cast<uint16_t*>(ws + p.y), dn.powers = ws + p.powers;
-  dn.depth = (int32_t)inner, dn.columns = (int32_t)dim, dn.choices = (int32_t)choices;
+  dn.depth = (int32_t)inner, dn.columns = (int32_t)dim;
   dn.column_blocks = (int32_t)((dim + 255) / 256);
   JoinArgs j{};
   j.ids = ids, j.place = place, j.weights = weights, j.y = dn.y, j.powers = dn.powers, j.out = out;
@@ -902,7 +904,8 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
                     grid_fits(tokens * j.groups_per_token, 256),
                 "too many tokens for one launch");
 
-  const GroupArgs group{ids, order, place, tiles, count, (int32_t)p.pairs, (int32_t)first, (int32_t)experts, 32 * p.rows};
+  const GroupArgs group{ids, row_tokens, place, tiles, count, (int32_t)p.pairs, (int32_t)choices, (int32_t)first,
+                        (int32_t)experts, 32 * p.rows};
   // (A wave for every 256 pairs, up to 16: with fewer the work-groups start and meet sooner.)
   const int64_t waves = (p.pairs + 255) / 256;
   auto list = [&](auto kernel) {
