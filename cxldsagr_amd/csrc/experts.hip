@@ -769,7 +769,9 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   p.pairs = tokens * choices;
   // Pair by pair up to three quarters as many pairs as experts (32 experts, 8 choices: 1 token
   // 80 -> 68 us, 3 182 -> 172, 4 would be 187 -> 219), where a token's codes fit into LDS.
-  if (p.pairs <= (total * 3 / 4 > choices ? total * 3 / 4 : choices) && choices * inner <= kPairCodes) {
+  const int64_t few = total * 3 / 4 > choices ? total * 3 / 4 : choices;
+  if (p.pairs <= few && choices * inner <= kPairCodes && grid_fits(p.pairs * (inner / 32), 256) &&
+      grid_fits(tokens * (dim / 32), 1024)) {
     p.parts = (int)(choices >= 16 ? 1 : 16 / choices);
     if (p.parts > inner / kBlock) p.parts = (int)(inner / kBlock);
     p.bytes = p.pairs * inner * 4;
@@ -806,7 +808,8 @@ int check_shape(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int
   DSA_CHECK_ARG(dim >= kBlock && dim % kBlock == 0 && dim <= 32768 && inner >= kBlock && inner % kBlock == 0 &&
                     inner <= 32768,
                 "dims must be whole blocks of 128, 32768 at most");
-  DSA_CHECK_ARG(experts >= 1 && experts <= kMaxExperts && total >= experts, "experts must number 1 to %d", kMaxExperts);
+  DSA_CHECK_ARG(experts >= 1 && experts <= kMaxExperts && total >= experts && total <= (1 << 30),
+                "experts must number 1 to %d, total at least as many and at most 2^30", kMaxExperts);
   DSA_CHECK_ARG(choices >= 1 && choices <= 64, "choices must number 1 to 64");
   DSA_CHECK_ARG(tokens >= 0 && tokens <= (1 << 22), "tokens must number 0 to 2^22");
   return kOk;

@@ -74,7 +74,7 @@ __device__ __forceinline__ double reciprocal_root(double v) {
 // i / threads. A work-group goes from row to row with the weight in registers and the next
 // row on its way.
 template <typename T, int kItems>
-__global__ __launch_bounds__(kThreads, kItems <= 2 ? 4 : 2) void residual_rms_norm(NormArgs a) {
+__global__ __launch_bounds__(kThreads, kItems * sizeof(T) <= 4 ? 4 : 2) void residual_rms_norm(NormArgs a) {
   using Item = Pack<T, 8>;
   __shared__ double shared[2][kThreads / 64];
   const int threads = blockDim.x, items = a.dim / 8;

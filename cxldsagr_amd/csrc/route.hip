@@ -293,7 +293,7 @@ extern "C" int dsa_route_experts(const void* logits, int64_t stride, int dtype, 
   DSA_CHECK_ARG(k >= 1 && k <= kMaxChoices && k <= top_groups * (experts / groups),
                 "k must be 1 to %d and within the experts of top_groups groups", kMaxChoices);
   DSA_CHECK_ARG(__builtin_isfinite((float)scale), "scale must be finite");
-  DSA_CHECK_ARG(grid_fits(tokens, 64), "too many tokens for one launch");
+  DSA_CHECK_ARG(tokens <= (1ll << 40) && grid_fits((tokens + 3) / 4, kThreads), "too many tokens for one launch");
   if (tokens == 0) return kOk;
   DSA_CHECK_ARG(logits && weights && ids, "null pointer");
   RouteArgs a{};

@@ -247,12 +247,12 @@ class ExpertWeights:
         tensors = (gate_up, gate_up_scale, down, down_scale)
         if any(t.device != down.device for t in tensors):
             raise ValueError("weights and scales must be on the same device")
-        if type(first) is not int or not 0 <= first <= 1 << 30:
+        if type(first) is not int or first < 0:
             raise ValueError("first must be a nonnegative integer")
         if total is None:
             total = first + experts
-        if type(total) is not int or total < first + experts:
-            raise ValueError("total must be at least first + E")
+        if type(total) is not int or not first + experts <= total <= 1 << 30:
+            raise ValueError("total must be at least first + E, at most 2^30")
         blocks, inner_blocks = dim // SCALE_BLOCK, inner // SCALE_BLOCK
         self.gate_up_scale = _exponents(gate_up_scale, (experts, 2 * inner_blocks, blocks),
                                         "gate_up_scale")

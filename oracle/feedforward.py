@@ -123,20 +123,23 @@ def expert_mlp(x, x_scale, gate_up, gate_up_scale, down, down_scale, ids, weight
     def sums(n):
         return 2 * (n + 2) * 2.0 ** -24
 
+    def terms(weight):  # (those that are not 0)
+        return int((weight != 0).sum(1).max())
+
     for e in range(len(wg)):
         token, choice = (ids.cpu() == e + first).nonzero(as_tuple=True)
         if not len(token):
             continue
         both, size = rows[token] @ wg[e].t(), rows[token].abs() @ wg[e].abs().t()
         gate, up = both[:, :inner], both[:, inner:]
-        off = sums(rows.shape[1]) * size
+        off = sums(terms(wg[e])) * size
         hidden = silu(gate) * up
         # (silu's slope is at most 1.1.)
         off = 1.1 * off[:, :inner] * (up.abs() + off[:, inner:]) + silu(gate).abs() * off[:, inner:]
         off = off + hidden.abs() * 2.0 ** -16 + 2.0 ** -126 * (1 + up.abs())
         hidden, moved = quantized(hidden, off)
         y, reach = hidden @ wd[e].t(), (hidden.abs() + moved) @ wd[e].abs().t()
-        inexact = moved @ wd[e].abs().t() + sums(inner) * reach
+        inexact = moved @ wd[e].abs().t() + sums(terms(wd[e])) * reach
         held = (y.abs() + inexact).view(len(token), -1, 64)
         held = (held * 2.0 ** -11 + held.amax(-1, keepdim=True) * 2.0 ** -38 + 2.0 ** -136).view(len(token), dim)
         w = weights[token, choice][:, None]

@@ -102,6 +102,7 @@ def _parts(**change):
         (dict(down_scale=z(2, 2, 1)), "e8m0 or FP32"),
         (dict(first=-1), "first"),
         (dict(first=4, total=5), "total"),
+        (dict(total=(1 << 30) + 1), "total"),
     ],
 )
 def test_weights(change, message):
@@ -206,6 +207,8 @@ def test_c_norm(args, message):
         ((0, 8, 0, 4, 8, 5, 0, 0, 2, 1, 1, 1.0, 0, 0), "k must"),
         ((0, 8, 0, 4, 8, 2, 0, 0, 1, 1, 1, float("inf"), 0, 0), "scale"),
         ((0, 8, 0, 1 << 31, 8, 2, 0, 0, 1, 1, 1, 1.0, 16, 16), "too many tokens"),
+        ((0, 8, 0, (1 << 26) - 1, 8, 2, 0, 0, 1, 1, 1, 1.0, 16, 16), "too many tokens"),
+        ((0, 8, 0, 1 << 62, 8, 2, 0, 0, 1, 1, 1, 1.0, 16, 16), "too many tokens"),
         ((0, 8, 0, 4, 8, 2, 0, 0, 1, 1, 1, 1.0, 16, 16), "null pointer"),
     ],
 )
@@ -220,6 +223,7 @@ def test_c_experts():
     _native.call(query, 0, 8, 256, 128, 4, 4, ctypes.byref(size))
     for args, message in [((4, 8, 100, 128, 4, 4), "whole blocks"), ((4, 8, 256, 0, 4, 4), "whole blocks"),
                           ((4, 8, 256, 128, 0, 4), "experts must"), ((4, 8, 256, 128, 4, 3), "experts must"),
+                          ((4, 8, 256, 128, 4, 1 << 31), "experts must"),
                           ((4, 65, 256, 128, 4, 4), "choices"), ((4, 0, 256, 128, 4, 4), "choices"),
                           ((-1, 8, 256, 128, 4, 4), "tokens"), (((1 << 22) + 1, 8, 256, 128, 4, 4), "tokens")]:
         with pytest.raises(ValueError, match=message):

@@ -18,9 +18,15 @@ def tokens_in_codes(gen, tokens, dim):
 
 
 def matrix(gen, experts, rows, columns):
-    codes = (torch.randn(experts, rows, columns, generator=gen) * 60).to(F8)
+    codes = torch.randn(experts, rows, columns, generator=gen) * 60
+    if columns > 8192:
+        # One of 64 columns, any in a block: a sum of as many terms as a shallow one's.
+        at = torch.randint(0, 64, (1, 1, columns // 64, 1), generator=gen)
+        codes = torch.where(torch.arange(64) == at, codes.view(experts, rows, -1, 64), 0).view(experts, rows, columns)
+    codes = codes.to(F8)
     scale = torch.exp2(torch.randint(-2, 2, (experts, rows // 128, columns // 128), generator=gen).float())
-    return codes, scale / 64 * 2.0 ** -round(torch.tensor(columns).double().log2().item() / 2)
+    terms = columns if columns <= 8192 else columns // 64
+    return codes, scale / 64 * 2.0 ** -round(torch.tensor(terms).double().log2().item() / 2)
 
 
 class Model:
@@ -71,13 +77,27 @@ def test_sizes(gpu, tokens, choices, dim, inner, experts):
     model.check(*model.tokens(tokens, choices, 0, experts))
 
 
-@pytest.mark.parametrize("rows", [15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 513])
-def test_rows_around_a_tile(gpu, rows):
-    """One expert with so many rows, one with a single one, one with none."""
-    model = Model(gpu, 256, 128, 3)
-    x, scale, ids, weights = model.tokens(rows + 1, 1, 1, 2)
-    ids[rows // 2] = 2
+@pytest.mark.parametrize("rows", [15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 513])
+@pytest.mark.parametrize("experts", [3, 2])
+def test_rows_around_a_tile(gpu, rows, experts):
+    """One expert with so many rows, one with a single one, one with none or none more."""
+    model = Model(gpu, 256, 128, experts)
+    x, scale, ids, weights = model.tokens(rows + 1, 1, experts - 2, experts - 1)
+    ids[rows // 2] = experts - 1
     model.check(x, scale, ids, weights)
+
+
+@pytest.mark.parametrize(
+    ("tokens", "choices", "dim", "inner", "experts", "total"),
+    [(60, 1, 16128, 128, 1, 1), (2, 2, 16128, 128, 2, 6), (1, 8, 128, 16128, 1, 1), (70, 1, 128, 16128, 1, 1),
+     (1, 64, 128, 1024, 3, 90), (3, 5, 256, 384, 4, 40), (6, 2, 384, 256, 8, 16), (7, 2, 384, 256, 8, 16),
+     (40, 1, 32768, 128, 1, 1)],
+)
+def test_deep_products_and_pairs_by_themselves(gpu, tokens, choices, dim, inner, experts, total):
+    """Depths whose scales or codes do not fit where those of others do; few tokens of many
+    experts, some of them other ranks'."""
+    model = Model(gpu, dim, inner, experts, first=(total - experts) // 2, total=total, seed=choices)
+    model.check(*model.tokens(tokens, choices, 0, total))
 
 
 def test_choices_of_other_ranks_none_and_twice(gpu):
@@ -89,14 +109,18 @@ def test_choices_of_other_ranks_none_and_twice(gpu):
     got = model.check(x, scale, ids, weights.nan_to_num())
     assert not got[0].any() and not got[2].any() and not got[3].any()
     assert torch.equal(model.run(x, scale, ids, weights), got)
+    one = model.run(x[:3], scale[:3], ids[:3], weights[:3])
+    assert not one[0].any() and not one[2].any()
+    want, bound = off.expert_mlp(x[1:2], scale[1:2], *model.parts, ids[1:2], weights[1:2], model.first)
+    assert ((one[1].cpu().double() - want[0]).abs() <= bound[0] + 2.0 ** -8 * (want[0].abs() + bound[0])).all()
     nothing = model.run(x, scale, torch.full_like(ids, 9), weights)
     assert nothing.shape == x.shape and not nothing.any()
     assert model.run(x[:0], scale[:0], ids[:0], weights[:0]).shape == (0, 256)
 
 
-@pytest.mark.parametrize("tokens", [9, 200])
-def test_a_row_s_infinities_and_nan_stay_in_it(gpu, tokens):
-    model = Model(gpu, 256, 128, 2)
+@pytest.mark.parametrize("tokens, total", [(9, 2), (200, 2), (9, 60)])
+def test_a_row_s_infinities_and_nan_stay_in_it(gpu, tokens, total):
+    model = Model(gpu, 256, 128, 2, total=total)
     x, scale, ids, weights = model.tokens(tokens, 2, 0, 2)
     clean = model.run(x, scale, ids, weights)
     scale.view(torch.uint8)[2, 1] = 255  # NaN
@@ -139,6 +163,16 @@ def test_inputs_that_are_not_contiguous_and_an_output_given(gpu):
                      ids.t().contiguous().t(), weights.repeat_interleave(2, 1)[:, ::2], out=out[:12])
     assert got.data_ptr() == out.data_ptr()
     assert torch.equal(out[:12], want) and (out[12] == 7).all()
+
+
+@pytest.mark.parametrize("tokens", [2, 60])
+def test_scales_at_any_address(gpu, tokens):
+    model = Model(gpu, 512, 128, 1)
+    x, scale, ids, weights = (t.to(gpu) for t in model.tokens(tokens, 1, 0, 1))
+    flat = torch.zeros(tokens * 4 + 1, dtype=torch.uint8, device=gpu)
+    flat[1:] = scale.view(torch.uint8).flatten()
+    got = model.run(x, flat[1:].view(E8).view(tokens, 4), ids, weights)
+    assert torch.equal(got, model.run(x, scale, ids, weights))
 
 
 def test_many_rows_are_each_as_in_small_calls(gpu):
