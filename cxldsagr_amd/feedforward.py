@@ -55,6 +55,19 @@ def _rows(tensor, aligned=False):
     return tensor, address, stride
 
 
+def _apart(out, tensor):
+    """Whether contiguous rows ``out`` share no memory with the rows ``tensor``, or are the
+    same rows."""
+    begin, other = out.data_ptr(), tensor.data_ptr()
+    rows, dim = tensor.shape
+    stride, size = tensor.stride(0), tensor.element_size()
+    if begin == other and (stride == dim or rows == 1):
+        return True
+    # (As far as its unit stride goes; other rows are copied before anything is written.)
+    return (tensor.stride(1) != 1 or begin >= other + ((rows - 1) * stride + dim) * size
+            or other >= begin + rows * dim * size)
+
+
 def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quantize=False,
                       residual_out=None):
     """``t = x + residual`` and ``t * weight / sqrt(mean(t^2) + eps)`` of every row.
@@ -67,8 +80,8 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
     rule of ``indexer.quantize_index``); ``values=False`` leaves them as codes only.
 
     Returns ``Normed(values, codes, scales, residual)``; ``residual`` is ``t``, in a new
-    tensor or in ``residual_out`` (contiguous; it may be ``residual`` itself). Forward
-    only.
+    tensor or in ``residual_out`` (contiguous; it may be ``residual`` or ``x`` itself, else
+    it must not overlap them). Forward only.
     """
     shape, dtype, device = x.shape, x.dtype, x.device
     if len(shape) != 2 or weight.shape != shape[1:]:
@@ -100,6 +113,9 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
             or residual_out.data_ptr() % 16):
         raise ValueError("residual_out must be a contiguous, 16-byte aligned tensor of x's shape, "
                          "type and device")
+    if residual_out is not None and tokens and not (_apart(residual_out, x)
+                                                    and _apart(residual_out, residual)):
+        raise ValueError("residual_out must be residual or x itself, or overlap neither")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         raise ValueError("residual RMS norm has no backward pass")
@@ -190,7 +206,7 @@ def _exponents(scale, shape, what):
     if scale.shape != shape:
         raise ValueError(f"{what} must be {list(shape)}: a scale for every 128 by 128")
     if scale.dtype == SCALES:
-        return scale.contiguous()
+        return scale.clone(memory_format=torch.contiguous_format)
     if scale.dtype != torch.float32:
         raise ValueError(f"{what} must be e8m0 or FP32")
     bits = scale.contiguous().view(torch.int32)
@@ -224,10 +240,10 @@ class ExpertWeights:
     scale for every 128 by 128: ``gate_up_scale`` ``[E, 2 I / 128, D / 128]``,
     ``down_scale`` ``[E, D / 128, I / 128]`` (e8m0, or fp32 powers of two, which are
     checked). The experts are those numbered ``first .. first + E - 1`` of the model's
-    ``total`` (default ``first + E``): other choices are other ranks'. ``total`` only
-    tells how many rows an expert may expect.
+    ``total`` (default ``first + E``, at most 2^30): other choices are other ranks'.
+    ``total`` only tells how many rows an expert may expect.
 
-    The codes are copied in another order; the given tensors are not kept.
+    Codes (in another order) and scales are copied; the given tensors are not kept.
     """
 
     def __init__(self, gate_up, gate_up_scale, down, down_scale, *, first=0, total=None):
@@ -278,7 +294,8 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
     (contiguous, of ``dtype``); a token without a choice here gives zeros. Products and
     sums are in 32 bits; ``silu(gate) * up`` is rounded to e4m3 codes with a
     power-of-two scale for every 128, and an expert's result, before it is weighted, to
-    11 bits. Forward only.
+    no fewer than 11 bits beside the largest of its 64 neighbours. ``out`` must not overlap
+    the inputs. Forward only.
     """
     if not isinstance(experts, ExpertWeights):
         raise ValueError("experts must be an ExpertWeights")

@@ -118,6 +118,38 @@ def test_weights_from_either_scale_type():
     assert (a.experts, a.dim, a.inner, a.first, a.total) == (2, 256, 128, 0, 2)
 
 
+@pytest.mark.parametrize("x, residual, out", [
+    (slice(8, 12), slice(0, 4), slice(1, 5)),  # rows of the residual, one on
+    (slice(0, 4), slice(8, 12), slice(3, 7)),  # x's last row
+])
+def test_a_sum_that_overlaps_is_refused(x, residual, out):
+    rows = torch.zeros(12, 256)
+    with pytest.raises(ValueError, match="overlap"):
+        residual_rms_norm(rows[x], torch.ones(256), rows[residual], residual_out=rows[out])
+
+
+def test_a_sum_over_a_row_for_all_is_refused():
+    rows = torch.zeros(4, 256)
+    with pytest.raises(ValueError, match="overlap"):
+        residual_rms_norm(torch.zeros(4, 256), torch.ones(256), rows[:1].expand(4, 256), residual_out=rows)
+
+
+def test_sums_in_place_or_beside_are_not():
+    rows = torch.zeros(12, 256)
+    for x, residual, out in [(slice(0, 4), slice(4, 8), slice(8, 12)), (slice(0, 4), slice(4, 8), slice(4, 8)),
+                             (slice(0, 4), slice(4, 8), slice(0, 4)), (slice(0, 4), slice(0, 4), slice(0, 4))]:
+        # (As far as a CPU's tensors get.)
+        with pytest.raises((ValueError, RuntimeError), match="(?i)gpu|gfx950|device"):
+            residual_rms_norm(rows[x], torch.ones(256), rows[residual], residual_out=rows[out])
+
+
+def test_given_scales_are_not_kept():
+    scale = torch.ones(2, 2, 2).to(E8)
+    own = ExpertWeights(**_parts(gate_up_scale=scale))
+    scale.view(torch.uint8).fill_(3)
+    assert int(own.gate_up_scale.view(torch.uint8).min()) == 127
+
+
 def test_tiles_hold_what_the_layout_says():
     codes = torch.randint(0, 256, (2, 512, 384), generator=torch.Generator().manual_seed(4), dtype=torch.uint8)
     parts = _parts(gate_up=codes.view(F8), gate_up_scale=torch.ones(2, 4, 3),
