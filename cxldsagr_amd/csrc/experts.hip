@@ -11,17 +11,28 @@
 //     row (its largest value just below 2^15 as fp16: 11 bits of each value; as bf16, 8, the
 //     result would be sqrt 2 times as far from the formula as its own rounding puts it);
 //  4. join: each token's y, weighted, in 32 bits, in the order of its choices.
+// With so few pairs that an expert seldom has two, two launches: each pair by itself, and the
+// token's results weighted and summed where they are formed.
 // No atomics on values: results do not depend on the order of work-groups.
 //
-// The products run on v_mfma_scale_f32_16x16x128_f8f6f4, weights as the first operand (rows:
-// 16 of a weight's), tokens as the second (columns), so that a lane's four results are
-// neighbours in the output's row. The instruction multiplies by each operand's scale, a
-// power of two per 32 values along K: the blocks of 128 cost nothing beyond that. Sums are
-// in 32 bits. Weights are laid out as the instruction reads them (ExpertWeights): a tile of
-// 16 rows by 128 is 2 KB, two planes of 16 bytes a lane, read by one wave straight into
-// registers; tiles of gate and up alternate, so that a lane holds g and u of the same h; and
-// the rows of a wave's four tiles are dealt out so that a lane's results in all of them are
-// neighbours (16 of y, 8 of h) and four lanes fill a line.
+// The products run on v_mfma_scale_f32_*_f8f6f4, weights as the first operand, tokens as the
+// second, so that a lane's results are of one token. The instruction multiplies by each
+// operand's scale, a power of two per 32 values along K: the blocks of 128 cost nothing beyond
+// that. Sums are in 32 bits, of which the unit's own way of adding a step's products leaves some
+// 16 (sums of 128, 1,024 and 7,168 products are 1.4e-5, 1.4e-5 and 1.5e-5 of their own size off,
+// in every form of its 8-bit instructions): one in 700 codes of h falls on the other side of a
+// border, and the result's error is 1.2 times that of products in 64 bits, 2.0e-3 of its size
+// against 1.7e-3, most of it the rounding to bf16. Weights are laid out as
+// waves read them (ExpertWeights), straight into registers: tiles of 16 rows by 128, 2 KB, in
+// planes of 16 bytes a lane; tiles of gate and up in turn, so that a lane holds g and u of the
+// same h; the rows of a wave's four tiles dealt out so that a lane's results are neighbours.
+//
+// What bounds it: reading the weights, up to some 100 rows an expert, where a read alone
+// reaches 6.2 TB/s (32 experts of 7,168 by 2,048 dims, 8 choices: 1 token 67 us, 5.2 TB/s; 64
+// tokens 250 us, 5.6; 128 experts, 128 tokens 893 us, 6.2); beyond that the matrix unit,
+// which the card's power holds to 1.4 - 1.7 GHz (8,192 tokens 2,830 us, 2.04 PFLOP/s: up 1,620,
+// down 1,040, join 220, which is y's way to memory and back; the library's product of the same
+// type 2.70).
 #include "attention_core.h"
 #include "quantize_core.h"
 #include "../../include/dsa_gfx950.h"
@@ -231,14 +242,18 @@ __device__ __forceinline__ v8i load_weight(const uint8_t* codes, int steps, int 
 
 // Row tiles: 32 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
 // registers, a step ahead; the rows' codes go into LDS straight from memory (two steps
-// ahead, four buffers), where all four waves read them, three operands ahead of their
-// products. Half-way through a step the waves meet: from there on the next step's rows may
-// be read. A row's eight 16-byte parts are turned by its index, so that the rows' reads of one
-// part fall on different banks.
+// ahead, four buffers), where all four waves read them, an operand ahead of its products.
+// Half-way through a step the waves meet: from there on the next step's rows may be read. A
+// row's eight 16-byte parts are turned by its index, so that the rows' reads of one part fall
+// on different banks.
 // Rows' scales: up lays those of all steps out in LDS before the first; the scales of h come
 // from memory a step ahead, where up has put them by tile.
 // Per step of 128 a CU's matrix units take 256 kRows clocks, its LDS 160 kRows (four waves'
-// reads and one write of 4 kRows KB at 128 bytes).
+// reads and one write of 4 kRows KB at 128 bytes). Two work-groups of 128 rows a CU: one's
+// start and end (11 and 8 of 144 thousand clocks of up, 6 and 9 of 51 of down) go on beside
+// the other's products. 256 rows by four waves of twice the accumulators, or by eight waves,
+// read a third less from L2 and were slower (8,192 tokens 2,890 and 3,170 us against 2,830);
+// 96 rows were faster at 640 tokens of 32 experts alone (370 us against 387).
 constexpr int kMaxSteps = 256;
 // Steps of up whose rows' scales LDS holds (of 128 rows with two work-groups a CU).
 constexpr int max_up_steps(int rows) { return rows <= 2 ? kMaxSteps : 124; }

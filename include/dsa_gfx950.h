@@ -693,15 +693,18 @@ int dsa_route_experts(const void* logits, int64_t stride, int dtype, int64_t tok
  * out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j] - first,
  * over the choices with 0 <= e < experts. x: e4m3 [tokens, dim], x_scale: exponent bytes
  * [tokens, dim / 128]; ids int32, weights f32 [tokens, choices] (1 .. 64 choices); dim and
- * inner in whole blocks of 128, tokens up to 2^22, experts 1 .. 1024 of the model's `total`
- * (which only steers tiles). Weights are e4m3 in tiles of 16 rows by 128 columns, 2048 bytes,
- * [experts][rows / 16][columns / 128][plane 2][g 4][row 16][16 bytes]: bytes 64 plane + 16 g ..
- * of a row's 128. gate_up has 2 inner rows, tiles of 16 gate rows and of 16 up rows in turn;
- * down has dim rows. Scales are exponent bytes per 128 by 128: gate_up_scale
- * [experts, 2 inner / 128, dim / 128] (gate's blocks, then up's), down_scale
- * [experts, dim / 128, inner / 128]. silu(gate) * up is rounded to e4m3 codes with a power of
- * two per 128; sums are in 32 bits; an expert's result is held in 11 bits before it is
- * weighted. out: [tokens, dim] of `dtype`. workspace: device memory of
+ * inner in whole blocks of 128 up to 32768, tokens up to 2^22, experts 1 .. 1024 of the
+ * model's `total` (up to 2^30; it only steers tiles). Weights are e4m3 in tiles of 16 rows by
+ * 128 columns, 2048 bytes, [experts][rows / 16][columns / 128][plane 2][g 4][row 16][16 bytes]:
+ * bytes 64 plane + 16 g .. of a row's 128. Four tiles hold 64 rows of down [dim, inner], dealt
+ * out: row 4 a + i of tile t is the 64's row 16 a + 4 t + i. Of gate_up [2 inner, dim] four
+ * tiles hold 32 rows of gate and the same 32 of up in turn (gate, up, gate, up): row 4 a + i of
+ * gate's tile t (0 or 1) is the 32's row 8 a + 4 t + i, up's likewise. Scales are exponent
+ * bytes per 128 by 128: gate_up_scale [experts, 2 inner / 128, dim / 128] (gate's blocks, then
+ * up's), down_scale [experts, dim / 128, inner / 128]. silu(gate) * up is rounded to e4m3 codes
+ * with a power of two per 128; sums are in 32 bits; an expert's result is held, before it is
+ * weighted, in fp16 with a power of two per 64 columns, or in 32 bits where pairs are taken by
+ * themselves. out: [tokens, dim] of `dtype`, apart from all inputs. workspace: device memory of
  * dsa_expert_mlp_workspace_bytes(...), 16-byte aligned, uninitialised; calls that overlap
  * need different ones.
  */
