@@ -184,3 +184,30 @@ def test_many_rows_are_each_as_in_small_calls(gpu):
     want, bound = off.expert_mlp(x[some], scale[some], *model.parts, ids[some], weights[some])
     bound = bound + 2.0 ** -8 * (want.abs() + bound)
     assert ((got[some.to(gpu)].cpu().double() - want).abs() <= bound).all()
+
+
+def test_offsets_that_pass_32_bits(gpu):
+    """Inputs, weights, hidden codes and results of more than 2^31 elements each: the last
+    and the first tokens as in a call of their own."""
+    from cxldsagr_amd.feedforward import ExpertWeights, expert_mlp
+
+    tokens, dim, inner, experts = 300_001, 7168, 4096, 40
+    gen = torch.Generator(device=gpu).manual_seed(51)
+
+    def codes(*shape):  # (magnitudes below 1, no NaN)
+        return torch.randint(0, 256, shape, generator=gen, device=gpu, dtype=torch.uint8).bitwise_and_(0xBF).view(F8)
+
+    def scales(*shape):
+        return torch.randint(118, 122, shape, generator=gen, device=gpu, dtype=torch.uint8).view(E8)
+
+    own = ExpertWeights(codes(experts, 2 * inner, dim), scales(experts, inner // 64, dim // 128),
+                        codes(experts, dim, inner), scales(experts, dim // 128, inner // 128))
+    x, scale = codes(tokens, dim), scales(tokens, dim // 128)
+    ids = torch.randint(0, experts, (tokens, 2), generator=gen, device=gpu, dtype=torch.int32)
+    ids[-3000:, 0] = experts - 1  # the last rows and the last weights of all
+    weights = torch.rand(tokens, 2, generator=gen, device=gpu)
+    assert min(x.numel(), own.gate_up.numel(), 2 * tokens * inner, 2 * tokens * dim) > 2 ** 31
+    got = expert_mlp(x, scale, own, ids, weights)
+    for part in (slice(tokens - 3000, tokens), slice(0, 3000)):
+        want = expert_mlp(x[part], scale[part], own, ids[part], weights[part])
+        assert want.abs().amax(1).min() > 0 and torch.equal(got[part], want)

@@ -114,3 +114,21 @@ def test_zeros_infinities_and_nan_stay_in_their_rows(gpu):
     assert got.values[3].isnan().all() and got.codes[3].float().isnan().all()
     # 64-bit squares: 1e38 does not overflow the mean.
     assert torch.equal(got.values[4].float(), torch.ones(256, device=gpu))
+
+
+@pytest.mark.parametrize("dim", [16384, 16383])
+def test_offsets_that_pass_32_bits(gpu, dim):
+    from cxldsagr_amd.feedforward import residual_rms_norm
+
+    tokens, quantize = 132_000, dim % 128 == 0
+    assert tokens * dim > 2 ** 31
+    gen = torch.Generator(device=gpu).manual_seed(8)
+    x, r = (torch.randn(tokens, dim, generator=gen, device=gpu, dtype=torch.bfloat16) for _ in range(2))
+    weight = torch.randn(dim, generator=gen, device=gpu)
+    got = residual_rms_norm(x, weight, r, quantize=quantize)
+    for part in (slice(tokens - 5, tokens), slice(0, 5)):
+        want = residual_rms_norm(x[part], weight, r[part], quantize=quantize)
+        assert torch.equal(got.values[part], want.values) and torch.equal(got.residual[part], want.residual)
+        if quantize:
+            for a, b in ((got.codes, want.codes), (got.scales, want.scales)):
+                assert torch.equal(a[part].view(torch.uint8), b.view(torch.uint8))

@@ -106,3 +106,17 @@ def test_many_tokens_are_each_as_alone(gpu, tokens):
     want, want_ids = off.route(logits[part], 8, bias=bias, groups=8, top_groups=4, scale=2.5)
     assert torch.equal(ids[part].cpu(), want_ids)
     assert ((weights[part].cpu().double() - want).abs() <= 12 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("experts, stride, tokens", [(1024, 1024, 2_100_001), (100, 70_003, 31_000)])
+def test_offsets_that_pass_32_bits(gpu, experts, stride, tokens):
+    from cxldsagr_amd.feedforward import route_experts
+
+    assert tokens * stride > 2 ** 31
+    gen = torch.Generator(device=gpu).manual_seed(15)
+    logits = torch.empty(tokens, stride, device=gpu, dtype=torch.bfloat16)[:, :experts]
+    logits.normal_(generator=gen)
+    weights, ids = route_experts(logits, 6)
+    for part in (slice(tokens - 7, tokens), slice(0, 7)):
+        want = route_experts(logits[part].contiguous(), 6)
+        assert torch.equal(weights[part], want[0]) and torch.equal(ids[part], want[1])
