@@ -100,6 +100,14 @@ def test_deep_products_and_pairs_by_themselves(gpu, tokens, choices, dim, inner,
     model.check(*model.tokens(tokens, choices, 0, total))
 
 
+@pytest.mark.parametrize("seed", [9, 11, 12, 13])
+def test_small_sums_of_large_products(gpu, seed):
+    """Results far smaller than the products in them, as exact as 32 bits can show them."""
+    model = Model(gpu, 128, 128, 1, first=2, total=11, seed=seed)
+    model.check(*model.tokens(339, 4, 2, 3), dtype=torch.float32)
+    model.check(*model.tokens(339, 4, 0, 11), dtype=torch.float32)
+
+
 def test_choices_of_other_ranks_none_and_twice(gpu):
     """Slices of the experts sum to the whole; what is not here adds nothing."""
     model = Model(gpu, 256, 128, 4, first=10, total=24)

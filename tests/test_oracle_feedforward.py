@@ -79,3 +79,22 @@ def test_experts_of_unit_weights():
     want = off.quantized(rows * rows * torch.sigmoid(rows))[0]
     assert torch.allclose(out[0], want[0], atol=1e-12) and torch.allclose(out[1], want[1] / 2, atol=1e-12)
     assert not out[2].any() and not bound[2].any()
+
+
+def test_what_the_unit_cuts_off():
+    row = torch.zeros(1, 24, dtype=torch.float64)
+    row[0, 0], row[0, 1], row[0, 2] = 1.75, 15 * 2.0 ** -13, -1.75 * 2.0 ** -13
+    row[0, 8], row[0, 9], row[0, 23] = -1.0, 2.0 ** -7, 2.0 ** -20
+    weight = torch.ones(3, 24, dtype=torch.float64)
+    weight[1] = -1.5
+    weight[2, 9] = 2.0 ** -8  # the product 2^-15 beside 1
+    # 15 units of 2^-13 stay, of 1.75 one does, of 2.625 two do; alone all is whole.
+    want = torch.tensor([[-0.75 * 2.0 ** -13, (0.625 - 0.5) * 2.0 ** -13, (0.25 - 0.75) * 2.0 ** -13]], dtype=torch.float64)
+    assert torch.equal(off.cut_off(row, weight), want)
+    assert not off.cut_off(torch.zeros(1, 24, dtype=torch.float64), weight).any()
+    assert torch.equal(off.cut_off(row, weight, torch.zeros_like(row)), want.abs())
+    # The first eight may be off: what each may lose of 1.75 (2 with what it may be off by).
+    moved = torch.zeros_like(row)
+    moved[0, 0] = 0.25
+    got = off.cut_off(row, weight[:1], moved)
+    assert torch.equal(got, torch.tensor([[(2.0 + 1.75) * 2.0 ** -13]], dtype=torch.float64))
