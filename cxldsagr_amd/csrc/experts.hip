@@ -23,8 +23,9 @@
 // of two. A product of 8 bits loses nothing down to 2^-6 of the largest, so that sums of normal
 // values, 128 to 7,168 of them, are 1.4e-5 to 1.5e-5 of their size off: one in 700 codes of h falls
 // on the other side of a border, and the result's error is 1.2 times that of products in 64 bits,
-// 2.0e-3 of its size against 1.7e-3, most of it the rounding to bf16. (16-bit products would need
-// twice the unit's time and the codes' conversion.) Weights are laid out as
+// 2.0e-3 of its size against 1.7e-3, most of it the rounding to bf16. 16-bit products, which lose
+// nothing, need twice the unit's time and the codes' conversion: up's are of those in tiles of 32
+// rows and of pairs by themselves. Weights are laid out as
 // waves read them (ExpertWeights), straight into registers: tiles of 16 rows by 128, 2 KB, in
 // planes of 16 bytes a lane; tiles of gate and up in turn, so that a lane holds g and u of the
 // same h; the rows of a wave's four tiles dealt out so that a lane's results are neighbours.
@@ -67,6 +68,38 @@ __device__ __forceinline__ v4f product(v8i w, v8i x, v4f c, uint32_t w_scale, ui
 template <int kW, int kX>
 __device__ __forceinline__ v16f product32(v8i w, v8i x, v16f c, uint32_t w_scale, uint32_t x_scale) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, kW, (int)w_scale, kX, (int)x_scale);
+}
+
+// The same products in 16 bits, of codes that are converted for it: the unit adds these with 32
+// bits throughout (sums of 7,168 are 1.2e-7 of their size off). They are up's where they cost
+// little, while reading the weights is what takes time (1 token 64.1 -> 65.1 us, 64 tokens 249.6
+// -> 251.1), and where h has few values, with many rows of few experts at up to a fifth more (500
+// of one of 7,168 by 2,048 dims 56.4 -> 69.1): 1.4e-5 moves one code of h in 700 by a step, and
+// among fewer than some 2^20 a single one of the largest may show in the result more than all
+// other roundings.
+// x takes both scales with it, 2^(a + b - 254) of their exponents' bytes, as the number whose
+// exponent the conversion takes (255: NaN; products that bf16's exponents do not hold are far
+// outside those of h).
+__device__ __forceinline__ float both_scales(uint32_t a, uint32_t b) {
+  const int e = min(max((int)(a + b) - 127, 0), 254);
+  return __uint_as_float((a == 255 || b == 255 ? 255u : (uint32_t)e) << 23);
+}
+// Eight of a lane's 32 codes (part 0 .. 3) times that.
+__device__ __forceinline__ v4u widened(v8i codes, int part, float scale) {
+  v4u wide;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t four = (uint32_t)codes[2 * part + i];
+    wide[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, false));
+    wide[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, true));
+  }
+  return wide;
+}
+__device__ __forceinline__ v4f wide_product(v4u w, v4u x, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f wide_product(v4u w, v4u x, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
 }
 
 // ------------------------------------------------------------ 1. groups --
@@ -281,6 +314,7 @@ __device__ __forceinline__ uint32_t turn_of(uint32_t row) { return (row & 7) ^ (
 
 template <int kRows, bool kUp>
 __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expert_product(ProductArgs a) {
+  constexpr bool kWide = kUp && kRows == 1;  // products in 16 bits
   constexpr int kSize = 32 * kRows;  // rows of a tile
   __shared__ TileLds<kRows, kUp> lds;
   // Work-groups go round the eight XCDs: each takes a run of the work, in which an expert's
@@ -440,8 +474,16 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
         __builtin_amdgcn_sched_barrier(0);
       }
       x[(q + kAhead) % kRing] = q + kAhead < kParts ? read(s & 3, q + kAhead) : read((s + 1) & 3, q + kAhead - kParts);
-      acc[m][0] = product32<0, m>(now[k][0], x[q % kRing], acc[m][0], ws, xs);
-      acc[m][1] = product32<kUp ? 1 : 0, m>(now[k][1], x[q % kRing], acc[m][1], ws, xs);
+      if constexpr (kWide) {
+        const float scale[2] = {both_scales(xs >> (8 * m) & 255, ws & 255), both_scales(xs >> (8 * m) & 255, ws >> 8)};
+        static_for<8>([&](auto part) {
+          constexpr int o = decltype(part)::value & 1, i = decltype(part)::value / 2;
+          acc[m][o] = wide_product(widened(now[k][o], i, 1.0f), widened(x[q % kRing], i, scale[o]), acc[m][o]);
+        });
+      } else {
+        acc[m][0] = product32<0, m>(now[k][0], x[q % kRing], acc[m][0], ws, xs);
+        acc[m][1] = product32<kUp ? 1 : 0, m>(now[k][1], x[q % kRing], acc[m][1], ws, xs);
+      }
     });
 #pragma unroll
     for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = next[i >> 1][i & 1];
@@ -649,8 +691,14 @@ __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) load(ring[d], begin + d < end ? begin + d : end - 1);
     auto multiply = [&](const Step& of) {
+      const float scale[2] = {both_scales(of.x_scale, of.w_scale[0]), both_scales(of.x_scale, of.w_scale[1])};
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = product(of.w[t], of.x, acc[t], of.w_scale[t & 1], of.x_scale);
+      for (int part = 0; part < 4; ++part) {
+        // (x with the scales of gate's tiles and of up's)
+        const v4u wide[2] = {widened(of.x, part, scale[0]), widened(of.x, part, scale[1])};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = wide_product(widened(of.w[t], part, 1.0f), wide[t & 1], acc[t]);
+      }
     };
     int s = begin;
     for (; s + kDepth <= end; s += kDepth) {
@@ -800,6 +848,10 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   const int64_t mean = p.pairs / total;
   p.rows = mean <= 16 ? 1 : mean <= 48 ? 2 : 4;
   if (dim > max_up_steps(4) * kBlock && p.rows > 2) p.rows = 2;
+  // Few values of h (of the pairs that are to be expected here) want 16-bit products. (In tiles
+  // of 64 rows these took longer, with half as many work-groups: 250 tokens, 2 of 2 experts of
+  // 4,096 by 2,048 dims, one here, 44.6 -> 53.7 us, 90 tokens, 6 of 16 of 4,096 by 512, 55.1 -> 63.6.)
+  if (p.pairs * experts / total * inner <= 1 << 20) p.rows = 1;
   const int64_t size = 32 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;

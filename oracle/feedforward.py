@@ -142,11 +142,12 @@ def cut_off(rows, weight, moved=None):
     return out
 
 
-def expert_mlp(x, x_scale, gate_up, gate_up_scale, down, down_scale, ids, weights, first=0):
+def expert_mlp(x, x_scale, gate_up, gate_up_scale, down, down_scale, ids, weights, first=0, cut_up=True):
     """``(out, bound)`` float64 [T, D]: ``bound`` is how far a kernel may be off before it
     rounds the result, that sums products on the matrix unit (eights of neighbours exactly
-    but for ``cut_off``; n of them in 32 bits, in any order, are off by at most (n + 2) 2^-24
-    of their magnitudes' sum, taken twice as the unit's rounding is its own), forms silu within 2^-16 of its value (an exponential and a
+    but for ``cut_off``, up's only with ``cut_up``; n of them in 32 bits, in any order, are
+    off by at most (n + 2) 2^-24 of their magnitudes' sum, taken twice as the unit's rounding
+    is its own), forms silu within 2^-16 of its value (an exponential and a
     reciprocal of 32 bits; the former's argument, in log2 units 127 at most where it is a
     normal number, is off by 2^-24 of that from its constant and as much from its product)
     and holds an expert's result in 11 bits (half a step: 2^-11) against the largest of 64."""
@@ -168,7 +169,9 @@ def expert_mlp(x, x_scale, gate_up, gate_up_scale, down, down_scale, ids, weight
             continue
         both, size = rows[token] @ wg[e].t(), rows[token].abs() @ wg[e].abs().t()
         gate, up = both[:, :inner], both[:, inner:]
-        off = sums(eights(wg[e])) * size + cut_off(rows[token], wg[e]).abs()
+        off = sums(eights(wg[e])) * size
+        if cut_up:
+            off = off + cut_off(rows[token], wg[e]).abs()
         hidden = silu(gate) * up
         # (silu's slope is at most 1.1.)
         off = 1.1 * off[:, :inner] * (up.abs() + off[:, inner:]) + silu(gate).abs() * off[:, inner:]

@@ -37,6 +37,7 @@ class Model:
         self.parts = (*matrix(gen, experts, 2 * inner, dim), *matrix(gen, experts, dim, inner))
         self.own = ExpertWeights(*(t.to(gpu) for t in self.parts), first=first, total=total)
         self.first, self.gen, self.gpu, self.dim = first, gen, gpu, dim
+        self.inner, self.part = inner, experts / (self.own.total)
 
     def tokens(self, tokens, choices, low, high):
         x, scale = tokens_in_codes(self.gen, tokens, self.dim)
@@ -51,7 +52,9 @@ class Model:
     def check(self, x, scale, ids, weights, dtype=torch.bfloat16):
         got = self.run(x, scale, ids, weights, dtype=dtype)
         assert got.dtype == dtype and got.shape == x.shape
-        want, bound = off.expert_mlp(x, scale, *self.parts, ids, weights, self.first)
+        # (Up to 2^20 values of h, or 16 rows an expert, up's products are in 16 bits.)
+        want, bound = off.expert_mlp(x, scale, *self.parts, ids, weights, self.first,
+                                     cut_up=ids.numel() * self.part * self.inner > 2 ** 20 and ids.numel() >= 17 * self.own.total)
         bound = bound + torch.finfo(dtype).eps / 2 * (want.abs() + bound) + 2.0 ** -25
         far = (got.cpu().double() - want).abs()
         assert (far <= bound).all(), (far / bound).max()
@@ -85,6 +88,38 @@ def test_rows_around_a_tile(gpu, rows, experts):
     x, scale, ids, weights = model.tokens(rows + 1, 1, experts - 2, experts - 1)
     ids[rows // 2] = experts - 1
     model.check(x, scale, ids, weights)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 16, 17, 31, 33, 47, 49, 63, 65, 96, 127, 129, 257, 300, 513])
+def test_rows_around_a_tile_of_long_calls(gpu, rows):
+    """More than 2^20 values of h: each expert with a row more or less than the next."""
+    inner, dim = (4096, 128) if rows > 1 else (16128, 256)
+    experts = max(2, -(-(2 ** 20 + 1) // (rows * inner)) + 1)
+    model = Model(gpu, dim, inner, experts)
+    ids = torch.repeat_interleave(torch.arange(experts), torch.tensor([rows - 1, rows + 1] * experts)[:experts])
+    x, scale, _, weights = model.tokens(len(ids), 1, 0, experts)
+    ids = ids[torch.randperm(len(ids), generator=model.gen)].int()[:, None]
+    assert ids.numel() * inner > 2 ** 20
+    model.check(x, scale, ids, weights)
+
+
+@pytest.mark.parametrize("tokens, experts, inner", [(1, 1, 4096), (2, 1, 2048), (40, 8, 1024)])
+def test_hidden_codes_of_few_values(gpu, tokens, experts, inner):
+    """Codes of h as the results of a down that picks them: those of 64 bits, but for one in
+    20,000 (silu's 2^-21 of a value, within a step of 1/8 to 1/16 of it, is half of that)."""
+    from cxldsagr_amd.feedforward import ExpertWeights
+
+    dim = inner
+    model = Model(gpu, dim, inner, experts)
+    model.parts = (*model.parts[:2], torch.eye(inner).expand(experts, inner, inner).contiguous().to(F8),
+                   torch.ones(experts, inner // 128, inner // 128))
+    model.own = ExpertWeights(*(t.to(gpu) for t in model.parts))
+    x, scale, ids, weights = model.tokens(tokens, 1, 0, experts)
+    got = model.run(x, scale, ids, torch.ones_like(weights), dtype=torch.float32).cpu().double()
+    rows = off.wide(x) * off.wide(scale).repeat_interleave(128, 1)
+    both = torch.stack([rows[t] @ off.weight_values(*(p[ids[t]] for p in model.parts[:2]))[0].t() for t in range(tokens)])
+    want, _ = off.quantized(off.silu(both[:, :inner]) * both[:, inner:])
+    assert int((got != want).sum()) <= 2 + want.numel() // 20000
 
 
 @pytest.mark.parametrize(
@@ -126,7 +161,7 @@ def test_choices_of_other_ranks_none_and_twice(gpu):
     assert model.run(x[:0], scale[:0], ids[:0], weights[:0]).shape == (0, 256)
 
 
-@pytest.mark.parametrize("tokens, total", [(9, 2), (200, 2), (9, 60)])
+@pytest.mark.parametrize("tokens, total", [(9, 2), (200, 2), (9, 60), (4200, 2)])
 def test_a_row_s_infinities_and_nan_stay_in_it(gpu, tokens, total):
     model = Model(gpu, 256, 128, 2, total=total)
     x, scale, ids, weights = model.tokens(tokens, 2, 0, 2)
@@ -142,18 +177,19 @@ def test_a_row_s_infinities_and_nan_stay_in_it(gpu, tokens, total):
     assert not got[6].isfinite().any() and not got[7].isfinite().any()
 
 
+@pytest.mark.parametrize("tokens", [6, 4200])
 @pytest.mark.parametrize("power", [-40, -20, 20, 40])
-def test_scales_far_from_one(gpu, power):
+def test_scales_far_from_one(gpu, power, tokens):
     """Exponents of tokens and weights that cancel in part; results far below and above 1."""
     model = Model(gpu, 256, 128, 2)
-    x, scale, ids, weights = model.tokens(6, 2, 0, 2)
+    x, scale, ids, weights = model.tokens(tokens, 2, 0, 2)
     scale = (scale.float() * 2.0 ** power).to(E8)
     model.parts = (*model.parts[:2], model.parts[2], model.parts[3] * 2.0 ** (power // 2))
     from cxldsagr_amd.feedforward import ExpertWeights
 
     model.own = ExpertWeights(*(t.to(gpu) for t in model.parts))
-    got = model.run(x, scale, ids, weights, dtype=torch.float32)
-    want, bound = off.expert_mlp(x, scale, *model.parts, ids, weights)
+    got = model.run(x, scale, ids, weights, dtype=torch.float32)[:6]
+    want, bound = off.expert_mlp(x[:6], scale[:6], *model.parts, ids[:6], weights[:6], cut_up=tokens > 6)
     bound = bound + 2.0 ** -24 * (want.abs() + bound) + 2.0 ** -149
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
