@@ -293,7 +293,8 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
     Returns ``[T, D]`` in ``dtype`` (bf16, fp16 or fp32), or writes it to ``out``
     (contiguous, of ``dtype``); a token without a choice here gives zeros. Sums are in
     32 bits, but for what the matrix unit cuts off each of eight neighbouring products
-    (below 2^-13 of the largest); ``silu(gate) * up`` is rounded to e4m3 codes with a
+    (below 2^-13 of the largest; nothing from gate's and up's up to 16 choices an expert or
+    2^20 hidden values); ``silu(gate) * up`` is rounded to e4m3 codes with a
     power-of-two scale for every 128 (the rule of ``indexer.quantize_index``: 2^-22 at
     least, so that what is below 2^-32 is lost), and an expert's result, before it is
     weighted, to no fewer than 11 bits (down to 2^-29 of the largest of its 64 neighbours).
