@@ -702,10 +702,11 @@ int dsa_route_experts(const void* logits, int64_t stride, int dtype, int64_t tok
  * gate's tile t (0 or 1) is the 32's row 8 a + 4 t + i, up's likewise. Scales are exponent
  * bytes per 128 by 128: gate_up_scale [experts, 2 inner / 128, dim / 128] (gate's blocks, then
  * up's), down_scale [experts, dim / 128, inner / 128]. silu(gate) * up is rounded to e4m3 codes
- * with a power of two per 128; sums are in 32 bits, but (not in up of few pairs) of eight
- * neighbouring products each cut at 2^-13 of the largest; an expert's result is held, before it is weighted, in fp16 with a power
- * of two per 64 columns, or in 32 bits where pairs are taken by themselves. out: [tokens, dim]
- * of `dtype`, apart from all inputs. workspace: device memory of
+ * with a power of two per 128; sums are in 32 bits, but (not gate's and up's of few pairs) of
+ * eight neighbouring products each cut at 2^-13 of the largest; an expert's result is held,
+ * before it is weighted, in fp16 with a power of two per 64 columns, or in 32 bits where pairs
+ * are taken by themselves. out: [tokens, dim] of `dtype`, apart from all inputs. workspace:
+ * device memory of
  * dsa_expert_mlp_workspace_bytes(...), 16-byte aligned, uninitialised; calls that overlap
  * need different ones.
  */
