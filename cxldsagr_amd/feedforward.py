@@ -42,6 +42,8 @@ class Normed(NamedTuple):
 
 
 _CODES = _native.DTYPE_CODES
+# (Two thirds of what new_empty takes.)
+_empty = torch.empty_strided
 
 
 def _rows(tensor, aligned=False):
@@ -127,14 +129,15 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
     if residual is not None:
         residual, residual_at, residual_stride = _rows(residual, quantize)
         if residual_out is None:
-            residual_out = x.new_empty(shape)
+            residual_out = _empty(shape, (dim, 1), dtype=dtype, device=device)
     if not weight.is_contiguous() or (quantize and weight.data_ptr() % 16):
         weight = weight.clone(memory_format=torch.contiguous_format)
-    out = x.new_empty(shape) if values else None
+    out = _empty(shape, (dim, 1), dtype=dtype, device=device) if values else None
     codes = scales = None
     if quantize:
-        codes = x.new_empty(shape, dtype=CODES)
-        scales = x.new_empty((tokens, dim // SCALE_BLOCK), dtype=SCALES)
+        codes = _empty(shape, (dim, 1), dtype=CODES, device=device)
+        blocks = dim // SCALE_BLOCK
+        scales = _empty((tokens, blocks), (blocks, 1), dtype=SCALES, device=device)
     if tokens:
         with _native.on_device(device):
             _native.call(
@@ -190,8 +193,8 @@ def route_experts(logits, k, *, bias=None, scoring="sigmoid", groups=1, top_grou
         raise ValueError("routing to experts has no backward pass")
     _native.require_gfx950(device, "routing to experts")
     logits, logits_at, stride = _rows(logits)
-    weights = logits.new_empty((tokens, k), dtype=torch.float32)
-    ids = logits.new_empty((tokens, k), dtype=torch.int32)
+    weights = _empty((tokens, k), (k, 1), dtype=torch.float32, device=device)
+    ids = _empty((tokens, k), (k, 1), dtype=torch.int32, device=device)
     if tokens:
         with _native.on_device(device):
             _native.call(
@@ -329,7 +332,7 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
         raise ValueError("the experts' MLP has no backward pass")
     _native.require_gfx950(device, "the experts' MLP")
     if out is None:
-        out = x.new_empty((tokens, dim), dtype=dtype)
+        out = _empty((tokens, dim), (dim, 1), dtype=dtype, device=device)
     if not tokens:
         return out
     x = x.contiguous()
@@ -340,7 +343,7 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
     with _native.on_device(device):
         needed = _native.size_of("dsa_expert_mlp_workspace_bytes", device.index, tokens, choices,
                                  dim, experts.inner, experts.experts, experts.total)
-        workspace = x.new_empty(needed, dtype=torch.uint8)
+        workspace = _empty((needed,), (1,), dtype=torch.uint8, device=device)
         _native.call(
             "dsa_expert_mlp_fp8", x.data_ptr(), x_scale.data_ptr(), tokens, dim, experts.inner,
             experts.gate_up.data_ptr(), experts.gate_up_scale.data_ptr(),
