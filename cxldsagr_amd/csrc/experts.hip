@@ -269,10 +269,19 @@ __device__ __forceinline__ WaveWeight weight_of(const ProductArgs& a, int expert
   return w;
 }
 
+// 16 bytes of a weight; kOnce: that no other work-group of the call wants, past the caches, of
+// which the rest of the call has more then.
+template <bool kOnce>
+__device__ __forceinline__ v4u load_part(const v4u* from) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(from);
+  return *from;
+}
+
 // Tile t of the wave's four, one step.
+template <bool kOnce>
 __device__ __forceinline__ v8i load_weight(const uint8_t* codes, int steps, int t, int s) {
   const v4u* from = reinterpret_cast<const v4u*>(codes + ((int64_t)t * steps + s) * kTile);
-  return joined(from[0], from[64]);
+  return joined(load_part<kOnce>(from), load_part<kOnce>(from + 64));
 }
 
 // Row tiles: 32 kRows rows by 256 columns. Each wave keeps its 64 columns of the weight in
@@ -301,9 +310,10 @@ struct TileLds {
 
 // The wave's weight tiles as two operands of 32 rows (up: gate's and up's), 64 deep: half k
 // of a step. Lane (r, h): rows r of tiles `first` and `second`, bytes 32 h .. of the half.
+template <bool kOnce>
 __device__ __forceinline__ v8i load_weight32(const uint8_t* codes, int64_t tile, int k) {
   const v4u* from = reinterpret_cast<const v4u*>(codes + tile + k * 1024);
-  return joined(from[0], from[16]);
+  return joined(load_part<kOnce>(from), load_part<kOnce>(from + 16));
 }
 
 // How a row's parts are turned: two rows and their eight parts are all 64 banks. 16 lanes are
@@ -312,7 +322,7 @@ __device__ __forceinline__ v8i load_weight32(const uint8_t* codes, int64_t tile,
 // row % 8 alone half of the LDS's time went to conflicts.)
 __device__ __forceinline__ uint32_t turn_of(uint32_t row) { return (row & 7) ^ (row >> 4 & 1); }
 
-template <int kRows, bool kUp>
+template <int kRows, bool kUp, bool kOnce>
 __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expert_product(ProductArgs a) {
   constexpr bool kWide = kUp && kRows == 1;  // products in 16 bits
   constexpr int kSize = 32 * kRows;  // rows of a tile
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
   for (int i = 0; i < kLoads; ++i) from[i] += once, fetch(1, i);
   v8i now[2][2];  // [half][operand]
 #pragma unroll
-  for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second, i >> 1);
+  for (int i = 0; i < 4; ++i) now[i >> 1][i & 1] = load_weight32<kOnce>(codes, (i & 1) * second, i >> 1);
 
   // The weight's scales of all steps. (Down: of a block of 128 columns each pair of waves,
   // up: of gate and up.)
@@ -463,7 +473,7 @@ __global__ __launch_bounds__(256, kRows == 1 ? 4 : kRows == 2 ? 3 : 2) void expe
           constexpr bool fetches = op < 2 * kLoads && op % 2 == 0;
           constexpr int i = op < 2 * kLoads ? op / 2 : op - kLoads;
           if constexpr (fetches) from[i] += on, fetch((s + 2) & 3, i);
-          else if constexpr (op < kOps) next[i >> 1][i & 1] = load_weight32(codes, (i & 1) * second + (int64_t)ahead * kTile, i >> 1);
+          else if constexpr (op < kOps) next[i >> 1][i & 1] = load_weight32<kOnce>(codes, (i & 1) * second + (int64_t)ahead * kTile, i >> 1);
         });
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -663,6 +673,7 @@ struct Step {
 
 // up: a work-group takes 32 columns of h, a quarter of the depth a wave, three steps at once
 // (what bounds it is reading the weight: 8 KB a step, of which a CU wants some 40 under way).
+template <bool kOnce>
 __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
   constexpr int kDepth = 3;
   __shared__ float part[4][4][16];
@@ -680,7 +691,7 @@ __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
   Step ring[kDepth];
   auto load = [&](Step& to, int s) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) to.w[t] = load_weight(w, steps, t, s);
+    for (int t = 0; t < 4; ++t) to.w[t] = load_weight<kOnce>(w, steps, t, s);
     to.w_scale[0] = gate[s], to.w_scale[1] = up[s];
     const v4u* from = reinterpret_cast<const v4u*>(x + s * kBlock);
     to.x = joined(from[0], from[4]);
@@ -731,7 +742,7 @@ __global__ __launch_bounds__(256, 2) void pair_hidden(PairArgs a) {
 // it forms the codes of all choices' h, then a wave takes a choice's part of the depth after
 // another: the products, and the weight.
 constexpr int kPairCodes = 65536;
-template <typename T>
+template <typename T, bool kOnce>
 __global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
   constexpr int kDepth = 4;
   __shared__ __align__(16) uint8_t codes[kPairCodes];
@@ -749,7 +760,7 @@ __global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
   const uint8_t* ws = nullptr;
   auto load = [&](auto& to, int s) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) to.w[t] = load_weight(w, steps, t, s);
+    for (int t = 0; t < 2; ++t) to.w[t] = load_weight<kOnce>(w, steps, t, s);
     to.scale = ws[s];
   };
   // A unit's expert (past the last: none) and its first weights.
@@ -825,6 +836,7 @@ struct Plan {
   int64_t pairs, tiles;       // of the longest call, and its row tiles at most
   int rows;                   // 32-row parts of a tile; 0: each pair by itself
   int parts;                  // of the depth of a pair's down
+  bool once;                  // whether a weight is read by one work-group, seldom by more
   // Offsets of the workspace's parts.
   int64_t count, list, tokens, place, codes, scales, y, powers, bytes;
 };
@@ -840,6 +852,10 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
     p.parts = (int)(choices >= 16 ? 1 : 16 / choices);
     if (p.parts > inner / kBlock) p.parts = (int)(inner / kBlock);
     p.bytes = p.pairs * inner * 4;
+    // One token's choices are of different experts, few pairs' seldom the same (8 experts a token,
+    // 32 of 7,168 by 2,048 dims here: 1 token 66.9 -> 63.5 us, 8 of 256 in all 85.7 -> 82.3; 16
+    // would be 129.6 -> 136.6).
+    p.once = tokens == 1 || p.pairs * 4 <= total;
     return p;
   }
   // Rows of an expert, on average: tiles that most experts fill once, as long as reading the
@@ -852,6 +868,10 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   // of 64 rows these took longer, with half as many work-groups: 250 tokens, 2 of 2 experts of
   // 4,096 by 2,048 dims, one here, 44.6 -> 53.7 us, 90 tokens, 6 of 16 of 4,096 by 512, 55.1 -> 63.6.)
   if (p.pairs * experts / total * inner <= 1 << 20) p.rows = 1;
+  // Most experts have one tile, whose columns are one work-group's (32 experts of 7,168 by 2,048
+  // dims: 12 rows 250 -> 232 us, 40 262 -> 239, 88 294 -> 266; 120 354 -> 350, 160 would be 402 ->
+  // 503; 16 of 4,096 by 1,408, 40 rows in tiles of 32, 77.8 -> 79.4).
+  p.once = mean * 4 <= 3 * 32 * p.rows;
   const int64_t size = 32 * p.rows;
   p.tiles = p.pairs / size + (experts < p.pairs ? experts : p.pairs);
   if (p.tiles > p.pairs) p.tiles = p.pairs;
@@ -890,9 +910,14 @@ int launch_product(const ProductArgs& a, const Plan& p, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, a);
   };
   const int64_t groups = (p.tiles * a.column_blocks + 7) / 8 * 8;
-  if (p.rows == 1) go(expert_product<1, kUp>, groups);
-  else if (p.rows == 2) go(expert_product<2, kUp>, groups);
-  else go(expert_product<4, kUp>, groups);
+  auto pick = [&](auto once) {
+    constexpr bool kOnce = decltype(once)::value;
+    if (p.rows == 1) go(expert_product<1, kUp, kOnce>, groups);
+    else if (p.rows == 2) go(expert_product<2, kUp, kOnce>, groups);
+    else go(expert_product<4, kUp, kOnce>, groups);
+  };
+  if (p.once) pick(std::true_type{});
+  else pick(std::false_type{});
   DSA_CHECK_LAUNCH("expert product");
   return kOk;
 }
@@ -934,7 +959,11 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
     one.first = (int32_t)first, one.experts = (int32_t)experts, one.parts = p.parts;
     one.w = static_cast<const uint8_t*>(gate_up), one.w_scale = static_cast<const uint8_t*>(gate_up_scale);
     one.blocks = (int32_t)(inner / 32);
-    hipLaunchKernelGGL(pair_hidden, dim3((unsigned)(p.pairs * one.blocks)), dim3(256), 0, stream, one);
+    auto up = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.pairs * one.blocks)), dim3(256), 0, stream, one);
+    };
+    if (p.once) up(pair_hidden<true>);
+    else up(pair_hidden<false>);
     DSA_CHECK_LAUNCH("hidden values of pairs");
     one.w = static_cast<const uint8_t*>(down), one.w_scale = static_cast<const uint8_t*>(down_scale);
     one.blocks = (int32_t)(dim / 32);
@@ -942,9 +971,14 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * one.blocks)), dim3(threads), 0, stream, one);
     };
-    if (dtype == DSA_DTYPE_BF16) go(pair_result<Bf16Bits>);
-    else if (dtype == DSA_DTYPE_F16) go(pair_result<_Float16>);
-    else go(pair_result<float>);
+    auto pick = [&](auto once) {
+      constexpr bool kOnce = decltype(once)::value;
+      if (dtype == DSA_DTYPE_BF16) go(pair_result<Bf16Bits, kOnce>);
+      else if (dtype == DSA_DTYPE_F16) go(pair_result<_Float16, kOnce>);
+      else go(pair_result<float, kOnce>);
+    };
+    if (p.once) pick(std::true_type{});
+    else pick(std::false_type{});
     DSA_CHECK_LAUNCH("results of pairs");
     return kOk;
   }
