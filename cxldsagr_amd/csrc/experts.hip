@@ -31,8 +31,8 @@
 // same h; the rows of a wave's four tiles dealt out so that a lane's results are neighbours.
 //
 // What bounds it: reading the weights, up to some 100 rows an expert, where a read alone
-// reaches 6.2 TB/s (32 experts of 7,168 by 2,048 dims, 8 choices: 1 token 67 us, 5.2 TB/s; 64
-// tokens 250 us, 5.6; 128 experts, 128 tokens 893 us, 6.2); beyond that the matrix unit,
+// reaches 6.2 TB/s (32 experts of 7,168 by 2,048 dims, 8 choices: 1 token 64 us, 5.5 TB/s; 64
+// tokens 234 us, 6.0; 128 experts, 128 tokens 878 us, 6.4); beyond that the matrix unit,
 // which the card's power holds to 1.4 - 1.7 GHz (8,192 tokens 2,830 us, 2.04 PFLOP/s: up 1,620,
 // down 1,040, join 220, which is y's way to memory and back; the library's product of the same
 // type 2.70).
