@@ -230,6 +230,18 @@ def test_many_rows_are_each_as_in_small_calls(gpu):
     assert ((got[some.to(gpu)].cpu().double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("tokens, dim, inner", [(8300, 16128, 128), (4161, 32768, 256)])
+def test_many_rows_of_deep_products(gpu, tokens, dim, inner):
+    """Depths whose rows' scales do not fit beside the largest tile, on some of the rows."""
+    model = Model(gpu, dim, inner, 1)
+    x, scale, ids, weights = model.tokens(tokens, 1, 0, 1)
+    got = model.run(x, scale, ids, weights)
+    some = torch.tensor([0, 1, 31, 32, 63, 64, 127, 128, tokens // 2, tokens - 65, tokens - 2, tokens - 1])
+    want, bound = off.expert_mlp(x[some], scale[some], *model.parts, ids[some], weights[some])
+    bound = bound + 2.0 ** -8 * (want.abs() + bound)
+    assert ((got[some.to(gpu)].cpu().double() - want).abs() <= bound).all()
+
+
 def test_offsets_that_pass_32_bits(gpu):
     """Inputs, weights, hidden codes and results of more than 2^31 elements each: the last
     and the first tokens as in a call of their own."""
