@@ -632,7 +632,8 @@ __global__ __launch_bounds__(256) void join_choices(JoinArgs a) {
       weight[i] = a.weights[pair];
       if (here[i]) {
         const int64_t row = a.place[pair];
-        y[i] = *reinterpret_cast<const v8hf*>(a.y + row * a.dim + column);
+        // (Past the caches: 8,192 tokens 2,943 -> 2,926 us.)
+        y[i] = __builtin_bit_cast(v8hf, __builtin_nontemporal_load(reinterpret_cast<const v4u*>(a.y + row * a.dim + column)));
         power[i] = a.powers[row * (a.dim / kWaveCols) + column / kWaveCols];
       }
     }
