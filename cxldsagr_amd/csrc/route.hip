@@ -2,7 +2,7 @@
 //   s = sigmoid(l) or softmax(l), rounded to 32 bits;  b = s + bias (32 bits);
 //   of each group of experts the best b, with a bias the sum of its two best (32 bits);
 //   the k largest b of the top_groups best groups, in that order, ties to the lower index;
-//   w = s, or s / (their sum + 1e-20), times scale.
+//   w = s, or s / (their sum + 1e-20), times scale, rounded once to 32 bits.
 // Scores are formed in 64 bits and rounded once, so that the order is that of the definition
 // and not of some exponential's last bits. A NaN is larger than every number (as in a sort),
 // so that it shows in the weights.
@@ -29,7 +29,7 @@ struct RouteArgs {
   int32_t* ids;
   int64_t stride, tokens;
   int32_t k, groups, top_groups, size, parts, log_parts, per, softmax, renormalize, vectors;
-  float scale;
+  double scale;
 };
 
 __device__ __forceinline__ float value_of(uint16_t v) { return bf16_to_f32(v); }
@@ -230,13 +230,17 @@ __global__ __launch_bounds__(kThreads) void route(RouteArgs a) {
   }
   __syncthreads();
   if (!live) return;
-  float sum = 0.0f;
-  if (a.renormalize)
-    for (int c = 0; c < a.k; ++c) sum += scores[local][chosen[local][c]];
+  // (In 64 bits up to the weight's own rounding: in 32 the sum, the quotient and the product each
+  // added theirs.)
+  double factor = a.scale;
+  if (a.renormalize) {
+    double sum = 1e-20;
+    for (int c = 0; c < a.k; ++c) sum += (double)scores[local][chosen[local][c]];
+    factor *= reciprocal(sum);
+  }
   for (int c = l; c < a.k; c += kLanes) {
     const int at = chosen[local][c], lane = at / kSlots;
-    const float w = scores[local][at];
-    a.weights[own * a.k + c] = (a.renormalize ? w / (sum + 1e-20f) : w) * a.scale;
+    a.weights[own * a.k + c] = (float)((double)scores[local][at] * factor);
     a.ids[own * a.k + c] = (lane >> a.log_parts) * a.size + (lane & (a.parts - 1)) * a.per + at % kSlots;
   }
 }
@@ -300,7 +304,7 @@ extern "C" int dsa_route_experts(const void* logits, int64_t stride, int dtype, 
   a.logits = logits, a.bias = bias, a.weights = weights, a.ids = ids;
   a.stride = stride, a.tokens = tokens, a.k = (int32_t)k;
   a.groups = (int32_t)groups, a.top_groups = (int32_t)top_groups, a.size = (int32_t)(experts / groups);
-  a.softmax = softmax != 0, a.renormalize = renormalize != 0, a.scale = (float)scale;
+  a.softmax = softmax != 0, a.renormalize = renormalize != 0, a.scale = scale;
   if (dtype == DSA_DTYPE_BF16) return launch_route<uint16_t>(a, stream);
   if (dtype == DSA_DTYPE_F16) return launch_route<_Float16>(a, stream);
   return launch_route<float>(a, stream);

@@ -120,3 +120,21 @@ def test_offsets_that_pass_32_bits(gpu, experts, stride, tokens):
     for part in (slice(tokens - 7, tokens), slice(0, 7)):
         want = route_experts(logits[part].contiguous(), 6)
         assert torch.equal(weights[part], want[0]) and torch.equal(ids[part], want[1])
+
+
+@pytest.mark.parametrize("tokens", [37, 5000])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("k", [1, 6, 64])
+def test_weights_are_rounded_once(gpu, k, scoring, tokens):
+    """From the scores of 32 bits (weights without a sum and a scale) the formula in 64 bits:
+    half a step, 2^-24 of the value, and what the 64 bits lose, below 2^-40."""
+    from cxldsagr_amd.feedforward import route_experts
+
+    gen = torch.Generator().manual_seed(16 + k)
+    logits = torch.randn(tokens, 128, generator=gen).mul(3).to(gpu)
+    scores, ids = route_experts(logits, k, scoring=scoring, renormalize=False)
+    wide = scores.double()
+    for renormalize, want in ((True, wide / (wide.sum(1, keepdim=True) + 1e-20) * 2.3), (False, wide * 2.3)):
+        weights, same = route_experts(logits, k, scoring=scoring, renormalize=renormalize, scale=2.3)
+        assert torch.equal(same, ids)
+        assert ((weights.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -40) * want + 2.0 ** -150).all()
