@@ -263,13 +263,16 @@ int launch_route(RouteArgs a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)((a.tokens + tokens - 1) / tokens)), dim3(kThreads), 0, stream, a);
   };
   // Four tokens a wave share the lanes' exchanges, half the instructions per token; with few
-  // tokens a whole wave for one ends sooner (256 experts: 2,048 tokens 5.5 us against 7.0,
-  // 4,096 7.4 against 7.2, 16,384 19.7 against 14.1; 64 experts: 1,024 3.6 against 3.5).
+  // tokens a whole wave for one ends sooner (a wave for one against four a wave: 256 experts 3,000
+  // tokens 6.2 us against 6.8, 4,096 7.2 against 6.8; 160 experts 2,048 5.4 against 5.8, 2,560 6.2
+  // against 5.8; 128 experts 1,024 3.9 against 4.3, 2,048 4.5 against 4.3; 64 experts 1,024 3.5
+  // against 3.4). A lane's slots come by fours, whole loads of 32 bits: with 16 for all beyond 8,
+  // 16,384 tokens of 160 experts took 13.2 us (10.6 with 12), of 192 12.7 (9.8), of 144 12.6 (10.4).
   plan(16);
   if (a.tokens >= 256 * a.per && a.groups <= 16 && a.per <= 16) {
     if (a.per <= 4) go(route<T, 16, 4>, 16, 4);
     else if (a.per <= 8) go(route<T, 16, 8>, 16, 8);
-    else if (a.per <= 10) go(route<T, 16, 10>, 16, 10);
+    else if (a.per <= 12) go(route<T, 16, 12>, 16, 12);
     else go(route<T, 16, 16>, 16, 16);
     DSA_CHECK_LAUNCH("routing to experts");
     return kOk;
