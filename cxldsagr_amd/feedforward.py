@@ -266,6 +266,8 @@ class ExpertWeights:
         tensors = (gate_up, gate_up_scale, down, down_scale)
         if any(t.device != down.device for t in tensors):
             raise ValueError("weights and scales must be on the same device")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+            raise ValueError("the experts' MLP has no backward pass")
         if type(first) is not int or first < 0:
             raise ValueError("first must be a nonnegative integer")
         if total is None:
@@ -328,7 +330,8 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
     code = _native.DTYPE_CODES.get(dtype)
     if code is None:
         raise ValueError("dtype must be bf16, fp16 or fp32")
-    if torch.is_grad_enabled() and weights.requires_grad:
+    if torch.is_grad_enabled() and (x.requires_grad or x_scale.requires_grad
+                                    or weights.requires_grad):
         raise ValueError("the experts' MLP has no backward pass")
     _native.require_gfx950(device, "the experts' MLP")
     if out is None:

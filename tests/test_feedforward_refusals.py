@@ -271,3 +271,24 @@ def test_c_experts():
             _native.call("dsa_expert_mlp_fp8", *{**good, **change}.values(), None)
     # No tokens: nothing is read.
     _native.call("dsa_expert_mlp_fp8", *{**good, "tokens": 0, "x": 0, "out": 0}.values(), None)
+
+
+@pytest.mark.parametrize("name", ["x", "x_scale", "weights"])
+def test_experts_refuse_what_wants_gradients(name):
+    args = dict(x=z(3, 256, dtype=F8), x_scale=z(3, 2, dtype=E8), experts=ExpertWeights(**_parts()),
+                ids=torch.zeros(3, 2, dtype=torch.int32), weights=torch.zeros(3, 2))
+    args[name].requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        expert_mlp(**args)
+    with torch.no_grad(), pytest.raises(NotImplementedError):  # (as far as a CPU's tensors get)
+        expert_mlp(**args)
+
+
+@pytest.mark.parametrize("name", sorted(_parts()))
+def test_weights_that_want_gradients_are_refused(name):
+    parts = _parts()
+    parts[name].requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        ExpertWeights(**parts)
+    with torch.no_grad():
+        assert ExpertWeights(**parts).experts == 2
