@@ -70,6 +70,14 @@ def _apart(out, tensor):
             or other >= begin + rows * dim * size)
 
 
+def _over(out, tensor):
+    """Whether contiguous ``out`` shares memory with ``tensor``, if that is contiguous too
+    (else it is copied before anything is written)."""
+    begin, other = out.data_ptr(), tensor.data_ptr()
+    return (begin < other + tensor.numel() * tensor.element_size()
+            and other < begin + out.numel() * out.element_size() and tensor.is_contiguous())
+
+
 def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quantize=False,
                       residual_out=None):
     """``t = x + residual`` and ``t * weight / sqrt(mean(t^2) + eps)`` of every row.
@@ -327,6 +335,8 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
                 or not out.is_contiguous() or out.data_ptr() % 16):
             raise ValueError("out must be a contiguous, 16-byte aligned [T, D] tensor of dtype on "
                              "the experts' device")
+        if tokens and (_over(out, x) or _over(out, x_scale) or _over(out, ids) or _over(out, weights)):
+            raise ValueError("out must not overlap the inputs")
     code = _native.DTYPE_CODES.get(dtype)
     if code is None:
         raise ValueError("dtype must be bf16, fp16 or fp32")

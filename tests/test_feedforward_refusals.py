@@ -292,3 +292,31 @@ def test_weights_that_want_gradients_are_refused(name):
         ExpertWeights(**parts)
     with torch.no_grad():
         assert ExpertWeights(**parts).experts == 2
+
+
+def test_an_output_over_an_input_is_refused():
+    own = ExpertWeights(**_parts())
+    whole = torch.zeros(8192, dtype=torch.uint8)
+
+    def at(offset, dtype, *shape):
+        size = torch.empty(shape, dtype=dtype).numel() * dtype.itemsize
+        return whole[offset:offset + size].view(dtype).view(shape)
+
+    out = at(2048, B16, 3, 256)  # 1,536 bytes
+    free = dict(x=at(0, F8, 3, 256), x_scale=at(1024, E8, 3, 2), ids=at(1100, torch.int32, 3, 2),
+                weights=at(1200, torch.float32, 3, 2))
+    over = dict(x=[at(2048, F8, 3, 256), at(2048 + 1520, F8, 3, 256), at(2048 - 752, F8, 3, 256)],
+                x_scale=[at(2048 + 1535, E8, 3, 2), at(2043, E8, 3, 2)], ids=[at(2028, torch.int32, 3, 2)],
+                weights=[at(2048 + 1532, torch.float32, 3, 2)])
+    for name, tensors in over.items():
+        for tensor in tensors:
+            with pytest.raises(ValueError, match="overlap"):
+                expert_mlp(**{**free, name: tensor}, experts=own, out=out)
+    # Neighbours are not, nor what is copied first, nor a call without tokens.
+    for change in (dict(x=at(2048 - 768, F8, 3, 256)), dict(x=at(2048 + 1536, F8, 3, 256)),
+                   dict(ids=at(2048, torch.int32, 2, 3).t())):
+        with pytest.raises(NotImplementedError):  # (as far as a CPU's tensors get)
+            expert_mlp(**{**free, **change}, experts=own, out=out)
+    none = {name: t[:0] for name, t in {**free, "x": over["x"][0]}.items()}
+    with pytest.raises(NotImplementedError):
+        expert_mlp(**none, experts=own, out=out[:0])
