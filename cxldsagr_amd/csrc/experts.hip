@@ -894,6 +894,10 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   return p;
 }
 
+// Work-groups of a product: up's tiles times 128 hidden columns, down's times 256 of the result.
+int64_t up_blocks(int64_t inner) { return inner / kBlock; }
+int64_t down_blocks(int64_t dim) { return (dim + 255) / 256; }
+
 int check_shape(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_t experts, int64_t total) {
   DSA_CHECK_ARG(dim >= kBlock && dim % kBlock == 0 && dim <= 32768 && inner >= kBlock && inner % kBlock == 0 &&
                     inner <= 32768,
@@ -902,6 +906,10 @@ int check_shape(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int
                 "experts must number 1 to %d, total at least as many and at most 2^30", kMaxExperts);
   DSA_CHECK_ARG(choices >= 1 && choices <= 64, "choices must number 1 to 64");
   DSA_CHECK_ARG(tokens >= 0 && tokens <= (1 << 22), "tokens must number 0 to 2^22");
+  // (Here, so that the size's query refuses what the call would.)
+  const int64_t tiles = plan_of(tokens, choices, dim, inner, experts, total).tiles;
+  DSA_CHECK_ARG(grid_fits(tiles * up_blocks(inner) + 7, 256) && grid_fits(tiles * down_blocks(dim) + 7, 256),
+                "too many tokens for one launch");
   return kOk;
 }
 
@@ -995,21 +1003,18 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   up.tiles = tiles, up.tile_count = count;
   up.codes = ws + p.codes, up.scales = ws + p.scales;
   up.depth = (int32_t)dim, up.columns = (int32_t)(2 * inner);
-  up.column_blocks = (int32_t)(inner / kBlock);
+  up.column_blocks = (int32_t)up_blocks(inner);
   ProductArgs dn{};
   dn.x = up.codes, dn.x_scale = up.scales;
   dn.w = static_cast<const uint8_t*>(down), dn.w_scale = static_cast<const uint8_t*>(down_scale);
   dn.tiles = tiles, dn.tile_count = count;
   dn.y = reinterpret_cast<uint16_t*>(ws + p.y), dn.powers = ws + p.powers;
   dn.depth = (int32_t)inner, dn.columns = (int32_t)dim;
-  dn.column_blocks = (int32_t)((dim + 255) / 256);
+  dn.column_blocks = (int32_t)down_blocks(dim);
   JoinArgs j{};
   j.ids = ids, j.place = place, j.weights = weights, j.y = dn.y, j.powers = dn.powers, j.out = out;
   j.choices = (int32_t)choices, j.first = (int32_t)first, j.experts = (int32_t)experts, j.dim = (int32_t)dim;
   j.groups_per_token = (int32_t)((dim / 8 + 255) / 256);
-  DSA_CHECK_ARG(grid_fits(p.tiles * up.column_blocks + 7, 256) && grid_fits(p.tiles * dn.column_blocks + 7, 256) &&
-                    grid_fits(tokens * j.groups_per_token, 256),
-                "too many tokens for one launch");
 
   const GroupArgs group{ids, row_tokens, place, tiles, count, (int32_t)p.pairs, (int32_t)choices, (int32_t)first,
                         (int32_t)experts, 32 * p.rows};
@@ -1025,8 +1030,16 @@ extern "C" int dsa_expert_mlp_fp8(const void* x, const void* x_scale, int64_t to
   DSA_CHECK_LAUNCH("grouping of pairs");
   if (const int status = launch_product<true>(up, p, stream)) return status;
   if (const int status = launch_product<false>(dn, p, stream)) return status;
+  // (A launch holds 2^24 - 1 work-groups; the tokens behind take another.)
+  const int64_t at_once = ((1ll << 24) - 1) / j.groups_per_token, out_bytes = dim * (dtype == DSA_DTYPE_F32 ? 4 : 2);
   auto join = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * j.groups_per_token)), dim3(256), 0, stream, j);
+    for (int64_t begin = 0; begin < tokens; begin += at_once) {
+      const int64_t some = tokens - begin < at_once ? tokens - begin : at_once;
+      JoinArgs of = j;
+      of.ids += begin * choices, of.place += begin * choices, of.weights += begin * choices;
+      of.out = static_cast<uint8_t*>(out) + begin * out_bytes;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(some * j.groups_per_token)), dim3(256), 0, stream, of);
+    }
   };
   if (dtype == DSA_DTYPE_BF16) join(join_choices<Bf16Bits>);
   else if (dtype == DSA_DTYPE_F16) join(join_choices<_Float16>);

@@ -301,7 +301,10 @@ def expert_mlp(x, x_scale, experts, ids, weights, *, dtype=torch.bfloat16, out=N
     ``residual_rms_norm`` gives them), ``experts`` an ``ExpertWeights``, ``ids`` int32
     and ``weights`` fp32 ``[T, k]``, k up to 64 (as ``route_experts`` gives them).
     Choices outside ``experts.first .. first + E - 1`` add nothing (an expert of another
-    rank, or -1 for none); a token may choose an expert twice. T up to 2^22.
+    rank, or -1 for none); a token may choose an expert twice. T up to 2^22, but refused
+    where the products' row tiles (of 32 to 128 choices) by their columns (I / 128 or
+    D / 256) would number 2^24. The workspace of a long call holds some 2 D + I bytes for
+    each of the T k choices, whichever rank's.
 
     Returns ``[T, D]`` in ``dtype`` (bf16, fp16 or fp32), or writes it to ``out``
     (contiguous, of ``dtype``); a token without a choice here gives zeros. Sums are in

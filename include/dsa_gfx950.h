@@ -693,8 +693,9 @@ int dsa_route_experts(const void* logits, int64_t stride, int dtype, int64_t tok
  * out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j] - first,
  * over the choices with 0 <= e < experts. x: e4m3 [tokens, dim], x_scale: exponent bytes
  * [tokens, dim / 128]; ids int32, weights f32 [tokens, choices] (1 .. 64 choices); dim and
- * inner in whole blocks of 128 up to 32768, tokens up to 2^22, experts 1 .. 1024 of the
- * model's `total` (up to 2^30; it only steers tiles). Weights are e4m3 in tiles of 16 rows by
+ * inner in whole blocks of 128 up to 32768, tokens up to 2^22 (fewer where a product would take
+ * 2^24 work-groups: refused, by the workspace's query too), experts 1 .. 1024 of the model's
+ * `total` (up to 2^30; it only steers tiles). Weights are e4m3 in tiles of 16 rows by
  * 128 columns, 2048 bytes, [experts][rows / 16][columns / 128][plane 2][g 4][row 16][16 bytes]:
  * bytes 64 plane + 16 g .. of a row's 128. Four tiles hold 64 rows of down [dim, inner], dealt
  * out: row 4 a + i of tile t is the 64's row 16 a + 4 t + i. Of gate_up [2 inner, dim] four

@@ -320,3 +320,15 @@ def test_an_output_over_an_input_is_refused():
     none = {name: t[:0] for name, t in {**free, "x": over["x"][0]}.items()}
     with pytest.raises(NotImplementedError):
         expert_mlp(**none, experts=own, out=out[:0])
+
+
+def test_sizes_of_too_many_tokens_are_refused_with_the_query():
+    size = ctypes.c_int64()
+    query = "dsa_expert_mlp_workspace_bytes"
+    for args in [(1 << 22, 64, 32768, 32768, 4, 4), (1 << 22, 64, 7168, 128, 256, 256), (1 << 22, 64, 128, 7168, 256, 256)]:
+        with pytest.raises(ValueError, match="too many tokens"):
+            _native.call(query, *args, ctypes.byref(size))
+    # The most tokens, of a choice and of eight.
+    for args in [(1 << 22, 1, 32768, 128, 1, 1), (1 << 22, 8, 7168, 2048, 256, 256)]:
+        _native.call(query, *args, ctypes.byref(size))
+        assert size.value > (1 << 22) * args[1] * (args[2] * 2 + args[3])

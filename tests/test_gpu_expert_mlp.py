@@ -267,3 +267,28 @@ def test_offsets_that_pass_32_bits(gpu):
     for part in (slice(tokens - 3000, tokens), slice(0, 3000)):
         want = expert_mlp(x[part], scale[part], own, ids[part], weights[part])
         assert want.abs().amax(1).min() > 0 and torch.equal(got[part], want)
+
+
+def test_the_most_tokens(gpu):
+    """2^22 tokens, the last of which is joined by a launch of its own; few have a choice here."""
+    from cxldsagr_amd.feedforward import expert_mlp
+
+    tokens, dim = 1 << 22, 6272  # four work-groups a token
+    model = Model(gpu, dim, 128, 1)
+    some = torch.tensor([0, 77, tokens - 3, tokens - 2, tokens - 1])
+    few, few_scale, few_ids, few_weights = model.tokens(len(some), 1, 0, 1)
+    x = torch.zeros(tokens, dim, dtype=torch.uint8, device=gpu)
+    scale = torch.zeros(tokens, dim // 128, dtype=torch.uint8, device=gpu)
+    ids = torch.full((tokens, 1), -1, dtype=torch.int32, device=gpu)
+    weights = torch.zeros(tokens, 1, device=gpu)
+    out = torch.empty(tokens, dim, dtype=torch.bfloat16, device=gpu).fill_(7.0)
+    for to, of in ((x, few.view(torch.uint8)), (scale, few_scale.view(torch.uint8)), (ids, few_ids), (weights, few_weights)):
+        to[some.to(gpu)] = of.to(gpu)
+    expert_mlp(x.view(F8), scale.view(E8), model.own, ids, weights, out=out)
+    want, bound = off.expert_mlp(few, few_scale, *model.parts, few_ids, few_weights)
+    bound = bound + 2.0 ** -8 * (want.abs() + bound) + 2.0 ** -25
+    assert ((out[some.to(gpu)].cpu().double() - want).abs() <= bound).all()
+    out[some.to(gpu)] = 0
+    assert not any(bool(part.any()) for part in out.split(1 << 18))
+    del x, scale, ids, weights, out
+    torch.cuda.empty_cache()
