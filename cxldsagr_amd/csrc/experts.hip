@@ -764,6 +764,9 @@ __global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
     for (int t = 0; t < 2; ++t) to.w[t] = load_weight<kOnce>(w, steps, t, s);
     to.scale = ws[s];
   };
+  // The choices that are here, a bit each (64 at most).
+  const uint32_t mine = lane < a.choices ? (uint32_t)a.ids[token * a.choices + lane] - (uint32_t)a.first : ~0u;
+  const uint64_t here = __ballot(mine < (uint32_t)a.experts);
   // A unit's expert (past the last: none) and its first weights.
   int begin = 0, end = 0;
   auto start = [&](int u) {
@@ -780,8 +783,9 @@ __global__ __launch_bounds__(1024) void pair_result(PairArgs a) {
   };
   bool some = start(wave);
 
-  // 16 lanes a block of 128. (Of choices that are not here: what memory held, and not used.)
+  // 16 lanes a block of 128. (Of choices that are not here nothing was written.)
   for (int i = threadIdx.x >> 4; i < a.choices * steps; i += blockDim.x >> 4) {
+    if (!(here >> (i / steps) & 1)) continue;
     const float4* from = reinterpret_cast<const float4*>(a.hidden + token * a.choices * a.inner + i * kBlock + (threadIdx.x & 15) * 8);
     const float4 one = from[0], two = from[1];
     const float v[8] = {one.x, one.y, one.z, one.w, two.x, two.y, two.z, two.w};

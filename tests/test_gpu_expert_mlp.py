@@ -292,3 +292,28 @@ def test_the_most_tokens(gpu):
     assert not any(bool(part.any()) for part in out.split(1 << 18))
     del x, scale, ids, weights, out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("choices, inner", [(8, 2048), (3, 384), (64, 128)])
+def test_pairs_of_other_ranks_are_not_read(gpu, choices, inner):
+    """A slice of many experts, pairs by themselves, over a workspace and a result of NaN: as over
+    zeros; tokens without a choice here are zeros."""
+    from cxldsagr_amd import _native
+
+    experts, total, dim, tokens = 8, 64 * choices, 384, 9
+    model = Model(gpu, dim, inner, experts, first=16, total=total)
+    x, scale, ids, weights = (t.to(gpu) for t in model.tokens(tokens, choices, 0, total))
+    ids[0], ids[1], ids[2, 0], ids[3] = 5, 17, 23, -1  # none, all, at least one, none
+    want = model.check(x, scale, ids, weights)
+    assert want[1].any() and want[2].any() and not want[0].any() and not want[3].any()
+    own = model.own
+    needed = _native.size_of("dsa_expert_mlp_workspace_bytes", 0, tokens, choices, dim, inner, experts, total)
+    assert needed == tokens * choices * inner * 4  # (the pairs' hidden values alone)
+    for fill in (0, 255):
+        workspace = torch.full((needed,), fill, dtype=torch.uint8, device=gpu)
+        out = torch.full((tokens, dim), float("nan"), dtype=torch.bfloat16, device=gpu)
+        _native.call("dsa_expert_mlp_fp8", x.data_ptr(), scale.data_ptr(), tokens, dim, inner, own.gate_up.data_ptr(),
+                     own.gate_up_scale.data_ptr(), own.down.data_ptr(), own.down_scale.data_ptr(), experts, own.first,
+                     total, ids.data_ptr(), weights.data_ptr(), choices, out.data_ptr(), 0, workspace.data_ptr(), needed,
+                     torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out, want)
