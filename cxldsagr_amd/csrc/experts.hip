@@ -849,10 +849,16 @@ struct Plan {
 Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_t experts, int64_t total) {
   Plan p{};
   p.pairs = tokens * choices;
-  // Pair by pair up to three quarters as many pairs as experts (32 experts, 8 choices: 1 token
-  // 80 -> 68 us, 3 182 -> 172, 4 would be 187 -> 219), where a token's codes fit into LDS.
+  // Pair by pair up to three quarters as many pairs as experts, where a token's codes fit into
+  // LDS and the weights of the pairs that are to be expected here stay below 500 MB: beyond that
+  // tiles fill the card and read what two pairs share once (8 choices of 7,168 by 2,048 dims, 44
+  // MB a pair; pairs by themselves and in tiles: 32 experts 1 token 65 us against 99, 2 tokens 120
+  // against 111; 256 experts 1 token 74 against 101, 12 681 against 558, 24 1,337 against 912; 32 of
+  // 256 here 10 tokens 95 against 103, 12 117 against 111, 24 202 against 143. 6 of 64 experts of
+  // 2,048 by 1,408: 6 tokens 57 against 58, 8 68 against 68).
   const int64_t few = total * 3 / 4 > choices ? total * 3 / 4 : choices;
-  if (p.pairs <= few && choices * inner <= kPairCodes && grid_fits(p.pairs * (inner / 32), 256) &&
+  const double weights = (double)p.pairs * experts / total * (3.0 * dim * inner);
+  if (p.pairs <= few && weights <= 5e8 && choices * inner <= kPairCodes && grid_fits(p.pairs * (inner / 32), 256) &&
       grid_fits(tokens * (dim / 32), 1024)) {
     p.parts = (int)(choices >= 16 ? 1 : 16 / choices);
     if (p.parts > inner / kBlock) p.parts = (int)(inner / kBlock);

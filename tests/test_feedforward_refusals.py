@@ -332,3 +332,15 @@ def test_sizes_of_too_many_tokens_are_refused_with_the_query():
     for args in [(1 << 22, 1, 32768, 128, 1, 1), (1 << 22, 8, 7168, 2048, 256, 256)]:
         _native.call(query, *args, ctypes.byref(size))
         assert size.value > (1 << 22) * args[1] * (args[2] * 2 + args[3])
+
+
+@pytest.mark.parametrize(("args", "alone"), [
+    ((1, 8, 7168, 2048, 32, 32), True), ((2, 8, 7168, 2048, 32, 32), False), ((1, 8, 7168, 2048, 256, 256), True),
+    ((24, 8, 7168, 2048, 256, 256), False), ((8, 8, 7168, 2048, 32, 256), True), ((24, 8, 7168, 2048, 32, 256), False),
+    ((6, 8, 1024, 512, 64, 64), True), ((12, 8, 1024, 512, 64, 64), False),
+])
+def test_pairs_are_taken_by_themselves_where_that_is_sooner(args, alone):
+    """The workspace is then the pairs' hidden values."""
+    size = ctypes.c_int64()
+    _native.call("dsa_expert_mlp_workspace_bytes", *args, ctypes.byref(size))
+    assert (size.value == args[0] * args[1] * args[3] * 4) == alone
