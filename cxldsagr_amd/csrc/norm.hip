@@ -1,11 +1,13 @@
 // The residual stream's sum and its root-mean-square norm, for every row:
 //   t = x + r (in 32 bits), y = t w / sqrt(mean t^2 + eps),
-// y rounded once to the element type, t too; and, where wanted, the e4m3 codes of the
-// rounded y with a power-of-two scale for every 128 values, as its exponent (e8m0).
+// y rounded to 32 bits and then to the element type, as a cast from 64 bits does, t from its 32;
+// and, where wanted, the e4m3 codes of the rounded y with a power-of-two scale for every 128
+// values, as its exponent (e8m0).
 //
-// The sum of squares is in 64 bits, y in 46 or more, so that y and its codes are the formula's
-// (a y of 32 bits lies on the other side of a rounding border in one of some 30,000 values,
-// and of a scale's border now and then, which doubles a whole block's step).
+// The sum of squares is in 64 bits, y in 46 or more before it is rounded, so that y and its codes
+// are those of that cast (a y formed in 32 bits lies on the other side of a rounding border in one
+// of some 30,000 values, and of a scale's border now and then, which doubles a whole block's
+// step). The 46 bits end at 2^-149: values below 2^-102 of a row's root mean square have fewer.
 //
 // Bound by memory: a row is read once, kept in registers over the sum, and written once.
 #include "quantize_core.h"
@@ -96,6 +98,13 @@ __device__ __forceinline__ double reciprocal_root(double v) {
   return r == r ? better : y;
 }
 
+// A product of 64 bits as one of 32. (With contraction the compiler makes its conversion and a
+// following one to fp16 a single one, which rounds once.)
+__device__ __forceinline__ float rounded_product(double v, double inverse, double weight) {
+#pragma clang fp contract(off)
+  return (float)(v * inverse * weight);
+}
+
 // Items of 8 elements, kItems a thread at most: item i is thread i % threads' item
 // i / threads. A work-group goes from row to row with the weight in registers and the next
 // row on its way.
@@ -155,7 +164,7 @@ __global__ __launch_bounds__(kThreads, kItems * sizeof(T) <= 4 ? 4 : 2) void res
     auto normed = [&](float v, float weight) {
 // (A product that becomes part of the sum would count its rounding twice.)
 #pragma clang fp contract(off)
-      if (!pairs) return (float)((double)v * inverse * weight);
+      if (!pairs) return rounded_product(v, inverse, weight);
       const float u = v * high, u_low = __builtin_fmaf(v, low, __builtin_fmaf(v, high, -u));
       const float y = u * weight, both = y + __builtin_fmaf(u_low, weight, __builtin_fmaf(u, weight, -y));
       return both == both ? both : y;  // (an infinity less itself)
@@ -215,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void residual_rms_norm_scalar(NormArgs a)
       const float t = total(i);
       if (a.residual_out) static_cast<T*>(a.residual_out)[base + i] = rounded<T>(t);
       const float w = a.wide_weight ? static_cast<const float*>(a.weight)[i] : value_of(static_cast<const T*>(a.weight)[i]);
-      if (a.values) static_cast<T*>(a.values)[base + i] = rounded<T>((float)((double)t * w * inverse));
+      if (a.values) static_cast<T*>(a.values)[base + i] = rounded<T>(rounded_product(t, inverse, w));
     }
   }
 }

@@ -132,3 +132,25 @@ def test_offsets_that_pass_32_bits(gpu, dim):
         if quantize:
             for a, b in ((got.codes, want.codes), (got.scales, want.scales)):
                 assert torch.equal(a[part].view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype, bits", [("bf16", 8), ("fp16", 11)])
+@pytest.mark.parametrize("dim", [7168, 7161])
+def test_values_are_rounded_to_32_bits_and_then_to_the_type(gpu, dtype, bits, dim):
+    """As a cast of the 64-bit value does: every value, and not all are those of one rounding.
+    (The kernel's 46 bits fall on another side of a border of 32 in one of 2^22 values, which
+    shows in 16 bits where that is next to a tie, one in 2^13 or fewer of these.)"""
+    from cxldsagr_amd.feedforward import residual_rms_norm
+
+    gen = torch.Generator(device=gpu).manual_seed(31)
+    tokens, dtype = 1024, TYPES[dtype]
+    x, r = (torch.randn(tokens, dim, generator=gen, device=gpu).to(dtype) for _ in range(2))
+    weight = 1 + 0.1 * torch.randn(dim, generator=gen, device=gpu)
+    got = residual_rms_norm(x, weight, r)
+    t = (x.float() + r.float()).double()
+    want = t / (t.square().mean(1, keepdim=True) + 1e-6).sqrt() * weight.double()
+    assert torch.equal(got.values, want.float().to(dtype))
+    part, power = torch.frexp(want)
+    once = torch.ldexp((part * 2.0 ** bits).round(), power - bits)  # (ties to even, as round)
+    normal = want.abs() >= torch.finfo(dtype).smallest_normal
+    assert int((once != got.values.double())[normal].sum()) > 0
