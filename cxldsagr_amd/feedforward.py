@@ -83,9 +83,11 @@ def residual_rms_norm(x, weight, residual=None, *, eps=1e-6, values=True, quanti
     """``t = x + residual`` and ``t * weight / sqrt(mean(t^2) + eps)`` of every row.
 
     ``x`` (and ``residual``) ``[T, D]`` in bf16, fp16 or fp32, any row stride, D up to
-    16384; ``weight`` ``[D]`` in fp32 or ``x``'s type. The sum is one of 32 bits, the
-    norm is formed in 64 from the sum before its rounding, and each output is rounded
-    once to ``x``'s type. With ``quantize`` (D in whole blocks of 128) the rounded
+    16384; ``weight`` ``[D]`` in fp32 or ``x``'s type. The sum is one of 32 bits, rounded
+    to ``x``'s type where it is returned; the norm is formed from the sum before that, to 46
+    bits or more, and rounded to 32 bits and then to ``x``'s type, as a cast from 64 bits
+    does (one rounding would give another value in one of some 130,000 in bf16, 17,000 in
+    fp16). With ``quantize`` (D in whole blocks of 128) the rounded
     values come as e4m3 codes too, with a power-of-two scale for every 128 of a row (the
     rule of ``indexer.quantize_index``); ``values=False`` leaves them as codes only.
 

@@ -664,11 +664,11 @@ int dsa_pool_release_rows(const int32_t* page_table, int64_t pages, int64_t host
  *
  * dsa_residual_rms_norm: t = x + residual (32 bits), y = t * weight / sqrt(mean t^2 + eps).
  * x, residual (or NULL): [tokens, dim] of `dtype` with row strides, dim 1 .. 16384; weight
- * [dim] of weight_dtype (dtype or fp32). Outputs are contiguous, each or NULL: values y and
- * residual_out t in `dtype`, rounded once; codes e4m3 [tokens, dim] of the rounded y with
- * scales [tokens, dim / 128], the exponent bytes (e8m0) of a power of two per 128 values
- * (amax * fl32(1/448) rounded up); both or neither, dim then in whole blocks of 128 and all
- * rows 16-byte aligned. residual_out may be residual, values x.
+ * [dim] of weight_dtype (dtype or fp32). Outputs are contiguous, each or NULL: values y (formed
+ * to 46 bits, rounded to fp32 and then to `dtype`) and residual_out t in `dtype`; codes e4m3
+ * [tokens, dim] of the rounded y with scales [tokens, dim / 128], the exponent bytes (e8m0) of a
+ * power of two per 128 values (amax * fl32(1/448) rounded up); both or neither, dim then in whole
+ * blocks of 128 and all rows 16-byte aligned. residual_out may be residual, values x.
  */
 int dsa_residual_rms_norm(const void* x, int64_t x_stride, const void* residual,
                           int64_t residual_stride, int dtype, const void* weight,
