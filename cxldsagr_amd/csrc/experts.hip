@@ -23,19 +23,20 @@
 // of two. A product of 8 bits loses nothing down to 2^-6 of the largest, so that sums of normal
 // values, 128 to 7,168 of them, are 1.4e-5 to 1.5e-5 of their size off: one in 700 codes of h falls
 // on the other side of a border, and the result's error is 1.2 times that of products in 64 bits,
-// 2.0e-3 of its size against 1.7e-3, most of it the rounding to bf16. 16-bit products, which lose
-// nothing, need twice the unit's time and the codes' conversion: up's are of those in tiles of 32
-// rows and of pairs by themselves. Weights are laid out as
-// waves read them (ExpertWeights), straight into registers: tiles of 16 rows by 128, 2 KB, in
+// 2.0e-3 of its size against 1.7e-3, most of it the rounding to bf16 (a row in which none of the
+// largest codes moves has that alone; one row in 100 is 5e-3 off, the worst of 8,000 of 512 hidden
+// values each 4e-2). 16-bit products, which lose nothing, need twice the unit's time and the codes'
+// conversion: up's are of those in tiles of 32 rows and of pairs by themselves. Weights are laid out
+// as waves read them (ExpertWeights), straight into registers: tiles of 16 rows by 128, 2 KB, in
 // planes of 16 bytes a lane; tiles of gate and up in turn, so that a lane holds g and u of the
 // same h; the rows of a wave's four tiles dealt out so that a lane's results are neighbours.
 //
-// What bounds it: reading the weights, up to some 100 rows an expert, where a read alone
-// reaches 6.2 TB/s (32 experts of 7,168 by 2,048 dims, 8 choices: 1 token 64 us, 5.5 TB/s; 64
-// tokens 234 us, 6.0; 128 experts, 128 tokens 878 us, 6.4); beyond that the matrix unit,
-// which the card's power holds to 1.4 - 1.7 GHz (8,192 tokens 2,830 us, 2.04 PFLOP/s: up 1,620,
-// down 1,040, join 220, which is y's way to memory and back; the library's product of the same
-// type 2.70).
+// What bounds it: reading the weights, up to some 100 rows an expert, where a kernel that only
+// reads reaches 6.2 TB/s, past the caches 6.9 (32 experts of 7,168 by 2,048 dims, 8 choices: 1
+// token 63 us, 5.6 TB/s; 64 tokens 232 us, 6.1; 128 experts, 128 tokens 860 us, 6.6); beyond that
+// the matrix unit, which the card's power holds to 1.4 - 1.7 GHz (8,192 tokens 2,840 us, 2.03
+// PFLOP/s: grouping 41, up 1,591, down 1,005, join 204, which is y's way to memory and back; the
+// library's product of the same type 2.67. All of one card; another card's calls were within 4 %).
 #include "attention_core.h"
 #include "quantize_core.h"
 #include "../../include/dsa_gfx950.h"
@@ -73,10 +74,13 @@ __device__ __forceinline__ v16f product32(v8i w, v8i x, v16f c, uint32_t w_scale
 // The same products in 16 bits, of codes that are converted for it: the unit adds these with 32
 // bits throughout (sums of 7,168 are 1.2e-7 of their size off). They are up's where they cost
 // little, while reading the weights is what takes time (1 token 64.1 -> 65.1 us, 64 tokens 249.6
-// -> 251.1), and where h has few values, with many rows of few experts at up to a fifth more (500
-// of one of 7,168 by 2,048 dims 56.4 -> 69.1): 1.4e-5 moves one code of h in 700 by a step, and
-// among fewer than some 2^20 a single one of the largest may show in the result more than all
-// other roundings.
+// -> 251.1), and where a call has few values of h, with many rows of few experts at up to a fifth
+// more (500 of one of 7,168 by 2,048 dims 56.4 -> 69.1). That is for a call's result as a whole, not
+// for a row's, whose error in 8 bits is the same however many come with it: 1.4e-5 moves one code of
+// h in 700 by a step, and where that is one of its row's largest, that row is up to 4e-2 of its size
+// off. Of many such rows the result is 2.0e-3 off; of fewer than some 2^20 values a single one may
+// be more of it than all other roundings (500 rows of one expert of 1,024 by 128 dims: 2.5e-3, in 16
+// bits 1.7e-3; 250 rows of two of 8 of 4,096 by 2,048: 2.2e-3; 8,000 of 1,024 by 128: 1.9e-3).
 // x takes both scales with it, 2^(a + b - 254) of their exponents' bytes, as the number whose
 // exponent the conversion takes (255: NaN; products that bf16's exponents do not hold are far
 // outside those of h).
@@ -216,13 +220,6 @@ struct ProductArgs {
 
 __device__ __forceinline__ float silu(float g) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -kLog2E));
-}
-
-__device__ __forceinline__ uint32_t max_over_groups(uint32_t v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = a[0] > a[1] ? a[0] : a[1];
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return b[0] > b[1] ? b[0] : b[1];
 }
 
 // h of kCount gates and ups of one row, and the largest magnitude's bits.
@@ -632,7 +629,8 @@ __global__ __launch_bounds__(256) void join_choices(JoinArgs a) {
       weight[i] = a.weights[pair];
       if (here[i]) {
         const int64_t row = a.place[pair];
-        // (Past the caches: 8,192 tokens 2,943 -> 2,926 us.)
+        // (Past the caches: 8,192 tokens 226 - 233 -> 201 - 209 us of this launch, less than the
+        // whole call varies by; 2,048 53 -> 51, 64 5.0 both.)
         y[i] = __builtin_bit_cast(v8hf, __builtin_nontemporal_load(reinterpret_cast<const v4u*>(a.y + row * a.dim + column)));
         power[i] = a.powers[row * (a.dim / kWaveCols) + column / kWaveCols];
       }
@@ -875,8 +873,9 @@ Plan plan_of(int64_t tokens, int64_t choices, int64_t dim, int64_t inner, int64_
   const int64_t mean = p.pairs / total;
   p.rows = mean <= 16 ? 1 : mean <= 48 ? 2 : 4;
   if (dim > max_up_steps(4) * kBlock && p.rows > 2) p.rows = 2;
-  // Few values of h (of the pairs that are to be expected here) want 16-bit products. (In tiles
-  // of 64 rows these took longer, with half as many work-groups: 250 tokens, 2 of 2 experts of
+  // Few values of h (of the pairs that are to be expected here) want 16-bit products, for the
+  // result as a whole (above wide_product). (In tiles of 64
+  // rows these took longer, with half as many work-groups: 250 tokens, 2 of 2 experts of
   // 4,096 by 2,048 dims, one here, 44.6 -> 53.7 us, 90 tokens, 6 of 16 of 4,096 by 512, 55.1 -> 63.6.)
   if (p.pairs * experts / total * inner <= 1 << 20) p.rows = 1;
   // Most experts have one tile, whose columns are one work-group's (32 experts of 7,168 by 2,048

@@ -682,7 +682,7 @@ int dsa_residual_rms_norm(const void* x, int64_t x_stride, const void* residual,
  * ties to the lower index, NaN above all, among the top_groups best of `groups` equal groups
  * (1 .. 64; a group counts as its best expert, with a bias as its two best's sum).
  * weights f32 and ids int32 [tokens, k], best first: s * scale, or with renormalize
- * s / (the k's sum + 1e-20) * scale.
+ * s / (the k's sum + 1e-20) * scale, in 64 bits from s and rounded once.
  */
 int dsa_route_experts(const void* logits, int64_t stride, int dtype, int64_t tokens,
                       int64_t experts, int64_t k, const float* bias, int softmax, int64_t groups,
